@@ -342,6 +342,86 @@ int mhc_stream_collapse(const void* H, int dtype_h, void* y, int dtype_y, int64_
 int mhc_convert(int n, const void* const* src, const int* src_dtype, void* const* dst, const int* dst_dtype,
                 const int64_t* count, mhc_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Inside the branch (no reference counterpart): the norm of its input, its
+ * experts' matrix products, dropout of its output.
+ * ------------------------------------------------------------------------ */
+
+/* RMS norm of R rows of D, D <= 16384, with the residual's addition:
+ *   h = x + residual (rounded to dtype; without a residual h = x, not written)
+ *   y = h * rstd * weight,  rstd = 1 / sqrt(mean_d h^2 + eps)
+ * x, residual, y, h [R,D] in `dtype`; weight [D] f32 or NULL (ones); rstd [R]
+ * f32, or NULL where no backward follows. */
+int mhc_rms_norm_forward(const void* x, const void* residual, int dtype,
+                         const float* weight, void* y, void* h, float* rstd,
+                         int64_t R, int64_t D, float eps, mhc_stream_t stream);
+
+/* The same with y in 8 bits: q [R,D] e4m3 values, and for every 32 of a row one
+ * power-of-two scale, scales [R, 4*ceil(D/128)] e8m0 bytes (127 + exponent; 255,
+ * NaN, where y is not finite; bytes past D/32 are 0).  The scale is the smallest
+ * that keeps the block's largest magnitude at or below 448, so nothing
+ * saturates.  D a multiple of 32; tensors 16-byte aligned. */
+int mhc_rms_norm_mx_forward(const void* x, const void* residual, int dtype,
+                            const float* weight, void* q, void* scales, void* h,
+                            int64_t R, int64_t D, float eps, mhc_stream_t stream);
+
+size_t mhc_rms_norm_backward_workspace_bytes(int64_t R, int64_t D);
+
+/* dx = rstd (g - n mean_d(g n)) + dh, g = weight dy, n = rstd h: the gradient of
+ * x and of the residual alike; dweight [D] f32 = sum_rows dy n.  dh (the gradient
+ * of h), dx or dweight may be NULL; without dweight no workspace is needed. */
+int mhc_rms_norm_backward(const void* dy, const void* h, const void* dh, int dtype,
+                          const float* weight, const float* rstd, void* dx,
+                          float* dweight, int64_t R, int64_t D,
+                          void* workspace, size_t workspace_bytes,
+                          mhc_stream_t stream);
+
+/* x [R,D] in 8 bits, as mhc_rms_norm_mx_forward writes y. */
+int mhc_quantize_mx(const void* x, int dtype, void* q, void* scales,
+                    int64_t R, int64_t D, mhc_stream_t stream);
+
+/* Dropout of n elements: y_i = [residual_i +] (u_i < kept ? x_i 65536 / kept : 0),
+ * kept = round((1 - p) 65536).  u_i is the 16-bit half i % 8 (low half of a word
+ * first) of Philox4x32-10's words for counter (i / 8, offset) and key seed, so the
+ * same call on a gradient, without the residual, is the backward.  `state`, when
+ * not NULL, holds {seed, offset} on the device in place of the arguments; `used`,
+ * when not NULL, gets what the call drew from. */
+int mhc_dropout(const void* x, const void* residual, int dtype, void* y, int64_t n,
+                double p, uint64_t seed, uint64_t offset, const int64_t* state,
+                int64_t* used, mhc_stream_t stream);
+
+/* Products grouped by expert.  Rows [offsets[e-1], offsets[e]) of the R rows belong
+ * to expert e (offsets[-1] = 0; offsets [E] i32 on the device, not decreasing; it
+ * is clamped to [0, R]).  Rows past offsets[E-1] belong to none: their outputs are
+ * zeros.  x [R,K], dy [R,N], weight [E,N,K], all in `dtype`; sums in f32.
+ * Widths up to 2^20, R < 2^31, E <= 4096.
+ *   forward          y[m,:]  = weight[e] x[m,:]
+ *   backward_input   dx[m,:] = weight[e]^T dy[m,:]
+ *   backward_weight  dw[e]   = sum_{m of e} dy[m,:] x[m,:]^T  (zeros for no rows) */
+int mhc_grouped_matmul_forward(const void* x, const void* weight, int dtype,
+                               const int32_t* offsets, void* y, int64_t R, int64_t K,
+                               int64_t N, int64_t E, mhc_stream_t stream);
+
+int mhc_grouped_matmul_backward_input(const void* dy, const void* weight, int dtype,
+                                      const int32_t* offsets, void* dx, int64_t R,
+                                      int64_t K, int64_t N, int64_t E,
+                                      mhc_stream_t stream);
+
+int mhc_grouped_matmul_backward_weight(const void* dy, const void* x, int dtype,
+                                       const int32_t* offsets, void* dw, int64_t R,
+                                       int64_t K, int64_t N, int64_t E,
+                                       mhc_stream_t stream);
+
+/* The forward product on 8-bit rows and weights with their scales, as
+ * mhc_quantize_mx and mhc_rms_norm_mx_forward write them (K a multiple of 32,
+ * values 16-byte and scales 4-byte aligned); y in dtype_y, bf16 or fp16.  The
+ * 8-bit matrix instruction drops what lies below 2^-13 of the largest of 16
+ * products before they join the fp32 sum, so no f32 result is offered. */
+int mhc_grouped_matmul_mx(const void* x, const void* x_scales, const void* weight,
+                          const void* weight_scales, const int32_t* offsets, void* y,
+                          int dtype_y, int64_t R, int64_t K, int64_t N, int64_t E,
+                          mhc_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,508 @@
+// RMS norm of a branch's input rows, with the residual's addition in front, backward, and with an
+// output in 8 bits; and the 8-bit quantiser alone.
+//
+//   h = x + residual   (rounded to the rows' type: the residual stream as it is stored)
+//   r = 1 / sqrt(mean_d h_d^2 + eps),   y_d = h_d r w_d
+//   dh_d = r (g_d - n_d mean_k(g_k n_k)) + (gradient of h),   g = w dy,  n = r h
+//   dw_d = sum_rows dy_d n_d
+//
+// All of it in fp32 from the stored values.  y is the norm of the *stored* h: the next layer reads
+// that h, and the backward has nothing else, so forward and backward see the same function.
+//
+// A team of TEAM lanes (a wave, or a workgroup) holds one row in registers, NV vectors per lane, so
+// each tensor passes the bus once; a workgroup walks over rows with the weight kept in registers.
+#include "stream_kernels.hpp"
+
+namespace mhc {
+
+int check_workspace(const char* who, const void* ws, size_t have, size_t need);
+
+// Sum over the wave, the same bits in every lane: DPP inside rows of 16, then two lane swaps.
+__device__ __forceinline__ float wave_total(float v) {
+  v = sum_all16(v);
+  const uint32_t b = __float_as_uint(v);
+  const auto p = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+  v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  const uint32_t c = __float_as_uint(v);
+  const auto q = __builtin_amdgcn_permlane32_swap(c, c, false, false);
+  return __uint_as_float(q[0]) + __uint_as_float(q[1]);
+}
+
+// Sum over a team.  `lds` holds 2 * (TEAM / 64) floats; `turn` alternates between its halves, so one
+// barrier per row is enough.
+template <int TEAM>
+__device__ __forceinline__ float team_sum(float v, float* lds, int turn) {
+  v = wave_total(v);
+  if constexpr (TEAM > 64) {
+    constexpr int NW = TEAM / 64;
+    float* p = lds + turn * NW;
+    if ((threadIdx.x & 63) == 0) p[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) v += p[i];
+  }
+  return v;
+}
+
+template <int TEAM>
+constexpr int kNormThreads = TEAM < 256 ? 256 : TEAM;
+
+// The vectors of a row that a lane holds: c = lane + v * TEAM, `ok` where c is inside the row.
+template <int W, bool RAG, int TEAM, int NV>
+struct RowPart {
+  uint32_t col[NV], skip[NV];
+  bool ok[NV];
+  __device__ __forceinline__ RowPart(uint32_t D) {
+    const uint32_t lane = threadIdx.x % TEAM, nch = (D + W - 1) / W;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const uint32_t c = lane + v * TEAM;
+      ok[v] = c < nch;
+      const RowCol<W, RAG> rc(ok[v] ? c : 0, D);
+      col[v] = rc.col;
+      skip[v] = rc.skip;
+    }
+  }
+};
+
+template <typename T, int W, bool RAG, int NV, bool NT, typename P>
+__device__ __forceinline__ void load_row(const T* row, int64_t D, const P& p, Frag<T, W> (&f)[NV]) {
+  const typename SpanOf<T, W, RAG>::type sp(row, D);
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+    if (p.ok[v]) f[v].template load<NT>(sp, p.col[v]);
+}
+
+template <int W, int NV, typename P>
+__device__ __forceinline__ void load_weight(const float* w, const P& p, float (&f)[NV][W]) {
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+#pragma unroll
+    for (int e = 0; e < W; ++e) f[v][e] = w && p.ok[v] ? w[p.col[v] + e] : (p.ok[v] ? 1.f : 0.f);
+}
+
+// 8-bit microscaled output: the smallest power of two that brings a block's largest magnitude to 448
+// (the largest e4m3 value) or below, so nothing saturates; bytes are 127 + exponent, 255 (NaN) for a
+// block that holds an infinity or a NaN.  From the bits: 448 = 1.75 * 2^8.
+__device__ __forceinline__ uint32_t mx_scale(float amax) {
+  const uint32_t b = __float_as_uint(amax);
+  if (b >= 0x7f800000u) return 255;
+  const int k = (int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return b == 0 || k < -127 ? 0 : (uint32_t)(k + 127);
+}
+
+// 2^-k of the scale byte 127 + k (exact; k = -127 gives 2^127).
+__device__ __forceinline__ float mx_inverse(uint32_t scale) { return __uint_as_float((254u - scale) << 23); }
+
+// W values over their block's scale in 8 bits, W / 4 dwords.  A block of scale NaN gets NaN throughout.
+template <int W>
+__device__ __forceinline__ void mx_pack(const float (&y)[W], uint32_t scale, uint32_t (&q)[W / 4]) {
+  const float inv = mx_inverse(scale);
+#pragma unroll
+  for (int i = 0; i < W / 4; ++i) {
+    int d = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i] * inv, y[4 * i + 1] * inv, 0, false);
+    d = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i + 2] * inv, y[4 * i + 3] * inv, d, true);
+    q[i] = scale == 255 ? 0x7f7f7f7fu : (uint32_t)d;
+  }
+}
+
+// Largest magnitude of a block of 32: 4 lanes of 8 values or 8 lanes of 4.  A NaN counts as the
+// largest (its bits, sign cleared, are above infinity's), so bits are compared.
+template <int W>
+__device__ __forceinline__ float block_amax(const float (&y)[W]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < W; ++e) m = max(m, __float_as_uint(y[e]) & 0x7fffffffu);
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, kDppQuadXor1, 0xF, 0xF, false));
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, kDppQuadXor2, 0xF, 0xF, false));
+  if constexpr (W == 4) m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xF, 0xF, false));  // row_half_mirror
+  return __uint_as_float(m);
+}
+
+constexpr int kMxBlock = 32;
+
+template <int W>
+__device__ __forceinline__ void mx_store(uint8_t* q, const uint32_t (&d)[W / 4]) {
+  if constexpr (W == 8) __builtin_nontemporal_store((uint64_t)d[1] << 32 | d[0], reinterpret_cast<uint64_t*>(q));
+  else __builtin_nontemporal_store(d[0], reinterpret_cast<uint32_t*>(q));
+}
+
+struct NormArgs {
+  const void *x, *res;
+  const float* w;
+  void *y, *h;        // y: rows in T, or 8-bit values
+  uint8_t* scales;    // 8-bit output only
+  float* rstd;        // may be null
+  int64_t R, D, ns;   // ns: scale bytes per row
+  float eps;
+};
+
+template <typename T, int W, bool RAG, int TEAM, int NV, bool RES, bool MX>
+__global__ __launch_bounds__(kNormThreads<TEAM>) void norm_fwd_kernel(NormArgs a) {
+  constexpr int NTH = kNormThreads<TEAM>, ROWS = NTH / TEAM;
+  __shared__ float lds[2 * (TEAM / 64)];
+  const int64_t D = a.D;
+  const RowPart<W, RAG, TEAM, NV> p((uint32_t)D);
+  float w[NV][W];
+  load_weight(a.w, p, w);
+  const float inv_d = 1.f / (float)D;
+  int turn = 0;
+  for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TEAM; row < a.R; row += (int64_t)gridDim.x * ROWS) {
+    Frag<T, W> xf[NV], rf[NV];
+    load_row<T, W, RAG, NV, true>((const T*)a.x + row * D, D, p, xf);
+    if constexpr (RES) load_row<T, W, RAG, NV, true>((const T*)a.res + row * D, D, p, rf);
+    float h[NV][W];
+    float ss = 0.f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      if (!p.ok[v]) {
+#pragma unroll
+        for (int e = 0; e < W; ++e) h[v][e] = 0.f;
+        continue;
+      }
+      xf[v].unpack(h[v]);
+      if constexpr (RES) {
+        float r[W];
+        rf[v].unpack(r);
+#pragma unroll
+        for (int e = 0; e < W; ++e) h[v][e] = to_f32(from_f32<T>(h[v][e] + r[e]));
+        const typename SpanOf<T, W, RAG>::type hs((T*)a.h + row * D, D);
+        st_from<T, W, true>(hs, p.col[v], h[v], p.skip[v]);
+      }
+#pragma unroll
+      for (int e = 0; e < W; ++e) ss += RAG && (uint32_t)e < p.skip[v] ? 0.f : h[v][e] * h[v][e];
+    }
+    ss = team_sum<TEAM>(ss, lds, turn);
+    turn ^= 1;
+    const float r = 1.f / sqrtf(ss * inv_d + a.eps);
+    if (a.rstd && threadIdx.x % TEAM == 0) a.rstd[row] = r;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      float y[W];
+#pragma unroll
+      for (int e = 0; e < W; ++e) y[e] = h[v][e] * r * w[v][e];
+      if constexpr (MX) {
+        const uint32_t s = mx_scale(block_amax(y));
+        uint32_t q[W / 4];
+        mx_pack(y, s, q);
+        if (p.ok[v]) {
+          mx_store<W>((uint8_t*)a.y + row * D + p.col[v], q);
+          if (p.col[v] % kMxBlock == 0) a.scales[row * a.ns + p.col[v] / kMxBlock] = (uint8_t)s;
+        }
+      } else if (p.ok[v]) {
+        const typename SpanOf<T, W, RAG>::type ys((T*)a.y + row * D, D);
+        st_from<T, W, true>(ys, p.col[v], y, p.skip[v]);
+      }
+    }
+    if constexpr (MX) {  // the scale row's filling
+      const int64_t pad = D / kMxBlock + threadIdx.x % TEAM;
+      if (pad < a.ns) a.scales[row * a.ns + pad] = 0;
+    }
+  }
+}
+
+struct NormBwdArgs {
+  const void *dy, *h, *dh;  // dh may be null
+  const float *w, *rstd;
+  void* dx;                 // may be null
+  float* part;              // [gridDim.x][D] partial weight gradients; null without one
+  int64_t R, D;
+};
+
+template <typename T, int W, bool RAG, int TEAM, int NV, bool DH>
+__global__ __launch_bounds__(kNormThreads<TEAM>) void norm_bwd_kernel(NormBwdArgs a) {
+  constexpr int NTH = kNormThreads<TEAM>, ROWS = NTH / TEAM;
+  __shared__ float lds[2 * (TEAM / 64)];
+  const int64_t D = a.D;
+  const RowPart<W, RAG, TEAM, NV> p((uint32_t)D);
+  float w[NV][W], dw[NV][W];
+  load_weight(a.w, p, w);
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+#pragma unroll
+    for (int e = 0; e < W; ++e) dw[v][e] = 0.f;
+  const float inv_d = 1.f / (float)D;
+  int turn = 0;
+  for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TEAM; row < a.R; row += (int64_t)gridDim.x * ROWS) {
+    Frag<T, W> yf[NV], hf[NV], gf[NV];
+    load_row<T, W, RAG, NV, true>((const T*)a.dy + row * D, D, p, yf);
+    load_row<T, W, RAG, NV, true>((const T*)a.h + row * D, D, p, hf);
+    if constexpr (DH) load_row<T, W, RAG, NV, true>((const T*)a.dh + row * D, D, p, gf);
+    const float r = a.rstd[row];
+    float g[NV][W], n[NV][W];
+    float c = 0.f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      if (!p.ok[v]) continue;
+      yf[v].unpack(g[v]);
+      hf[v].unpack(n[v]);
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        n[v][e] *= r;
+        dw[v][e] += g[v][e] * n[v][e];
+        g[v][e] *= w[v][e];
+        c += RAG && (uint32_t)e < p.skip[v] ? 0.f : g[v][e] * n[v][e];
+      }
+    }
+    c = team_sum<TEAM>(c, lds, turn) * inv_d;
+    turn ^= 1;
+    if (!a.dx) continue;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      if (!p.ok[v]) continue;
+      float d[W];
+#pragma unroll
+      for (int e = 0; e < W; ++e) d[e] = r * (g[v][e] - n[v][e] * c);
+      if constexpr (DH) {
+        float u[W];
+        gf[v].unpack(u);
+#pragma unroll
+        for (int e = 0; e < W; ++e) d[e] += u[e];
+      }
+      const typename SpanOf<T, W, RAG>::type ds((T*)a.dx + row * D, D);
+      st_from<T, W, true>(ds, p.col[v], d, p.skip[v]);
+    }
+  }
+  if (!a.part) return;
+  float* out = a.part + (int64_t)blockIdx.x * D;
+  if constexpr (TEAM < 256) {  // the workgroup's four rows' sums, in wave order
+    __shared__ float sum[ROWS][TEAM * NV * W];
+    const int team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int e = 0; e < W; ++e) sum[team][(v * W + e) * TEAM + lane] = dw[v][e];
+    __syncthreads();
+    if (team) return;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        const int i = (v * W + e) * TEAM + lane;
+        dw[v][e] = (sum[0][i] + sum[1][i]) + (sum[2][i] + sum[3][i]);
+      }
+  }
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    if (!p.ok[v]) continue;
+#pragma unroll
+    for (int e = 0; e < W; ++e)
+      if (!RAG || (uint32_t)e >= p.skip[v]) out[p.col[v] + e] = dw[v][e];
+  }
+}
+
+// dw[d] = sum over the partial records, 16 groups of them side by side, in fp64 (they are the sum's largest terms).
+constexpr int kDwCols = 64;
+
+__global__ __launch_bounds__(1024) void norm_dw_reduce_kernel(const float* __restrict__ part, float* __restrict__ dw,
+                                                              int n, int64_t D) {
+  __shared__ double sum[16][kDwCols];
+  const int col = threadIdx.x % kDwCols, grp = threadIdx.x / kDwCols;
+  const int64_t d = (int64_t)blockIdx.x * kDwCols + col;
+  double s = 0.;
+  if (d < D)
+    for (int i = grp; i < n; i += 16) s += part[i * D + d];
+  sum[grp][col] = s;
+  __syncthreads();
+  if (grp || d >= D) return;
+#pragma unroll
+  for (int i = 1; i < 16; ++i) s += sum[i][col];
+  dw[d] = (float)s;
+}
+
+// The quantiser alone: a lane per vector, rows of whole blocks.
+template <typename T, int W>
+__global__ __launch_bounds__(kThreads) void quantize_mx_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
+                                                               uint8_t* __restrict__ scales, int64_t R, int64_t D,
+                                                               int64_t ns) {
+  // A row has ns blocks; those past D are filled.  Lanes of one block are neighbours.
+  constexpr int LANES = kMxBlock / W;
+  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int64_t block = i / LANES, row = block / ns, b = block - row * ns;
+  const int64_t col = b * kMxBlock + (i % LANES) * W;
+  const bool in = row < R && col < D;
+  float v[W];
+#pragma unroll
+  for (int e = 0; e < W; ++e) v[e] = 0.f;
+  if (in) ld<T, W, true>(x + row * D + col, v);
+  const uint32_t s = mx_scale(block_amax(v));
+  uint32_t d[W / 4];
+  mx_pack(v, s, d);
+  if (in) mx_store<W>(q + row * D + col, d);
+  if (row < R && i % LANES == 0) scales[row * ns + b] = (uint8_t)s;
+}
+
+// Rows of up to this many elements fit the registers of the widest team.
+constexpr int64_t kNormMaxDim = 16384;
+
+// Workgroups of the backward, each with a partial weight gradient.
+constexpr int64_t kNormBwdBlocks = 512;
+
+template <int T, int N>
+struct Team {
+  static constexpr int TEAM = T, NV = N;
+};
+
+// The team and vectors per lane for rows of `nch` vectors.
+template <class F>
+static int with_team(int64_t nch, F&& fn) {
+  if (nch <= 64) return fn(Team<64, 1>{});
+  if (nch <= 128) return fn(Team<64, 2>{});
+  if (nch <= 256) return fn(Team<64, 4>{});
+  if (nch <= 512) return fn(Team<256, 2>{});
+  if (nch <= 1024) return fn(Team<256, 4>{});
+  return fn(Team<1024, 4>{});
+}
+
+// Whole vectors, ragged vectors, or (rows below one vector) single elements.
+template <int WV, class F>
+static int with_row_width(int64_t D, std::initializer_list<const void*> ptrs, F&& fn) {
+  bool vec = D % WV == 0;
+  for (const void* p : ptrs) vec = vec && (!p || aligned16(p));
+  if (vec) return fn(std::integral_constant<int, WV>{}, std::false_type{});
+  if (D >= WV) return fn(std::integral_constant<int, WV>{}, std::true_type{});
+  return fn(std::integral_constant<int, 1>{}, std::false_type{});
+}
+
+static int64_t norm_blocks(int64_t R, int rows, int64_t cap) {
+  const int64_t n = (R + rows - 1) / rows;
+  return n < cap ? n : cap;
+}
+
+static int check_rows(const char* who, int64_t R, int64_t D) {
+  if (R < 0 || D < 0) {
+    set_error("%s: negative size (R=%lld D=%lld)", who, (long long)R, (long long)D);
+    return MHC_ERR_ARG;
+  }
+  if (D > kNormMaxDim) {
+    set_error("%s: rows of %lld elements; at most %lld", who, (long long)D, (long long)kNormMaxDim);
+    return MHC_ERR_ARG;
+  }
+  return MHC_OK;
+}
+
+static int64_t mx_scale_row(int64_t D) { return (D + 127) / 128 * 4; }
+
+template <bool MX>
+static int norm_forward(const char* who, NormArgs a, int dtype, hipStream_t st) {
+  return MHC_DISPATCH_DTYPE(dtype, [&] {
+    auto go = [&](auto wc, auto rag) {
+      constexpr int W = decltype(wc)::value;
+      constexpr bool RAG = decltype(rag)::value;
+      return with_team((a.D + W - 1) / W, [&](auto team) -> int {
+        constexpr int TEAM = decltype(team)::TEAM, NV = decltype(team)::NV, NTH = kNormThreads<TEAM>;
+        const dim3 grid((unsigned)norm_blocks(a.R, NTH / TEAM, 8 * (int64_t)num_cus()));
+        if (a.res) norm_fwd_kernel<T, W, RAG, TEAM, NV, true, MX><<<grid, NTH, 0, st>>>(a);
+        else norm_fwd_kernel<T, W, RAG, TEAM, NV, false, MX><<<grid, NTH, 0, st>>>(a);
+        return hip_status(hipGetLastError(), who);
+      });
+    };
+    if constexpr (MX) return go(std::integral_constant<int, Vec<T>::N>{}, std::false_type{});
+    else return with_row_width<Vec<T>::N>(a.D, {a.x, a.res, a.y, a.h}, go);
+  });
+}
+
+static bool all_aligned16(std::initializer_list<const void*> ptrs) {
+  for (const void* p : ptrs)
+    if (!aligned16(p)) return false;
+  return true;
+}
+
+}  // namespace mhc
+
+using namespace mhc;
+
+extern "C" int mhc_rms_norm_forward(const void* x, const void* residual, int dtype, const float* weight, void* y,
+                                    void* h, float* rstd, int64_t R, int64_t D, float eps, mhc_stream_t stream) {
+  if (int rc = check_rows("rms_norm_forward", R, D)) return rc;
+  if (R * D == 0) return MHC_OK;
+  if (!x || !y || (residual && !h)) {
+    set_error("rms_norm_forward: null pointer");
+    return MHC_ERR_ARG;
+  }
+  return norm_forward<false>("rms_norm_forward launch",
+                             NormArgs{x, residual, weight, y, h, nullptr, rstd, R, D, 0, eps}, dtype,
+                             (hipStream_t)stream);
+}
+
+extern "C" int mhc_rms_norm_mx_forward(const void* x, const void* residual, int dtype, const float* weight, void* q,
+                                       void* scales, void* h, int64_t R, int64_t D, float eps, mhc_stream_t stream) {
+  if (int rc = check_rows("rms_norm_mx_forward", R, D)) return rc;
+  if (R * D == 0) return MHC_OK;
+  if (!x || !q || !scales || (residual && !h)) {
+    set_error("rms_norm_mx_forward: null pointer");
+    return MHC_ERR_ARG;
+  }
+  if (D % kMxBlock || !all_aligned16({x, residual, q, h})) {
+    set_error("rms_norm_mx_forward: rows of whole blocks of %d and 16-byte aligned tensors required", kMxBlock);
+    return MHC_ERR_ARG;
+  }
+  return norm_forward<true>("rms_norm_mx_forward launch",
+                            NormArgs{x, residual, weight, q, h, (uint8_t*)scales, nullptr, R, D, mx_scale_row(D), eps},
+                            dtype, (hipStream_t)stream);
+}
+
+extern "C" size_t mhc_rms_norm_backward_workspace_bytes(int64_t R, int64_t D) {
+  if (R <= 0 || D <= 0) return 0;
+  return (size_t)(norm_blocks(R, 1, kNormBwdBlocks) * D) * sizeof(float);
+}
+
+extern "C" int mhc_rms_norm_backward(const void* dy, const void* h, const void* dh, int dtype, const float* weight,
+                                     const float* rstd, void* dx, float* dweight, int64_t R, int64_t D,
+                                     void* workspace, size_t workspace_bytes, mhc_stream_t stream) {
+  if (int rc = check_rows("rms_norm_backward", R, D)) return rc;
+  hipStream_t st = (hipStream_t)stream;
+  if (R * D == 0) return dweight ? fill_zero(dweight, D, st) : (int)MHC_OK;  // an empty sum
+  if (!dy || !h || !rstd || (!dx && !dweight)) {
+    set_error("rms_norm_backward: null pointer");
+    return MHC_ERR_ARG;
+  }
+  if (dweight)
+    if (int rc = check_workspace("rms_norm_backward", workspace, workspace_bytes,
+                                 mhc_rms_norm_backward_workspace_bytes(R, D)))
+      return rc;
+  const NormBwdArgs a{dy, h, dh, weight, rstd, dx, dweight ? (float*)workspace : nullptr, R, D};
+  unsigned blocks = 0;
+  const int rc = MHC_DISPATCH_DTYPE(dtype, [&] {
+    return with_row_width<Vec<T>::N>(D, {dy, h, dh, dx}, [&](auto wc, auto rag) {
+      constexpr int W = decltype(wc)::value;
+      constexpr bool RAG = decltype(rag)::value;
+      return with_team((D + W - 1) / W, [&](auto team) -> int {
+        constexpr int TEAM = decltype(team)::TEAM, NV = decltype(team)::NV, NTH = kNormThreads<TEAM>;
+        blocks = (unsigned)norm_blocks(R, NTH / TEAM, kNormBwdBlocks);
+        if (dh) norm_bwd_kernel<T, W, RAG, TEAM, NV, true><<<blocks, NTH, 0, st>>>(a);
+        else norm_bwd_kernel<T, W, RAG, TEAM, NV, false><<<blocks, NTH, 0, st>>>(a);
+        return hip_status(hipGetLastError(), "rms_norm_backward launch");
+      });
+    });
+  });
+  if (rc || !dweight) return rc;
+  norm_dw_reduce_kernel<<<dim3((unsigned)((D + kDwCols - 1) / kDwCols)), 1024, 0, st>>>(a.part, dweight, (int)blocks, D);
+  return hip_status(hipGetLastError(), "rms_norm_backward reduce launch");
+}
+
+extern "C" int mhc_quantize_mx(const void* x, int dtype, void* q, void* scales, int64_t R, int64_t D,
+                               mhc_stream_t stream) {
+  if (R < 0 || D < 0 || D % kMxBlock) {
+    set_error("quantize_mx: bad size (R=%lld D=%lld; D in whole blocks of %d)", (long long)R, (long long)D, kMxBlock);
+    return MHC_ERR_ARG;
+  }
+  if (R * D == 0) return MHC_OK;
+  if (!x || !q || !scales || !all_aligned16({x, q})) {
+    set_error("quantize_mx: null pointer, or a tensor that is not 16-byte aligned");
+    return MHC_ERR_ARG;
+  }
+  const int64_t ns = mx_scale_row(D);
+  hipStream_t st = (hipStream_t)stream;
+  return MHC_DISPATCH_DTYPE(dtype, [&] {
+    constexpr int W = Vec<T>::N;
+    const int64_t n = (R * ns * (kMxBlock / W) + kThreads - 1) / kThreads;
+    if (n >= ((int64_t)1 << 32) / kThreads) {  // the runtime takes fewer than 2^32 work items
+      set_error("quantize_mx: %lld elements are too many for a call", (long long)(R * D));
+      return (int)MHC_ERR_ARG;
+    }
+    quantize_mx_kernel<T, W><<<dim3((unsigned)n), kThreads, 0, st>>>((const T*)x, (uint8_t*)q, (uint8_t*)scales, R, D, ns);
+    return hip_status(hipGetLastError(), "quantize_mx launch");
+  });
+}

@@ -8,6 +8,7 @@ PyTorch and run anywhere.
 """
 
 from . import streams  # stream expand / collapse (not in __all__, which is the reference's)
+from . import branch  # the operators inside a branch (likewise)
 from .module import HyperConnection
 from .ops import (
     sinkhorn_knopp,

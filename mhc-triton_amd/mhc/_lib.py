@@ -25,6 +25,8 @@ _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I = ctypes.c_int
 _F = ctypes.c_float
+_D = ctypes.c_double
+_U64 = ctypes.c_uint64
 _SZ = ctypes.c_size_t
 
 # name -> (restype, argtypes); mirrors include/mhc_abi.h
@@ -66,6 +68,16 @@ _SIGNATURES = {
              _I64, _I64, _I64, _I, _F, _P, _SZ, _P]),
     "mhc_layer_static_backward": (
         _I, [_P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I, _P, _SZ, _P]),
+    "mhc_rms_norm_forward": (_I, [_P, _P, _I, _P, _P, _P, _P, _I64, _I64, _F, _P]),
+    "mhc_rms_norm_mx_forward": (_I, [_P, _P, _I, _P, _P, _P, _P, _I64, _I64, _F, _P]),
+    "mhc_rms_norm_backward_workspace_bytes": (_SZ, [_I64, _I64]),
+    "mhc_rms_norm_backward": (_I, [_P, _P, _P, _I, _P, _P, _P, _P, _I64, _I64, _P, _SZ, _P]),
+    "mhc_quantize_mx": (_I, [_P, _I, _P, _P, _I64, _I64, _P]),
+    "mhc_dropout": (_I, [_P, _P, _I, _P, _I64, _D, _U64, _U64, _P, _P, _P]),
+    "mhc_grouped_matmul_forward": (_I, [_P, _P, _I, _P, _P, _I64, _I64, _I64, _I64, _P]),
+    "mhc_grouped_matmul_backward_input": (_I, [_P, _P, _I, _P, _P, _I64, _I64, _I64, _I64, _P]),
+    "mhc_grouped_matmul_backward_weight": (_I, [_P, _P, _I, _P, _P, _I64, _I64, _I64, _I64, _P]),
+    "mhc_grouped_matmul_mx": (_I, [_P, _P, _P, _P, _P, _P, _I, _I64, _I64, _I64, _I64, _P]),
 }
 
 ABI_VERSION = 3

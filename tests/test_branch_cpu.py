@@ -1,0 +1,173 @@
+"""``mhc.branch`` without a GPU: the oracle's pins, refusals, the C ABI's host-side checks, and the
+torch.library fakes."""
+
+import numpy as np
+import pytest
+import torch
+
+from mhc import _branch, branch
+from oracle import branch_oracle as O
+
+BF, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.mark.parametrize("ctr,key,out", [
+    # known answers published with the generator
+    ((0, 0, 0, 0), (0, 0), (0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8)),
+    ((0xFFFFFFFF,) * 4, (0xFFFFFFFF,) * 2, (0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD)),
+    ((0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344), (0xA4093822, 0x299F31D0),
+     (0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1)),
+])
+def test_oracle_philox_known_answers(ctr, key, out):
+    got = O.philox([ctr[0]], [ctr[1]], ctr[2] | ctr[3] << 32, key[0] | key[1] << 32)
+    assert tuple(int(w[0]) for w in got) == out
+
+
+def test_oracle_e4m3_and_scales():
+    v = torch.tensor([0.0, 448.0, 440.0, 1.0, 1.0625, 2.0 ** -9, 2.0 ** -10, 1.5 * 2.0 ** -9, 0.3, -27.0, 2.0 ** -6])
+    assert np.array_equal(O.e4m3_round(v.numpy()), v.to(torch.float8_e4m3fn).double().numpy())
+    assert O.mx_exponent([448.0, 448.0001, 224.0, 0.0, 1e-45, 1.0, 1.75, 1.7500001]).tolist() == [
+        0, 1, -1, -127, -127, -8, -8, -7]
+    for k, top in enumerate((448.0, 3.0, 1e30, 2.0 ** -100)):
+        e = float(O.mx_exponent(top))
+        assert top / 2 ** e <= 448 < top / 2 ** (e - 1), k
+
+
+def test_oracle_gradients_against_differences():
+    r = np.random.default_rng(0)
+    h, dy, dh, w = r.standard_normal((3, 5)), r.standard_normal((3, 5)), r.standard_normal((3, 5)), r.standard_normal(5)
+    dx, dw, _, _ = O.rms_norm_backward(dy, h, dh, w)
+    loss = lambda h, w: (O.rms_norm(h, w)[0] * dy).sum() + (h * dh).sum()  # noqa: E731
+    v, u, t = r.standard_normal(h.shape), r.standard_normal(5), 1e-6
+    assert abs((loss(h + t * v, w) - loss(h - t * v, w)) / (2 * t) - (dx * v).sum()) < 1e-8
+    assert abs((loss(h, w + t * u) - loss(h, w - t * u)) / (2 * t) - (dw * u).sum()) < 1e-8
+    x, wt, g = r.standard_normal((7, 4)), r.standard_normal((3, 6, 4)), r.standard_normal((7, 6))
+    off = [2, 2, 6]
+    dx, dw, _, _ = O.grouped_matmul_backward(g, x, wt, off)
+    vx, vw = r.standard_normal(x.shape), r.standard_normal(wt.shape)
+    f = lambda x, w: (O.grouped_matmul(x, w, off)[0] * g).sum()  # noqa: E731
+    assert abs((f(x + vx, wt) - f(x - vx, wt)) / 2 - (dx * vx).sum()) < 1e-10
+    assert abs((f(x, wt + vw) - f(x, wt - vw)) / 2 - (dw * vw).sum()) < 1e-10
+    assert not dw[1].any() and not dx[6].any()
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.randn(4, 32)
+    off = torch.tensor([2, 4], dtype=torch.int32)
+    for call in (lambda: branch.rms_norm(x), lambda: branch.rms_norm_mx(x), lambda: branch.quantize_mx(x),
+                 lambda: branch.dropout(x, 0.1, (1, 2)), lambda: branch.grouped_matmul(x, torch.randn(2, 8, 32), off)):
+        with pytest.raises(RuntimeError, match="ROCm GPU"):
+            call()
+
+
+def _refusals():
+    x = torch.zeros(4, 64)
+    off = torch.zeros(2, dtype=torch.int32)
+    w = torch.zeros(2, 8, 64)
+    q, s = torch.zeros(4, 64).to(_branch.F8), torch.zeros(4, 4, dtype=torch.uint8).view(_branch.E8)
+    wq, ws = torch.zeros(2, 8, 64).to(_branch.F8), torch.zeros(2, 8, 4, dtype=torch.uint8).view(_branch.E8)
+    mx = lambda **k: branch.grouped_matmul_mx(*{**dict(q=q, s=s, wq=wq, ws=ws, off=off), **k}.values())  # noqa: E731
+    return [
+        ("weight width", AssertionError, lambda: branch.rms_norm(x, torch.ones(63))),
+        ("scalar", AssertionError, lambda: branch.rms_norm(torch.zeros(()))),
+        ("row too wide", ValueError, lambda: branch.rms_norm(torch.zeros(1, 16385))),
+        ("residual shape", AssertionError, lambda: branch.rms_norm(x, residual=torch.zeros(64))),
+        ("residual dtype", TypeError, lambda: branch.rms_norm(x, residual=x.to(BF))),
+        ("not whole blocks", ValueError, lambda: _branch._mx_outputs(torch.zeros(4, 48))),
+        ("p", ValueError, lambda: branch.dropout(x, 1.5, (0, 0))),
+        ("p nan", ValueError, lambda: branch.dropout(x, float("nan"), (0, 0))),
+        ("seed range", ValueError, lambda: branch.dropout(x, 0.5, (-1, 0))),
+        ("seed type", TypeError, lambda: branch.dropout(x, 0.5, 7)),
+        ("rng shape", AssertionError, lambda: branch.dropout(x, 0.5, torch.zeros(3, dtype=torch.int64))),
+        ("dropout residual", AssertionError, lambda: branch.dropout(x, 0.5, (0, 0), residual=x[:2])),
+        ("weight dims", AssertionError, lambda: branch.grouped_matmul(x, w[0], off)),
+        ("in width", AssertionError, lambda: branch.grouped_matmul(x[:, :32], w, off)),
+        ("rows dims", AssertionError, lambda: branch.grouped_matmul(x[None], w, off)),
+        ("offsets count", AssertionError, lambda: _branch._offsets(off, 3)),
+        ("offsets dtype", TypeError, lambda: _branch._offsets(off.float(), 2)),
+        ("8-bit types", TypeError, lambda: mx(q=x)),
+        ("grad needed", RuntimeError, lambda: branch.quantize_mx(x.clone().requires_grad_())),
+        ("grad needed", RuntimeError, lambda: branch.rms_norm_mx(x, torch.ones(64, requires_grad=True))),
+    ]
+
+
+@pytest.mark.parametrize("i", range(20))
+def test_refusals(i):
+    cases = _refusals()
+    assert len(cases) == 20
+    name, error, call = cases[i]
+    with pytest.raises(error):
+        call()
+
+
+def test_abi_refusals_before_any_device_work():
+    from mhc import _lib
+
+    lib = _lib.load()
+    assert lib.mhc_rms_norm_forward(None, None, 1, None, None, None, None, 4, 64, 1e-6, None) == 1
+    assert lib.mhc_rms_norm_forward(None, None, 1, None, None, None, None, 0, 64, 1e-6, None) == 0
+    assert lib.mhc_rms_norm_forward(16, 16, 1, None, 16, None, None, 4, 64, 1e-6, None) == 1  # residual without h
+    assert lib.mhc_rms_norm_forward(16, None, 1, None, 16, None, None, 4, 16385, 1e-6, None) == 1
+    assert b"16384" in lib.mhc_last_error()
+    assert lib.mhc_rms_norm_forward(16, None, 9, None, 16, None, None, 4, 64, 1e-6, None) == 2
+    assert lib.mhc_rms_norm_mx_forward(16, None, 1, None, 16, 16, None, 4, 48, 1e-6, None) == 1
+    assert lib.mhc_rms_norm_mx_forward(24, None, 1, None, 16, 16, None, 4, 64, 1e-6, None) == 1  # alignment
+    assert lib.mhc_rms_norm_backward(16, 16, None, 1, None, 16, 16, 16, 4, 64, None, 0, None) == 3
+    need = lib.mhc_rms_norm_backward_workspace_bytes(4, 64)
+    assert need == 4 * 64 * 4 and lib.mhc_rms_norm_backward_workspace_bytes(0, 64) == 0
+    assert lib.mhc_rms_norm_backward(16, 16, None, 1, None, 16, 16, 16, 4, 64, 256, need - 1, None) == 3
+    assert lib.mhc_quantize_mx(16, 1, 16, 16, 4, 33, None) == 1
+    assert lib.mhc_dropout(None, None, 1, None, -1, 0.1, 0, 0, None, None, None) == 1
+    assert lib.mhc_dropout(None, None, 1, None, 8, 0.1, 0, 0, None, None, None) == 1
+    assert lib.mhc_dropout(16, None, 1, 16, 8, 1.1, 0, 0, None, None, None) == 1
+    assert lib.mhc_dropout(None, None, 1, None, 0, 0.1, 0, 0, None, None, None) == 0
+    for name in ("forward", "backward_input", "backward_weight"):
+        fn = getattr(lib, f"mhc_grouped_matmul_{name}")
+        assert fn(None, None, 1, None, None, 4, 8, 8, 2, None) == 1
+        assert fn(16, 16, 1, 16, 16, 4, -8, 8, 2, None) == 1
+        assert fn(16, 16, 1, 16, 16, 1 << 31, 8, 8, 2, None) == 1
+        assert fn(16, 16, 1, 16, 16, 4, 8, 8, 4097, None) == 1
+        assert fn(None, None, 1, None, None, 0, 0, 8, 2, None) == 0
+        assert fn(16, 16, 5, 16, 16, 4, 8, 8, 2, None) == 2
+    assert lib.mhc_grouped_matmul_mx(16, 16, 16, 16, 16, 16, 1, 4, 48, 8, 2, None) == 1
+    assert lib.mhc_grouped_matmul_mx(24, 16, 16, 16, 16, 16, 1, 4, 64, 8, 2, None) == 1
+    assert b"aligned" in lib.mhc_last_error()
+    assert lib.mhc_grouped_matmul_mx(16, 16, 16, 16, 16, 16, 0, 4, 64, 8, 2, None) == 2  # no fp32 results
+
+
+OPS = {"norm", "add_norm", "norm_backward", "norm_mx", "quantize_mx", "grouped_matmul",
+       "grouped_matmul_backward_input", "grouped_matmul_backward_weight", "grouped_matmul_mx", "dropout"}
+
+
+def test_every_launcher_is_registered():
+    assert {n for n in dir(torch.ops.mhc_branch) if not n.startswith("_") and n != "name"} == OPS
+    for n in OPS:
+        assert torch._C._dispatch_has_kernel_for_dispatch_key(f"mhc_branch::{n}", "CUDA"), n
+        assert not torch._C._dispatch_has_kernel_for_dispatch_key(f"mhc_branch::{n}", "CPU"), n
+
+
+def test_fakes_and_traced_gradients():
+    """Meta tensors through the traced functions: every gradient has its input's shape and dtype."""
+    from mhc import _branch_library as L
+
+    e = lambda *s, dt=BF: torch.empty(*s, device="meta", dtype=dt).requires_grad_(dt in (BF, F32))  # noqa: E731
+    x, res, w = e(6, 64), e(6, 64), e(64, dt=F32)
+    y, h = L.rms_norm(x, w, res, 1e-6)
+    assert y.shape == h.shape == x.shape and y.dtype == h.dtype == BF
+    g = torch.autograd.grad((y.sum() + h.sum()), (x, w, res))
+    assert [(t.shape, t.dtype) for t in g] == [(t.shape, t.dtype) for t in (x, w, res)]
+    y = L.rms_norm(x, None, None, 1e-6)
+    assert torch.autograd.grad(y.sum(), x)[0].shape == x.shape
+    q, s, h = L.rms_norm_mx(x.detach(), w.detach(), res.detach(), 1e-6)
+    assert (q.dtype, s.dtype, s.shape, h.dtype) == (_branch.F8, _branch.E8, (6, 4), BF)
+    assert L.quantize_mx(e(3, 5, 160).detach())[1].shape == (3, 5, 8)
+    wt, off = e(3, 16, 64), e(3, dt=torch.int32)
+    y = L.grouped_matmul(x, wt, off)
+    assert y.shape == (6, 16) and y.dtype == BF
+    g = torch.autograd.grad(y.sum(), (x, wt))
+    assert [(t.shape, t.dtype) for t in g] == [(t.shape, t.dtype) for t in (x, wt)]
+    wq, ws = L.quantize_mx(wt.detach())
+    assert L.grouped_matmul_mx(q, s, wq, ws, off, torch.float16).dtype == torch.float16
+    y = L.dropout(x, 0.1, e(2, dt=torch.int64), res)
+    g = torch.autograd.grad(y.sum(), (x, res))
+    assert [(t.shape, t.dtype) for t in g] == [(t.shape, t.dtype) for t in (x, res)]
