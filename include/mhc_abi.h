@@ -394,7 +394,7 @@ int mhc_dropout(const void* x, const void* residual, int dtype, void* y, int64_t
  * to expert e (offsets[-1] = 0; offsets [E] i32 on the device, not decreasing; it
  * is clamped to [0, R]).  Rows past offsets[E-1] belong to none: their outputs are
  * zeros.  x [R,K], dy [R,N], weight [E,N,K], all in `dtype`; sums in f32.
- * Widths up to 2^20, R < 2^31, E <= 4096.
+ * Widths up to 2^20, R <= 2^31 - 4096, E <= 4096.
  *   forward          y[m,:]  = weight[e] x[m,:]
  *   backward_input   dx[m,:] = weight[e]^T dy[m,:]
  *   backward_weight  dw[e]   = sum_{m of e} dy[m,:] x[m,:]^T  (zeros for no rows) */

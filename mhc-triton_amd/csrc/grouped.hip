@@ -11,27 +11,78 @@
 
 namespace mhc {
 
-template <typename T, typename TO, bool A_KR, bool B_KR, Role ROLE>
-static int launch_grouped(GroupedArgs a, const char* who, hipStream_t st) {
-  constexpr int BM = 128, BN = 128;
-  a.vec = a.lda % kElems<T> == 0 && a.ldb % kElems<T> == 0 && aligned16(a.A) && aligned16(a.B);
+// Row tiles (kRows) or output tiles (kWeight) of a launch, at most.
+template <Role ROLE, int BM, int BN>
+static int64_t set_tiles(GroupedArgs& a) {
   a.tiles_j = (int)((a.J + BN - 1) / BN);
-  int64_t tiles;
   if (ROLE == Role::kWeight) {
     a.tiles_i = (int)((a.I + BM - 1) / BM);
-    tiles = (int64_t)a.E * a.tiles_i * a.tiles_j;
-  } else {
-    const int64_t most = a.R / BM + a.E + 1;
-    a.tiles_i = (int)(a.R < most ? a.R : most);
-    tiles = (int64_t)a.tiles_i * a.tiles_j;
+    return (int64_t)a.E * (((int64_t)a.tiles_i * a.tiles_j + 7) / 8 * 8);  // an eighth of each expert's for each XCD
   }
-  if (tiles >= ((int64_t)1 << 32) / 256) {
-    set_error("%s: %lld tiles are too many for a call", who, (long long)tiles);
-    return MHC_ERR_ARG;
-  }
-  if (a.vec) grouped_kernel<T, TO, A_KR, B_KR, BM, BN, ROLE, true><<<dim3((unsigned)tiles), 256, 0, st>>>(a);
-  else grouped_kernel<T, TO, A_KR, B_KR, BM, BN, ROLE, false><<<dim3((unsigned)tiles), 256, 0, st>>>(a);
+  const int64_t most = a.R / BM + a.E + 1;
+  a.tiles_i = (int)(a.R < most ? a.R : most);
+  return (int64_t)a.tiles_i * a.tiles_j;
+}
+
+static int check_tiles(const char* who, int64_t tiles, int threads) {
+  if (tiles < ((int64_t)1 << 32) / threads - 8) return MHC_OK;
+  set_error("%s: %lld tiles are too many for a call", who, (long long)tiles);
+  return MHC_ERR_ARG;
+}
+
+template <typename T, typename TO, bool A_KR, bool B_KR, int BM, int BN, int WI, int WJ, int ST, Role ROLE>
+static int launch_direct(GroupedArgs a, const char* who, hipStream_t st) {
+  constexpr int NTH = 64 * WI * WJ;
+  const int64_t tiles = set_tiles<ROLE, BM, BN>(a);
+  if (int rc = check_tiles(who, tiles, NTH)) return rc;
+  // whole runs of eight: one for each XCD
+  grouped_direct_kernel<T, TO, A_KR, B_KR, BM, BN, WI, WJ, ST, ROLE>
+      <<<dim3((unsigned)((tiles + 7) / 8 * 8)), NTH, 0, st>>>(a);
   return hip_status(hipGetLastError(), who);
+}
+
+template <typename T, typename TO, int FI, int NJ, int WAVES, int U>
+static int launch_few(GroupedArgs a, const char* who, hipStream_t st) {
+  const int64_t tiles = set_tiles<Role::kRows, 16 * FI, 16 * NJ>(a);
+  if (int rc = check_tiles(who, tiles, 64 * WAVES)) return rc;
+  grouped_few_kernel<T, TO, FI, NJ, WAVES, U><<<dim3((unsigned)tiles), 64 * WAVES, 0, st>>>(a);
+  return hip_status(hipGetLastError(), who);
+}
+
+template <typename T, bool A_KR, bool B_KR, int BM, int BN, Role ROLE>
+static int launch_general(GroupedArgs a, const char* who, hipStream_t st) {
+  const int64_t tiles = set_tiles<ROLE, BM, BN>(a);
+  if (int rc = check_tiles(who, tiles, 256)) return rc;
+  grouped_kernel<T, A_KR, B_KR, BM, BN, ROLE><<<dim3((unsigned)tiles), 256, 0, st>>>(a);
+  return hip_status(hipGetLastError(), who);
+}
+
+// Tiles that hold rows, as far as the host can tell: an expert's last row tile is half full.
+template <Role ROLE, int BM, int BN>
+static int64_t likely_tiles(const GroupedArgs& a) {
+  const int64_t j = (a.J + BN - 1) / BN;
+  if (ROLE == Role::kWeight) return a.E * ((a.I + BM - 1) / BM) * j;
+  return ((a.R + BM - 1) / BM + (a.E < a.R ? a.E : a.R) / 2) * j;
+}
+
+template <typename T, typename TO, bool A_KR, bool B_KR, Role ROLE>
+static int launch_grouped(GroupedArgs a, const char* who, hipStream_t st) {
+  const bool vec = a.lda % kElems<T> == 0 && a.ldb % kElems<T> == 0 && aligned16(a.A) && aligned16(a.B);
+  const int cus = num_cus();
+  if (vec) {
+    if constexpr (!A_KR && !B_KR)
+      if (a.R <= 16 * (int64_t)a.E) return launch_few<T, TO, 1, 2, 4, 2>(a, who, st);
+    if (likely_tiles<ROLE, 256, 256>(a) >= cus / 2) return launch_direct<T, TO, A_KR, B_KR, 256, 256, 2, 4, 2, ROLE>(a, who, st);
+    if (likely_tiles<ROLE, 128, 128>(a) >= cus) return launch_direct<T, TO, A_KR, B_KR, 128, 128, 2, 2, 2, ROLE>(a, who, st);
+    if (__is_same(T, Mx) || likely_tiles<ROLE, 64, 64>(a) >= cus)
+      return launch_direct<T, TO, A_KR, B_KR, 64, 64, 2, 2, 4, ROLE>(a, who, st);
+    if constexpr (!__is_same(T, Mx)) return launch_direct<T, TO, A_KR, B_KR, 32, 32, 2, 2, 4, ROLE>(a, who, st);
+  }
+  if constexpr (!__is_same(T, Mx)) {
+    if (likely_tiles<ROLE, 128, 128>(a) >= 2 * cus) return launch_general<T, A_KR, B_KR, 128, 128, ROLE>(a, who, st);
+    return launch_general<T, A_KR, B_KR, 64, 64, ROLE>(a, who, st);
+  }
+  return MHC_OK;
 }
 
 static int check_grouped(const char* who, int64_t R, int64_t K, int64_t N, int64_t E) {
@@ -40,10 +91,11 @@ static int check_grouped(const char* who, int64_t R, int64_t K, int64_t N, int64
               (long long)E);
     return MHC_ERR_ARG;
   }
-  // A row's byte offsets inside a tile are 32-bit, as are tile counts; offsets are int32.
-  if (R >= ((int64_t)1 << 31) || K > kMaxWidth || N > kMaxWidth || E > kMaxExperts) {
-    set_error("%s: R=%lld K=%lld N=%lld E=%lld exceeds 2^31-1 rows, widths of %lld or %lld experts", who, (long long)R,
-              (long long)K, (long long)N, (long long)E, (long long)kMaxWidth, (long long)kMaxExperts);
+  // A row's byte offsets inside a tile are 32-bit, as are tile counts; offsets are int32, and the weight
+  // gradient counts up to two slabs past the last row.
+  if (R > kMaxRows || K > kMaxWidth || N > kMaxWidth || E > kMaxExperts) {
+    set_error("%s: R=%lld K=%lld N=%lld E=%lld exceeds %lld rows, widths of %lld or %lld experts", who, (long long)R,
+              (long long)K, (long long)N, (long long)E, (long long)kMaxRows, (long long)kMaxWidth, (long long)kMaxExperts);
     return MHC_ERR_ARG;
   }
   return MHC_OK;

@@ -19,6 +19,7 @@ struct Mx { uint8_t v; };  // e4m3 values with a power-of-two scale for every 32
 template <typename T> constexpr int kElems = 16 / (int)sizeof(T);  // values per 16-byte chunk
 template <typename T> constexpr int kSlab = 128 / (int)sizeof(T);  // values of k per slab
 
+constexpr int64_t kMaxRows = ((int64_t)1 << 31) - 4096;
 constexpr int64_t kMaxWidth = (int64_t)1 << 20;
 constexpr int64_t kMaxExperts = 4096;
 
@@ -83,37 +84,39 @@ __device__ __forceinline__ RowTile find_tile(const int32_t* offsets, int E, int6
   return {-1, 0, 0};
 }
 
-// A 16-byte chunk at p of which `n` values (the rest zero) may be read.
-template <typename T, bool VEC>
+// A 16-byte chunk at p, of any alignment, of which `n` values (the rest zero) may be read.
+template <typename T>
 __device__ __forceinline__ u32x4 load_chunk(const T* p, int64_t n) {
   u32x4 v = {0, 0, 0, 0};
   if (n >= kElems<T>) {
-    if constexpr (VEC) v = *reinterpret_cast<const u32x4*>(p);
-    else v = load16_any(p, false);
+    v = load16_any(p, false);
   } else if (n > 0) {
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (i < n) v[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[i] << (16 * (i % 2));
-    } else if constexpr (sizeof(T) == 4) {
+    } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (i < n) v[i] = reinterpret_cast<const uint32_t*>(p)[i];
     }
-    // 8-bit rows are whole chunks
   }
   return v;
 }
 
-// Slot of 16-byte chunk c of k-row r (KR).
-template <typename T>
+// Slot of 16-byte chunk c of k-row r (KR, PER chunks a row; its own inverse).  16 bits: the eight rows
+// that half a wave reads 32 bytes each from (four by the lanes, two by the groups) fall on different banks;
+// 32 bits: the four rows of 64 bytes.
+template <typename T, int PER>
 __device__ __forceinline__ int kr_slot(int r, int c) {
-  if constexpr (sizeof(T) == 2) return c ^ (2 * ((r & 3) | ((r >> 1) & 4)));
-  else return c ^ (4 * ((r >> 2) & 3));
+  if constexpr (sizeof(T) == 4) return c ^ (4 * ((r >> 2) & (PER >= 16 ? 3 : 1)));
+  else if constexpr (PER >= 16) return c ^ (2 * ((r & 3) | ((r >> 1) & 4)));
+  else if constexpr (PER == 8) return c ^ (2 * (((r >> 1) & 1) | ((r >> 2) & 2)));  // two rows share the banks' width
+  else return c ^ (2 * ((r >> 3) & 1));  // four do
 }
 
 // Global -> registers -> LDS for one slab of one operand (NTH threads).
-template <typename T, bool KR, int BM, int NTH, bool VEC>
+template <typename T, bool KR, int BM, int NTH>
 struct Stage {
   static constexpr int CH = BM * 8 / NTH;          // chunks per thread
   static constexpr int PER = BM / kElems<T>;       // KR: chunks per k-row
@@ -126,10 +129,10 @@ struct Stage {
       const int i = q * NTH + threadIdx.x;
       if constexpr (KR) {
         const int row = i / PER, c = (i % PER) * kElems<T>;
-        r[q] = load_chunk<T, VEC>(base + (k0 + row) * ld + c, k0 + row < klim ? rows - c : 0);
+        r[q] = load_chunk<T>(base + (k0 + row) * ld + c, k0 + row < klim ? rows - c : 0);
       } else {
         const int row = i / 8, c = (i % 8) * kElems<T>;
-        r[q] = load_chunk<T, VEC>(base + row * ld + k0 + c, row < rows ? klim - k0 - c : 0);
+        r[q] = load_chunk<T>(base + row * ld + k0 + c, row < rows ? klim - k0 - c : 0);
       }
     }
   }
@@ -139,7 +142,7 @@ struct Stage {
       const int i = q * NTH + threadIdx.x;
       if constexpr (KR) {
         const int row = i / PER;
-        lds[row * PER + kr_slot<T>(row, i % PER)] = r[q];
+        lds[row * PER + kr_slot<T, PER>(row, i % PER)] = r[q];
       } else {
         const int row = i / 8;
         lds[row * 8 + ((i % 8) ^ (row & 7))] = r[q];
@@ -167,8 +170,8 @@ __device__ __forceinline__ u32x4 load_frag(const u32x4* lds, int row, int h) {
     const int c = (row >> 3) + ((i & 3) >> 1);  // chunk of the lane's four columns
     const char* p = reinterpret_cast<const char*>(lds);
     const int r0 = 32 * h + 8 * g + (i >> 2), r1 = r0 + 4;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + (r0 * PER + kr_slot<T>(r0, c)) * 16 + (i & 1) * 8));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + (r1 * PER + kr_slot<T>(r1, c)) * 16 + (i & 1) * 8));
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + (r0 * PER + kr_slot<T, PER>(r0, c)) * 16 + (i & 1) * 8));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + (r1 * PER + kr_slot<T, PER>(r1, c)) * 16 + (i & 1) * 8));
     return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   } else {
     constexpr int PER = BM / 4;
@@ -177,7 +180,7 @@ __device__ __forceinline__ u32x4 load_frag(const u32x4* lds, int row, int h) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int r = 16 * h + 4 * g + j, c = row + i;
-      v[j] = p[(r * PER + kr_slot<T>(r, c >> 2)) * 4 + (c & 3)];
+      v[j] = p[(r * PER + kr_slot<T, PER>(r, c >> 2)) * 4 + (c & 3)];
     }
     return v;
   }
@@ -226,15 +229,15 @@ __device__ __forceinline__ void store4(TO* p, f32x4 v, int64_t n, bool vec) {
   }
 }
 
-// The general kernel: any size and alignment, operands staged through registers.  256 threads, four
-// waves of a quarter of the tile each.
-template <typename T, typename TO, bool A_KR, bool B_KR, int BM, int BN, Role ROLE, bool VEC>
+// The general kernel: any size and alignment, operands staged through registers (unaligned 16-byte loads,
+// single values at a row's end).  256 threads, four waves of a quarter of the tile each; the next slab's
+// loads are in flight while one is multiplied, and two slabs of LDS make one barrier a slab enough.
+template <typename T, bool A_KR, bool B_KR, int BM, int BN, Role ROLE>
 __global__ __launch_bounds__(256) void grouped_kernel(GroupedArgs a) {
   constexpr int NTH = 256, FI = BM / 32, FJ = BN / 32;
-  __shared__ u32x4 lds[(BM + BN) * 8];
-  u32x4 *la = lds, *lb = lds + BM * 8;
+  __shared__ u32x4 lds[2 * (BM + BN) * 8];
   const T *A = (const T*)a.A, *B = (const T*)a.B;
-  TO* out = (TO*)a.out;
+  T* out = (T*)a.out;
   int64_t rows, k0 = 0, klim, i0 = 0;  // the tile's rows, the range of k, the first row
   int64_t j0;
   int e;
@@ -252,6 +255,7 @@ __global__ __launch_bounds__(256) void grouped_kernel(GroupedArgs a) {
   } else {
     const int per = a.tiles_i * a.tiles_j;
     e = blockIdx.x / per;
+    if (e >= a.E) return;
     const int t = blockIdx.x % per;
     i0 = (int64_t)(t / a.tiles_j) * BM;
     j0 = (int64_t)(t % a.tiles_j) * BN;
@@ -271,38 +275,248 @@ __global__ __launch_bounds__(256) void grouped_kernel(GroupedArgs a) {
   for (int i = 0; i < FI; ++i)
 #pragma unroll
     for (int j = 0; j < FJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  Stage<T, A_KR, BM, NTH, VEC> sa;
-  Stage<T, B_KR, BN, NTH, VEC> sb;
-  for (; k0 < klim; k0 += kSlab<T>) {
+  Stage<T, A_KR, BM, NTH> sa;
+  Stage<T, B_KR, BN, NTH> sb;
+  if (k0 < klim) {
     sa.load(A, a.lda, rows, k0, klim);
     sb.load(B, a.ldb, cols, k0, klim);
-    __syncthreads();
+  }
+  for (int s = 0; k0 < klim; k0 += kSlab<T>, s ^= 1) {
+    u32x4 *la = lds + s * (BM + BN) * 8, *lb = la + BM * 8;
     sa.store(la);
     sb.store(lb);
     __syncthreads();
-    if constexpr (__is_same(T, Mx)) {
-      uint32_t s_a[FI], s_b[FJ];
-      const bool block = k0 + 32 * (lane >> 4) < klim;  // a scale row's filling is not read
+    if (k0 + kSlab<T> < klim) {
+      sa.load(A, a.lda, rows, k0 + kSlab<T>, klim);
+      sb.load(B, a.ldb, cols, k0 + kSlab<T>, klim);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      u32x4 fb[FJ];
+#pragma unroll
+      for (int j = 0; j < FJ; ++j) fb[j] = load_frag<T, B_KR, BN>(lb, wj + 16 * j, h);
 #pragma unroll
       for (int i = 0; i < FI; ++i) {
-        const int r = wi + 16 * i + (lane & 15);
-        s_a[i] = block && r < rows ? a.sa[(i0 + r) * a.ns + k0 / 32 + (lane >> 4)] : 0;
+        const u32x4 fa = load_frag<T, A_KR, BM>(la, wi + 16 * i, h);
+#pragma unroll
+        for (int j = 0; j < FJ; ++j) acc[i][j] = mma<T>(fb[j], fa, acc[i][j]);
       }
+    }
+  }
+  const bool vec = a.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(T) - 1)) == 0;
+#pragma unroll
+  for (int i = 0; i < FI; ++i) {
+    const int r = wi + 16 * i + (lane & 15);
+    if (r >= rows) continue;
+#pragma unroll
+    for (int j = 0; j < FJ; ++j) {
+      const int c = wj + 16 * j + 4 * (lane >> 4);
+      store4(out + (i0 + r) * a.ldo + j0 + c, acc[i][j], cols - c, vec);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The direct kernel: operands of whole 16-byte chunks go from global memory into LDS without passing
+// registers (buffer loads to LDS; a lane's 16 bytes land at the wave's base + 16 * lane, so the swizzle
+// is in the addresses that the lanes read from).  ST slabs are in flight; one barrier a slab: behind it,
+// the slab waited for is complete and the one multiplied before is free.
+//
+// Ranges are checked by the buffer: rows past the tile's and, for a k-row operand, k past the group's end
+// read as zeros; chunks past a row's end get an offset past any buffer.
+// ---------------------------------------------------------------------------
+constexpr int kNowhere = 0x7ffffff0;
+
+template <typename T, bool KR, int BM, int NTH>
+struct Direct {
+  static constexpr int CH = BM * 8 / NTH;    // loads a lane makes per slab
+  static constexpr int PER = BM / kElems<T>; // KR: chunks per k-row
+  const char* base;
+  int64_t ld;  // bytes
+  int off[CH];
+  int col;     // KC: the lane's first value in a slab
+  int span;    // KC: the buffer's bytes; KR: bytes of a row that may be read
+
+  // rows: KC rows of the tile, KR columns.
+  __device__ __forceinline__ Direct(const T* p, int64_t ld_, int rows, int klim) {
+    base = reinterpret_cast<const char*>(p);
+    ld = ld_ * (int64_t)sizeof(T);
+#pragma unroll
+    for (int q = 0; q < CH; ++q) {
+      const int i = q * NTH + threadIdx.x;
+      if constexpr (KR) {
+        const int row = i / PER, c = kr_slot<T, PER>(row, i % PER);
+        off[q] = c * kElems<T> < rows ? (int)(row * ld) + c * 16 : kNowhere;
+      } else {
+        const int row = i / 8;
+        off[q] = (int)(row * ld) + (((i % 8) ^ (row & 7)) * 16);
+      }
+    }
+    const int lane = threadIdx.x;
+    col = ((lane % 8) ^ ((lane / 8) & 7)) * kElems<T>;
+    span = KR ? (int)(rows * (int64_t)sizeof(T)) : (int)((rows - 1) * ld + klim * (int64_t)sizeof(T));
+  }
+
+  // The slab at k0 into lds; past klim it reads zeros.
+  __device__ __forceinline__ void load(u32x4* lds, int k0, int klim) const {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if constexpr (KR) {
+      const int left = klim - k0;
+      const int n = left <= 0 ? 0 : min(left, kSlab<T>) - 1;
+      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<char*>(base + k0 * ld), 0, left <= 0 ? 0 : (int)(n * ld) + span, kBufRsrcDword3);
+#pragma unroll
+      for (int q = 0; q < CH; ++q)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(lds + q * NTH + wave * 64),
+                                                 16, off[q], 0, 0, 0);
+    } else {
+      // k goes into the scalar offset, which the range check leaves out: rows past the tile's are caught by
+      // their own offsets, k past the row's end (the last slab, or those after it) by the lane.
+      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, span, kBufRsrcDword3);
+      const int k = k0 * (int)sizeof(T);
+      const bool in = k0 + col < klim;
+#pragma unroll
+      for (int q = 0; q < CH; ++q)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(lds + q * NTH + wave * 64),
+                                                 16, in ? off[q] : kNowhere, k, 0, 0);
+    }
+  }
+};
+
+// Waits until at most N of the wave's loads are in flight, then for the whole workgroup.
+template <int N>
+__device__ __forceinline__ void slab_ready() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Tile `at` of the workgroup's XCD, in the order in which the workgroups of an XCD (every eighth) should take them:
+// each XCD a run of its own, and in a run four row tiles side by side through all column tiles, so that
+// what the XCD's CUs work on at a time shares rows and columns in its L2.
+__device__ __forceinline__ bool xcd_tile(int tiles_i, int tiles_j, int at, int* ti, int* tj) {
+  const int total = tiles_i * tiles_j, run = (total + 7) / 8;
+  const int t = (blockIdx.x % 8) * run + at;
+  if (at >= run || t >= total) return false;
+  const int band = t / (4 * tiles_j), high = min(4, tiles_i - 4 * band), in = t - band * 4 * tiles_j;
+  *ti = 4 * band + in % high;
+  *tj = in / high;
+  return true;
+}
+
+// Row tiles in all.
+template <int BM>
+__device__ __forceinline__ int count_tiles(const int32_t* offsets, int E, int64_t R) {
+  const int lane = threadIdx.x & 63;
+  int n = 0;
+  for (int base = 0; base <= E; base += 64) {
+    const int e = base + lane;
+    if (e <= E) {
+      const Group g = group_of(offsets, e, E, R);
+      n += (int)((g.hi - g.lo + BM - 1) / BM);
+    }
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
+  return n;
+}
+
+template <typename T, typename TO, bool A_KR, bool B_KR, int BM, int BN, int WI, int WJ, int ST, Role ROLE>
+__global__ __launch_bounds__(64 * WI * WJ, WI * WJ == 4 && BM == 256 ? 1 : 2) void grouped_direct_kernel(GroupedArgs a) {
+#ifdef __HIP_DEVICE_COMPILE__  // the host's compiler drops instantiations with 16-byte loads to LDS
+  static_assert(!__is_same(T, Mx) || BM % 64 == 0, "a wave's scales are all A's or all B's");
+  constexpr bool MX = __is_same(T, Mx), AHEAD = !MX && BM == 256;
+  constexpr int NTH = 64 * WI * WJ, FI = BM / WI / 16, FJ = BN / WJ / 16;
+  constexpr int kSlabChunks = (BM + BN) * 8;
+  // Mx: every wave loads as many scales (past the tile's rows: zeros into the array's end)
+  constexpr int SQ = MX ? (BM + BN + NTH - 1) / NTH : 0, kScaleDwords = SQ * NTH;
+  __shared__ u32x4 lds[ST * kSlabChunks];
+  __shared__ uint32_t lds_s[MX ? ST * kScaleDwords : 1];
+  const T *A = (const T*)a.A, *B = (const T*)a.B;
+  TO* out = (TO*)a.out;
+  int64_t i0;
+  int rows, k0 = 0, klim;  // rows of the tile; the range of k
+  int e, ti, tj;
+  if constexpr (ROLE == Role::kRows) {
+    const int tiles = __builtin_amdgcn_readfirstlane(count_tiles<BM>(a.offsets, a.E, a.R));
+    if (!xcd_tile(tiles, a.tiles_j, blockIdx.x / 8, &ti, &tj)) return;
+    const RowTile t = find_tile<BM>(a.offsets, a.E, a.R, ti);
+    if (t.e < 0) return;
+    e = __builtin_amdgcn_readfirstlane(t.e);
+    i0 = __builtin_amdgcn_readfirstlane((int)t.lo);
+    rows = __builtin_amdgcn_readfirstlane((int)(t.hi - t.lo));
+    klim = e < a.E ? (int)a.K : 0;
+    A += i0 * a.lda;
+    B += (int64_t)(e < a.E ? e : 0) * a.b_expert;
+  } else {
+    // Every XCD takes an eighth of each expert's tiles: the experts' rows, and so their tiles' times, differ.
+    const int run = (a.tiles_i * a.tiles_j + 7) / 8, at = blockIdx.x / 8;
+    e = at / run;
+    if (!xcd_tile(a.tiles_i, a.tiles_j, at - e * run, &ti, &tj)) return;
+    i0 = (int64_t)ti * BM;
+    const Group g = group_of(a.offsets, e, a.E, a.R);
+    rows = (int)(a.I - i0 < BM ? a.I - i0 : BM);
+    k0 = __builtin_amdgcn_readfirstlane((int)g.lo);
+    klim = __builtin_amdgcn_readfirstlane((int)g.hi);
+    A += i0;
+    out += (int64_t)e * a.o_expert;
+  }
+  const int64_t j0 = (int64_t)tj * BN;
+  const int cols = (int)(a.J - j0 < BN ? a.J - j0 : BN);
+  B += B_KR ? j0 : j0 * a.ldb;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wi = (wave / WJ) * (BM / WI), wj = (wave % WJ) * (BN / WJ);
+  f32x4 acc[FI][FJ];
+#pragma unroll
+  for (int i = 0; i < FI; ++i)
+#pragma unroll
+    for (int j = 0; j < FJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  const Direct<T, A_KR, BM, NTH> da(A, a.lda, rows, klim);
+  const Direct<T, B_KR, BN, NTH> db(B, a.ldb, cols, klim);
+  constexpr int kLoads = da.CH + db.CH + SQ;  // per wave and slab
+  const uint8_t *pa = nullptr, *pb = nullptr;
+  if constexpr (MX) {
+    pa = a.sa + i0 * a.ns;
+    pb = a.sb + ((int64_t)(e < a.E ? e : 0) * a.J + j0) * a.ns;
+  }
+  auto issue = [&](int s, int k) {
+    u32x4* p = lds + s * kSlabChunks;
+    da.load(p, k, klim);
+    db.load(p + BM * 8, k, klim);
+    if constexpr (MX) {  // four scales of a row are one dword; a wave's rows are all A's or all B's
+#pragma unroll
+      for (int q = 0; q < SQ; ++q) {
+        const int r0 = q * NTH + wave * 64;
+        const bool of_a = r0 < BM;
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint8_t*>(of_a ? pa : pb), 0, (int)((of_a ? rows : cols) * a.ns), kBufRsrcDword3);
+        const int row = r0 + lane - (of_a ? 0 : BM);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            r, (__attribute__((address_space(3))) void*)(lds_s + s * kScaleDwords + r0), 4,
+            k < klim ? row * (int)a.ns + k / 32 : kNowhere, 0, 0, 0);
+      }
+    }
+  };
+  auto multiply = [&](int s, int k) {
+    const u32x4 *la = lds + s * kSlabChunks, *lb = la + BM * 8;
+    if constexpr (MX) {
+      const uint8_t* sc = reinterpret_cast<const uint8_t*>(lds_s + s * kScaleDwords) + (lane & 15) * 4 + (lane >> 4);
+      const bool block = k + 32 * (lane >> 4) < klim;  // a scale row's filling is not used
+      u32x4 fb[FJ][2];
+      uint32_t s_b[FJ];
 #pragma unroll
       for (int j = 0; j < FJ; ++j) {
-        const int r = wj + 16 * j + (lane & 15);
-        s_b[j] = block && r < cols ? a.sb[((int64_t)e * a.J + j0 + r) * a.ns + k0 / 32 + (lane >> 4)] : 0;
+        fb[j][0] = load_frag<T, false, BN>(lb, wj + 16 * j, 0);
+        fb[j][1] = load_frag<T, false, BN>(lb, wj + 16 * j, 1);
+        s_b[j] = block ? sc[(BM + wj + 16 * j) * 4] : 0;
       }
-      u32x4 fb[FJ][2];
-#pragma unroll
-      for (int j = 0; j < FJ; ++j)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) fb[j][h] = load_frag<T, false, BN>(lb, wj + 16 * j, h);
 #pragma unroll
       for (int i = 0; i < FI; ++i) {
         const u32x4 a0 = load_frag<T, false, BM>(la, wi + 16 * i, 0), a1 = load_frag<T, false, BM>(la, wi + 16 * i, 1);
+        const uint32_t s_a = block ? sc[(wi + 16 * i) * 4] : 0;
 #pragma unroll
-        for (int j = 0; j < FJ; ++j) acc[i][j] = mma_mx(fb[j][0], fb[j][1], a0, a1, s_b[j], s_a[i], acc[i][j]);
+        for (int j = 0; j < FJ; ++j) acc[i][j] = mma_mx(fb[j][0], fb[j][1], a0, a1, s_b[j], s_a, acc[i][j]);
       }
     } else {
 #pragma unroll
@@ -317,7 +531,87 @@ __global__ __launch_bounds__(256) void grouped_kernel(GroupedArgs a) {
           for (int j = 0; j < FJ; ++j) acc[i][j] = mma<T>(fb[j], fa, acc[i][j]);
         }
       }
+      if constexpr (FI >= FJ) {
+        // One row fragment ahead of the matrix instructions that use it, and the second half's columns
+        // spread over the first half's end.
+        constexpr int RA = !A_KR ? 1 : (sizeof(T) == 2 ? 2 : 4), RB = !B_KR ? 1 : (sizeof(T) == 2 ? 2 : 4);
+        constexpr int MM = FJ * (sizeof(T) == 4 ? 4 : 1);
+        __builtin_amdgcn_sched_group_barrier(0x100, FJ * RB + 2 * RA, 0);
+#pragma unroll
+        for (int n = 0; n < 2 * FI; ++n) {
+          __builtin_amdgcn_sched_group_barrier(0x008, MM, 0);
+          if (n >= FI - FJ && n < FI) __builtin_amdgcn_sched_group_barrier(0x100, RB, 0);
+          if (n < 2 * FI - 2) __builtin_amdgcn_sched_group_barrier(0x100, RA, 0);
+        }
+      }
     }
+  };
+
+  if constexpr (AHEAD) {
+    // Fragments are read half a slab ahead of the matrix instructions that use them.  Between a slab's halves
+    // every wave has read all of it and the next one has arrived: one barrier a slab, and the loads of slab
+    // n + 2 go out there, a whole slab's time before they are needed.
+    if (k0 < klim) {
+      u32x4 fa[2][FI], fb[2][FJ];
+      constexpr int RA = !A_KR ? 1 : (sizeof(T) == 2 ? 2 : 4), RB = !B_KR ? 1 : (sizeof(T) == 2 ? 2 : 4);
+      constexpr int MM = FI * FJ * (sizeof(T) == 4 ? 4 : 1), DS = FI * RA + FJ * RB;
+      auto read = [&](int s, int h) {
+        const u32x4 *la = lds + s * kSlabChunks, *lb = la + BM * 8;
+#pragma unroll
+        for (int j = 0; j < FJ; ++j) fb[h][j] = load_frag<T, B_KR, BN>(lb, wj + 16 * j, h);
+#pragma unroll
+        for (int i = 0; i < FI; ++i) fa[h][i] = load_frag<T, A_KR, BM>(la, wi + 16 * i, h);
+      };
+      auto mult = [&](int h) {
+#pragma unroll
+        for (int i = 0; i < FI; ++i)
+#pragma unroll
+          for (int j = 0; j < FJ; ++j) acc[i][j] = mma<T>(fb[h][j], fa[h][i], acc[i][j]);
+      };
+      issue(0, k0);
+      issue(1, k0 + kSlab<T>);
+      slab_ready<kLoads>();
+      read(0, 0);
+      int s = 0;
+      for (; k0 < klim; k0 += kSlab<T>, s ^= 1) {
+        read(s, 1);
+        mult(0);
+#pragma unroll
+        for (int n = 0; n < DS; ++n) {
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x008, MM / DS, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        issue(s, k0 + 2 * kSlab<T>);
+        read(s ^ 1, 0);
+        mult(1);
+#pragma unroll
+        for (int n = 0; n < DS; ++n) {
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          if (n < kLoads) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x008, MM / DS, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing lands in LDS after the workgroup's end
+    }
+  } else if (k0 < klim) {
+#pragma unroll
+    for (int s = 0; s < ST - 1; ++s) issue(s, k0 + s * kSlab<T>);
+    int s = 0;
+    for (; k0 < klim; k0 += kSlab<T>) {
+      slab_ready<(ST - 2) * kLoads>();
+      int next = s + ST - 1;
+      next = next >= ST ? next - ST : next;
+      issue(next, k0 + (ST - 1) * kSlab<T>);
+      multiply(s, k0);
+      s = s + 1 == ST ? 0 : s + 1;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing lands in LDS after the workgroup's end
   }
   const bool vec = a.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(TO) - 1)) == 0;
 #pragma unroll
@@ -329,6 +623,116 @@ __global__ __launch_bounds__(256) void grouped_kernel(GroupedArgs a) {
       const int c = wj + 16 * j + 4 * (lane >> 4);
       store4(out + (i0 + r) * a.ldo + j0 + c, acc[i][j], cols - c, vec);
     }
+  }
+#endif
+}
+
+// ---------------------------------------------------------------------------
+// Few rows an expert (decoding): out[i, j] for up to 16 FI rows and 16 NJ columns, both operands with k
+// contiguous.  What counts is how fast the weights arrive, and nothing is used twice, so fragments come
+// from global memory straight into registers: a lane holds 16-byte chunks g and 4 + g of 128 bytes of a
+// row (a unit).  The waves of a workgroup take every WAVES-th unit, each with U of them in flight, and
+// add up through LDS in wave order.
+// ---------------------------------------------------------------------------
+template <typename T, typename TO, int FI, int NJ, int WAVES, int U>
+__global__ __launch_bounds__(64 * WAVES) void grouped_few_kernel(GroupedArgs a) {
+  constexpr bool MX = __is_same(T, Mx);
+  __shared__ f32x4 sum[WAVES][FI * NJ][64];
+  const int ti = blockIdx.x / a.tiles_j;
+  const int j0 = (int)(blockIdx.x % a.tiles_j) * 16 * NJ;
+  const RowTile t = find_tile<16 * FI>(a.offsets, a.E, a.R, ti);
+  if (t.e < 0) return;
+  const int e = __builtin_amdgcn_readfirstlane(t.e);
+  const int64_t i0 = __builtin_amdgcn_readfirstlane((int)t.lo);
+  const int rows = __builtin_amdgcn_readfirstlane((int)(t.hi - t.lo));
+  const int klim = e < a.E ? (int)a.K : 0;
+  const int cols = min((int)a.J - j0, 16 * NJ);
+  const int lane = threadIdx.x & 63, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t wrow = (int64_t)(e < a.E ? e : 0) * a.J + j0;  // the tile's first weight row
+  const int lda = (int)(a.lda * (int64_t)sizeof(T)), ldb = (int)(a.ldb * (int64_t)sizeof(T));
+  const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<char*>((const char*)a.A + i0 * lda), 0, (rows - 1) * lda + klim * (int)sizeof(T), kBufRsrcDword3);
+  const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<char*>((const char*)a.B + wrow * ldb), 0, (cols - 1) * ldb + klim * (int)sizeof(T), kBufRsrcDword3);
+  const int ns = (int)a.ns;
+  const __amdgpu_buffer_rsrc_t rsa = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t*>(MX ? a.sa + i0 * a.ns : nullptr), 0, MX ? rows * ns : 0, kBufRsrcDword3);
+  const __amdgpu_buffer_rsrc_t rsb = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t*>(MX ? a.sb + wrow * a.ns : nullptr), 0, MX ? cols * ns : 0, kBufRsrcDword3);
+  f32x4 acc[FI][NJ];
+#pragma unroll
+  for (int i = 0; i < FI; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  struct Unit {
+    u32x4 a[FI][2], b[NJ][2];
+    uint32_t sa[FI], sb[NJ];
+  };
+  // Ranges as in the direct kernel: rows past the tile's by the buffer, k past the end by the lane.
+  auto load = [&](Unit& u, int unit) {
+    const int k = unit * kSlab<T>;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const bool in = k + (4 * h + g) * kElems<T> < klim;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int off = in ? (16 * j + (lane & 15)) * ldb + (4 * h + g) * 16 : kNowhere;
+        u.b[j][h] = __builtin_amdgcn_raw_buffer_load_b128(rb, off, unit * 128, 2);  // streamed
+      }
+#pragma unroll
+      for (int i = 0; i < FI; ++i) {
+        const int off = in ? (16 * i + (lane & 15)) * lda + (4 * h + g) * 16 : kNowhere;
+        u.a[i][h] = __builtin_amdgcn_raw_buffer_load_b128(ra, off, unit * 128, 0);
+      }
+    }
+    if constexpr (MX) {
+      const bool in = k + 32 * g < klim;  // a scale row's filling is not read
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+        u.sb[j] = __builtin_amdgcn_raw_buffer_load_b8(rsb, in ? (16 * j + (lane & 15)) * ns + g : kNowhere, unit * 4, 0);
+#pragma unroll
+      for (int i = 0; i < FI; ++i)
+        u.sa[i] = __builtin_amdgcn_raw_buffer_load_b8(rsa, in ? (16 * i + (lane & 15)) * ns + g : kNowhere, unit * 4, 0);
+    }
+  };
+  auto multiply = [&](const Unit& u) {
+#pragma unroll
+    for (int i = 0; i < FI; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        if constexpr (MX) {
+          acc[i][j] = mma_mx(u.b[j][0], u.b[j][1], u.a[i][0], u.a[i][1], u.sb[j], u.sa[i], acc[i][j]);
+        } else {
+          acc[i][j] = mma<T>(u.b[j][0], u.a[i][0], acc[i][j]);
+          acc[i][j] = mma<T>(u.b[j][1], u.a[i][1], acc[i][j]);
+        }
+      }
+  };
+  const int units = (klim + kSlab<T> - 1) / kSlab<T>;
+  Unit u[U];
+#pragma unroll
+  for (int n = 0; n < U; ++n) load(u[n], wave + n * WAVES);  // past the end: zeros
+  for (int at = wave; at < units; at += U * WAVES) {
+#pragma unroll
+    for (int n = 0; n < U; ++n) {
+      multiply(u[n]);
+      load(u[n], at + (U + n) * WAVES);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < FI; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) sum[wave][i * NJ + j][lane] = acc[i][j];
+  __syncthreads();
+  TO* out = (TO*)a.out;
+  const bool vec = a.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(TO) - 1)) == 0;
+  for (int f = wave; f < FI * NJ; f += WAVES) {
+    f32x4 v = sum[0][f][lane];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) v += sum[w][f][lane];
+    const int r = f / NJ * 16 + (lane & 15), c = f % NJ * 16 + 4 * g;
+    if (r < rows) store4(out + (i0 + r) * a.ldo + j0 + c, v, cols - c, vec);
   }
 }
 

@@ -363,7 +363,8 @@ def offsets_of(split, R, E, dtype=torch.int32):
     (64, 128, 256, 8, "even"), (300, 72, 136, 5, "empty ends"), (300, 129, 65, 5, "one has all"),
     (1000, 256, 200, 70, "single rows"), (257, 500, 1001, 3, "even"), (130, 96, 64, 4, "none"),
     (700, 640, 384, 130, "even"), (1024, 1024, 512, 4, "empty ends"), (90, 2048, 264, 6, "empty ends"),
-    (2000, 512, 768, 2, "one has all"),
+    (2000, 512, 768, 2, "one has all"), (300, 136, 2056, 4, "even"), (1100, 1032, 1048, 5, "empty ends"),
+    (2100, 1032, 2056, 5, "empty ends"), (4100, 264, 2048, 3, "one has all"), (1500, 1026, 1030, 6, "even"),
 ])
 def test_grouped_matmul(R, K, N, E, split, dtype):
     dt = DT[dtype]
@@ -472,7 +473,7 @@ def test_grouped_matmul_strides_alignment_and_repeatability():
 @pytest.mark.parametrize("R,K,N,E,split", [
     (1, 32, 8, 1, "even"), (3, 96, 33, 2, "even"), (64, 128, 128, 8, "even"), (129, 160, 257, 5, "empty ends"),
     (40, 1024, 64, 40, "single rows"), (600, 512, 384, 3, "one has all"), (16, 4096, 72, 4, "even"),
-    (77, 64, 100, 3, "none"),
+    (77, 64, 100, 3, "none"), (900, 416, 1100, 5, "empty ends"), (4200, 288, 2056, 3, "empty ends"),
 ])
 def test_grouped_matmul_mx(R, K, N, E, split, out):
     x, w = rand(R, K, seed=1), rand(E, N, K, seed=2, scale=K ** -0.5)
