@@ -4,7 +4,7 @@
 // which the GPU worked 44): a ctypes call marshals 20-30 arguments, a Python autograd node costs
 // 5 us forward and takes the GIL in the engine's thread backward.
 //
-// The nodes are the ones of mhc/_layer.py, mhc/ops.py and mhc/streams.py (their docstrings hold the
+// The nodes are the ones of mhc/_layer.py, mhc/ops.py, mhc/streams.py and mhc/branch.py (their docstrings hold the
 // reasoning): the same inputs, outputs and saved tensors in the same roles.  Every function returns
 // None when a call is not the plain case -- a tensor subclass, a CPU tensor, mixed devices, an
 // unsupported dtype or shape, a functorch transform, a torch-function or torch-dispatch mode,
@@ -769,6 +769,240 @@ PyObject* py_ends(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------------------
+// mhc.branch: rms_norm, dropout, grouped_matmul
+// ---------------------------------------------------------------------------
+
+// A tensor or None.
+bool optional_tensor(PyObject* o, const Tensor& like, Tensor* out) {
+  return o == Py_None || (tensors(&o, 1, out) && out->device() == like.device());
+}
+
+Tensor empty_like_plain(const Tensor& t) { return at::empty(t.sizes(), t.options().requires_grad(false)); }
+
+Tensor whole(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+
+at::IntArrayRef row_sizes(const Tensor& t) { return t.sizes().slice(0, t.dim() - 1); }
+
+int64_t row_count(const Tensor& t) { return t.size(-1) ? t.numel() / t.size(-1) : 0; }
+
+struct NormOut { Tensor x, y, h, rstd; };
+
+NormOut norm_forward(const Tensor& x_in, const Tensor& weight, const Tensor& residual, double eps, bool keep) {
+  const c10::DeviceGuard guard(x_in.device());
+  NormOut o;
+  o.x = x_in.contiguous();
+  const Tensor res = whole(residual), w = f32(weight);
+  o.y = empty_like_plain(o.x);
+  if (res.defined()) o.h = empty_like_plain(o.x);
+  if (keep) o.rstd = empty_f32(row_sizes(o.x), o.x);
+  check(mhc_rms_norm_forward(ptr(o.x), ptr(res), code(o.x), fptr(w), ptr(o.y), ptr(o.h), wptr(o.rstd), row_count(o.x),
+                             o.x.size(-1), (float)eps, stream(o.x)),
+        "rms_norm_forward");
+  return o;
+}
+
+struct RmsNorm : Function<RmsNorm> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& weight,
+                               const std::optional<Tensor>& residual, double eps) {
+    const Tensor w = weight.value_or(Tensor());
+    NormOut o = norm_forward(x, w, residual.value_or(Tensor()), eps, true);
+    ctx->save_for_backward({o.h.defined() ? o.h : o.x, w, o.rstd});
+    ctx->set_materialize_grads(false);
+    if (o.h.defined()) return {o.y, o.h};
+    return {o.y};
+  }
+
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    const variable_list s = saved(ctx);
+    const Tensor dh_in = g.size() > 1 ? g[1] : Tensor();
+    // inputs that were None do not count
+    const bool has_w = s[1].defined(), has_res = g.size() > 1;
+    const bool need_w = has_w && ctx->needs_input_grad(1), need_res = has_res && ctx->needs_input_grad(1 + has_w);
+    const bool need_x = ctx->needs_input_grad(0) || need_res;
+    Tensor dx = dh_in, dw;
+    if (g[0].defined() && (need_x || need_w)) {
+      const c10::DeviceGuard guard(s[0].device());
+      const Tensor h = s[0].contiguous(), w = f32(s[1]), rstd = f32(s[2]);
+      const Tensor dy = in_dtype(g[0], h.scalar_type()), dh = in_dtype(dh_in, h.scalar_type());
+      const int64_t R = row_count(h), D = h.size(-1);
+      dx = need_x ? empty_like_plain(h) : Tensor();
+      if (need_w) dw = empty_f32({D}, h);
+      const Workspace ws(need_w ? mhc_rms_norm_backward_workspace_bytes(R, D) : 0, h);
+      check(mhc_rms_norm_backward(ptr(dy), ptr(h), ptr(dh), code(h), fptr(w), fptr(rstd), ptr(dx), wptr(dw), R, D,
+                                  ws.p(), ws.bytes, stream(h)),
+            "rms_norm_backward");
+    }
+    return {ctx->needs_input_grad(0) ? dx : Tensor(), dw.defined() ? grad_like(dw, s[1]) : Tensor(),
+            need_res ? dx : Tensor(), Tensor()};
+  }
+};
+
+std::optional<Tensor> given(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
+
+PyObject* py_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor x, w, res;
+  double eps;
+  if (n != 4 || !tensors(a, 1, &x) || !optional_tensor(a[1], x, &w) || !optional_tensor(a[2], x, &res) ||
+      !number(a[3], &eps))
+    return none();
+  if (code(x) < 0 || x.dim() < 1 || x.size(-1) > 16384 || (w.defined() && w.sizes() != x.sizes().slice(x.dim() - 1)) ||
+      (w.defined() && !w.is_floating_point()) ||
+      (res.defined() && (res.sizes() != x.sizes() || res.scalar_type() != x.scalar_type())))
+    return none();
+  variable_list out;
+  {
+    ReleaseGil gil;
+    if (wants_grad({x, w, res})) {
+      out = RmsNorm::apply(x, given(w), given(res), eps);
+    } else {
+      NormOut o = norm_forward(x, w, res, eps, false);
+      out = {o.y};
+      if (o.h.defined()) out.push_back(o.h);
+    }
+  }
+  return out.size() == 1 ? THPVariable_Wrap(out[0]) : tuple_of(out);
+  END_HANDLE_TH_ERRORS
+}
+
+struct Draw { uint64_t seed = 0, offset = 0; };
+
+Tensor dropout_forward(const Tensor& x_in, const Tensor& residual, double p, const Draw& d, const Tensor& state,
+                       Tensor* used) {
+  const c10::DeviceGuard guard(x_in.device());
+  const Tensor x = x_in.contiguous(), res = whole(residual), st = whole(state);
+  const Tensor y = empty_like_plain(x);
+  if (used) *used = at::empty({2}, x.options().dtype(at::kLong).requires_grad(false));
+  check(mhc_dropout(ptr(x), ptr(res), code(x), ptr(y), x.numel(), p, d.seed, d.offset,
+                    static_cast<const int64_t*>(ptr(st)), used ? static_cast<int64_t*>(ptr(*used)) : nullptr, stream(x)),
+        "dropout");
+  return y;
+}
+
+struct Dropout : Function<Dropout> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& residual,
+                        const std::optional<Tensor>& state, double p, int64_t seed, int64_t offset) {
+    Tensor used;
+    const Tensor y = dropout_forward(x, residual.value_or(Tensor()), p, {(uint64_t)seed, (uint64_t)offset},
+                                     state.value_or(Tensor()), state ? &used : nullptr);
+    ctx->saved_data["res"] = residual.has_value();
+    // a device state may move on before the backward: what the forward drew from is kept
+    if (used.defined()) ctx->save_for_backward({used});
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["seed"] = seed;
+    ctx->saved_data["offset"] = offset;
+    ctx->saved_data["dtype"] = (int64_t)x.scalar_type();
+    return y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    const variable_list s = saved(ctx);
+    Tensor dx;
+    if (ctx->needs_input_grad(0))
+      dx = dropout_forward(in_dtype(g[0], (at::ScalarType)ctx->saved_data["dtype"].toInt()), Tensor(),
+                           ctx->saved_data["p"].toDouble(),
+                           {(uint64_t)ctx->saved_data["seed"].toInt(), (uint64_t)ctx->saved_data["offset"].toInt()},
+                           s.empty() ? Tensor() : s[0], nullptr);
+    const bool need_res = ctx->saved_data["res"].toBool() && ctx->needs_input_grad(1);
+    return {dx, need_res ? g[0] : Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+bool number(PyObject* o, uint64_t* v) {
+  if (!PyLong_CheckExact(o)) return false;
+  *v = PyLong_AsUnsignedLongLong(o);
+  if (*v == (uint64_t)-1 && PyErr_Occurred()) { PyErr_Clear(); return false; }
+  return true;
+}
+
+PyObject* py_dropout(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor x, res, state;
+  double p;
+  Draw d;
+  if (n != 4 || !tensors(a, 1, &x) || !optional_tensor(a[1], x, &res) || !number(a[2], &p)) return none();
+  if (PyTuple_CheckExact(a[3])) {
+    if (PyTuple_GET_SIZE(a[3]) != 2 || !number(PyTuple_GET_ITEM(a[3], 0), &d.seed) ||
+        !number(PyTuple_GET_ITEM(a[3], 1), &d.offset))
+      return none();
+  } else if (a[3] == Py_None || !optional_tensor(a[3], x, &state) || state.scalar_type() != at::kLong ||
+             state.sizes() != at::IntArrayRef({2})) {
+    return none();
+  }
+  if (code(x) < 0 || !(p >= 0. && p <= 1.) ||
+      (res.defined() && (res.sizes() != x.sizes() || res.scalar_type() != x.scalar_type())))
+    return none();
+  Tensor y;
+  {
+    ReleaseGil gil;
+    if (wants_grad({x, res})) y = Dropout::apply(x, given(res), given(state), p, (int64_t)d.seed, (int64_t)d.offset);
+    else y = dropout_forward(x, res, p, d, state, nullptr);
+  }
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+Tensor int_offsets(const Tensor& t) { return t.to(at::kInt).contiguous(); }
+
+Tensor grouped_forward(const Tensor& x_in, const Tensor& w_in, const Tensor& off_in) {
+  const c10::DeviceGuard guard(x_in.device());
+  const Tensor x = x_in.contiguous(), w = w_in.contiguous(), off = int_offsets(off_in);
+  const Tensor y = at::empty({x.size(0), w.size(1)}, x.options().requires_grad(false));
+  check(mhc_grouped_matmul_forward(ptr(x), ptr(w), code(x), static_cast<const int32_t*>(ptr(off)), ptr(y), x.size(0),
+                                   x.size(1), w.size(1), w.size(0), stream(x)),
+        "grouped_matmul_forward");
+  return y;
+}
+
+struct GroupedMatmul : Function<GroupedMatmul> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& off) {
+    ctx->save_for_backward({x, w, off});
+    return grouped_forward(x, w, off);
+  }
+
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    const variable_list s = saved(ctx);
+    const c10::DeviceGuard guard(s[0].device());
+    const at::ScalarType dt = s[0].scalar_type();
+    const Tensor dy = in_dtype(g[0], dt), off = int_offsets(s[2]);
+    const int32_t* o = static_cast<const int32_t*>(ptr(off));
+    const int64_t R = s[0].size(0), K = s[0].size(1), N = s[1].size(1), E = s[1].size(0);
+    Tensor dx, dw;
+    if (ctx->needs_input_grad(0)) {
+      const Tensor w = in_dtype(s[1], dt);
+      dx = at::empty({R, K}, dy.options().requires_grad(false));
+      check(mhc_grouped_matmul_backward_input(ptr(dy), ptr(w), code(dy), o, ptr(dx), R, K, N, E, stream(dy)),
+            "grouped_matmul_backward_input");
+    }
+    if (ctx->needs_input_grad(1)) {
+      const Tensor x = s[0].contiguous();
+      dw = at::empty({E, N, K}, dy.options().requires_grad(false));
+      check(mhc_grouped_matmul_backward_weight(ptr(dy), ptr(x), code(dy), o, ptr(dw), R, K, N, E, stream(dy)),
+            "grouped_matmul_backward_weight");
+    }
+    return {dx, dw, Tensor()};
+  }
+};
+
+PyObject* py_grouped_matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor t[3];
+  if (n != 3 || !tensors(a, 3, t)) return none();
+  if (code(t[0]) < 0 || t[1].scalar_type() != t[0].scalar_type() || t[0].dim() != 2 || t[1].dim() != 3 ||
+      t[0].size(1) != t[1].size(2) || t[2].sizes() != t[1].sizes().slice(0, 1) ||
+      (t[2].scalar_type() != at::kInt && t[2].scalar_type() != at::kLong))
+    return none();
+  Tensor y;
+  {
+    ReleaseGil gil;
+    if (wants_grad({t[0], t[1]})) y = GroupedMatmul::apply(t[0], t[1], t[2]);
+    else y = grouped_forward(t[0], t[1], t[2]);
+  }
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* py_set_error(PyObject*, PyObject* cls) {
   Py_INCREF(cls);
   Py_XDECREF(g_error);
@@ -783,7 +1017,9 @@ PyMethodDef methods[] = {
     {"layer_add", FAST(py_layer_add)},           {"sinkhorn", FAST(py_sinkhorn)},
     {"stream_mix", FAST(py_stream_mix)},         {"add_residual", FAST(py_add_residual)},
     {"dynamic_weights", FAST(py_dynamic_weights)}, {"expand", FAST(py_ends<true>)},
-    {"collapse", FAST(py_ends<false>)},          {"set_error", py_set_error, METH_O, nullptr},
+    {"collapse", FAST(py_ends<false>)},          {"rms_norm", FAST(py_rms_norm)},
+    {"dropout", FAST(py_dropout)},               {"grouped_matmul", FAST(py_grouped_matmul)},
+    {"set_error", py_set_error, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -28,6 +28,7 @@ import torch
 
 from . import _branch as _k
 from . import _branch_library as _l
+from . import _lib
 from ._branch import Rng
 
 __all__ = ["rms_norm", "rms_norm_mx", "quantize_mx", "grouped_matmul", "grouped_matmul_mx", "dropout"]
@@ -107,6 +108,10 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: O
     """
     if torch.compiler.is_compiling():
         return _l.rms_norm(x, weight, residual, float(eps))
+    if x.is_cuda:
+        out = _lib.native().rms_norm(x, weight, residual, float(eps))
+        if out is not None:
+            return out
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         return _RmsNorm.apply(x, weight, residual, float(eps))
     y, h, _ = _k.rms_norm_forward(x, weight, residual, float(eps), want_rstd=False)
@@ -149,6 +154,10 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor)
     """
     if torch.compiler.is_compiling():
         return _l.grouped_matmul(x, weight, offsets)
+    if x.is_cuda:
+        y = _lib.native().grouped_matmul(x, weight, offsets)
+        if y is not None:
+            return y
     return _GroupedMatmul.apply(x, weight, offsets)
 
 
@@ -176,4 +185,8 @@ def dropout(x: torch.Tensor, p: float, rng: Rng, residual: Optional[torch.Tensor
         p = 0.0
     if torch.compiler.is_compiling():
         return _l.dropout(x, float(p), rng, residual)
+    if x.is_cuda:
+        y = _lib.native().dropout(x, residual, float(p), rng)
+        if y is not None:
+            return y
     return _Dropout.apply(x, residual, float(p), rng)

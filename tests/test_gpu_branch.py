@@ -12,6 +12,7 @@ import pytest
 import torch
 
 from helpers import assert_rounded_once, to_np
+from test_gpu_native_nodes import both, same
 from mhc import _branch, branch
 from oracle import branch_oracle as O
 
@@ -615,6 +616,42 @@ def test_compiled_equals_eager():
         return branch.grouped_matmul_mx(q, s, *branch.quantize_mx(wt), off), h
 
     assert all(torch.equal(a, b) for a, b in zip(g(*args[:5]), torch.compile(g, fullgraph=True, backend="aot_eager")(*args[:5])))
+
+
+@pytest.mark.parametrize("grads", [(), ("x",), ("w",), ("res",), ("wt",), ("x", "w", "res", "wt")])
+@pytest.mark.parametrize("state", [False, True])
+def test_native_and_python_nodes_agree(monkeypatch, grads, state):
+    """The C++ nodes and the Python nodes make the same launches: the same bits."""
+    leaves = {"x": rand(40, 128, seed=1, dtype=torch.bfloat16), "w": rand(128, seed=2, dtype=torch.float16),
+              "res": rand(40, 128, seed=3, dtype=torch.bfloat16), "wt": rand(3, 128, 128, seed=4, dtype=torch.bfloat16)}
+    off = torch.tensor([7, 7, 40], device=DEV)
+    dy = rand(40, 128, seed=5, dtype=torch.bfloat16).T.contiguous().T
+
+    def step():
+        for n, t in leaves.items():
+            t.requires_grad_(n in grads)
+        y, h = branch.rms_norm(leaves["x"], leaves["w"], residual=leaves["res"])
+        y = branch.grouped_matmul(branch.rms_norm(y), leaves["wt"], off)
+        y = branch.dropout(y, 0.3, torch.tensor([3, 4], device=DEV) if state else (3, 4), residual=h)
+        return [y.detach(), *(torch.autograd.grad(y, [leaves[n] for n in grads], dy) if grads else ())]
+
+    got, want = both(monkeypatch, step)
+    same(got, want)
+
+
+def test_calls_the_native_nodes_leave_alone():
+    from mhc import _lib
+
+    n = _lib.native()
+    x, w = torch.ones(4, 8, device=DEV), torch.ones(2, 8, 8, device=DEV)
+    off = torch.tensor([2, 4], dtype=torch.int32, device=DEV)
+    assert n.rms_norm(x, None, None, 1e-6) is not None and n.grouped_matmul(x, w, off) is not None
+    for out in (n.rms_norm(x, x, None, 1e-6), n.rms_norm(x.double(), None, None, 1e-6), n.rms_norm(x, None, x[:2], 1e-6),
+                n.rms_norm(x, None, None, 1), n.dropout(x, None, 0.5, (-1, 0)), n.dropout(x, None, 1.5, (0, 0)),
+                n.dropout(x, None, 0.5, (0, 1 << 64)), n.dropout(x, None, 0.5, off), n.dropout(x, None, 0.5, None),
+                n.grouped_matmul(x, w[0], off), n.grouped_matmul(x, w, off[:1]), n.grouped_matmul(x, w, off.cpu()),
+                n.grouped_matmul(x, w.half(), off), n.grouped_matmul(x.cpu(), w, off)):
+        assert out is None
 
 
 def test_wrong_devices_and_dtypes_are_refused():
