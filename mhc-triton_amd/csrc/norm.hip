@@ -9,7 +9,7 @@
 // All of it in fp32 from the stored values.  y is the norm of the *stored* h: the next layer reads
 // that h, and the backward has nothing else, so forward and backward see the same function.
 //
-// A team of TEAM lanes (a wave, or a workgroup) holds one row in registers, NV vectors per lane, so
+// A team (a wave, or a workgroup) holds one row in registers, NV vectors per lane, so
 // each tensor passes the bus once; a workgroup walks over rows with the weight kept in registers.
 #include "stream_kernels.hpp"
 
@@ -28,36 +28,41 @@ __device__ __forceinline__ float wave_total(float v) {
   return __uint_as_float(q[0]) + __uint_as_float(q[1]);
 }
 
-// Sum over a team.  `lds` holds 2 * (TEAM / 64) floats; `turn` alternates between its halves, so one
-// barrier per row is enough.
-template <int TEAM>
-__device__ __forceinline__ float team_sum(float v, float* lds, int turn) {
+// A team is a wave (WAVE: four rows a workgroup of 256) or the whole workgroup, of as many waves as the row
+// needs, 16 at most.
+constexpr int kTeamWaves = 16;
+
+template <bool WAVE>
+__device__ __forceinline__ uint32_t team_lane() { return WAVE ? threadIdx.x & 63 : threadIdx.x; }
+template <bool WAVE>
+__device__ __forceinline__ uint32_t team_size() { return WAVE ? 64 : blockDim.x; }
+template <bool WAVE>
+constexpr int kTeamRows = WAVE ? 4 : 1;
+
+// Sum over a team, in wave order.  `turn` alternates between the halves of `lds`, so one barrier per row
+// is enough.
+template <bool WAVE>
+__device__ __forceinline__ float team_sum(float v, float (&lds)[2][kTeamWaves], int turn) {
   v = wave_total(v);
-  if constexpr (TEAM > 64) {
-    constexpr int NW = TEAM / 64;
-    float* p = lds + turn * NW;
-    if ((threadIdx.x & 63) == 0) p[threadIdx.x >> 6] = v;
+  if constexpr (!WAVE) {
+    if ((threadIdx.x & 63) == 0) lds[turn][threadIdx.x >> 6] = v;
     __syncthreads();
-    v = 0.f;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) v += p[i];
+    v = lds[turn][0];
+    for (uint32_t i = 1; i < blockDim.x / 64; ++i) v += lds[turn][i];
   }
   return v;
 }
 
-template <int TEAM>
-constexpr int kNormThreads = TEAM < 256 ? 256 : TEAM;
-
-// The vectors of a row that a lane holds: c = lane + v * TEAM, `ok` where c is inside the row.
-template <int W, bool RAG, int TEAM, int NV>
+// The vectors of a row that a lane holds: c = lane + v * team, `ok` where c is inside the row.
+template <int W, bool RAG, bool WAVE, int NV>
 struct RowPart {
   uint32_t col[NV], skip[NV];
   bool ok[NV];
   __device__ __forceinline__ RowPart(uint32_t D) {
-    const uint32_t lane = threadIdx.x % TEAM, nch = (D + W - 1) / W;
+    const uint32_t lane = team_lane<WAVE>(), nch = (D + W - 1) / W;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const uint32_t c = lane + v * TEAM;
+      const uint32_t c = lane + v * team_size<WAVE>();
       ok[v] = c < nch;
       const RowCol<W, RAG> rc(ok[v] ? c : 0, D);
       col[v] = rc.col;
@@ -77,9 +82,18 @@ __device__ __forceinline__ void load_row(const T* row, int64_t D, const P& p, Fr
 template <int W, int NV, typename P>
 __device__ __forceinline__ void load_weight(const float* w, const P& p, float (&f)[NV][W]) {
 #pragma unroll
-  for (int v = 0; v < NV; ++v)
+  for (int v = 0; v < NV; ++v) {
 #pragma unroll
-    for (int e = 0; e < W; ++e) f[v][e] = w && p.ok[v] ? w[p.col[v] + e] : (p.ok[v] ? 1.f : 0.f);
+    for (int e = 0; e < W; ++e) f[v][e] = p.ok[v] ? 1.f : 0.f;
+    if (!w || !p.ok[v]) continue;
+    if constexpr (W >= 4) {
+#pragma unroll
+      for (int q = 0; q < W / 4; ++q) RawVec<float>::unpack(__builtin_bit_cast(f32x4, load16_any(w + p.col[v] + 4 * q, false)), f[v] + 4 * q);
+    } else {
+#pragma unroll
+      for (int e = 0; e < W; ++e) f[v][e] = w[p.col[v] + e];
+    }
+  }
 }
 
 // 8-bit microscaled output: the smallest power of two that brings a block's largest magnitude to 448
@@ -138,17 +152,17 @@ struct NormArgs {
   float eps;
 };
 
-template <typename T, int W, bool RAG, int TEAM, int NV, bool RES, bool MX>
-__global__ __launch_bounds__(kNormThreads<TEAM>) void norm_fwd_kernel(NormArgs a) {
-  constexpr int NTH = kNormThreads<TEAM>, ROWS = NTH / TEAM;
-  __shared__ float lds[2 * (TEAM / 64)];
+template <typename T, int W, bool RAG, bool WAVE, int NV, bool RES, bool MX>
+__global__ __launch_bounds__(WAVE ? 256 : 64 * kTeamWaves) void norm_fwd_kernel(NormArgs a) {
+  constexpr int ROWS = kTeamRows<WAVE>;
+  __shared__ float lds[2][kTeamWaves];
   const int64_t D = a.D;
-  const RowPart<W, RAG, TEAM, NV> p((uint32_t)D);
+  const RowPart<W, RAG, WAVE, NV> p((uint32_t)D);
   float w[NV][W];
   load_weight(a.w, p, w);
   const float inv_d = 1.f / (float)D;
   int turn = 0;
-  for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TEAM; row < a.R; row += (int64_t)gridDim.x * ROWS) {
+  for (int64_t row = (int64_t)blockIdx.x * ROWS + (WAVE ? threadIdx.x / 64 : 0); row < a.R; row += (int64_t)gridDim.x * ROWS) {
     Frag<T, W> xf[NV], rf[NV];
     load_row<T, W, RAG, NV, true>((const T*)a.x + row * D, D, p, xf);
     if constexpr (RES) load_row<T, W, RAG, NV, true>((const T*)a.res + row * D, D, p, rf);
@@ -173,10 +187,10 @@ __global__ __launch_bounds__(kNormThreads<TEAM>) void norm_fwd_kernel(NormArgs a
 #pragma unroll
       for (int e = 0; e < W; ++e) ss += RAG && (uint32_t)e < p.skip[v] ? 0.f : h[v][e] * h[v][e];
     }
-    ss = team_sum<TEAM>(ss, lds, turn);
+    ss = team_sum<WAVE>(ss, lds, turn);
     turn ^= 1;
     const float r = 1.f / sqrtf(ss * inv_d + a.eps);
-    if (a.rstd && threadIdx.x % TEAM == 0) a.rstd[row] = r;
+    if (a.rstd && team_lane<WAVE>() == 0) a.rstd[row] = r;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       float y[W];
@@ -196,7 +210,7 @@ __global__ __launch_bounds__(kNormThreads<TEAM>) void norm_fwd_kernel(NormArgs a
       }
     }
     if constexpr (MX) {  // the scale row's filling
-      const int64_t pad = D / kMxBlock + threadIdx.x % TEAM;
+      const int64_t pad = D / kMxBlock + team_lane<WAVE>();
       if (pad < a.ns) a.scales[row * a.ns + pad] = 0;
     }
   }
@@ -210,12 +224,12 @@ struct NormBwdArgs {
   int64_t R, D;
 };
 
-template <typename T, int W, bool RAG, int TEAM, int NV, bool DH>
-__global__ __launch_bounds__(kNormThreads<TEAM>) void norm_bwd_kernel(NormBwdArgs a) {
-  constexpr int NTH = kNormThreads<TEAM>, ROWS = NTH / TEAM;
-  __shared__ float lds[2 * (TEAM / 64)];
+template <typename T, int W, bool RAG, bool WAVE, int NV, bool DH>
+__global__ __launch_bounds__(WAVE ? 256 : 64 * kTeamWaves) void norm_bwd_kernel(NormBwdArgs a) {
+  constexpr int ROWS = kTeamRows<WAVE>;
+  __shared__ float lds[2][kTeamWaves];
   const int64_t D = a.D;
-  const RowPart<W, RAG, TEAM, NV> p((uint32_t)D);
+  const RowPart<W, RAG, WAVE, NV> p((uint32_t)D);
   float w[NV][W], dw[NV][W];
   load_weight(a.w, p, w);
 #pragma unroll
@@ -224,28 +238,41 @@ __global__ __launch_bounds__(kNormThreads<TEAM>) void norm_bwd_kernel(NormBwdArg
     for (int e = 0; e < W; ++e) dw[v][e] = 0.f;
   const float inv_d = 1.f / (float)D;
   int turn = 0;
-  for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TEAM; row < a.R; row += (int64_t)gridDim.x * ROWS) {
-    Frag<T, W> yf[NV], hf[NV], gf[NV];
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  int64_t row = (int64_t)blockIdx.x * ROWS + (WAVE ? threadIdx.x / 64 : 0);
+  Frag<T, W> yf[NV], hf[NV], gf[NV];
+  float r = 0.f;
+  auto load = [&](int64_t row) {
     load_row<T, W, RAG, NV, true>((const T*)a.dy + row * D, D, p, yf);
     load_row<T, W, RAG, NV, true>((const T*)a.h + row * D, D, p, hf);
     if constexpr (DH) load_row<T, W, RAG, NV, true>((const T*)a.dh + row * D, D, p, gf);
-    const float r = a.rstd[row];
-    float g[NV][W], n[NV][W];
+    r = a.rstd[row];
+  };
+  if (row < a.R) load(row);
+  for (; row < a.R; row += step) {
+    float g[NV][W], n[NV][W], u[NV][W];
+    const float rs = r;
     float c = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       if (!p.ok[v]) continue;
       yf[v].unpack(g[v]);
       hf[v].unpack(n[v]);
+      if constexpr (DH) gf[v].unpack(u[v]);
+    }
+    if (row + step < a.R) load(row + step);  // on their way while this row is summed
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      if (!p.ok[v]) continue;
 #pragma unroll
       for (int e = 0; e < W; ++e) {
-        n[v][e] *= r;
+        n[v][e] *= rs;
         dw[v][e] += g[v][e] * n[v][e];
         g[v][e] *= w[v][e];
         c += RAG && (uint32_t)e < p.skip[v] ? 0.f : g[v][e] * n[v][e];
       }
     }
-    c = team_sum<TEAM>(c, lds, turn) * inv_d;
+    c = team_sum<WAVE>(c, lds, turn) * inv_d;
     turn ^= 1;
     if (!a.dx) continue;
 #pragma unroll
@@ -253,12 +280,9 @@ __global__ __launch_bounds__(kNormThreads<TEAM>) void norm_bwd_kernel(NormBwdArg
       if (!p.ok[v]) continue;
       float d[W];
 #pragma unroll
-      for (int e = 0; e < W; ++e) d[e] = r * (g[v][e] - n[v][e] * c);
-      if constexpr (DH) {
-        float u[W];
-        gf[v].unpack(u);
-#pragma unroll
-        for (int e = 0; e < W; ++e) d[e] += u[e];
+      for (int e = 0; e < W; ++e) {
+        d[e] = rs * (g[v][e] - n[v][e] * c);
+        if constexpr (DH) d[e] += u[v][e];
       }
       const typename SpanOf<T, W, RAG>::type ds((T*)a.dx + row * D, D);
       st_from<T, W, true>(ds, p.col[v], d, p.skip[v]);
@@ -266,7 +290,8 @@ __global__ __launch_bounds__(kNormThreads<TEAM>) void norm_bwd_kernel(NormBwdArg
   }
   if (!a.part) return;
   float* out = a.part + (int64_t)blockIdx.x * D;
-  if constexpr (TEAM < 256) {  // the workgroup's four rows' sums, in wave order
+  if constexpr (WAVE) {  // the workgroup's four rows' sums, in wave order
+    constexpr int TEAM = 64;
     __shared__ float sum[ROWS][TEAM * NV * W];
     const int team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM;
 #pragma unroll
@@ -292,22 +317,32 @@ __global__ __launch_bounds__(kNormThreads<TEAM>) void norm_bwd_kernel(NormBwdArg
   }
 }
 
-// dw[d] = sum over the partial records, 16 groups of them side by side, in fp64 (they are the sum's largest terms).
-constexpr int kDwCols = 64;
+// dw[d] = sum over the partial records in fp64 (they are the sum's largest terms): 16 columns a workgroup, 16
+// groups of records side by side, eight loads of a lane in flight.
+constexpr int kDwCols = 16, kDwGroups = 16;
 
-__global__ __launch_bounds__(1024) void norm_dw_reduce_kernel(const float* __restrict__ part, float* __restrict__ dw,
-                                                              int n, int64_t D) {
-  __shared__ double sum[16][kDwCols];
+__global__ __launch_bounds__(kDwCols * kDwGroups) void norm_dw_reduce_kernel(const float* __restrict__ part,
+                                                                            float* __restrict__ dw, int n, int64_t D) {
+  __shared__ double sum[kDwGroups][kDwCols];
   const int col = threadIdx.x % kDwCols, grp = threadIdx.x / kDwCols;
   const int64_t d = (int64_t)blockIdx.x * kDwCols + col;
   double s = 0.;
-  if (d < D)
-    for (int i = grp; i < n; i += 16) s += part[i * D + d];
+  if (d < D) {
+    int i = grp;
+    for (; i + 7 * kDwGroups < n; i += 8 * kDwGroups) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = part[(int64_t)(i + k * kDwGroups) * D + d];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += v[k];
+    }
+    for (; i < n; i += kDwGroups) s += part[(int64_t)i * D + d];
+  }
   sum[grp][col] = s;
   __syncthreads();
   if (grp || d >= D) return;
 #pragma unroll
-  for (int i = 1; i < 16; ++i) s += sum[i][col];
+  for (int i = 1; i < kDwGroups; ++i) s += sum[i][col];
   dw[d] = (float)s;
 }
 
@@ -336,23 +371,34 @@ __global__ __launch_bounds__(kThreads) void quantize_mx_kernel(const T* __restri
 // Rows of up to this many elements fit the registers of the widest team.
 constexpr int64_t kNormMaxDim = 16384;
 
-// Workgroups of the backward, each with a partial weight gradient.
-constexpr int64_t kNormBwdBlocks = 512;
+// A workgroup a row (or four) forward, four of them a CU: they start and end apart, which is worth the
+// weight's vectors read again for each.  16384 x 4096 bf16 with a residual: two to eight workgroups a CU that
+// loop over rows 92-99 us, a row each 86.6 (6.2 TB/s) and 89.0 without the limit.
+constexpr int64_t kNormFwdBlocks = (int64_t)1 << 22;
 
-template <int T, int N>
+// Workgroups of the backward at most, each with a partial weight gradient: half as many of four waves that
+// each hold a sum.  More write and add up more partials, fewer leave CUs waiting (us at 256 / 512 / 1024):
+// 16384 x 4096 bf16 with a residual 117 / 92 / 104, 3069 x 1500 fp16 (waves) 12.5 / 17 / 21.  A team has two
+// rows at least, for the same reason: 1000 x 256 bf16 7.6 -> 5.7 us.
+constexpr int64_t kNormBwdBlocks = 512;
+constexpr int kBwdRows = 2;
+
+template <bool W, int N>
 struct Team {
-  static constexpr int TEAM = T, NV = N;
+  static constexpr bool WAVE = W;
+  static constexpr int NV = N;
 };
 
-// The team and vectors per lane for rows of `nch` vectors.
+// The team for rows of `nch` vectors, fn(Team, threads): a wave up to 256 vectors; beyond, a workgroup
+// of as many waves as two vectors a lane need (four, past 16 waves).  D = 7168 bf16, seven waves of two
+// against four of four: to 8 bits 75.7 -> 72.1 us.
 template <class F>
 static int with_team(int64_t nch, F&& fn) {
-  if (nch <= 64) return fn(Team<64, 1>{});
-  if (nch <= 128) return fn(Team<64, 2>{});
-  if (nch <= 256) return fn(Team<64, 4>{});
-  if (nch <= 512) return fn(Team<256, 2>{});
-  if (nch <= 1024) return fn(Team<256, 4>{});
-  return fn(Team<1024, 4>{});
+  if (nch <= 64) return fn(Team<true, 1>{}, 256);
+  if (nch <= 128) return fn(Team<true, 2>{}, 256);
+  if (nch <= 256) return fn(Team<true, 4>{}, 256);
+  if (nch <= 2 * 64 * kTeamWaves) return fn(Team<false, 2>{}, (int)((nch + 127) / 128 * 64));
+  return fn(Team<false, 4>{}, (int)((nch + 255) / 256 * 64));
 }
 
 // Whole vectors, ragged vectors, or (rows below one vector) single elements.
@@ -390,11 +436,13 @@ static int norm_forward(const char* who, NormArgs a, int dtype, hipStream_t st) 
     auto go = [&](auto wc, auto rag) {
       constexpr int W = decltype(wc)::value;
       constexpr bool RAG = decltype(rag)::value;
-      return with_team((a.D + W - 1) / W, [&](auto team) -> int {
-        constexpr int TEAM = decltype(team)::TEAM, NV = decltype(team)::NV, NTH = kNormThreads<TEAM>;
-        const dim3 grid((unsigned)norm_blocks(a.R, NTH / TEAM, 8 * (int64_t)num_cus()));
-        if (a.res) norm_fwd_kernel<T, W, RAG, TEAM, NV, true, MX><<<grid, NTH, 0, st>>>(a);
-        else norm_fwd_kernel<T, W, RAG, TEAM, NV, false, MX><<<grid, NTH, 0, st>>>(a);
+      return with_team((a.D + W - 1) / W, [&](auto team, int threads) -> int {
+        constexpr bool WAVE = decltype(team)::WAVE;
+        constexpr int NV = decltype(team)::NV;
+        const dim3 grid((unsigned)norm_blocks(a.R, kTeamRows<WAVE>, kNormFwdBlocks));
+        const size_t cap = WAVE || threads > 512 ? 0 : occupancy_lds(4);
+        if (a.res) norm_fwd_kernel<T, W, RAG, WAVE, NV, true, MX><<<grid, threads, cap, st>>>(a);
+        else norm_fwd_kernel<T, W, RAG, WAVE, NV, false, MX><<<grid, threads, cap, st>>>(a);
         return hip_status(hipGetLastError(), who);
       });
     };
@@ -445,7 +493,7 @@ extern "C" int mhc_rms_norm_mx_forward(const void* x, const void* residual, int 
 
 extern "C" size_t mhc_rms_norm_backward_workspace_bytes(int64_t R, int64_t D) {
   if (R <= 0 || D <= 0) return 0;
-  return (size_t)(norm_blocks(R, 1, kNormBwdBlocks) * D) * sizeof(float);
+  return (size_t)(norm_blocks(R, kBwdRows, kNormBwdBlocks) * D) * sizeof(float);
 }
 
 extern "C" int mhc_rms_norm_backward(const void* dy, const void* h, const void* dh, int dtype, const float* weight,
@@ -468,17 +516,18 @@ extern "C" int mhc_rms_norm_backward(const void* dy, const void* h, const void* 
     return with_row_width<Vec<T>::N>(D, {dy, h, dh, dx}, [&](auto wc, auto rag) {
       constexpr int W = decltype(wc)::value;
       constexpr bool RAG = decltype(rag)::value;
-      return with_team((D + W - 1) / W, [&](auto team) -> int {
-        constexpr int TEAM = decltype(team)::TEAM, NV = decltype(team)::NV, NTH = kNormThreads<TEAM>;
-        blocks = (unsigned)norm_blocks(R, NTH / TEAM, kNormBwdBlocks);
-        if (dh) norm_bwd_kernel<T, W, RAG, TEAM, NV, true><<<blocks, NTH, 0, st>>>(a);
-        else norm_bwd_kernel<T, W, RAG, TEAM, NV, false><<<blocks, NTH, 0, st>>>(a);
+      return with_team((D + W - 1) / W, [&](auto team, int threads) -> int {
+        constexpr bool WAVE = decltype(team)::WAVE;
+        constexpr int NV = decltype(team)::NV;
+        blocks = (unsigned)norm_blocks(R, kBwdRows * kTeamRows<WAVE>, WAVE ? kNormBwdBlocks / 2 : kNormBwdBlocks);
+        if (dh) norm_bwd_kernel<T, W, RAG, WAVE, NV, true><<<blocks, threads, 0, st>>>(a);
+        else norm_bwd_kernel<T, W, RAG, WAVE, NV, false><<<blocks, threads, 0, st>>>(a);
         return hip_status(hipGetLastError(), "rms_norm_backward launch");
       });
     });
   });
   if (rc || !dweight) return rc;
-  norm_dw_reduce_kernel<<<dim3((unsigned)((D + kDwCols - 1) / kDwCols)), 1024, 0, st>>>(a.part, dweight, (int)blocks, D);
+  norm_dw_reduce_kernel<<<dim3((unsigned)((D + kDwCols - 1) / kDwCols)), kDwCols * kDwGroups, 0, st>>>(a.part, dweight, (int)blocks, D);
   return hip_status(hipGetLastError(), "rms_norm_backward reduce launch");
 }
 
