@@ -33,7 +33,9 @@ static int check_tiles(const char* who, int64_t tiles, int threads) {
 template <typename T, typename TO, bool A_KR, bool B_KR, int BM, int BN, int WI, int WJ, int ST, Role ROLE>
 static int launch_direct(GroupedArgs a, const char* who, hipStream_t st) {
   constexpr int NTH = 64 * WI * WJ;
-  const int64_t tiles = set_tiles<ROLE, BM, BN>(a);
+  a.cus = num_cus();
+  // the 256-tiles of the last round may go in quarters
+  const int64_t tiles = set_tiles<ROLE, BM, BN>(a) + (BM == 256 && ROLE == Role::kRows ? 2 * a.cus + 16 : 0);
   if (int rc = check_tiles(who, tiles, NTH)) return rc;
   // whole runs of eight: one for each XCD
   grouped_direct_kernel<T, TO, A_KR, B_KR, BM, BN, WI, WJ, ST, ROLE>

@@ -33,8 +33,7 @@ struct GroupedArgs {
   int64_t ns;
   int64_t R, I, J, K;      // rows in all; the product's sizes (kRows: I = R, kWeight: K = R)
   int64_t lda, ldb, ldo, b_expert, o_expert;
-  int E, tiles_i, tiles_j;
-  bool vec;
+  int E, tiles_i, tiles_j, cus;
 };
 
 // Rows of one expert, clamped to [0, R) whatever the offsets hold.
@@ -229,6 +228,56 @@ __device__ __forceinline__ void store4(TO* p, f32x4 v, int64_t n, bool vec) {
   }
 }
 
+// The tile's results, acc[i][j] of wave (wi, wj), to out rows of ldo: through LDS, so that whole rows of 16-byte
+// chunks leave the workgroup.  (Four neighbours a lane straight from the registers cost 20 us a tile of 256 x 256
+// bf16; 16384 x 4096 outputs at K = 64: 105 -> STOREUS us.)  Chunk c of row r waits at slot c ^ (r & 15).
+template <typename TO, int BM, int BN, int NTH, int CHUNKS, int FI, int FJ>
+__device__ __forceinline__ void store_tile(u32x4* lds, const f32x4 (&acc)[FI][FJ], int wi, int wj, TO* out, int64_t ldo,
+                                           int rows, int cols) {
+  constexpr int CPR = BN / kElems<TO>, MASK = (CPR < 16 ? CPR : 16) - 1;
+  constexpr int RP = BM * CPR <= CHUNKS ? BM : BM / 2;  // rows at a time
+  constexpr int Q = (RP * CPR + NTH - 1) / NTH;
+  static_assert(RP * CPR <= CHUNKS && RP % 16 == 0, "the tile fits in two passes");
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int p = 0; p < BM / RP; ++p) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < FI; ++i) {
+      if (RP < BM && (wi + 16 * i) / RP != p) continue;
+      const int r = wi + 16 * i + (lane & 15) - p * RP;
+#pragma unroll
+      for (int j = 0; j < FJ; ++j) {
+        const int c = wj + 16 * j + 4 * (lane >> 4);
+        const f32x4 v = acc[i][j];
+        if constexpr (sizeof(TO) == 4) {
+          lds[r * CPR + ((c / 4) ^ (r & MASK))] = __builtin_bit_cast(u32x4, v);
+        } else {
+          TO t[4] = {from_f32<TO>(v[0]), from_f32<TO>(v[1]), from_f32<TO>(v[2]), from_f32<TO>(v[3])};
+          reinterpret_cast<s16x4*>(lds)[2 * (r * CPR + ((c / 8) ^ (r & MASK))) + (c / 4) % 2] = *reinterpret_cast<s16x4*>(t);
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int at = q * NTH + threadIdx.x, r = at / CPR, c = at % CPR;
+      const int n = cols - c * kElems<TO>;  // values of the chunk that exist
+      if (r >= RP || p * RP + r >= rows || n <= 0) continue;
+      const u32x4 v = lds[r * CPR + (c ^ (r & MASK))];
+      TO* to = out + (int64_t)(p * RP + r) * ldo + c * kElems<TO>;
+      if (n >= kElems<TO>) {
+        store16_any(to, v, false);
+      } else {
+        for (int k = 0; k < n; ++k) {
+          if constexpr (sizeof(TO) == 4) reinterpret_cast<uint32_t*>(to)[k] = v[k];
+          else reinterpret_cast<uint16_t*>(to)[k] = (uint16_t)(v[k / 2] >> (16 * (k & 1)));
+        }
+      }
+    }
+  }
+}
+
 // The general kernel: any size and alignment, operands staged through registers (unaligned 16-byte loads,
 // single values at a row's end).  256 threads, four waves of a quarter of the tile each; the next slab's
 // loads are in flight while one is multiplied, and two slabs of LDS make one barrier a slab enough.
@@ -303,17 +352,7 @@ __global__ __launch_bounds__(256) void grouped_kernel(GroupedArgs a) {
       }
     }
   }
-  const bool vec = a.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(T) - 1)) == 0;
-#pragma unroll
-  for (int i = 0; i < FI; ++i) {
-    const int r = wi + 16 * i + (lane & 15);
-    if (r >= rows) continue;
-#pragma unroll
-    for (int j = 0; j < FJ; ++j) {
-      const int c = wj + 16 * j + 4 * (lane >> 4);
-      store4(out + (i0 + r) * a.ldo + j0 + c, acc[i][j], cols - c, vec);
-    }
-  }
+  store_tile<T, BM, BN, NTH, 2 * (BM + BN) * 8>(lds, acc, wi, wj, out + i0 * a.ldo + j0, a.ldo, (int)rows, (int)cols);
 }
 
 // ---------------------------------------------------------------------------
@@ -383,6 +422,33 @@ struct Direct {
   }
 };
 
+// Scales of 8-bit operands on their way to LDS: a thread has a row, and takes four slabs' scales (16 bytes) at a
+// time, a slab before they are used.  A dword a slab straight to LDS asked L2 for as many lines as the values
+// themselves do (8192 x 7168 x 2048 over 16 experts: 236 -> 219 us).  What fills a row past K / 32 is not used.
+struct ScaleFeed {
+  __amdgpu_buffer_rsrc_t r;
+  int off, ns, blocks;  // the row's offset (past any buffer: none); bytes of a row, and how many of them count
+  u32x4 quad;
+
+  __device__ __forceinline__ void load(int slab) {
+    if (4 * slab + 16 <= ns) {
+      quad = __builtin_amdgcn_raw_buffer_load_b128(r, off, 4 * slab, 0);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        quad[j] = __builtin_amdgcn_raw_buffer_load_b32(r, 4 * (slab + j) < ns ? off : kNowhere, 4 * (slab + j), 0);
+    }
+  }
+  // The scales of slab n, which follow one another.
+  __device__ __forceinline__ uint32_t take(int n) {
+    uint32_t v = n & 2 ? (n & 1 ? quad[3] : quad[2]) : (n & 1 ? quad[1] : quad[0]);
+    const int left = blocks - 4 * n;
+    if (left < 4) v = left <= 0 ? 0 : v & ((1u << (8 * left)) - 1);
+    if ((n & 3) == 3) load(n + 1);
+    return v;
+  }
+};
+
 // Waits until at most N of the wave's loads are in flight, then for the whole workgroup.
 template <int N>
 __device__ __forceinline__ void slab_ready() {
@@ -391,17 +457,19 @@ __device__ __forceinline__ void slab_ready() {
   asm volatile("" ::: "memory");
 }
 
-// Tile `at` of the workgroup's XCD, in the order in which the workgroups of an XCD (every eighth) should take them:
-// each XCD a run of its own, and in a run four row tiles side by side through all column tiles, so that
-// what the XCD's CUs work on at a time shares rows and columns in its L2.
-__device__ __forceinline__ bool xcd_tile(int tiles_i, int tiles_j, int at, int* ti, int* tj) {
-  const int total = tiles_i * tiles_j, run = (total + 7) / 8;
-  const int t = (blockIdx.x % 8) * run + at;
-  if (at >= run || t >= total) return false;
+// Tile t of tiles_i x tiles_j: four row tiles side by side through all column tiles, so that neighbours share
+// rows and columns.  Each XCD (every eighth workgroup) takes a run of neighbours, for its L2.
+__device__ __forceinline__ void band_tile(int t, int tiles_i, int tiles_j, int* ti, int* tj) {
   const int band = t / (4 * tiles_j), high = min(4, tiles_i - 4 * band), in = t - band * 4 * tiles_j;
   *ti = 4 * band + in % high;
   *tj = in / high;
-  return true;
+}
+
+// Place `at` of this workgroup's XCD in n places split into eight runs; false past the run's end.
+__device__ __forceinline__ bool xcd_place(int n, int at, int* t) {
+  const int run = (n + 7) / 8;
+  *t = (blockIdx.x % 8) * run + at;
+  return at < run && *t < n;
 }
 
 // Row tiles in all.
@@ -421,49 +489,31 @@ __device__ __forceinline__ int count_tiles(const int32_t* offsets, int E, int64_
   return n;
 }
 
-template <typename T, typename TO, bool A_KR, bool B_KR, int BM, int BN, int WI, int WJ, int ST, Role ROLE>
-__global__ __launch_bounds__(64 * WI * WJ, WI * WJ == 4 && BM == 256 ? 1 : 2) void grouped_direct_kernel(GroupedArgs a) {
+// What a workgroup is to do: `rows` x `cols` results of expert e from (i0, j0) on, k from k0 to klim.
+struct Task {
+  int e;
+  int64_t i0, j0;
+  int rows, cols, k0, klim;
+};
+
+// LDS of a tile in 16-byte chunks: per slab A, B and (8 bits) a dword of scales for each thread.
+template <typename T, int BM, int BN, int NTH>
+constexpr int kSlabChunks = (BM + BN) * 8 + (__is_same(T, Mx) ? NTH / 4 : 0);
+
 #ifdef __HIP_DEVICE_COMPILE__  // the host's compiler drops instantiations with 16-byte loads to LDS
-  static_assert(!__is_same(T, Mx) || BM % 64 == 0, "a wave's scales are all A's or all B's");
-  constexpr bool MX = __is_same(T, Mx), AHEAD = !MX && BM == 256;
+template <typename T, typename TO, bool A_KR, bool B_KR, int BM, int BN, int WI, int WJ, int ST, Role ROLE>
+__device__ __forceinline__ void direct_tile(const GroupedArgs& a, const Task& task, u32x4* lds) {
+  constexpr bool MX = __is_same(T, Mx), AHEAD = sizeof(T) == 2 && BM == 256 && BN == 256;
   constexpr int NTH = 64 * WI * WJ, FI = BM / WI / 16, FJ = BN / WJ / 16;
-  constexpr int kSlabChunks = (BM + BN) * 8;
-  // Mx: every wave loads as many scales (past the tile's rows: zeros into the array's end)
-  constexpr int SQ = MX ? (BM + BN + NTH - 1) / NTH : 0, kScaleDwords = SQ * NTH;
-  __shared__ u32x4 lds[ST * kSlabChunks];
-  __shared__ uint32_t lds_s[MX ? ST * kScaleDwords : 1];
-  const T *A = (const T*)a.A, *B = (const T*)a.B;
-  TO* out = (TO*)a.out;
-  int64_t i0;
-  int rows, k0 = 0, klim;  // rows of the tile; the range of k
-  int e, ti, tj;
-  if constexpr (ROLE == Role::kRows) {
-    const int tiles = __builtin_amdgcn_readfirstlane(count_tiles<BM>(a.offsets, a.E, a.R));
-    if (!xcd_tile(tiles, a.tiles_j, blockIdx.x / 8, &ti, &tj)) return;
-    const RowTile t = find_tile<BM>(a.offsets, a.E, a.R, ti);
-    if (t.e < 0) return;
-    e = __builtin_amdgcn_readfirstlane(t.e);
-    i0 = __builtin_amdgcn_readfirstlane((int)t.lo);
-    rows = __builtin_amdgcn_readfirstlane((int)(t.hi - t.lo));
-    klim = e < a.E ? (int)a.K : 0;
-    A += i0 * a.lda;
-    B += (int64_t)(e < a.E ? e : 0) * a.b_expert;
-  } else {
-    // Every XCD takes an eighth of each expert's tiles: the experts' rows, and so their tiles' times, differ.
-    const int run = (a.tiles_i * a.tiles_j + 7) / 8, at = blockIdx.x / 8;
-    e = at / run;
-    if (!xcd_tile(a.tiles_i, a.tiles_j, at - e * run, &ti, &tj)) return;
-    i0 = (int64_t)ti * BM;
-    const Group g = group_of(a.offsets, e, a.E, a.R);
-    rows = (int)(a.I - i0 < BM ? a.I - i0 : BM);
-    k0 = __builtin_amdgcn_readfirstlane((int)g.lo);
-    klim = __builtin_amdgcn_readfirstlane((int)g.hi);
-    A += i0;
-    out += (int64_t)e * a.o_expert;
-  }
-  const int64_t j0 = (int64_t)tj * BN;
-  const int cols = (int)(a.J - j0 < BN ? a.J - j0 : BN);
-  B += B_KR ? j0 : j0 * a.ldb;
+  constexpr int kSlabChunks = mhc::kSlabChunks<T, BM, BN, NTH>;
+  static_assert(!MX || BM + BN <= NTH, "a thread has one row's scales");
+  const int e = task.e, rows = task.rows, cols = task.cols, klim = task.klim;
+  int k0 = task.k0;
+  const int64_t i0 = task.i0, j0 = task.j0;
+  const bool row_role = ROLE == Role::kRows;
+  const T* A = (const T*)a.A + (row_role ? i0 * a.lda : i0);
+  const T* B = (const T*)a.B + (row_role ? (int64_t)(e < a.E ? e : 0) * a.b_expert : 0) + (B_KR ? j0 : j0 * a.ldb);
+  TO* out = (TO*)a.out + (row_role ? 0 : (int64_t)e * a.o_expert);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = (wave / WJ) * (BM / WI), wj = (wave % WJ) * (BN / WJ);
   f32x4 acc[FI][FJ];
@@ -474,49 +524,55 @@ __global__ __launch_bounds__(64 * WI * WJ, WI * WJ == 4 && BM == 256 ? 1 : 2) vo
 
   const Direct<T, A_KR, BM, NTH> da(A, a.lda, rows, klim);
   const Direct<T, B_KR, BN, NTH> db(B, a.ldb, cols, klim);
-  constexpr int kLoads = da.CH + db.CH + SQ;  // per wave and slab
-  const uint8_t *pa = nullptr, *pb = nullptr;
+  constexpr int kLoads = da.CH + db.CH;  // per wave and slab
+  ScaleFeed feed{};
   if constexpr (MX) {
-    pa = a.sa + i0 * a.ns;
-    pb = a.sb + ((int64_t)(e < a.E ? e : 0) * a.J + j0) * a.ns;
+    static_assert(BM % 64 == 0, "a wave's rows are all A's or all B's");
+    const bool of_a = wave * 64 < BM;
+    const int row = (int)threadIdx.x - (of_a ? 0 : BM);
+    feed.ns = (int)a.ns;
+    feed.blocks = klim / 32;
+    feed.r = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(of_a ? a.sa + i0 * a.ns : a.sb + ((int64_t)(e < a.E ? e : 0) * a.J + j0) * a.ns), 0,
+        (of_a ? rows : cols) * feed.ns, kBufRsrcDword3);
+    feed.off = row < (of_a ? rows : cols) ? row * feed.ns : kNowhere;
+    feed.load(0);
   }
   auto issue = [&](int s, int k) {
     u32x4* p = lds + s * kSlabChunks;
+    if constexpr (MX) reinterpret_cast<uint32_t*>(p + (BM + BN) * 8)[threadIdx.x] = feed.take(k / kSlab<T>);
     da.load(p, k, klim);
     db.load(p + BM * 8, k, klim);
-    if constexpr (MX) {  // four scales of a row are one dword; a wave's rows are all A's or all B's
-#pragma unroll
-      for (int q = 0; q < SQ; ++q) {
-        const int r0 = q * NTH + wave * 64;
-        const bool of_a = r0 < BM;
-        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<uint8_t*>(of_a ? pa : pb), 0, (int)((of_a ? rows : cols) * a.ns), kBufRsrcDword3);
-        const int row = r0 + lane - (of_a ? 0 : BM);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            r, (__attribute__((address_space(3))) void*)(lds_s + s * kScaleDwords + r0), 4,
-            k < klim ? row * (int)a.ns + k / 32 : kNowhere, 0, 0, 0);
-      }
-    }
   };
   auto multiply = [&](int s, int k) {
     const u32x4 *la = lds + s * kSlabChunks, *lb = la + BM * 8;
     if constexpr (MX) {
-      const uint8_t* sc = reinterpret_cast<const uint8_t*>(lds_s + s * kScaleDwords) + (lane & 15) * 4 + (lane >> 4);
-      const bool block = k + 32 * (lane >> 4) < klim;  // a scale row's filling is not used
+      // The instruction takes its scale from the low byte.
+      const uint32_t* sc = reinterpret_cast<const uint32_t*>(la + (BM + BN) * 8) + (lane & 15);
+      const int shift = 8 * (lane >> 4);
       u32x4 fb[FJ][2];
-      uint32_t s_b[FJ];
+      uint32_t s_b[FJ], s_a[FI];
+#pragma unroll
+      for (int j = 0; j < FJ; ++j) s_b[j] = sc[BM + wj + 16 * j] >> shift;
+#pragma unroll
+      for (int i = 0; i < FI; ++i) s_a[i] = sc[wi + 16 * i] >> shift;
 #pragma unroll
       for (int j = 0; j < FJ; ++j) {
         fb[j][0] = load_frag<T, false, BN>(lb, wj + 16 * j, 0);
         fb[j][1] = load_frag<T, false, BN>(lb, wj + 16 * j, 1);
-        s_b[j] = block ? sc[(BM + wj + 16 * j) * 4] : 0;
       }
 #pragma unroll
       for (int i = 0; i < FI; ++i) {
         const u32x4 a0 = load_frag<T, false, BM>(la, wi + 16 * i, 0), a1 = load_frag<T, false, BM>(la, wi + 16 * i, 1);
-        const uint32_t s_a = block ? sc[(wi + 16 * i) * 4] : 0;
 #pragma unroll
-        for (int j = 0; j < FJ; ++j) acc[i][j] = mma_mx(fb[j][0], fb[j][1], a0, a1, s_b[j], s_a, acc[i][j]);
+        for (int j = 0; j < FJ; ++j) acc[i][j] = mma_mx(fb[j][0], fb[j][1], a0, a1, s_b[j], s_a[i], acc[i][j]);
+      }
+      // one row fragment ahead of the matrix instructions that use it, and no more: registers
+      __builtin_amdgcn_sched_group_barrier(0x100, 2 * FJ + 4, 0);
+#pragma unroll
+      for (int n = 0; n < FI; ++n) {
+        __builtin_amdgcn_sched_group_barrier(0x008, FJ, 0);
+        if (n < FI - 2) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
       }
     } else {
 #pragma unroll
@@ -604,6 +660,7 @@ __global__ __launch_bounds__(64 * WI * WJ, WI * WJ == 4 && BM == 256 ? 1 : 2) vo
     for (int s = 0; s < ST - 1; ++s) issue(s, k0 + s * kSlab<T>);
     int s = 0;
     for (; k0 < klim; k0 += kSlab<T>) {
+      if constexpr (MX) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // scales written
       slab_ready<(ST - 2) * kLoads>();
       int next = s + ST - 1;
       next = next >= ST ? next - ST : next;
@@ -613,17 +670,79 @@ __global__ __launch_bounds__(64 * WI * WJ, WI * WJ == 4 && BM == 256 ? 1 : 2) vo
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing lands in LDS after the workgroup's end
   }
-  const bool vec = a.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(TO) - 1)) == 0;
-#pragma unroll
-  for (int i = 0; i < FI; ++i) {
-    const int r = wi + 16 * i + (lane & 15);
-    if (r >= rows) continue;
-#pragma unroll
-    for (int j = 0; j < FJ; ++j) {
-      const int c = wj + 16 * j + 4 * (lane >> 4);
-      store4(out + (i0 + r) * a.ldo + j0 + c, acc[i][j], cols - c, vec);
+  store_tile<TO, BM, BN, NTH, ST * kSlabChunks>(lds, acc, wi, wj, out + i0 * a.ldo + j0, a.ldo, rows, cols);
+}
+#endif
+
+// Row tile ti of expert rows, column tile tj.
+template <int BM, int BN>
+__device__ __forceinline__ Task row_task(const GroupedArgs& a, int ti, int tj) {
+  const RowTile t = find_tile<BM>(a.offsets, a.E, a.R, ti);
+  Task k;
+  k.e = __builtin_amdgcn_readfirstlane(t.e);
+  k.i0 = __builtin_amdgcn_readfirstlane((int)t.lo);
+  k.rows = __builtin_amdgcn_readfirstlane((int)(t.hi - t.lo));
+  k.j0 = (int64_t)tj * BN;
+  k.cols = (int)(a.J - k.j0 < BN ? a.J - k.j0 : BN);
+  k.k0 = 0;
+  k.klim = k.e < a.E ? (int)a.K : 0;  // the rows of no expert: zeros
+  return k;
+}
+
+template <typename T, typename TO, bool A_KR, bool B_KR, int BM, int BN, int WI, int WJ, int ST, Role ROLE>
+__global__ __launch_bounds__(64 * WI * WJ, 2) void grouped_direct_kernel(GroupedArgs a) {
+#ifdef __HIP_DEVICE_COMPILE__
+  __shared__ u32x4 lds[ST * kSlabChunks<T, BM, BN, 64 * WI * WJ>];
+  // Tiles of 256 x 256 of rows: what is left after whole rounds of the CUs, if it is half a round at most, goes in
+  // quarters, so that the last round does not leave most CUs idle.
+  constexpr bool QUARTERS = BM == 256 && ROLE == Role::kRows;
+  int t, ti, tj;
+  Task k;
+  if constexpr (ROLE == Role::kRows) {
+    const int tiles = __builtin_amdgcn_readfirstlane(count_tiles<BM>(a.offsets, a.E, a.R));
+    const int total = tiles * a.tiles_j, left = total % a.cus;
+    const int split = QUARTERS && left <= a.cus / 2 ? left : 0, whole = total - split;
+    const int at = blockIdx.x / 8, runs = (whole + 7) / 8;
+    int part = -1;
+    if (!xcd_place(whole, at, &t)) {
+      if (!QUARTERS || at < runs || !xcd_place(4 * split, at - runs, &t)) return;
+      part = t % 4;
+      t = whole + t / 4;
     }
+    band_tile(t, tiles, a.tiles_j, &ti, &tj);
+    k = row_task<BM, BN>(a, ti, tj);
+    if (k.e < 0) return;
+    if constexpr (QUARTERS) {
+      if (part >= 0) {
+        const int di = part / 2 * 128, dj = part % 2 * 128;
+        if (di >= k.rows || dj >= k.cols) return;
+        k.i0 += di;
+        k.j0 += dj;
+        k.rows = min(k.rows - di, 128);
+        k.cols = min(k.cols - dj, 128);
+        direct_tile<T, TO, A_KR, B_KR, 128, 128, 2, 4, ST, ROLE>(a, k, lds);
+        return;
+      }
+      if (k.rows <= 128) {  // an expert's last rows
+        direct_tile<T, TO, A_KR, B_KR, 128, 256, 2, 4, ST, ROLE>(a, k, lds);
+        return;
+      }
+    }
+  } else {
+    // Every XCD takes an eighth of each expert's tiles: the experts' rows, and so their tiles' times, differ.
+    const int run = (a.tiles_i * a.tiles_j + 7) / 8, at = blockIdx.x / 8;
+    k.e = at / run;
+    if (!xcd_place(a.tiles_i * a.tiles_j, at - k.e * run, &t)) return;
+    band_tile(t, a.tiles_i, a.tiles_j, &ti, &tj);
+    const Group g = group_of(a.offsets, k.e, a.E, a.R);
+    k.i0 = (int64_t)ti * BM;
+    k.rows = (int)(a.I - k.i0 < BM ? a.I - k.i0 : BM);
+    k.j0 = (int64_t)tj * BN;
+    k.cols = (int)(a.J - k.j0 < BN ? a.J - k.j0 : BN);
+    k.k0 = __builtin_amdgcn_readfirstlane((int)g.lo);
+    k.klim = __builtin_amdgcn_readfirstlane((int)g.hi);
   }
+  direct_tile<T, TO, A_KR, B_KR, BM, BN, WI, WJ, ST, ROLE>(a, k, lds);
 #endif
 }
 
