@@ -55,7 +55,7 @@ template <typename T, bool A_KR, bool B_KR, int BM, int BN, Role ROLE>
 static int launch_general(GroupedArgs a, const char* who, hipStream_t st) {
   const int64_t tiles = set_tiles<ROLE, BM, BN>(a);
   if (int rc = check_tiles(who, tiles, 256)) return rc;
-  grouped_kernel<T, A_KR, B_KR, BM, BN, ROLE><<<dim3((unsigned)tiles), 256, 0, st>>>(a);
+  grouped_kernel<T, A_KR, B_KR, BM, BN, ROLE><<<dim3((unsigned)((tiles + 7) / 8 * 8)), 256, 0, st>>>(a);
   return hip_status(hipGetLastError(), who);
 }
 
@@ -67,24 +67,31 @@ static int64_t likely_tiles(const GroupedArgs& a) {
   return ((a.R + BM - 1) / BM + (a.E < a.R ? a.E : a.R) / 2) * j;
 }
 
+// Which kernel.  Few rows an expert: at 8 each the kernel that takes weights into registers still wins, past
+// 16 it reads the rows too often (us for 1 / 8 / 16 / 32 rows an expert, registers against tiles: 32 experts of
+// 2048 to 4096 bf16 100 / 111 / 131 / 211 against 133; 8 bits 56 / 64 / 75 / 123 against 74 to 78).  In 8 bits its
+// four waves need four units of four slabs: K = 1024 over 64 experts 38 against 32 us.
+// Tiles: the largest of 256, 128, 64 and 32 that give the CUs enough of them (half of the CUs in 256s, which go in
+// quarters then).  The general kernel takes what is not whole aligned 16-byte chunks.
 template <typename T, typename TO, bool A_KR, bool B_KR, Role ROLE>
 static int launch_grouped(GroupedArgs a, const char* who, hipStream_t st) {
-  const bool vec = a.lda % kElems<T> == 0 && a.ldb % kElems<T> == 0 && aligned16(a.A) && aligned16(a.B);
+  constexpr bool MX = __is_same(T, Mx);
+  const bool chunks = a.lda % kElems<T> == 0 && a.ldb % kElems<T> == 0 && aligned16(a.A) && aligned16(a.B);
   const int cus = num_cus();
-  if (vec) {
+  if (chunks) {
     if constexpr (!A_KR && !B_KR)
-      if (a.R <= 16 * (int64_t)a.E) return launch_few<T, TO, 1, 2, 4, 2>(a, who, st);
-    if (likely_tiles<ROLE, 256, 256>(a) >= cus / 2) return launch_direct<T, TO, A_KR, B_KR, 256, 256, 2, 4, 2, ROLE>(a, who, st);
+      if (a.R <= 8 * (int64_t)a.E && (!MX || a.K >= 2048)) return launch_few<T, TO, 1, 2, 4, 2>(a, who, st);
+    if (likely_tiles<ROLE, 256, 256>(a) >= cus / 2)
+      return launch_direct<T, TO, A_KR, B_KR, 256, 256, 2, 4, 2, ROLE>(a, who, st);
     if (likely_tiles<ROLE, 128, 128>(a) >= cus) return launch_direct<T, TO, A_KR, B_KR, 128, 128, 2, 2, 2, ROLE>(a, who, st);
-    if (__is_same(T, Mx) || likely_tiles<ROLE, 64, 64>(a) >= cus)
-      return launch_direct<T, TO, A_KR, B_KR, 64, 64, 2, 2, 4, ROLE>(a, who, st);
-    if constexpr (!__is_same(T, Mx)) return launch_direct<T, TO, A_KR, B_KR, 32, 32, 2, 2, 4, ROLE>(a, who, st);
+    if (MX || likely_tiles<ROLE, 64, 64>(a) >= cus) return launch_direct<T, TO, A_KR, B_KR, 64, 64, 2, 2, 4, ROLE>(a, who, st);
+    if constexpr (!MX) return launch_direct<T, TO, A_KR, B_KR, 32, 32, 2, 2, 4, ROLE>(a, who, st);
   }
-  if constexpr (!__is_same(T, Mx)) {
+  if constexpr (!MX) {
     if (likely_tiles<ROLE, 128, 128>(a) >= 2 * cus) return launch_general<T, A_KR, B_KR, 128, 128, ROLE>(a, who, st);
     return launch_general<T, A_KR, B_KR, 64, 64, ROLE>(a, who, st);
   }
-  return MHC_OK;
+  return MHC_OK;  // 8-bit operands are whole chunks (checked at the entry)
 }
 
 static int check_grouped(const char* who, int64_t R, int64_t K, int64_t N, int64_t E) {

@@ -83,22 +83,33 @@ __device__ __forceinline__ RowTile find_tile(const int32_t* offsets, int E, int6
   return {-1, 0, 0};
 }
 
-// A 16-byte chunk at p, of any alignment, of which `n` values (the rest zero) may be read.
+// A 16-byte chunk at p, of any alignment, of which `n` values (the rest zero) may be read.  Of a row of 16-bit
+// values of at least a chunk (`wide`) the last, partial chunk is read so that it ends with the row and shifted
+// into place: a load a value cost the tiles at a row's end more than all the rest.
 template <typename T>
-__device__ __forceinline__ u32x4 load_chunk(const T* p, int64_t n) {
+__device__ __forceinline__ u32x4 load_chunk(const T* p, int n, bool wide) {
   u32x4 v = {0, 0, 0, 0};
-  if (n >= kElems<T>) {
+  if (n <= 0) return v;
+  const int back = n < kElems<T> ? kElems<T> - n : 0;
+  if (sizeof(T) == 4 && back == 0) {
     v = load16_any(p, false);
-  } else if (n > 0) {
-    if constexpr (sizeof(T) == 2) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < n) v[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[i] << (16 * (i % 2));
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i < n) v[i] = reinterpret_cast<const uint32_t*>(p)[i];
+  } else if (sizeof(T) == 2 && wide) {
+    v = load16_any(p - back, false);
+    if (back) {
+      uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
+      const int bits = back * 8 * (int)sizeof(T);
+      lo = bits < 64 ? lo >> bits | hi << (64 - bits) : hi >> (bits - 64);
+      hi = bits < 64 ? hi >> bits : 0;
+      v = u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
     }
+  } else if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+      if (i < n) v[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[i] << (16 * (i % 2));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      if (i < n) v[i] = reinterpret_cast<const uint32_t*>(p)[i];
   }
   return v;
 }
@@ -121,18 +132,18 @@ struct Stage {
   static constexpr int PER = BM / kElems<T>;       // KR: chunks per k-row
   u32x4 r[CH];
 
-  // rows: KC valid rows of the tile; KR valid columns.  k0: the slab's first k, klim: the end of k.
-  __device__ __forceinline__ void load(const T* base, int64_t ld, int64_t rows, int64_t k0, int64_t klim) {
+  // rows: KC valid rows of the tile; KR valid columns.  k0: the slab's first k, klim: the end of k.  wide: a row
+  // in memory has a chunk at least.
+  __device__ __forceinline__ void load(const T* base, int64_t ld, int rows, int k0, int klim, bool wide) {
+    const bool whole = !KR && k0 + kSlab<T> <= klim;  // no row ends inside the slab
 #pragma unroll
     for (int q = 0; q < CH; ++q) {
       const int i = q * NTH + threadIdx.x;
-      if constexpr (KR) {
-        const int row = i / PER, c = (i % PER) * kElems<T>;
-        r[q] = load_chunk<T>(base + (k0 + row) * ld + c, k0 + row < klim ? rows - c : 0);
-      } else {
-        const int row = i / 8, c = (i % 8) * kElems<T>;
-        r[q] = load_chunk<T>(base + row * ld + k0 + c, row < rows ? klim - k0 - c : 0);
-      }
+      const int row = KR ? i / PER : i / 8, c = (KR ? i % PER : i % 8) * kElems<T>;
+      const T* p = base + (KR ? (int64_t)(k0 + row) * ld + c : row * ld + k0 + c);
+      const bool in = KR ? k0 + row < klim : row < rows;
+      if (whole) r[q] = in ? load16_any(p, false) : u32x4{0, 0, 0, 0};
+      else r[q] = load_chunk<T>(p, !in ? 0 : KR ? rows - c : klim - k0 - c, wide);
     }
   }
   __device__ __forceinline__ void store(u32x4* lds) const {
@@ -228,9 +239,41 @@ __device__ __forceinline__ void store4(TO* p, f32x4 v, int64_t n, bool vec) {
   }
 }
 
+// Tile t of tiles_i x tiles_j: four row tiles side by side through all column tiles, so that neighbours share
+// rows and columns.  Each XCD (every eighth workgroup) takes a run of neighbours, for its L2.
+__device__ __forceinline__ void band_tile(int t, int tiles_i, int tiles_j, int* ti, int* tj) {
+  const int band = t / (4 * tiles_j), high = min(4, tiles_i - 4 * band), in = t - band * 4 * tiles_j;
+  *ti = 4 * band + in % high;
+  *tj = in / high;
+}
+
+// Place `at` of this workgroup's XCD in n places split into eight runs; false past the run's end.
+__device__ __forceinline__ bool xcd_place(int n, int at, int* t) {
+  const int run = (n + 7) / 8;
+  *t = (blockIdx.x % 8) * run + at;
+  return at < run && *t < n;
+}
+
+// Row tiles in all.
+template <int BM>
+__device__ __forceinline__ int count_tiles(const int32_t* offsets, int E, int64_t R) {
+  const int lane = threadIdx.x & 63;
+  int n = 0;
+  for (int base = 0; base <= E; base += 64) {
+    const int e = base + lane;
+    if (e <= E) {
+      const Group g = group_of(offsets, e, E, R);
+      n += (int)((g.hi - g.lo + BM - 1) / BM);
+    }
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
+  return n;
+}
+
 // The tile's results, acc[i][j] of wave (wi, wj), to out rows of ldo: through LDS, so that whole rows of 16-byte
 // chunks leave the workgroup.  (Four neighbours a lane straight from the registers cost 20 us a tile of 256 x 256
-// bf16; 16384 x 4096 outputs at K = 64: 105 -> STOREUS us.)  Chunk c of row r waits at slot c ^ (r & 15).
+// bf16; 16384 x 4096 outputs at K = 64: 105 -> 41 us.)  Chunk c of row r waits at slot c ^ (r & 15).
 template <typename TO, int BM, int BN, int NTH, int CHUNKS, int FI, int FJ>
 __device__ __forceinline__ void store_tile(u32x4* lds, const f32x4 (&acc)[FI][FJ], int wi, int wj, TO* out, int64_t ldo,
                                            int rows, int cols) {
@@ -287,35 +330,38 @@ __global__ __launch_bounds__(256) void grouped_kernel(GroupedArgs a) {
   __shared__ u32x4 lds[2 * (BM + BN) * 8];
   const T *A = (const T*)a.A, *B = (const T*)a.B;
   T* out = (T*)a.out;
-  int64_t rows, k0 = 0, klim, i0 = 0;  // the tile's rows, the range of k, the first row
-  int64_t j0;
+  int64_t i0, j0;
+  int rows, k0 = 0, klim;  // the tile's rows, the range of k
   int e;
+  int t, ti, tj;
   if constexpr (ROLE == Role::kRows) {
-    const int ti = blockIdx.x / a.tiles_j;
-    j0 = (int64_t)(blockIdx.x % a.tiles_j) * BN;
-    const RowTile t = find_tile<BM>(a.offsets, a.E, a.R, ti);
-    if (t.e < 0) return;
-    e = t.e;
-    rows = t.hi - t.lo;
-    klim = t.e < a.E ? a.K : 0;
-    i0 = t.lo;
-    A += t.lo * a.lda;
+    const int tiles = __builtin_amdgcn_readfirstlane(count_tiles<BM>(a.offsets, a.E, a.R));
+    if (!xcd_place(tiles * a.tiles_j, blockIdx.x / 8, &t)) return;
+    band_tile(t, tiles, a.tiles_j, &ti, &tj);
+    const RowTile k = find_tile<BM>(a.offsets, a.E, a.R, ti);
+    if (k.e < 0) return;
+    e = k.e;
+    rows = (int)(k.hi - k.lo);
+    klim = k.e < a.E ? (int)a.K : 0;
+    i0 = k.lo;
+    A += i0 * a.lda;
     B += (int64_t)(e < a.E ? e : 0) * a.b_expert;
   } else {
-    const int per = a.tiles_i * a.tiles_j;
-    e = blockIdx.x / per;
-    if (e >= a.E) return;
-    const int t = blockIdx.x % per;
-    i0 = (int64_t)(t / a.tiles_j) * BM;
-    j0 = (int64_t)(t % a.tiles_j) * BN;
+    const int run = (a.tiles_i * a.tiles_j + 7) / 8, at = blockIdx.x / 8;
+    e = at / run;
+    if (!xcd_place(a.tiles_i * a.tiles_j, at - e * run, &t)) return;
+    band_tile(t, a.tiles_i, a.tiles_j, &ti, &tj);
+    i0 = (int64_t)ti * BM;
     const Group g = group_of(a.offsets, e, a.E, a.R);
-    rows = a.I - i0 < BM ? a.I - i0 : BM;
-    k0 = g.lo;
-    klim = g.hi;
+    rows = (int)(a.I - i0 < BM ? a.I - i0 : BM);
+    k0 = (int)g.lo;
+    klim = (int)g.hi;
     A += i0;
     out += (int64_t)e * a.o_expert;
   }
-  const int64_t cols = a.J - j0 < BN ? a.J - j0 : BN;
+  j0 = (int64_t)tj * BN;
+  const int cols = (int)(a.J - j0 < BN ? a.J - j0 : BN);
+  const bool wa = a.lda >= kElems<T>, wb = a.ldb >= kElems<T>;
   B += B_KR ? j0 : j0 * a.ldb;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wi = (wave >> 1) * (BM / 2), wj = (wave & 1) * (BN / 2);
@@ -327,8 +373,8 @@ __global__ __launch_bounds__(256) void grouped_kernel(GroupedArgs a) {
   Stage<T, A_KR, BM, NTH> sa;
   Stage<T, B_KR, BN, NTH> sb;
   if (k0 < klim) {
-    sa.load(A, a.lda, rows, k0, klim);
-    sb.load(B, a.ldb, cols, k0, klim);
+    sa.load(A, a.lda, rows, k0, klim, wa);
+    sb.load(B, a.ldb, cols, k0, klim, wb);
   }
   for (int s = 0; k0 < klim; k0 += kSlab<T>, s ^= 1) {
     u32x4 *la = lds + s * (BM + BN) * 8, *lb = la + BM * 8;
@@ -336,8 +382,8 @@ __global__ __launch_bounds__(256) void grouped_kernel(GroupedArgs a) {
     sb.store(lb);
     __syncthreads();
     if (k0 + kSlab<T> < klim) {
-      sa.load(A, a.lda, rows, k0 + kSlab<T>, klim);
-      sb.load(B, a.ldb, cols, k0 + kSlab<T>, klim);
+      sa.load(A, a.lda, rows, k0 + kSlab<T>, klim, wa);
+      sb.load(B, a.ldb, cols, k0 + kSlab<T>, klim, wb);
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -352,7 +398,7 @@ __global__ __launch_bounds__(256) void grouped_kernel(GroupedArgs a) {
       }
     }
   }
-  store_tile<T, BM, BN, NTH, 2 * (BM + BN) * 8>(lds, acc, wi, wj, out + i0 * a.ldo + j0, a.ldo, (int)rows, (int)cols);
+  store_tile<T, BM, BN, NTH, 2 * (BM + BN) * 8>(lds, acc, wi, wj, out + i0 * a.ldo + j0, a.ldo, rows, cols);
 }
 
 // ---------------------------------------------------------------------------
@@ -391,8 +437,7 @@ struct Direct {
         off[q] = (int)(row * ld) + (((i % 8) ^ (row & 7)) * 16);
       }
     }
-    const int lane = threadIdx.x;
-    col = ((lane % 8) ^ ((lane / 8) & 7)) * kElems<T>;
+    col = (((int)threadIdx.x % 8) ^ (((int)threadIdx.x / 8) & 7)) * kElems<T>;
     span = KR ? (int)(rows * (int64_t)sizeof(T)) : (int)((rows - 1) * ld + klim * (int64_t)sizeof(T));
   }
 
@@ -455,38 +500,6 @@ __device__ __forceinline__ void slab_ready() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
-}
-
-// Tile t of tiles_i x tiles_j: four row tiles side by side through all column tiles, so that neighbours share
-// rows and columns.  Each XCD (every eighth workgroup) takes a run of neighbours, for its L2.
-__device__ __forceinline__ void band_tile(int t, int tiles_i, int tiles_j, int* ti, int* tj) {
-  const int band = t / (4 * tiles_j), high = min(4, tiles_i - 4 * band), in = t - band * 4 * tiles_j;
-  *ti = 4 * band + in % high;
-  *tj = in / high;
-}
-
-// Place `at` of this workgroup's XCD in n places split into eight runs; false past the run's end.
-__device__ __forceinline__ bool xcd_place(int n, int at, int* t) {
-  const int run = (n + 7) / 8;
-  *t = (blockIdx.x % 8) * run + at;
-  return at < run && *t < n;
-}
-
-// Row tiles in all.
-template <int BM>
-__device__ __forceinline__ int count_tiles(const int32_t* offsets, int E, int64_t R) {
-  const int lane = threadIdx.x & 63;
-  int n = 0;
-  for (int base = 0; base <= E; base += 64) {
-    const int e = base + lane;
-    if (e <= E) {
-      const Group g = group_of(offsets, e, E, R);
-      n += (int)((g.hi - g.lo + BM - 1) / BM);
-    }
-  }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
-  return n;
 }
 
 // What a workgroup is to do: `rows` x `cols` results of expert e from (i0, j0) on, k from k0 to klim.
@@ -786,7 +799,6 @@ __global__ __launch_bounds__(64 * WAVES) void grouped_few_kernel(GroupedArgs a) 
 
   struct Unit {
     u32x4 a[FI][2], b[NJ][2];
-    uint32_t sa[FI], sb[NJ];
   };
   // Ranges as in the direct kernel: rows past the tile's by the buffer, k past the end by the lane.
   auto load = [&](Unit& u, int unit) {
@@ -797,7 +809,7 @@ __global__ __launch_bounds__(64 * WAVES) void grouped_few_kernel(GroupedArgs a) 
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         const int off = in ? (16 * j + (lane & 15)) * ldb + (4 * h + g) * 16 : kNowhere;
-        u.b[j][h] = __builtin_amdgcn_raw_buffer_load_b128(rb, off, unit * 128, 2);  // streamed
+        u.b[j][h] = __builtin_amdgcn_raw_buffer_load_b128(rb, off, unit * 128, 0);
       }
 #pragma unroll
       for (int i = 0; i < FI; ++i) {
@@ -805,38 +817,70 @@ __global__ __launch_bounds__(64 * WAVES) void grouped_few_kernel(GroupedArgs a) 
         u.a[i][h] = __builtin_amdgcn_raw_buffer_load_b128(ra, off, unit * 128, 0);
       }
     }
-    if constexpr (MX) {
-      const bool in = k + 32 * g < klim;  // a scale row's filling is not read
-#pragma unroll
-      for (int j = 0; j < NJ; ++j)
-        u.sb[j] = __builtin_amdgcn_raw_buffer_load_b8(rsb, in ? (16 * j + (lane & 15)) * ns + g : kNowhere, unit * 4, 0);
-#pragma unroll
-      for (int i = 0; i < FI; ++i)
-        u.sa[i] = __builtin_amdgcn_raw_buffer_load_b8(rsa, in ? (16 * i + (lane & 15)) * ns + g : kNowhere, unit * 4, 0);
-    }
-  };
-  auto multiply = [&](const Unit& u) {
-#pragma unroll
-    for (int i = 0; i < FI; ++i)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        if constexpr (MX) {
-          acc[i][j] = mma_mx(u.b[j][0], u.b[j][1], u.a[i][0], u.a[i][1], u.sb[j], u.sa[i], acc[i][j]);
-        } else {
-          acc[i][j] = mma<T>(u.b[j][0], u.a[i][0], acc[i][j]);
-          acc[i][j] = mma<T>(u.b[j][1], u.a[i][1], acc[i][j]);
-        }
-      }
   };
   const int units = (klim + kSlab<T> - 1) / kSlab<T>;
   Unit u[U];
+  if constexpr (MX) {
+    // A wave takes four units in a row, whose scales are 16 bytes of a row: one load for all of them (a byte
+    // a unit and lane: 120 -> 108 us for 128 rows over 32 experts, 4096 to 4096).
+    static_assert(U == 2, "units two ahead");
+    const int blocks = klim / 32;
+    auto scales = [&](__amdgpu_buffer_rsrc_t r, int row, int unit) -> u32x4 {
+      u32x4 v;
+      if (4 * unit + 16 <= ns) {
+        v = __builtin_amdgcn_raw_buffer_load_b128(r, row * ns, 4 * unit, 0);
+      } else {
 #pragma unroll
-  for (int n = 0; n < U; ++n) load(u[n], wave + n * WAVES);  // past the end: zeros
-  for (int at = wave; at < units; at += U * WAVES) {
+        for (int n = 0; n < 4; ++n)
+          v[n] = __builtin_amdgcn_raw_buffer_load_b32(r, 4 * (unit + n) < ns ? row * ns : kNowhere, 4 * (unit + n), 0);
+      }
+      return v;
+    };
+    auto first_unit = [&](int group) { return 4 * (wave + group * WAVES); };
+    const int groups = (units + 4 * WAVES - 1) / (4 * WAVES);  // of this wave; some past the end
+    u32x4 sb[NJ], sa[FI], next_b[NJ], next_a[FI];
+    auto load_scales = [&](int unit) {
 #pragma unroll
-    for (int n = 0; n < U; ++n) {
-      multiply(u[n]);
-      load(u[n], at + (U + n) * WAVES);
+      for (int j = 0; j < NJ; ++j) next_b[j] = scales(rsb, 16 * j + (lane & 15), unit);
+#pragma unroll
+      for (int i = 0; i < FI; ++i) next_a[i] = scales(rsa, 16 * i + (lane & 15), unit);
+    };
+    load_scales(first_unit(0));
+    load(u[0], first_unit(0));
+    load(u[1], first_unit(0) + 1);
+    for (int n = 0; n < groups; ++n) {
+      const int at = first_unit(n);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) sb[j] = next_b[j];
+#pragma unroll
+      for (int i = 0; i < FI; ++i) sa[i] = next_a[i];
+      load_scales(first_unit(n + 1));
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const bool block = 4 * (at + q) + g < blocks;  // a scale row's filling is not used
+#pragma unroll
+        for (int i = 0; i < FI; ++i)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j)
+            acc[i][j] = mma_mx(u[q % 2].b[j][0], u[q % 2].b[j][1], u[q % 2].a[i][0], u[q % 2].a[i][1],
+                               block ? sb[j][q] >> (8 * g) : 0, block ? sa[i][q] >> (8 * g) : 0, acc[i][j]);
+        load(u[q % 2], q < 2 ? at + q + 2 : first_unit(n + 1) + q - 2);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int n = 0; n < U; ++n) load(u[n], wave + n * WAVES);  // past the end: zeros
+    for (int at = wave; at < units; at += U * WAVES) {
+#pragma unroll
+      for (int n = 0; n < U; ++n) {
+#pragma unroll
+        for (int i = 0; i < FI; ++i)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) acc[i][j] = mma<T>(u[n].b[j][h], u[n].a[i][h], acc[i][j]);
+        load(u[n], at + (U + n) * WAVES);
+      }
     }
   }
 #pragma unroll

@@ -28,6 +28,35 @@ __device__ __forceinline__ float wave_total(float v) {
   return __uint_as_float(q[0]) + __uint_as_float(q[1]);
 }
 
+// The same in fp64: both halves of a value take the same lanes.
+template <class F>
+__device__ __forceinline__ double both_halves(double v, F&& f) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, (uint64_t)f((uint32_t)(b >> 32)) << 32 | f((uint32_t)b));
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double v) {
+  return both_halves(v, [](uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, false); });
+}
+__device__ __forceinline__ double wave_total(double v) {
+  v += dpp64<kDppQuadXor1>(v);
+  v += dpp64<kDppQuadXor2>(v);
+  v += dpp64<kDppRowRor8>(v);
+  v += dpp64<kDppRowRor4>(v);
+  v = both_halves(v, [](uint32_t x) { return __builtin_amdgcn_permlane16_swap(x, x, false, false)[0]; }) +
+      both_halves(v, [](uint32_t x) { return __builtin_amdgcn_permlane16_swap(x, x, false, false)[1]; });
+  return both_halves(v, [](uint32_t x) { return __builtin_amdgcn_permlane32_swap(x, x, false, false)[0]; }) +
+         both_halves(v, [](uint32_t x) { return __builtin_amdgcn_permlane32_swap(x, x, false, false)[1]; });
+}
+
+// 1 / sqrt(m) to fp64's precision but for a few units: fp32's and a Newton step where fp32 holds m.
+__device__ __forceinline__ double rsqrt64(double m) {
+  const float f = (float)m;
+  if (!(f > 1e-37f && f < 1e37f)) return 1. / sqrt(m);
+  const double r = (double)__builtin_amdgcn_rsqf(f);
+  return r * (1.5 - 0.5 * m * r * r);
+}
+
 // A team is a wave (WAVE: four rows a workgroup of 256) or the whole workgroup, of as many waves as the row
 // needs, 16 at most.
 constexpr int kTeamWaves = 16;
@@ -41,8 +70,8 @@ constexpr int kTeamRows = WAVE ? 4 : 1;
 
 // Sum over a team, in wave order.  `turn` alternates between the halves of `lds`, so one barrier per row
 // is enough.
-template <bool WAVE>
-__device__ __forceinline__ float team_sum(float v, float (&lds)[2][kTeamWaves], int turn) {
+template <bool WAVE, typename F>
+__device__ __forceinline__ F team_sum(F v, F (&lds)[2][kTeamWaves], int turn) {
   v = wave_total(v);
   if constexpr (!WAVE) {
     if ((threadIdx.x & 63) == 0) lds[turn][threadIdx.x >> 6] = v;
@@ -155,7 +184,11 @@ struct NormArgs {
 template <typename T, int W, bool RAG, bool WAVE, int NV, bool RES, bool MX>
 __global__ __launch_bounds__(WAVE ? 256 : 64 * kTeamWaves) void norm_fwd_kernel(NormArgs a) {
   constexpr int ROWS = kTeamRows<WAVE>;
-  __shared__ float lds[2][kTeamWaves];
+  // 8 bits: the sum and r in fp64, and y = h w r from fp32 products with their errors, rounded to fp32 once.  A
+  // block's scale doubles where its largest value passes a boundary, so an error of y there is one of the
+  // whole block.
+  using Sum = std::conditional_t<MX, double, float>;
+  __shared__ Sum lds[2][kTeamWaves];
   const int64_t D = a.D;
   const RowPart<W, RAG, WAVE, NV> p((uint32_t)D);
   float w[NV][W];
@@ -167,7 +200,7 @@ __global__ __launch_bounds__(WAVE ? 256 : 64 * kTeamWaves) void norm_fwd_kernel(
     load_row<T, W, RAG, NV, true>((const T*)a.x + row * D, D, p, xf);
     if constexpr (RES) load_row<T, W, RAG, NV, true>((const T*)a.res + row * D, D, p, rf);
     float h[NV][W];
-    float ss = 0.f;
+    Sum ss = 0;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       if (!p.ok[v]) {
@@ -185,17 +218,28 @@ __global__ __launch_bounds__(WAVE ? 256 : 64 * kTeamWaves) void norm_fwd_kernel(
         st_from<T, W, true>(hs, p.col[v], h[v], p.skip[v]);
       }
 #pragma unroll
-      for (int e = 0; e < W; ++e) ss += RAG && (uint32_t)e < p.skip[v] ? 0.f : h[v][e] * h[v][e];
+      for (int e = 0; e < W; ++e) ss += RAG && (uint32_t)e < p.skip[v] ? (Sum)0 : (Sum)h[v][e] * (Sum)h[v][e];
     }
     ss = team_sum<WAVE>(ss, lds, turn);
     turn ^= 1;
-    const float r = 1.f / sqrtf(ss * inv_d + a.eps);
-    if (a.rstd && team_lane<WAVE>() == 0) a.rstd[row] = r;
+    Sum r;
+    if constexpr (MX) r = rsqrt64(ss / (double)D + (double)a.eps);
+    else r = 1.f / sqrtf(ss * inv_d + a.eps);
+    if (a.rstd && team_lane<WAVE>() == 0) a.rstd[row] = (float)r;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       float y[W];
 #pragma unroll
-      for (int e = 0; e < W; ++e) y[e] = h[v][e] * r * w[v][e];
+      for (int e = 0; e < W; ++e) {
+        if constexpr (MX) {
+          const float hi = (float)r, lo = (float)(r - (double)hi);
+          const float p = h[v][e] * w[v][e], err = fmaf(h[v][e], w[v][e], -p);
+          const float q = p * hi, rest = fmaf(p, lo, fmaf(err, hi, fmaf(p, hi, -q)));
+          y[e] = q + (rest == rest ? rest : 0.f);  // no error term for what is not finite
+        } else {
+          y[e] = h[v][e] * r * w[v][e];
+        }
+      }
       if constexpr (MX) {
         const uint32_t s = mx_scale(block_amax(y));
         uint32_t q[W / 4];
