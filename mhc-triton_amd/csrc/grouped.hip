@@ -43,11 +43,11 @@ static int launch_direct(GroupedArgs a, const char* who, hipStream_t st) {
   return hip_status(hipGetLastError(), who);
 }
 
-template <typename T, typename TO, int FI, int NJ, int WAVES, int U>
+template <typename T, typename TO, int FI, int NJ, int WAVES, int U, bool CHUNKS>
 static int launch_few(GroupedArgs a, const char* who, hipStream_t st) {
   const int64_t tiles = set_tiles<Role::kRows, 16 * FI, 16 * NJ>(a);
   if (int rc = check_tiles(who, tiles, 64 * WAVES)) return rc;
-  grouped_few_kernel<T, TO, FI, NJ, WAVES, U><<<dim3((unsigned)tiles), 64 * WAVES, 0, st>>>(a);
+  grouped_few_kernel<T, TO, FI, NJ, WAVES, U, CHUNKS><<<dim3((unsigned)tiles), 64 * WAVES, 0, st>>>(a);
   return hip_status(hipGetLastError(), who);
 }
 
@@ -80,7 +80,7 @@ static int launch_grouped(GroupedArgs a, const char* who, hipStream_t st) {
   const int cus = num_cus();
   if (chunks) {
     if constexpr (!A_KR && !B_KR)
-      if (a.R <= 8 * (int64_t)a.E && (!MX || a.K >= 2048)) return launch_few<T, TO, 1, 2, 4, 2>(a, who, st);
+      if (a.R <= 8 * (int64_t)a.E && (!MX || a.K >= 2048)) return launch_few<T, TO, 1, 2, 4, 2, true>(a, who, st);
     if (likely_tiles<ROLE, 256, 256>(a) >= cus / 2)
       return launch_direct<T, TO, A_KR, B_KR, 256, 256, 2, 4, 2, ROLE>(a, who, st);
     if (likely_tiles<ROLE, 128, 128>(a) >= cus) return launch_direct<T, TO, A_KR, B_KR, 128, 128, 2, 2, 2, ROLE>(a, who, st);
@@ -88,6 +88,8 @@ static int launch_grouped(GroupedArgs a, const char* who, hipStream_t st) {
     if constexpr (!MX) return launch_direct<T, TO, A_KR, B_KR, 32, 32, 2, 2, 4, ROLE>(a, who, st);
   }
   if constexpr (!MX) {
+    if constexpr (!A_KR && !B_KR)
+      if (a.R <= 8 * (int64_t)a.E) return launch_few<T, TO, 1, 2, 4, 2, false>(a, who, st);
     if (likely_tiles<ROLE, 128, 128>(a) >= 2 * cus) return launch_general<T, A_KR, B_KR, 128, 128, ROLE>(a, who, st);
     return launch_general<T, A_KR, B_KR, 64, 64, ROLE>(a, who, st);
   }

@@ -114,6 +114,25 @@ __device__ __forceinline__ u32x4 load_chunk(const T* p, int n, bool wide) {
   return v;
 }
 
+// The same in two steps, for rows of at least a chunk.  The load is the same for every lane, so that the compiler
+// can keep count of the loads in flight: a row's last, partial chunk is read so that it ends with the row, one with nothing to read from
+// `safe`.  chunk_fix, once it has arrived, shifts the former into place and clears the latter.
+template <typename T>
+__device__ __forceinline__ u32x4 chunk_load(const T* p, int n, const T* safe) {
+  const int back = n < kElems<T> ? kElems<T> - n : 0;
+  return load16_any(n > 0 ? p - back : safe, false);
+}
+template <typename T>
+__device__ __forceinline__ u32x4 chunk_fix(u32x4 v, int n) {
+  const int bits = n >= kElems<T> ? 0 : (kElems<T> - max(n, 1)) * 8 * (int)sizeof(T);
+  uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
+  const uint64_t carry = bits == 0 ? 0 : hi << (64 - (bits & 63)) % 64;  // bits = 64: lo is replaced below
+  lo = bits < 64 ? lo >> (bits & 63) | carry : hi >> (bits & 63);
+  hi = bits < 64 ? hi >> (bits & 63) : 0;
+  if (n <= 0) lo = hi = 0;
+  return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+}
+
 // Slot of 16-byte chunk c of k-row r (KR, PER chunks a row; its own inverse).  16 bits: the eight rows
 // that half a wave reads 32 bytes each from (four by the lanes, two by the groups) fall on different banks;
 // 32 bits: the four rows of 64 bytes.
@@ -125,38 +144,44 @@ __device__ __forceinline__ int kr_slot(int r, int c) {
   else return c ^ (2 * ((r >> 3) & 1));  // four do
 }
 
-// Global -> registers -> LDS for one slab of one operand (NTH threads).
+// Global -> registers -> LDS for one slab of one operand (NTH threads).  16-bit k-rows are loaded in two steps
+// (8000 x 2001 x 3001 bf16: dx 260 -> 200 us, dw 297 -> 204), the others with what is past an end left out: there
+// loads of rows that are none cost more than the branches (the same product's fwd 161 against 183).
 template <typename T, bool KR, int BM, int NTH>
 struct Stage {
   static constexpr int CH = BM * 8 / NTH;          // chunks per thread
   static constexpr int PER = BM / kElems<T>;       // KR: chunks per k-row
+  static constexpr bool TWO = KR && sizeof(T) == 2;
   u32x4 r[CH];
 
-  // rows: KC valid rows of the tile; KR valid columns.  k0: the slab's first k, klim: the end of k.  wide: a row
-  // in memory has a chunk at least.
+  __device__ __forceinline__ static int row(int q) { return (q * NTH + (int)threadIdx.x) / (KR ? PER : 8); }
+  __device__ __forceinline__ static int chunk(int q) { return (q * NTH + (int)threadIdx.x) % (KR ? PER : 8); }
+  // Values of chunk q that exist.  rows: KC valid rows of the tile; KR valid columns.
+  __device__ __forceinline__ static int left(int q, int rows, int k0, int klim) {
+    const int c = chunk(q) * kElems<T>;
+    if constexpr (KR) return k0 + row(q) < klim ? rows - c : 0;
+    else return row(q) < rows ? klim - k0 - c : 0;
+  }
+
+  // wide: a row in memory has a chunk at least.
   __device__ __forceinline__ void load(const T* base, int64_t ld, int rows, int k0, int klim, bool wide) {
     const bool whole = !KR && k0 + kSlab<T> <= klim;  // no row ends inside the slab
 #pragma unroll
     for (int q = 0; q < CH; ++q) {
-      const int i = q * NTH + threadIdx.x;
-      const int row = KR ? i / PER : i / 8, c = (KR ? i % PER : i % 8) * kElems<T>;
-      const T* p = base + (KR ? (int64_t)(k0 + row) * ld + c : row * ld + k0 + c);
-      const bool in = KR ? k0 + row < klim : row < rows;
-      if (whole) r[q] = in ? load16_any(p, false) : u32x4{0, 0, 0, 0};
-      else r[q] = load_chunk<T>(p, !in ? 0 : KR ? rows - c : klim - k0 - c, wide);
+      const int c = chunk(q) * kElems<T>, n = left(q, rows, k0, klim);
+      const T* p = base + (KR ? (int64_t)(k0 + row(q)) * ld + c : row(q) * ld + k0 + c);
+      if (TWO && wide) r[q] = chunk_load<T>(p, n, base + (int64_t)k0 * ld + min(0, rows - kElems<T>));
+      else if (whole) r[q] = row(q) < rows ? load16_any(p, false) : u32x4{0, 0, 0, 0};
+      else r[q] = load_chunk<T>(p, n, wide);
     }
   }
-  __device__ __forceinline__ void store(u32x4* lds) const {
+  __device__ __forceinline__ void store(u32x4* lds, int rows, int k0, int klim, bool wide) const {
+    const bool ends = TWO && wide && (rows < BM || k0 + kSlab<T> > klim);  // the operand, or k, ends inside the slab
 #pragma unroll
     for (int q = 0; q < CH; ++q) {
-      const int i = q * NTH + threadIdx.x;
-      if constexpr (KR) {
-        const int row = i / PER;
-        lds[row * PER + kr_slot<T, PER>(row, i % PER)] = r[q];
-      } else {
-        const int row = i / 8;
-        lds[row * 8 + ((i % 8) ^ (row & 7))] = r[q];
-      }
+      const u32x4 v = ends ? chunk_fix<T>(r[q], left(q, rows, k0, klim)) : r[q];
+      if constexpr (KR) lds[row(q) * PER + kr_slot<T, PER>(row(q), chunk(q))] = v;
+      else lds[row(q) * 8 + (chunk(q) ^ (row(q) & 7))] = v;
     }
   }
 };
@@ -322,7 +347,7 @@ __device__ __forceinline__ void store_tile(u32x4* lds, const f32x4 (&acc)[FI][FJ
 }
 
 // The general kernel: any size and alignment, operands staged through registers (unaligned 16-byte loads,
-// single values at a row's end).  256 threads, four waves of a quarter of the tile each; the next slab's
+// single values at a short row's end).  256 threads, four waves of a quarter of the tile each; the next slab's
 // loads are in flight while one is multiplied, and two slabs of LDS make one barrier a slab enough.
 template <typename T, bool A_KR, bool B_KR, int BM, int BN, Role ROLE>
 __global__ __launch_bounds__(256) void grouped_kernel(GroupedArgs a) {
@@ -378,8 +403,8 @@ __global__ __launch_bounds__(256) void grouped_kernel(GroupedArgs a) {
   }
   for (int s = 0; k0 < klim; k0 += kSlab<T>, s ^= 1) {
     u32x4 *la = lds + s * (BM + BN) * 8, *lb = la + BM * 8;
-    sa.store(la);
-    sb.store(lb);
+    sa.store(la, rows, k0, klim, wa);
+    sb.store(lb, cols, k0, klim, wb);
     __syncthreads();
     if (k0 + kSlab<T> < klim) {
       sa.load(A, a.lda, rows, k0 + kSlab<T>, klim, wa);
@@ -766,7 +791,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void grouped_direct_kernel(Grouped
 // row (a unit).  The waves of a workgroup take every WAVES-th unit, each with U of them in flight, and
 // add up through LDS in wave order.
 // ---------------------------------------------------------------------------
-template <typename T, typename TO, int FI, int NJ, int WAVES, int U>
+template <typename T, typename TO, int FI, int NJ, int WAVES, int U, bool CHUNKS>
 __global__ __launch_bounds__(64 * WAVES) void grouped_few_kernel(GroupedArgs a) {
   constexpr bool MX = __is_same(T, Mx);
   __shared__ f32x4 sum[WAVES][FI * NJ][64];
@@ -800,21 +825,25 @@ __global__ __launch_bounds__(64 * WAVES) void grouped_few_kernel(GroupedArgs a) 
   struct Unit {
     u32x4 a[FI][2], b[NJ][2];
   };
-  // Ranges as in the direct kernel: rows past the tile's by the buffer, k past the end by the lane.
+  // Whole chunks: ranges as in the direct kernel, rows past the tile's by the buffer, k past the end by the lane.
+  // Otherwise the general kernel's loads.
   auto load = [&](Unit& u, int unit) {
     const int k = unit * kSlab<T>;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const bool in = k + (4 * h + g) * kElems<T> < klim;
+      const int c = k + (4 * h + g) * kElems<T>;
+      const bool in = c < klim;
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        const int off = in ? (16 * j + (lane & 15)) * ldb + (4 * h + g) * 16 : kNowhere;
-        u.b[j][h] = __builtin_amdgcn_raw_buffer_load_b128(rb, off, unit * 128, 0);
+        const int row = 16 * j + (lane & 15);
+        if constexpr (CHUNKS) u.b[j][h] = __builtin_amdgcn_raw_buffer_load_b128(rb, in ? row * ldb + (4 * h + g) * 16 : kNowhere, unit * 128, 0);
+        else u.b[j][h] = load_chunk<T>((const T*)a.B + (wrow + row) * a.ldb + c, row < cols ? klim - c : 0, klim >= kElems<T>);
       }
 #pragma unroll
       for (int i = 0; i < FI; ++i) {
-        const int off = in ? (16 * i + (lane & 15)) * lda + (4 * h + g) * 16 : kNowhere;
-        u.a[i][h] = __builtin_amdgcn_raw_buffer_load_b128(ra, off, unit * 128, 0);
+        const int row = 16 * i + (lane & 15);
+        if constexpr (CHUNKS) u.a[i][h] = __builtin_amdgcn_raw_buffer_load_b128(ra, in ? row * lda + (4 * h + g) * 16 : kNowhere, unit * 128, 0);
+        else u.a[i][h] = load_chunk<T>((const T*)a.A + (i0 + row) * a.lda + c, row < rows ? klim - c : 0, klim >= kElems<T>);
       }
     }
   };
