@@ -388,7 +388,7 @@ __global__ __launch_bounds__(256) void grouped_kernel(GroupedArgs a) {
   const int cols = (int)(a.J - j0 < BN ? a.J - j0 : BN);
   const bool wa = a.lda >= kElems<T>, wb = a.ldb >= kElems<T>;
   B += B_KR ? j0 : j0 * a.ldb;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wave = threadIdx.x >> 6;
   const int wi = (wave >> 1) * (BM / 2), wj = (wave & 1) * (BN / 2);
   f32x4 acc[FI][FJ];
 #pragma unroll

@@ -264,14 +264,38 @@ struct NormBwdArgs {
   const void *dy, *h, *dh;  // dh may be null
   const float *w, *rstd;
   void* dx;                 // may be null
-  float* part;              // [gridDim.x][D] partial weight gradients; null without one
+  float* part;              // [row_blocks][D] partial weight gradients; null without one
+  float* dw;                // few rows: the weight gradient itself, by the workgroups past row_blocks
   int64_t R, D;
+  uint32_t row_blocks;
 };
+
+// The weight gradient of few rows: 64 columns a workgroup, its waves a share of the rows each.
+constexpr int64_t kFewRows = 64;
+
+template <typename T>
+__device__ __forceinline__ void few_rows_dw(const NormBwdArgs& a) {
+  __shared__ double sum[kTeamWaves][64];
+  const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int64_t d = (int64_t)(blockIdx.x - a.row_blocks) * 64 + (threadIdx.x & 63);
+  double s = 0.;
+  if (d < a.D) {
+#pragma unroll 4
+    for (int64_t r = wave; r < a.R; r += waves)
+      s += (double)(to_f32(((const T*)a.dy)[r * a.D + d]) * (to_f32(((const T*)a.h)[r * a.D + d]) * a.rstd[r]));
+  }
+  sum[wave][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (wave || d >= a.D) return;
+  for (int i = 1; i < waves; ++i) s += sum[i][threadIdx.x];
+  a.dw[d] = (float)s;
+}
 
 template <typename T, int W, bool RAG, bool WAVE, int NV, bool DH>
 __global__ __launch_bounds__(WAVE ? 256 : 64 * kTeamWaves) void norm_bwd_kernel(NormBwdArgs a) {
   constexpr int ROWS = kTeamRows<WAVE>;
   __shared__ float lds[2][kTeamWaves];
+  if (blockIdx.x >= a.row_blocks) return few_rows_dw<T>(a);
   const int64_t D = a.D;
   const RowPart<W, RAG, WAVE, NV> p((uint32_t)D);
   float w[NV][W], dw[NV][W];
@@ -282,7 +306,7 @@ __global__ __launch_bounds__(WAVE ? 256 : 64 * kTeamWaves) void norm_bwd_kernel(
     for (int e = 0; e < W; ++e) dw[v][e] = 0.f;
   const float inv_d = 1.f / (float)D;
   int turn = 0;
-  const int64_t step = (int64_t)gridDim.x * ROWS;
+  const int64_t step = (int64_t)a.row_blocks * ROWS;
   int64_t row = (int64_t)blockIdx.x * ROWS + (WAVE ? threadIdx.x / 64 : 0);
   Frag<T, W> yf[NV], hf[NV], gf[NV];
   float r = 0.f;
@@ -536,7 +560,7 @@ extern "C" int mhc_rms_norm_mx_forward(const void* x, const void* residual, int 
 }
 
 extern "C" size_t mhc_rms_norm_backward_workspace_bytes(int64_t R, int64_t D) {
-  if (R <= 0 || D <= 0) return 0;
+  if (R <= kFewRows || D <= 0) return 0;
   return (size_t)(norm_blocks(R, kBwdRows, kNormBwdBlocks) * D) * sizeof(float);
 }
 
@@ -554,7 +578,10 @@ extern "C" int mhc_rms_norm_backward(const void* dy, const void* h, const void* 
     if (int rc = check_workspace("rms_norm_backward", workspace, workspace_bytes,
                                  mhc_rms_norm_backward_workspace_bytes(R, D)))
       return rc;
-  const NormBwdArgs a{dy, h, dh, weight, rstd, dx, dweight ? (float*)workspace : nullptr, R, D};
+  // Few rows: the weight gradient in the same launch, without partials (64 x 4096 bf16 6.7 -> 3.5 us, and a
+  // launch less on the host).
+  const bool few = dweight && R <= kFewRows;
+  NormBwdArgs a{dy, h, dh, weight, rstd, dx, dweight && !few ? (float*)workspace : nullptr, few ? dweight : nullptr, R, D, 0};
   unsigned blocks = 0;
   const int rc = MHC_DISPATCH_DTYPE(dtype, [&] {
     return with_row_width<Vec<T>::N>(D, {dy, h, dh, dx}, [&](auto wc, auto rag) {
@@ -564,13 +591,15 @@ extern "C" int mhc_rms_norm_backward(const void* dy, const void* h, const void* 
         constexpr bool WAVE = decltype(team)::WAVE;
         constexpr int NV = decltype(team)::NV;
         blocks = (unsigned)norm_blocks(R, kBwdRows * kTeamRows<WAVE>, WAVE ? kNormBwdBlocks / 2 : kNormBwdBlocks);
-        if (dh) norm_bwd_kernel<T, W, RAG, WAVE, NV, true><<<blocks, threads, 0, st>>>(a);
-        else norm_bwd_kernel<T, W, RAG, WAVE, NV, false><<<blocks, threads, 0, st>>>(a);
+        a.row_blocks = !few ? blocks : dx ? (unsigned)norm_blocks(R, kTeamRows<WAVE>, kNormBwdBlocks) : 0;
+        const dim3 grid(a.row_blocks + (few ? (unsigned)((D + 63) / 64) : 0));
+        if (dh) norm_bwd_kernel<T, W, RAG, WAVE, NV, true><<<grid, threads, 0, st>>>(a);
+        else norm_bwd_kernel<T, W, RAG, WAVE, NV, false><<<grid, threads, 0, st>>>(a);
         return hip_status(hipGetLastError(), "rms_norm_backward launch");
       });
     });
   });
-  if (rc || !dweight) return rc;
+  if (rc || !dweight || few) return rc;
   norm_dw_reduce_kernel<<<dim3((unsigned)((D + kDwCols - 1) / kDwCols)), kDwCols * kDwGroups, 0, st>>>(a.part, dweight, (int)blocks, D);
   return hip_status(hipGetLastError(), "rms_norm_backward reduce launch");
 }

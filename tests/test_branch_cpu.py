@@ -112,10 +112,10 @@ def test_abi_refusals_before_any_device_work():
     assert lib.mhc_rms_norm_forward(16, None, 9, None, 16, None, None, 4, 64, 1e-6, None) == 2
     assert lib.mhc_rms_norm_mx_forward(16, None, 1, None, 16, 16, None, 4, 48, 1e-6, None) == 1
     assert lib.mhc_rms_norm_mx_forward(24, None, 1, None, 16, 16, None, 4, 64, 1e-6, None) == 1  # alignment
-    assert lib.mhc_rms_norm_backward(16, 16, None, 1, None, 16, 16, 16, 4, 64, None, 0, None) == 3
-    need = lib.mhc_rms_norm_backward_workspace_bytes(4, 64)
-    assert need == 2 * 64 * 4 and lib.mhc_rms_norm_backward_workspace_bytes(0, 64) == 0
-    assert lib.mhc_rms_norm_backward(16, 16, None, 1, None, 16, 16, 16, 4, 64, 256, need - 1, None) == 3
+    assert lib.mhc_rms_norm_backward(16, 16, None, 1, None, 16, 16, 16, 100, 64, None, 0, None) == 3
+    need = lib.mhc_rms_norm_backward_workspace_bytes(100, 64)
+    assert need == 50 * 64 * 4 and lib.mhc_rms_norm_backward_workspace_bytes(64, 64) == 0
+    assert lib.mhc_rms_norm_backward(16, 16, None, 1, None, 16, 16, 16, 100, 64, 256, need - 1, None) == 3
     assert lib.mhc_quantize_mx(16, 1, 16, 16, 4, 33, None) == 1
     assert lib.mhc_dropout(None, None, 1, None, -1, 0.1, 0, 0, None, None, None) == 1
     assert lib.mhc_dropout(None, None, 1, None, 8, 0.1, 0, 0, None, None, None) == 1
