@@ -10,6 +10,7 @@
 //
 // Bound by the bus (two or three tensors), as long as the generator stays below it: its twenty 32x32-bit
 // products per call are quarter rate, which is why a call serves eight elements (halves) and not four.
+// 16384 x 4096 bf16: with a residual 62 us (6.4 TB/s), a gradient 44.5 us (6.0 TB/s).
 #include "stream_kernels.hpp"
 
 namespace mhc {
