@@ -71,8 +71,10 @@ static int64_t likely_tiles(const GroupedArgs& a) {
 // 16 it reads the rows too often (us for 1 / 8 / 16 / 32 rows an expert, registers against tiles: 32 experts of
 // 2048 to 4096 bf16 100 / 111 / 131 / 211 against 133; 8 bits 56 / 64 / 75 / 123 against 74 to 78).  In 8 bits its
 // four waves need four units of four slabs: K = 1024 over 64 experts 38 against 32 us.
-// Tiles: the largest of 256, 128, 64 and 32 that give the CUs enough of them (half of the CUs in 256s, which go in
-// quarters then).  The general kernel takes what is not whole aligned 16-byte chunks.
+// Tiles: the largest of 256, 128, 64 and 32 that gives every CU one, 256 only where experts have as many rows (bf16
+// fwd / dx / dw, 256 against 128: 4096 rows of 4096 to 4096 over 8 experts 118 / 126 / 169 and 154 / 167 / 197 us, 8192 of
+// 1024 to 1024 over 8, half a tile a CU, 29 / 37 / 38 and 25 / 22 / 23, 4096 of 2048 to 1024 over 32 47 / 32 / 50 and
+// 27 / 28 / 45).  The general kernel takes what is not whole aligned 16-byte chunks.
 template <typename T, typename TO, bool A_KR, bool B_KR, Role ROLE>
 static int launch_grouped(GroupedArgs a, const char* who, hipStream_t st) {
   constexpr bool MX = __is_same(T, Mx);
@@ -81,7 +83,7 @@ static int launch_grouped(GroupedArgs a, const char* who, hipStream_t st) {
   if (chunks) {
     if constexpr (!A_KR && !B_KR)
       if (a.R <= 8 * (int64_t)a.E && (!MX || a.K >= 2048)) return launch_few<T, TO, 1, 2, 4, 2, true>(a, who, st);
-    if (likely_tiles<ROLE, 256, 256>(a) >= cus / 2)
+    if (likely_tiles<ROLE, 256, 256>(a) >= cus && (ROLE == Role::kWeight || a.R >= 256 * (int64_t)a.E))
       return launch_direct<T, TO, A_KR, B_KR, 256, 256, 2, 4, 2, ROLE>(a, who, st);
     if (likely_tiles<ROLE, 128, 128>(a) >= cus) return launch_direct<T, TO, A_KR, B_KR, 128, 128, 2, 2, 2, ROLE>(a, who, st);
     if (MX || likely_tiles<ROLE, 64, 64>(a) >= cus) return launch_direct<T, TO, A_KR, B_KR, 64, 64, 2, 2, 4, ROLE>(a, who, st);
