@@ -682,7 +682,7 @@ __device__ __forceinline__ void direct_tile(const GroupedArgs& a, const Task& ta
           __builtin_amdgcn_sched_group_barrier(0x008, MM / DS, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);

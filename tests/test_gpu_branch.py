@@ -366,6 +366,8 @@ def offsets_of(split, R, E, dtype=torch.int32):
     (700, 640, 384, 130, "even"), (1024, 1024, 512, 4, "empty ends"), (90, 2048, 264, 6, "empty ends"),
     (2000, 512, 768, 2, "one has all"), (300, 136, 2056, 4, "even"), (1100, 1032, 1048, 5, "empty ends"),
     (2100, 1032, 2056, 5, "empty ends"), (4100, 264, 2048, 3, "one has all"), (1500, 1026, 1030, 6, "even"),
+    (4100, 264, 4104, 3, "even"), (4100, 4104, 264, 3, "empty ends"), (600, 2056, 2312, 3, "even"),
+    (4360, 136, 4104, 16, "single rows"),
 ])
 def test_grouped_matmul(R, K, N, E, split, dtype):
     dt = DT[dtype]
@@ -423,6 +425,30 @@ def test_grouped_matmul_rows_of_other_experts_do_not_leak(dtype):
     assert torch.isnan(y1[50:90]).all() and torch.isnan(g1[1][1]).all()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_grouped_matmul_large_tiles_do_not_leak(dtype):
+    """The same where experts end inside the largest tiles, one of them has no rows and K ends inside a slab."""
+    dt, (R, K, N, E) = DT[dtype], (2500, 2056, 4104, 4)
+    ends = [1000, 1000, 1277, 2300]
+    off = torch.tensor(ends, dtype=torch.int32, device=DEV)
+    x, w, dy = rand(R, K, seed=1, dtype=dt), rand(E, N, K, seed=2, dtype=dt), rand(R, N, seed=3, dtype=dt)
+    clean = [t.clone().requires_grad_() for t in (x, w)]
+    y0 = branch.grouped_matmul(*clean, off)
+    g0 = torch.autograd.grad(y0, clean, dy)
+    for t in (x, dy):
+        t[1000:1277] = float("nan")
+        t[2300:] = float("inf")
+    w[1:3] = float("inf")
+    dirty = [t.clone().requires_grad_() for t in (x, w)]
+    y1 = branch.grouped_matmul(*dirty, off)
+    g1 = torch.autograd.grad(y1, dirty, dy)
+    for a, b in ((y0, y1), (g0[0], g1[0])):
+        assert torch.equal(a[:1000], b[:1000]) and torch.equal(a[1277:2300], b[1277:2300])
+        assert torch.isnan(b[1000:1277]).all() and not b[2300:].any()
+    assert torch.equal(g0[1][[0, 3]], g1[1][[0, 3]])
+    assert not g1[1][1].any() and torch.isnan(g1[1][2]).all()
+
+
 def test_grouped_matmul_offsets_out_of_range_are_clamped():
     x, w = rand(20, 32, seed=1), rand(3, 16, 32, seed=2)
     want = branch.grouped_matmul(x, w, torch.tensor([0, 20, 20], dtype=torch.int32, device=DEV))
@@ -475,6 +501,7 @@ def test_grouped_matmul_strides_alignment_and_repeatability():
     (1, 32, 8, 1, "even"), (3, 96, 33, 2, "even"), (64, 128, 128, 8, "even"), (129, 160, 257, 5, "empty ends"),
     (40, 1024, 64, 40, "single rows"), (600, 512, 384, 3, "one has all"), (16, 4096, 72, 4, "even"),
     (77, 64, 100, 3, "none"), (900, 416, 1100, 5, "empty ends"), (4200, 288, 2056, 3, "empty ends"),
+    (4200, 288, 4104, 3, "empty ends"),
 ])
 def test_grouped_matmul_mx(R, K, N, E, split, out):
     x, w = rand(R, K, seed=1), rand(E, N, K, seed=2, scale=K ** -0.5)
@@ -488,6 +515,34 @@ def test_grouped_matmul_mx(R, K, N, E, split, out):
     ref, size = O.grouped_matmul(mx_values(q, s), mx_values(wq, ws), off.tolist())
     assert y.dtype == DT[out]
     close(y, ref, size, (K + 8) * 2.0 ** -23, "y")
+
+
+def test_grouped_matmul_mx_one_slab():
+    """The largest tiles at the shortest K, 18 million results.  The instruction cuts each of a group's 16 products,
+    but the largest, at 2^-13 of that one: 15 * 2^-13 of the groups' largest products, which the bound of the test above
+    leaves out (34 of these results are past it).  Bit by bit the tiles of every size agree."""
+    R, K, N, E = 4200, 128, 4360, 3
+    x, w = rand(R, K, seed=1), rand(E, N, K, seed=2, scale=K ** -0.5)
+    x *= torch.exp2((torch.arange(K, device=DEV) // 32) % 7 - 3.0)
+    w *= torch.exp2((torch.arange(N, device=DEV) % 5) - 2.0)[None, :, None]
+    q, s = branch.quantize_mx(x)
+    wq, ws = branch.quantize_mx(w)
+    y = branch.grouped_matmul_mx(q, s, wq, ws, offsets_of("one has all", R, E), out_dtype=torch.bfloat16)
+    for rows in (40, 600):  # 64-tiles and 128-tiles
+        for i in range(0, R, rows):
+            c = slice(i, i + rows)
+            part = branch.grouped_matmul_mx(q[c], s[c], wq[1:2], ws[1:2], offsets_of("even", rows, 1), out_dtype=torch.bfloat16)
+            assert torch.equal(part, y[c])
+    xv, wv = torch.from_numpy(mx_values(q, s)).to(DEV), torch.from_numpy(mx_values(wq, ws)).to(DEV)[1]
+    cut = torch.zeros(R, N, dtype=torch.float64, device=DEV)
+    for g in range(0, K, 16):
+        largest = torch.zeros_like(cut)
+        for k in range(g, g + 16):
+            largest = torch.maximum(largest, xv[:, k, None].abs() * wv[None, :, k].abs())
+        cut += 15 * 2.0 ** -13 * largest
+    ref = xv @ wv.T
+    allowed = cut + (K + 8) * 2.0 ** -23 * (xv.abs() @ wv.abs().T) + 1.01 * HALF_ULP[torch.bfloat16] * ref.abs()
+    assert bool(((y.double() - ref).abs() <= allowed).all())
 
 
 def test_grouped_matmul_mx_special_scales():
