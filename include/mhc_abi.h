@@ -391,8 +391,8 @@ int mhc_dropout(const void* x, const void* residual, int dtype, void* y, int64_t
                 int64_t* used, mhc_stream_t stream);
 
 /* Products grouped by expert.  Rows [offsets[e-1], offsets[e]) of the R rows belong
- * to expert e (offsets[-1] = 0; offsets [E] i32 on the device, not decreasing; it
- * is clamped to [0, R]).  Rows past offsets[E-1] belong to none: their outputs are
+ * to expert e (offsets[-1] = 0; offsets [E] i32 on the device, not decreasing: they
+ * count clamped to [0, R] and as their running maximum).  Rows past offsets[E-1] belong to none: their outputs are
  * zeros.  x [R,K], dy [R,N], weight [E,N,K], all in `dtype`; sums in f32.
  * Widths up to 2^20, R <= 2^31 - 4096, E <= 4096.
  *   forward          y[m,:]  = weight[e] x[m,:]

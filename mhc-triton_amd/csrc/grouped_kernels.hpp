@@ -36,16 +36,36 @@ struct GroupedArgs {
   int E, tiles_i, tiles_j, cus;
 };
 
-// Rows of one expert, clamped to [0, R) whatever the offsets hold.
+// Rows of one expert.  Whatever the offsets hold, they count clamped to [0, R] and as their running maximum, so that
+// the experts' rows never overlap, leave none out and fit the launch's tiles.
 struct Group {
   int64_t lo, hi;
 };
 
-__device__ __forceinline__ Group group_of(const int32_t* offsets, int e, int E, int64_t R) {
-  int64_t lo = e > 0 ? offsets[e - 1] : 0, hi = e < E ? offsets[e] : R;
-  lo = lo < 0 ? 0 : (lo > R ? R : lo);
-  hi = hi < lo ? lo : (hi > R ? R : hi);
-  return {lo, hi};
+// Of expert e < E; the whole wave calls.
+__device__ __forceinline__ Group group_of(const int32_t* offsets, int e, int64_t R) {
+  int lo = 0;
+  for (int i = threadIdx.x & 63; i < e; i += 64) lo = max(lo, offsets[i]);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) lo = max(lo, __shfl_xor(lo, off, 64));
+  lo = min(lo, (int)R);
+  return {lo, max(lo, min(offsets[e], (int)R))};
+}
+
+// Of experts base to base + 63, a lane each; expert E has the rows past the last offset.  `end` is the last lane's
+// end, and before the call that of expert base - 1.
+__device__ __forceinline__ Group groups_of(const int32_t* offsets, int base, int E, int64_t R, int* end) {
+  const int lane = threadIdx.x & 63, e = base + lane;
+  int hi = max(e < E ? min(offsets[e], (int)R) : (int)R, *end);
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int v = __shfl_up(hi, off, 64);
+    if (lane >= off) hi = max(hi, v);
+  }
+  const int before = __shfl_up(hi, 1, 64);
+  const Group g{lane ? before : *end, hi};
+  *end = __shfl(hi, 63, 64);
+  return g;
 }
 
 struct RowTile {
@@ -57,11 +77,9 @@ struct RowTile {
 template <int BM>
 __device__ __forceinline__ RowTile find_tile(const int32_t* offsets, int E, int64_t R, int t) {
   const int lane = threadIdx.x & 63;
-  int before = 0;
+  int before = 0, end = 0;
   for (int base = 0; base <= E; base += 64) {
-    const int e = base + lane;
-    Group g{0, 0};
-    if (e <= E) g = group_of(offsets, e, E, R);
+    const Group g = groups_of(offsets, base, E, R, &end);
     const int n = (int)((g.hi - g.lo + BM - 1) / BM);
     int upto = n;
 #pragma unroll
@@ -282,14 +300,10 @@ __device__ __forceinline__ bool xcd_place(int n, int at, int* t) {
 // Row tiles in all.
 template <int BM>
 __device__ __forceinline__ int count_tiles(const int32_t* offsets, int E, int64_t R) {
-  const int lane = threadIdx.x & 63;
-  int n = 0;
+  int n = 0, end = 0;
   for (int base = 0; base <= E; base += 64) {
-    const int e = base + lane;
-    if (e <= E) {
-      const Group g = group_of(offsets, e, E, R);
-      n += (int)((g.hi - g.lo + BM - 1) / BM);
-    }
+    const Group g = groups_of(offsets, base, E, R, &end);
+    n += (int)((g.hi - g.lo + BM - 1) / BM);
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
@@ -379,7 +393,7 @@ __global__ __launch_bounds__(256) void grouped_kernel(GroupedArgs a) {
     if (!xcd_place(a.tiles_i * a.tiles_j, at - e * run, &t)) return;
     band_tile(t, a.tiles_i, a.tiles_j, &ti, &tj);
     i0 = (int64_t)ti * BM;
-    const Group g = group_of(a.offsets, e, a.E, a.R);
+    const Group g = group_of(a.offsets, e, a.R);
     rows = (int)(a.I - i0 < BM ? a.I - i0 : BM);
     k0 = (int)g.lo;
     klim = (int)g.hi;
@@ -778,7 +792,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void grouped_direct_kernel(Grouped
     k.e = at / run;
     if (!xcd_place(a.tiles_i * a.tiles_j, at - k.e * run, &t)) return;
     band_tile(t, a.tiles_i, a.tiles_j, &ti, &tj);
-    const Group g = group_of(a.offsets, k.e, a.E, a.R);
+    const Group g = group_of(a.offsets, k.e, a.R);
     k.i0 = (int64_t)ti * BM;
     k.rows = (int)(a.I - k.i0 < BM ? a.I - k.i0 : BM);
     k.j0 = (int64_t)tj * BN;

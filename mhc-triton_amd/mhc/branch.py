@@ -150,7 +150,8 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor)
     Rows are sorted by expert: expert e has rows ``offsets[e-1]`` to ``offsets[e]`` (``offsets[-1]`` counting as 0),
     the running sum of the experts' row counts, int32 (int64 is converted) on the GPU.  It is read there
     only, so any split, experts without rows among them, serves a captured graph.  Rows past the last offset
-    belong to no expert: they give zeros and get zero gradients.  Differentiable in x and weight.
+    belong to no expert: they give zeros and get zero gradients; offsets out of range count clamped, offsets that
+    run backwards as their running maximum.  Differentiable in x and weight.
     """
     if torch.compiler.is_compiling():
         return _l.grouped_matmul(x, weight, offsets)

@@ -456,6 +456,29 @@ def test_grouped_matmul_offsets_out_of_range_are_clamped():
     assert torch.equal(want, got)
 
 
+@pytest.mark.parametrize("R,K", [(60, 32), (3000, 32), (3000, 33)])
+def test_grouped_matmul_offsets_that_run_backwards(R, K):
+    """They count as their running maximum, in whatever kernel: experts share no row and leave none out."""
+    x, w = rand(R, K, seed=1), rand(3, 40, K, seed=2)
+    y = branch.grouped_matmul(x, w, torch.tensor([R * 2 // 3, R // 6, R], dtype=torch.int32, device=DEV))
+    for rows, e in ((slice(0, R // 6), 0), (slice(R * 2 // 3, R), 2)):
+        ref, size = O.grouped_matmul(to_np(x[rows]), to_np(w[e:e + 1]), [x[rows].shape[0]])
+        close(y[rows], ref, size, (K + 8) * 2.0 ** -23, "y")
+
+
+@pytest.mark.parametrize("E", [5, 70, 200])
+@pytest.mark.parametrize("K", [32, 33])
+def test_grouped_matmul_offsets_count_as_their_running_maximum(K, E):
+    R, N = 900, 40
+    x, w = rand(R, K, seed=1).requires_grad_(), rand(E, N, K, seed=2).requires_grad_()
+    dy = rand(R, N, seed=3)
+    off = torch.from_numpy(np.random.default_rng(4).integers(-50, R // 2, E).astype(np.int32)).to(DEV)
+    off[E // 2:] += R // 2 + 20
+    got = [branch.grouped_matmul(x, w, o) for o in (off, off.clamp(0, R).cummax(0).values.int())]
+    grads = [torch.autograd.grad(y, (x, w), dy) for y in got]
+    assert torch.equal(*got) and all(torch.equal(a, b) for a, b in zip(*grads))
+
+
 def test_grouped_matmul_empty_sizes():
     off = torch.zeros(3, dtype=torch.int32, device=DEV)
     for R, K, N in ((0, 8, 8), (4, 0, 8), (4, 8, 0)):
