@@ -25,6 +25,7 @@ from __future__ import annotations
 from typing import Optional, Tuple, Union
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _branch as _k
 from . import _branch_library as _l
@@ -40,7 +41,7 @@ class _RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps: float):
         x = x.contiguous()
-        y, h, rstd = _k.rms_norm_forward(x, weight, residual, eps)
+        y, h, rstd = _k.rms_norm_forward(x, weight, residual, eps, want_rstd=any(ctx.needs_input_grad))
         ctx.save_for_backward(x if h is None else h, weight, rstd)
         ctx.set_materialize_grads(False)
         return y if h is None else (y, h)
@@ -96,6 +97,9 @@ class _GroupedMatmul(torch.autograd.Function):
 def _inference_only(name: str, *tensors) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"mhc: {name} has no backward; call it under torch.no_grad()")
+    # a launcher reads a dual tensor's values and would drop its tangent
+    if not torch.compiler.is_compiling() and any(t is not None and unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"mhc: {name} has no forward-mode derivative")
 
 
 def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
@@ -112,10 +116,7 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: O
         out = _lib.native().rms_norm(x, weight, residual, float(eps))
         if out is not None:
             return out
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
-        return _RmsNorm.apply(x, weight, residual, float(eps))
-    y, h, _ = _k.rms_norm_forward(x, weight, residual, float(eps), want_rstd=False)
-    return y if h is None else (y, h)
+    return _RmsNorm.apply(x, weight, residual, float(eps))
 
 
 def rms_norm_mx(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
@@ -167,6 +168,7 @@ def grouped_matmul_mx(q: torch.Tensor, scales: torch.Tensor, weight_q: torch.Ten
     """``grouped_matmul`` of 8-bit rows and weights, each with its scales as ``quantize_mx`` gives them; the
     result is in ``out_dtype``, bfloat16 or float16 (the 8-bit matrix instruction's sums fall short of fp32).
     No backward."""
+    _inference_only("grouped_matmul_mx", q, scales, weight_q, weight_scales)
     if torch.compiler.is_compiling():
         return _l.grouped_matmul_mx(q, scales, weight_q, weight_scales, offsets, out_dtype)
     return _k.grouped_matmul_mx(q, scales, weight_q, weight_scales, offsets, out_dtype)

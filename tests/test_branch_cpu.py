@@ -171,3 +171,58 @@ def test_fakes_and_traced_gradients():
     y = L.dropout(x, 0.1, e(2, dt=torch.int64), res)
     g = torch.autograd.grad(y.sum(), (x, res))
     assert [(t.shape, t.dtype) for t in g] == [(t.shape, t.dtype) for t in (x, res)]
+
+
+def _forward_mode_calls(device):
+    """name -> call on tensors of which f makes one dual (forward-mode AD)."""
+    x, w, off = torch.ones(4, 64, device=device), torch.ones(64, device=device), torch.tensor([2, 4], device=device)
+    wt = torch.ones(2, 64, 64, device=device)
+    q, s = x.to(_branch.F8), torch.full((4, 4), 127, dtype=torch.uint8, device=device).view(_branch.E8)
+    wq, ws = wt.to(_branch.F8), torch.full((2, 64, 4), 127, dtype=torch.uint8, device=device).view(_branch.E8)
+    return {
+        "norm": lambda f: branch.rms_norm(f(x)),
+        "norm weight": lambda f: branch.rms_norm(x, f(w)),
+        "norm residual": lambda f: branch.rms_norm(x, w, residual=f(x)),
+        "norm mx": lambda f: branch.rms_norm_mx(f(x)),
+        "norm mx weight": lambda f: branch.rms_norm_mx(x, f(w)),
+        "quantize": lambda f: branch.quantize_mx(f(x)),
+        "dropout": lambda f: branch.dropout(f(x), 0.5, (1, 2)),
+        "grouped": lambda f: branch.grouped_matmul(f(x), wt, off),
+        "grouped weight": lambda f: branch.grouped_matmul(x, f(wt), off),
+        "grouped mx": lambda f: branch.grouped_matmul_mx(f(q), s, wq, ws, off),
+        "grouped mx weight": lambda f: branch.grouped_matmul_mx(q, s, f(wq), ws, off),
+    }
+
+
+def forward_mode_is_refused(name, device):
+    """No operator has a forward-mode derivative: a dual tensor is refused, not computed without its tangent.
+    Without one the same call runs, with gradients off and with them on."""
+    from torch.autograd.forward_ad import dual_level, make_dual
+
+    call = _forward_mode_calls(device)[name]
+    for mode in (torch.no_grad, torch.enable_grad):
+        with mode(), dual_level():
+            call(lambda t: t)
+            with pytest.raises(NotImplementedError):
+                call(lambda t: make_dual(t, t.clone()))
+
+
+@pytest.mark.parametrize("name", list(_forward_mode_calls("cpu")))
+def test_forward_mode_is_refused(monkeypatch, name):
+    """Stand-in launchers that, as the real ones do, read the values and return new tensors."""
+    new = torch.empty_like
+    monkeypatch.setattr(_branch, "rms_norm_forward", lambda x, w, res, eps, want_rstd=True: (
+        new(x), None if res is None else new(x), new(x) if want_rstd else None))
+    monkeypatch.setattr(_branch, "rms_norm_mx", lambda x, w, res, eps: (new(x), new(x), None))
+    monkeypatch.setattr(_branch, "quantize_mx", lambda x: (new(x), new(x)))
+    monkeypatch.setattr(_branch, "dropout", lambda x, p, rng, res, want_used: (new(x), None))
+    monkeypatch.setattr(_branch, "grouped_matmul_forward", lambda x, w, off: new(x))
+    monkeypatch.setattr(_branch, "grouped_matmul_mx", lambda q, *rest: new(q))
+    forward_mode_is_refused(name, "cpu")
+
+
+def test_8_bit_products_refuse_operands_that_need_gradients():
+    q, s = torch.zeros(4, 64).to(_branch.F8), torch.zeros(4, 4, dtype=torch.uint8).view(_branch.E8)
+    wq, ws = torch.zeros(2, 8, 64).to(_branch.F8), torch.zeros(2, 8, 4, dtype=torch.uint8).view(_branch.E8)
+    with pytest.raises(RuntimeError, match="no backward"):
+        branch.grouped_matmul_mx(q.requires_grad_(), s, wq, ws, torch.zeros(2, dtype=torch.int32))
