@@ -943,7 +943,10 @@ PyObject* py_dropout(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-Tensor int_offsets(const Tensor& t) { return t.to(at::kInt).contiguous(); }
+// int64 offsets are narrowed to the nearest int32: the kernels clamp what is out of range.
+Tensor int_offsets(const Tensor& t) {
+  return (t.scalar_type() == at::kInt ? t : at::clamp(t, INT32_MIN, INT32_MAX).to(at::kInt)).contiguous();
+}
 
 Tensor grouped_forward(const Tensor& x_in, const Tensor& w_in, const Tensor& off_in) {
   const c10::DeviceGuard guard(x_in.device());

@@ -184,6 +184,8 @@ def _offsets(offsets: torch.Tensor, E: int) -> torch.Tensor:
         raise ShapeError(f"offsets must be ({E},), the end of each expert's rows, got {tuple(offsets.shape)}")
     if offsets.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"mhc: offsets must be int32 or int64, got {offsets.dtype}")
+    if offsets.dtype == torch.int64:  # narrowed to the nearest: the kernels clamp what is out of range
+        offsets = offsets.clamp(-(1 << 31), (1 << 31) - 1)
     return offsets.to(torch.int32).contiguous()
 
 

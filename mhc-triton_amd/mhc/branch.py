@@ -149,7 +149,7 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor)
     """Each row of x (rows, in) times its expert's weight (experts, out, in): (rows, out) in x's dtype.
 
     Rows are sorted by expert: expert e has rows ``offsets[e-1]`` to ``offsets[e]`` (``offsets[-1]`` counting as 0),
-    the running sum of the experts' row counts, int32 (int64 is converted) on the GPU.  It is read there
+    the running sum of the experts' row counts, int32 on the GPU (int64 is narrowed, two more launches).  It is read there
     only, so any split, experts without rows among them, serves a captured graph.  Rows past the last offset
     belong to no expert: they give zeros and get zero gradients; offsets out of range count clamped, offsets that
     run backwards as their running maximum.  Differentiable in x and weight.

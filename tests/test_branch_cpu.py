@@ -226,3 +226,11 @@ def test_8_bit_products_refuse_operands_that_need_gradients():
     wq, ws = torch.zeros(2, 8, 64).to(_branch.F8), torch.zeros(2, 8, 4, dtype=torch.uint8).view(_branch.E8)
     with pytest.raises(RuntimeError, match="no backward"):
         branch.grouped_matmul_mx(q.requires_grad_(), s, wq, ws, torch.zeros(2, dtype=torch.int32))
+
+
+def test_wide_offsets_are_narrowed_to_the_nearest():
+    """int64 offsets outside 32 bits stay out of range, on the side on which they were."""
+    wide = torch.tensor([-2 ** 40, -2 ** 31 - 1, -2 ** 31, 7, 2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 32 + 3, 2 ** 63 - 1])
+    got = _branch._offsets(wide, 9)
+    assert got.dtype == torch.int32
+    assert got.tolist() == [-2 ** 31] * 3 + [7] + [2 ** 31 - 1] * 5
