@@ -76,13 +76,12 @@ def dropout_factors(n, p, seed, offset, first=0):
 
 
 def groups(offsets, rows):
-    """[(expert, lo, hi)] of offsets, clamped to [0, rows]."""
+    """[(expert, lo, hi)]: offsets count clamped to [0, rows] and as their running maximum."""
     out, lo = [], 0
     for e, hi in enumerate(offsets):
-        lo = min(max(lo, 0), rows)
-        end = min(max(int(hi), lo), rows)
-        out.append((e, lo, end))
-        lo = int(hi)
+        hi = max(lo, min(int(hi), rows))
+        out.append((e, lo, hi))
+        lo = hi
     return out
 
 

@@ -234,3 +234,13 @@ def test_wide_offsets_are_narrowed_to_the_nearest():
     got = _branch._offsets(wide, 9)
     assert got.dtype == torch.int32
     assert got.tolist() == [-2 ** 31] * 3 + [7] + [2 ** 31 - 1] * 5
+
+
+@pytest.mark.parametrize("offsets,want", [
+    ([2, 2, 6], [(0, 0, 2), (1, 2, 2), (2, 2, 6)]),
+    ([5, 3, 8], [(0, 0, 5), (1, 5, 5), (2, 5, 8)]),
+    ([-4, 20, 1], [(0, 0, 0), (1, 0, 8), (2, 8, 8)]),
+    ([6, -1, 2, 7], [(0, 0, 6), (1, 6, 6), (2, 6, 6), (3, 6, 7)]),
+])
+def test_oracle_offsets_count_as_their_running_maximum(offsets, want):
+    assert O.groups(offsets, 8) == want

@@ -4,13 +4,28 @@ import pytest
 import torch
 
 from test_branch_cpu import _forward_mode_calls, forward_mode_is_refused
-from test_gpu_branch import rand
+from helpers import to_np
+from test_gpu_branch import DT, close, rand
 from test_gpu_native_nodes import both, same
 from mhc import branch
+from oracle import branch_oracle as O
 
 pytestmark = pytest.mark.gpu
 
 DEV = "cuda"
+
+
+def against_oracle(y, dx, dw, x, w, dy, offsets):
+    """The bounds of fp32 sums of as many terms, as in test_gpu_branch.py; rows of no expert are zeros."""
+    (R, K), N = x.shape, w.shape[1]
+    o = list(offsets)
+    ref, size = O.grouped_matmul(to_np(x), to_np(w), o)
+    rx, rw, sx, sw = O.grouped_matmul_backward(to_np(dy), to_np(x), to_np(w), o)
+    close(y, ref, size, (K + 8) * 2.0 ** -23, "y")
+    close(dx, rx, sx, (N + 8) * 2.0 ** -23, "dx")
+    close(dw, rw, sw, (R + 8) * 2.0 ** -23, "dw")
+    end = max(0, max(o)) if o else 0
+    assert not y[end:].any() and not dx[end:].any()
 
 
 @pytest.mark.parametrize("name", list(_forward_mode_calls("cpu")))
@@ -35,3 +50,21 @@ def test_int64_offsets_outside_32_bits_are_clamped(monkeypatch, wide):
     want = step(in_range)
     for got in both(monkeypatch, lambda: step(wide)):
         same(got, want)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("R,K,N,E", [
+    (60, 32, 40, 8), (60, 33, 40, 8),         # few rows: whole chunks, any alignment
+    (600, 96, 72, 3), (600, 97, 71, 3),       # small tiles
+    (3000, 256, 5000, 3), (3000, 5000, 264, 3),  # the largest tiles, with quarters (of y, of dx)
+])
+def test_offsets_that_run_backwards_against_the_oracle(R, K, N, E, dtype):
+    """Every row and both gradients: the rows belong to the running maximum's experts."""
+    dt = DT[dtype]
+    x, w = rand(R, K, seed=1, dtype=dt).requires_grad_(), rand(E, N, K, seed=2, dtype=dt, scale=K ** -0.5).requires_grad_()
+    dy = rand(R, N, seed=3, dtype=dt)
+    o = [R // 3, R // 6, -R, R * 5 // 6, R // 2, R * 2 // 3, R - 7, R - 9][:E - 1] + [R - 4]
+    off = torch.tensor(o, dtype=torch.int32, device=DEV)
+    y = branch.grouped_matmul(x, w, off)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    against_oracle(y, dx, dw, x, w, dy, o)
