@@ -208,14 +208,20 @@ def grouped_matmul_mx(q, scales, weight_q, weight_scales, offsets, out_dtype):
 # Dropout
 # --------------------------------------------------------------------------
 
+# rng: a device state, or None and the words of a pair of ints (low and high 32 bits of the seed, of the offset):
+# traced ints are symbols, and one past int64 can neither pass a schema nor enter a graph whole.
+
 @_op("dropout")
-def _dropout(x: Tensor, residual: Optional[Tensor], p: float, rng: Tensor) -> Tuple[Tensor, Tensor]:
+def _dropout(x: Tensor, residual: Optional[Tensor], p: float, rng: Optional[Tensor],
+             words: List[int]) -> Tuple[Tensor, Tensor]:
+    if rng is None:
+        rng = (words[0] | words[1] << 32, words[2] | words[3] << 32)
     return _k.dropout(x, p, rng, residual, want_used=True)
 
 
 @_dropout.register_fake
-def _(x, residual, p, rng):
-    return x.new_empty(x.shape), rng.new_empty(2)
+def _(x, residual, p, rng, words):
+    return x.new_empty(x.shape), x.new_empty(2, dtype=torch.int64)
 
 
 def _dropout_setup(ctx, inputs, output):
@@ -224,15 +230,18 @@ def _dropout_setup(ctx, inputs, output):
 
 
 def _dropout_bwd(ctx, dy, _):
-    dx = torch.ops.mhc_branch.dropout(dy, None, ctx.p, ctx.saved_tensors[0])[0] if ctx.needs_input_grad[0] else None
-    return dx, dy if ctx.needs_input_grad[1] else None, None, None
+    used, = ctx.saved_tensors
+    dx = torch.ops.mhc_branch.dropout(dy, None, ctx.p, used, [])[0] if ctx.needs_input_grad[0] else None
+    return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
 
 
 torch.library.register_autograd("mhc_branch::dropout", _dropout_bwd, setup_context=_dropout_setup)
 
 
 def dropout(x, p, rng, residual):
+    words = []
     if not isinstance(rng, Tensor):
         _k.check_rng(x, rng)
-        rng = torch.tensor([v - (1 << 64) if v >> 63 else v for v in rng], dtype=torch.int64, device=x.device)
-    return torch.ops.mhc_branch.dropout(x, residual, p, rng)[0]
+        words = [w for v in rng for w in (v & 0xFFFFFFFF, v >> 32)]
+        rng = None
+    return torch.ops.mhc_branch.dropout(x, residual, p, rng, words)[0]

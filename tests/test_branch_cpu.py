@@ -244,3 +244,31 @@ def test_wide_offsets_are_narrowed_to_the_nearest():
 ])
 def test_oracle_offsets_count_as_their_running_maximum(offsets, want):
     assert O.groups(offsets, 8) == want
+
+
+@pytest.mark.parametrize("backend", ["aot_eager", "inductor"])
+def test_traced_dropout_takes_every_pair_of_ints(backend):
+    """Traced ints become symbols once they change between calls; the pairs still reach the op whole, and its
+    backward draws from what the forward drew from.  A stand-in op writes down what it got."""
+    seen = []
+
+    def op(x, residual, p, rng, words):
+        u64 = (1 << 64) - 1
+        if rng is None:
+            rng = torch.tensor([v - (1 << 64) if v >> 63 else v for v in (words[0] | words[1] << 32, words[2] | words[3] << 32)])
+        seen.append(tuple(v & u64 for v in rng.tolist()))
+        return x.clone(), rng.clone()
+
+    torch._dynamo.reset()
+    with torch.library._scoped_library("mhc_branch", "IMPL") as lib:
+        lib.impl("dropout", op, "CPU")
+        f = torch.compile(lambda x, rng: branch.dropout(x, 0.5, rng), fullgraph=True, backend=backend)
+        for pair in [(7, 0), (7, 1), (8, 2), (2 ** 63 + 5, 3), (9, 2 ** 64 - 1), (2 ** 64 - 1, 2 ** 63), (2 ** 31, 2 ** 32), (0, 0)]:
+            x = torch.ones(8, requires_grad=True)
+            f(x, pair).sum().backward()
+            assert seen == [pair, pair]
+            seen.clear()
+        for pair in ((-1, 0), (0, 2 ** 64)):
+            with pytest.raises(Exception, match=r"2\^64"):
+                f(torch.ones(8), pair)
+    torch._dynamo.reset()

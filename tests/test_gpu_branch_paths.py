@@ -68,3 +68,21 @@ def test_offsets_that_run_backwards_against_the_oracle(R, K, N, E, dtype):
     y = branch.grouped_matmul(x, w, off)
     dx, dw = torch.autograd.grad(y, (x, w), dy)
     against_oracle(y, dx, dw, x, w, dy, o)
+
+
+@pytest.mark.parametrize("backend", ["aot_eager", "inductor"])
+def test_compiled_dropout_from_pairs_of_ints(backend):
+    """The same mask as eager, forward and backward, also once the ints have become symbols and past 2^63."""
+    x, res, dy = rand(64, 96, seed=1).requires_grad_(), rand(64, 96, seed=2).requires_grad_(), rand(64, 96, seed=3)
+
+    def f(x, res, rng):
+        return branch.dropout(x, 0.3, rng, residual=res)
+
+    torch._dynamo.reset()
+    compiled = torch.compile(f, fullgraph=True, backend=backend)
+    for pair in [(7, 0), (7, 1), (8, 2), (2 ** 63 + 5, 3), (2 ** 64 - 1, 2 ** 64 - 2), (2 ** 31, 2 ** 32)]:
+        want, got = f(x, res, pair), compiled(x, res, pair)
+        assert torch.equal(got, want)
+        for a, b in zip(torch.autograd.grad(got, (x, res), dy), torch.autograd.grad(want, (x, res), dy)):
+            assert torch.equal(a, b)
+    torch._dynamo.reset()
