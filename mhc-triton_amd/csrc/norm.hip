@@ -446,7 +446,8 @@ constexpr int64_t kNormMaxDim = 16384;
 // A workgroup a row (or four) forward, four of them a CU: they start and end apart, which is worth the
 // weight's vectors read again for each.  16384 x 4096 bf16 with a residual: two to eight workgroups a CU that
 // loop over rows 92-99 us, a row each 86.6 (6.2 TB/s) and 89.0 without the limit.
-constexpr int64_t kNormFwdBlocks = (int64_t)1 << 22;
+constexpr int64_t kNormFwdBlocks = ((int64_t)1 << 22) - 1;
+static_assert(kNormFwdBlocks * 64 * kTeamWaves < (int64_t)1 << 32, "the runtime takes fewer than 2^32 work items");
 
 // Workgroups of the backward at most, each with a partial weight gradient: half as many of four waves that
 // each hold a sum.  More write and add up more partials, fewer leave CUs waiting (us at 256 / 512 / 1024):

@@ -86,3 +86,21 @@ def test_compiled_dropout_from_pairs_of_ints(backend):
         for a, b in zip(torch.autograd.grad(got, (x, res), dy), torch.autograd.grad(want, (x, res), dy)):
             assert torch.equal(a, b)
     torch._dynamo.reset()
+
+
+def test_more_rows_than_a_launch_has_workgroups():
+    """Workgroups of 1024 threads come to 2^32 work items at 2^22 rows: a launch holds fewer and loops."""
+    D, R = 15392, (1 << 22) + 5
+    torch.cuda.empty_cache()
+    need = R * D * 3 + R * 4 * 121 + (4 << 30)
+    if torch.cuda.mem_get_info()[0] < need:
+        pytest.skip(f"needs {need >> 30} GiB of GPU memory")
+    x = torch.empty(R, D, device=DEV, dtype=torch.bfloat16).fill_(0.5)
+    x[-9:] = rand(9, D, seed=1, dtype=torch.bfloat16)
+    x[:3] = rand(3, D, seed=2, dtype=torch.bfloat16)
+    q, s = (t.view(torch.uint8) for t in branch.rms_norm_mx(x))
+    for rows in (slice(0, 4), slice(R // 2, R // 2 + 2), slice(R - 9, R)):
+        qa, sa = (t.view(torch.uint8) for t in branch.rms_norm_mx(x[rows].clone()))
+        assert torch.equal(q[rows], qa) and torch.equal(s[rows], sa)
+    del x, q, s
+    torch.cuda.empty_cache()
