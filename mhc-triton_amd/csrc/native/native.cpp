@@ -20,6 +20,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../../include/mhc_abi.h"
@@ -786,6 +787,14 @@ at::IntArrayRef row_sizes(const Tensor& t) { return t.sizes().slice(0, t.dim() -
 
 int64_t row_count(const Tensor& t) { return t.size(-1) ? t.numel() / t.size(-1) : 0; }
 
+// A gradient that a launcher computed.  Under create_graph, where something that went into it is differentiable,
+// it carries a node that raises: it would count as a constant otherwise.
+Tensor first_order(const Tensor& grad, const char* name, bool differentiable) {
+  if (!grad.defined() || !at::GradMode::is_enabled() || !differentiable) return grad;
+  const auto node = std::make_shared<torch::autograd::DelayedError>(std::string("mhc: ") + name + " has no second derivative", 1);
+  return (*node)({grad.detach().set_requires_grad(true)})[0];
+}
+
 struct NormOut { Tensor x, y, h, rstd; };
 
 NormOut norm_forward(const Tensor& x_in, const Tensor& weight, const Tensor& residual, double eps, bool keep) {
@@ -832,9 +841,10 @@ struct RmsNorm : Function<RmsNorm> {
       check(mhc_rms_norm_backward(ptr(dy), ptr(h), ptr(dh), code(h), fptr(w), fptr(rstd), ptr(dx), wptr(dw), R, D,
                                   ws.p(), ws.bytes, stream(h)),
             "rms_norm_backward");
+      dx = first_order(dx, "rms_norm", need_x);
+      if (dw.defined()) dw = first_order(grad_like(dw, s[1]), "rms_norm", need_x || g[0].requires_grad());
     }
-    return {ctx->needs_input_grad(0) ? dx : Tensor(), dw.defined() ? grad_like(dw, s[1]) : Tensor(),
-            need_res ? dx : Tensor(), Tensor()};
+    return {ctx->needs_input_grad(0) ? dx : Tensor(), dw, need_res ? dx : Tensor(), Tensor()};
   }
 };
 
@@ -899,11 +909,13 @@ struct Dropout : Function<Dropout> {
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
     const variable_list s = saved(ctx);
     Tensor dx;
-    if (ctx->needs_input_grad(0))
+    if (ctx->needs_input_grad(0)) {
       dx = dropout_forward(in_dtype(g[0], (at::ScalarType)ctx->saved_data["dtype"].toInt()), Tensor(),
                            ctx->saved_data["p"].toDouble(),
                            {(uint64_t)ctx->saved_data["seed"].toInt(), (uint64_t)ctx->saved_data["offset"].toInt()},
                            s.empty() ? Tensor() : s[0], nullptr);
+      dx = first_order(dx, "dropout", g[0].requires_grad());
+    }
     const bool need_res = ctx->saved_data["res"].toBool() && ctx->needs_input_grad(1);
     return {dx, need_res ? g[0] : Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
@@ -977,12 +989,14 @@ struct GroupedMatmul : Function<GroupedMatmul> {
       dx = at::empty({R, K}, dy.options().requires_grad(false));
       check(mhc_grouped_matmul_backward_input(ptr(dy), ptr(w), code(dy), o, ptr(dx), R, K, N, E, stream(dy)),
             "grouped_matmul_backward_input");
+      dx = first_order(dx, "grouped_matmul", g[0].requires_grad() || s[1].requires_grad());
     }
     if (ctx->needs_input_grad(1)) {
       const Tensor x = s[0].contiguous();
       dw = at::empty({E, N, K}, dy.options().requires_grad(false));
       check(mhc_grouped_matmul_backward_weight(ptr(dy), ptr(x), code(dy), o, ptr(dw), R, K, N, E, stream(dy)),
             "grouped_matmul_backward_weight");
+      dw = first_order(dw, "grouped_matmul", g[0].requires_grad() || s[0].requires_grad());
     }
     return {dx, dw, Tensor()};
   }

@@ -35,6 +35,15 @@ from ._branch import Rng
 __all__ = ["rms_norm", "rms_norm_mx", "quantize_mx", "grouped_matmul", "grouped_matmul_mx", "dropout"]
 
 
+def _first_order(grad: Optional[torch.Tensor], name: str, *differentiable: bool) -> Optional[torch.Tensor]:
+    """A gradient that a launcher computed.  Under create_graph, where something that went into it is differentiable,
+    it carries a node that raises: it would count as a constant otherwise."""
+    if grad is None or not torch.is_grad_enabled() or not any(differentiable):
+        return grad
+    return torch._C._functions.DelayedError(f"mhc: {name} has no second derivative".encode(), 1)(
+        grad.detach().requires_grad_())
+
+
 class _RmsNorm(torch.autograd.Function):
     """(x, weight, residual) -> y, or (y, h) with a residual.  Keeps h (x without a residual) and rstd."""
 
@@ -53,8 +62,11 @@ class _RmsNorm(torch.autograd.Function):
         dx, dw = dh, None
         if dy is not None:
             dx, dw = _k.rms_norm_backward(dy, h, dh, weight, rstd, need_x, ctx.needs_input_grad[1])
+            dw = None if dw is None else dw.to(weight.dtype)
+            dx = _first_order(dx, "rms_norm", need_x)
+            dw = _first_order(dw, "rms_norm", need_x, dy.requires_grad)
         return (dx if ctx.needs_input_grad[0] else None,
-                None if dw is None else dw.to(weight.dtype),
+                dw,
                 dx if ctx.needs_input_grad[2] else None,
                 None)
 
@@ -74,6 +86,7 @@ class _Dropout(torch.autograd.Function):
         dx = None
         if ctx.needs_input_grad[0]:
             dx, _ = _k.dropout(dy, ctx.p, ctx.rng if ctx.rng is not None else ctx.saved_tensors[0])
+            dx = _first_order(dx, "dropout", dy.requires_grad)
         return dx, dy if ctx.needs_input_grad[1] else None, None, None
 
 
@@ -89,8 +102,10 @@ class _GroupedMatmul(torch.autograd.Function):
         dx = dw = None
         if ctx.needs_input_grad[0]:
             dx = _k.grouped_matmul_backward_input(dy, weight, offsets)
+            dx = _first_order(dx, "grouped_matmul", dy.requires_grad, weight.requires_grad)
         if ctx.needs_input_grad[1]:
             dw = _k.grouped_matmul_backward_weight(dy, x, offsets)
+            dw = _first_order(dw, "grouped_matmul", dy.requires_grad, x.requires_grad)
         return dx, dw, None
 
 

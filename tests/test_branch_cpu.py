@@ -272,3 +272,59 @@ def test_traced_dropout_takes_every_pair_of_ints(backend):
             with pytest.raises(Exception, match=r"2\^64"):
                 f(torch.ones(8), pair)
     torch._dynamo.reset()
+
+
+def _leaf(*shape, device, grad=True, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(shape, generator=g).to(device).requires_grad_(grad)
+
+
+# (operator, which of its inputs need gradients, whether dy depends on something differentiated, gradients that go on)
+SECOND_ORDER = [
+    ("norm", "x", False, "x"), ("norm", "w", False, ""), ("norm", "w", True, "w"), ("norm", "xw", False, "xw"),
+    ("norm", "xwr", True, "xwr"), ("norm", "r", False, "r"),
+    ("dropout", "x", False, ""), ("dropout", "x", True, "x"), ("dropout", "xr", True, "xr"),
+    ("grouped", "x", False, ""), ("grouped", "w", False, ""), ("grouped", "xw", False, "xw"), ("grouped", "x", True, "x"),
+]
+
+
+def second_derivatives_raise(op, need, dy_grad, graph, device):
+    """Under create_graph a gradient that depends on something differentiated has a graph, and going back through
+    the operator's part of it raises; one that depends on nothing has none.  The values are the same."""
+    x, r = (_leaf(8, 32, device=device, grad=n in need, seed=i) for i, n in enumerate("xr"))
+    w = _leaf(*((2, 32, 32) if op == "grouped" else (32,)), device=device, grad="w" in need, seed=3)
+    dy = _leaf(8, 32, device=device, grad=dy_grad, seed=4)
+    res = r if "r" in need else None
+    if op == "norm":
+        y = branch.rms_norm(x, w, residual=res)
+        y = y if res is None else y[0]
+    elif op == "dropout":
+        y = branch.dropout(x, 0.5, (1, 2), residual=res)
+    else:
+        y = branch.grouped_matmul(x, w, torch.tensor([3, 8], dtype=torch.int32, device=device))
+    leaves = {n: t for n, t in zip("xwr", (x, w, r)) if n in need}
+    plain = torch.autograd.grad(y, list(leaves.values()), dy, retain_graph=True)
+    grads = torch.autograd.grad(y, list(leaves.values()), dy, create_graph=True)
+    for n, g, p in zip(leaves, grads, plain):
+        assert torch.equal(g, p) and g.dtype == leaves[n].dtype
+        assert g.requires_grad == (n in graph), n
+        if op == "dropout" and n == "r":  # dy itself
+            assert torch.equal(torch.autograd.grad(g.sum(), dy)[0], torch.ones_like(dy))
+        elif n in graph:
+            with pytest.raises(RuntimeError, match="no second derivative"):
+                (g.square().sum() + x.sum()).backward()
+
+
+@pytest.mark.parametrize("op,need,dy_grad,graph", SECOND_ORDER)
+def test_second_derivatives_raise(monkeypatch, op, need, dy_grad, graph):
+    """The Python nodes, with stand-in launchers that return new tensors."""
+    one = lambda t: torch.ones(t.shape)  # noqa: E731
+    monkeypatch.setattr(_branch, "rms_norm_forward", lambda x, w, res, eps, want_rstd=True: (
+        one(x), None if res is None else one(x), torch.ones(8)))
+    monkeypatch.setattr(_branch, "rms_norm_backward", lambda dy, h, dh, w, rstd, need_dx=True, need_dw=True: (
+        one(h) if need_dx else None, one(w) if need_dw else None))
+    monkeypatch.setattr(_branch, "dropout", lambda x, p, rng, res=None, want_used=False: (one(x), None))
+    monkeypatch.setattr(_branch, "grouped_matmul_forward", lambda x, w, off: one(x))
+    monkeypatch.setattr(_branch, "grouped_matmul_backward_input", lambda dy, w, off: one(dy))
+    monkeypatch.setattr(_branch, "grouped_matmul_backward_weight", lambda dy, x, off: torch.ones(2, 32, 32))
+    second_derivatives_raise(op, need, dy_grad, graph, "cpu")

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from test_branch_cpu import _forward_mode_calls, forward_mode_is_refused
+from test_branch_cpu import SECOND_ORDER, _forward_mode_calls, forward_mode_is_refused, second_derivatives_raise
 from helpers import to_np
 from test_gpu_branch import DT, close, rand
 from test_gpu_native_nodes import both, same
@@ -104,3 +104,8 @@ def test_more_rows_than_a_launch_has_workgroups():
         assert torch.equal(q[rows], qa) and torch.equal(s[rows], sa)
     del x, q, s
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("op,need,dy_grad,graph", SECOND_ORDER)
+def test_second_derivatives_raise(monkeypatch, op, need, dy_grad, graph):
+    both(monkeypatch, lambda: second_derivatives_raise(op, need, dy_grad, graph, DEV))
