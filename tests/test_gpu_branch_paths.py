@@ -5,7 +5,7 @@ import torch
 
 from test_branch_cpu import SECOND_ORDER, _forward_mode_calls, forward_mode_is_refused, second_derivatives_raise
 from helpers import to_np
-from test_gpu_branch import DT, close, rand
+from test_gpu_branch import DT, HALF_ULP, close, mx_values, offsets_of, rand
 from test_gpu_native_nodes import both, same
 from mhc import branch
 from oracle import branch_oracle as O
@@ -109,3 +109,151 @@ def test_more_rows_than_a_launch_has_workgroups():
 @pytest.mark.parametrize("op,need,dy_grad,graph", SECOND_ORDER)
 def test_second_derivatives_raise(monkeypatch, op, need, dy_grad, graph):
     both(monkeypatch, lambda: second_derivatives_raise(op, need, dy_grad, graph, DEV))
+
+
+# --------------------------------------------------------------------------
+# RMS norm of more than 64 rows: partial weight gradients, rows in a loop
+# --------------------------------------------------------------------------
+# Bounds.  A sum over a row adds at most 16 terms a lane, six levels in a wave and 16 waves: 38 roundings of 2^-24 of
+# the terms' magnitudes, and half of that in rstd; with the roundings around it y is within 24 * 2^-24 of itself.  dx has
+# rstd three times and two sums: below 128 * 2^-24 of its terms.  The weight gradient adds few rows in fp32 and
+# the rest in fp64: 32 * 2^-24.
+Y_TOL, DX_TOL, DW_TOL = 2.0 ** -19, 2.0 ** -17, 2.0 ** -19
+
+
+def check_norm(x, w, res, dy, dh):
+    leaves = [t for t in (x, w, res) if t is not None]
+    out = branch.rms_norm(x, w, residual=res)
+    y, h = (out, x) if res is None else out
+    if res is not None:
+        assert torch.equal(h, x + res)
+    grads = torch.autograd.grad((y,) if res is None else (y, h), leaves, (dy,) if res is None else (dy, dh))
+    if res is not None:
+        assert torch.equal(grads[0], grads[2])
+    ref, _ = O.rms_norm(to_np(h), to_np(w))
+    rx, rw, sx, sw = O.rms_norm_backward(to_np(dy), to_np(h), None if res is None else to_np(dh), to_np(w))
+    close(y, ref, ref, Y_TOL, "y")
+    close(grads[0], rx, sx, DX_TOL, "dx")
+    close(grads[1], rw, sw, DW_TOL, "dw")
+
+
+# a row in a wave of one, two and four vectors a lane, in workgroups of every width, below one vector
+NORM_WIDTHS = {
+    "16": [3, 7, 504, 513, 1024, 1030, 1500, 2048, 2050, 4096, 4099, 7168, 8191, 16383, 16384],
+    "32": [1, 3, 256, 258, 512, 750, 1022, 1024, 1026, 4096, 8190, 8192, 8193, 12290, 16383, 16384],
+}
+
+
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("dtype,D", [(t, D) for t in DT for D in NORM_WIDTHS["32" if t == "fp32" else "16"]])
+def test_rms_norm_of_many_rows(D, dtype, residual):
+    R, dt = (2101 if D <= 2048 else 1100 if D <= 4100 else 1027 if D < 8193 else 517), DT[dtype]
+    x, dy = rand(R, D, seed=1, dtype=dt, scale=1.5).requires_grad_(), rand(R, D, seed=4, dtype=dt)
+    w = rand(D, seed=2).add_(1.0).requires_grad_()
+    res = rand(R, D, seed=3, dtype=dt).requires_grad_() if residual else None
+    check_norm(x, w, res, dy, rand(R, D, seed=5, dtype=dt) if residual else None)
+
+
+@pytest.mark.parametrize("dtype,D", [("bf16", 512), ("fp16", 2048), ("bf16", 4096), ("fp32", 1024), ("fp32", 8192), ("fp32", 12288)])
+def test_rms_norm_of_many_unaligned_rows(dtype, D):
+    """Rows of whole vectors, an element past a 16-byte boundary."""
+    R, dt = 300, DT[dtype]
+    off = lambda seed: rand(R * D + 1, seed=seed, dtype=dt)[1:].view(R, D)  # noqa: E731
+    x, res, dy, dh = off(1).requires_grad_(), off(3).requires_grad_(), off(4), off(5)
+    check_norm(x, rand(D, seed=2).add_(1.0).requires_grad_(), res, dy, dh)
+
+
+@pytest.mark.parametrize("R", [65, 1100])
+@pytest.mark.parametrize("dtype,D", [("bf16", 512), ("bf16", 1500), ("fp16", 2050), ("bf16", 4096), ("fp32", 1000), ("fp32", 9001)])
+def test_rms_norm_of_many_rows_each_gradient_alone(dtype, D, R):
+    """dx without dw and dw without dx: the bits that both together have."""
+    dt = DT[dtype]
+    x, dy, w = rand(R, D, seed=1, dtype=dt), rand(R, D, seed=4, dtype=dt), rand(D, seed=2)
+    lx, lw = x.clone().requires_grad_(), w.clone().requires_grad_()
+    dx, dw = torch.autograd.grad(branch.rms_norm(lx, lw), (lx, lw), dy)
+    assert torch.equal(torch.autograd.grad(branch.rms_norm(lx, w), lx, dy)[0], dx)
+    assert torch.equal(torch.autograd.grad(branch.rms_norm(x, lw), lw, dy)[0], dw)
+
+
+# --------------------------------------------------------------------------
+# Expert products: few rows an expert, unaligned tiles
+# --------------------------------------------------------------------------
+
+FEW_SPLITS = ["even", "one has all", "empty ends", "single rows", "none"]
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("split", FEW_SPLITS)
+@pytest.mark.parametrize("R,K,N,E", [(100, 1001, 37, 16), (100, 1500, 65, 16), (100, 1504, 72, 16), (128, 200, 130, 16),
+                                     (500, 260, 34, 70)])
+def test_grouped_matmul_of_few_rows(R, K, N, E, split, dtype):
+    """At most eight rows an expert on average: several tiles of one expert, experts without any, rows of none; rows
+    of whole chunks, and of any alignment over several units of 128 bytes."""
+    dt = DT[dtype]
+    x = rand(R, K, seed=1, dtype=dt).requires_grad_()
+    w = rand(E, N, K, seed=2, dtype=dt, scale=K ** -0.5).requires_grad_()
+    dy = rand(R, N, seed=3, dtype=dt)
+    off = offsets_of(split, R, E)
+    y = branch.grouped_matmul(x, w, off)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    against_oracle(y, dx, dw, x, w, dy, off.tolist())
+
+
+def test_grouped_matmul_of_few_rows_does_not_leak():
+    """NaN and infinity in one expert's rows and weights and in the rows of none stay there."""
+    R, N, E = 100, 37, 16
+    off = torch.tensor([5, 5, 31, 40] + [40 + 4 * i for i in range(11)] + [90], dtype=torch.int32, device=DEV)
+    for K in (1001, 1500, 1504):
+        for dt in DT.values():
+            x, w = rand(R, K, seed=1, dtype=dt), rand(E, N, K, seed=2, dtype=dt)
+            want = branch.grouped_matmul(x, w, off)
+            x[5:31], x[90:] = float("nan"), float("inf")
+            w[1:3] = float("inf")
+            got = branch.grouped_matmul(x, w, off)
+            assert torch.equal(got[:5], want[:5]) and torch.equal(got[31:90], want[31:90])
+            assert torch.isnan(got[5:31]).all() and not got[90:].any()
+
+
+@pytest.mark.parametrize("out", ["bf16", "fp16"])
+@pytest.mark.parametrize("split", FEW_SPLITS)
+@pytest.mark.parametrize("K,N", [(2048, 40), (2080, 33), (4128, 257), (4224, 100)])
+def test_grouped_matmul_mx_of_few_rows(K, N, split, out):
+    """8 bits: the last unit and the last scales of a row partial, odd widths, NaN in the scales' filling.  The bound is
+    the instruction's: of 16 products all but the largest are cut at 2^-13 of that one."""
+    R, E = 100, 16
+    x, w = rand(R, K, seed=1), rand(E, N, K, seed=2, scale=K ** -0.5)
+    x *= torch.exp2((torch.arange(K, device=DEV) // 32) % 7 - 3.0)
+    w *= torch.exp2((torch.arange(N, device=DEV) % 5) - 2.0)[None, :, None]
+    (q, s), (wq, ws) = branch.quantize_mx(x), branch.quantize_mx(w)
+    xv, wv = (torch.from_numpy(mx_values(*t)).to(DEV) for t in ((q, s), (wq, ws)))
+    for t in (s, ws):
+        t.view(torch.uint8)[..., K // 32:] = 255
+    off = offsets_of(split, R, E)
+    y = branch.grouped_matmul_mx(q, s, wq, ws, off, out_dtype=DT[out])
+    ref, allowed = torch.zeros(R, N, dtype=torch.float64, device=DEV), torch.zeros(R, N, dtype=torch.float64, device=DEV)
+    for e, lo, hi in O.groups(off.tolist(), R):
+        for r in range(lo, hi):
+            terms = xv[r] * wv[e]
+            ref[r] = terms.sum(1)
+            cut = 15 * 2.0 ** -13 * terms.abs().view(N, -1, 16).amax(2).sum(1)
+            allowed[r] = cut + (K + 8) * 2.0 ** -23 * terms.abs().sum(1)
+    allowed += 1.01 * HALF_ULP[DT[out]] * ref.abs() + (2.0 ** -25 if out == "fp16" else 0.0)
+    assert y.dtype == DT[out]
+    assert bool(((y.double() - ref).abs() <= allowed).all())
+    end = max(off.tolist())
+    assert not y[end:].any()
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("R,K,N", [(2900, 129, 2801), (2900, 2801, 129), (2900, 2801, 136), (300, 2801, 2901), (301, 2800, 2901)])
+def test_grouped_matmul_unaligned_large_tiles(R, K, N, dtype):
+    """Unaligned rows and enough tiles of 128 x 128 (22 x 24, 66 x 23 of the weight gradient) for two a CU: y, dx and dw
+    each, one operand of whole chunks beside an odd one, an expert without rows, rows of none."""
+    dt, E = DT[dtype], 3
+    x = rand(R, K, seed=1, dtype=dt).requires_grad_()
+    w = rand(E, N, K, seed=2, dtype=dt, scale=K ** -0.5).requires_grad_()
+    dy = rand(R, N, seed=3, dtype=dt)
+    o = [R * 2 // 5, R * 2 // 5, R - 13]
+    y = branch.grouped_matmul(x, w, torch.tensor(o, dtype=torch.int32, device=DEV))
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    against_oracle(y, dx, dw, x, w, dy, o)
