@@ -462,17 +462,21 @@ struct Team {
   static constexpr int NV = N;
 };
 
-// The team for rows of `nch` vectors, fn(Team, threads): a wave up to 256 vectors; beyond, a workgroup
+// The team for rows of `nch` vectors of W, fn(Team, threads): a wave up to 256 vectors; beyond, a workgroup
 // of as many waves as two vectors a lane need (four, past 16 waves).  D = 7168 bf16, seven waves of two
-// against four of four: to 8 bits 75.7 -> 72.1 us.
-template <class F>
+// against four of four: to 8 bits 75.7 -> 72.1 us.  Single elements are rows below one vector, and 16-bit rows
+// end at 16 waves of two.
+template <int W, class F>
 static int with_team(int64_t nch, F&& fn) {
-  if (nch <= 64) return fn(Team<true, 1>{}, 256);
-  if (nch <= 128) return fn(Team<true, 2>{}, 256);
-  if (nch <= 256) return fn(Team<true, 4>{}, 256);
-  if (nch <= 2 * 64 * kTeamWaves) return fn(Team<false, 2>{}, (int)((nch + 127) / 128 * 64));
-  return fn(Team<false, 4>{}, (int)((nch + 255) / 256 * 64));
+  if (W == 1 || nch <= 64) return fn(Team<true, 1>{}, 256);
+  if constexpr (W > 1) {
+    if (nch <= 128) return fn(Team<true, 2>{}, 256);
+    if (nch <= 256) return fn(Team<true, 4>{}, 256);
+    if (W >= 8 || nch <= 2 * 64 * kTeamWaves) return fn(Team<false, 2>{}, (int)((nch + 127) / 128 * 64));
+    if constexpr (W < 8) return fn(Team<false, 4>{}, (int)((nch + 255) / 256 * 64));
+  }
 }
+static_assert(kNormMaxDim <= 8 * 2 * 64 * kTeamWaves && kNormMaxDim <= 4 * 4 * 64 * kTeamWaves, "the widest rows fit");
 
 // Whole vectors, ragged vectors, or (rows below one vector) single elements.
 template <int WV, class F>
@@ -509,7 +513,7 @@ static int norm_forward(const char* who, NormArgs a, int dtype, hipStream_t st) 
     auto go = [&](auto wc, auto rag) {
       constexpr int W = decltype(wc)::value;
       constexpr bool RAG = decltype(rag)::value;
-      return with_team((a.D + W - 1) / W, [&](auto team, int threads) -> int {
+      return with_team<W>((a.D + W - 1) / W, [&](auto team, int threads) -> int {
         constexpr bool WAVE = decltype(team)::WAVE;
         constexpr int NV = decltype(team)::NV;
         const dim3 grid((unsigned)norm_blocks(a.R, kTeamRows<WAVE>, kNormFwdBlocks));
@@ -592,7 +596,7 @@ extern "C" int mhc_rms_norm_backward(const void* dy, const void* h, const void* 
     return with_row_width<Vec<T>::N>(D, {dy, h, dh, dx}, [&](auto wc, auto rag) {
       constexpr int W = decltype(wc)::value;
       constexpr bool RAG = decltype(rag)::value;
-      return with_team((D + W - 1) / W, [&](auto team, int threads) -> int {
+      return with_team<W>((D + W - 1) / W, [&](auto team, int threads) -> int {
         constexpr bool WAVE = decltype(team)::WAVE;
         constexpr int NV = decltype(team)::NV;
         blocks = (unsigned)norm_blocks(R, kBwdRows * kTeamRows<WAVE>, WAVE ? kNormBwdBlocks / 2 : kNormBwdBlocks);
