@@ -539,10 +539,11 @@ struct ScaleFeed {
   }
 };
 
-// Waits until at most N of the wave's loads are in flight, then for the whole workgroup.
+// Waits until at most N of the wave's loads are in flight and its LDS accesses are done, then for the whole workgroup:
+// behind it, slabs may be read that were waited for, and those overwritten that were read before.
 template <int N>
 __device__ __forceinline__ void slab_ready() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
@@ -718,7 +719,6 @@ __device__ __forceinline__ void direct_tile(const GroupedArgs& a, const Task& ta
     for (int s = 0; s < ST - 1; ++s) issue(s, k0 + s * kSlab<T>);
     int s = 0;
     for (; k0 < klim; k0 += kSlab<T>) {
-      if constexpr (MX) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // scales written
       slab_ready<(ST - 2) * kLoads>();
       int next = s + ST - 1;
       next = next >= ST ? next - ST : next;
