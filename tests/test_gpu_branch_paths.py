@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from test_branch_cpu import SECOND_ORDER, _forward_mode_calls, forward_mode_is_refused, second_derivatives_raise
+from test_branch_cpu import OPS, SECOND_ORDER, _forward_mode_calls, forward_mode_is_refused, second_derivatives_raise
 from helpers import to_np
 from test_gpu_branch import DT, HALF_ULP, close, mx_values, offsets_of, rand
 from test_gpu_native_nodes import both, same
@@ -257,3 +257,83 @@ def test_grouped_matmul_unaligned_large_tiles(R, K, N, dtype):
     y = branch.grouped_matmul(x, w, torch.tensor(o, dtype=torch.int32, device=DEV))
     dx, dw = torch.autograd.grad(y, (x, w), dy)
     against_oracle(y, dx, dw, x, w, dy, o)
+
+
+# --------------------------------------------------------------------------
+# Registrations, uninitialised memory
+# --------------------------------------------------------------------------
+
+def _registered_ops():
+    """name -> arguments of each op; several of one op side by side."""
+    bf = torch.bfloat16
+    x, res, w, dy = (rand(6, 64, seed=i, dtype=bf) for i in (1, 2, 3, 4))
+    w, off, wt = rand(64, seed=3), torch.tensor([2, 2, 5], dtype=torch.int32, device=DEV), rand(3, 16, 64, seed=5, dtype=bf)
+    rstd, state = rand(6, seed=6).abs(), torch.tensor([3, 4], device=DEV)
+    (q, s), (wq, ws) = branch.quantize_mx(x), branch.quantize_mx(wt)
+    rg = lambda t: t.clone().requires_grad_()  # noqa: E731
+    return [
+        ("norm", (rg(x.float()), rg(w), 1e-6)), ("norm", (x, None, 1e-6)),
+        ("add_norm", (rg(x.float()), rg(w), rg(res.float()), 1e-6)),
+        ("norm_backward", (dy, x, res, w, rstd, True)), ("norm_backward", (dy, x, None, None, rstd, False)),
+        ("norm_mx", (x, w, res, 1e-6)), ("norm_mx", (x, None, None, 1e-6)), ("quantize_mx", (x,)),
+        ("grouped_matmul", (rg(x.float()), rg(wt.float()), off)),
+        ("grouped_matmul_backward_input", (rand(6, 16, seed=7, dtype=bf), wt, off)),
+        ("grouped_matmul_backward_weight", (rand(6, 16, seed=7, dtype=bf), x, off)),
+        ("grouped_matmul_mx", (q, s, wq, ws, off, torch.float16)),
+        ("dropout", (rg(x.float()), rg(res.float()), 0.3, state, [])), ("dropout", (rg(x.float()), None, 0.3, None, [1, 2, 3, 4])),
+    ]
+
+
+@pytest.mark.parametrize("i", range(14))
+def test_opcheck(i):
+    cases = _registered_ops()
+    assert len(cases) == 14 and {n for n, _ in cases} == OPS
+    name, args = cases[i]
+    checks = ("test_schema", "test_autograd_registration", "test_faketensor", "test_aot_dispatch_dynamic")
+    # the schema check compares inputs before and after with products, which torch does not have in 8 bits
+    torch.library.opcheck(getattr(torch.ops.mhc_branch, name).default, args, test_utils=checks[name == "grouped_matmul_mx":])
+
+
+def test_outputs_and_workspaces_are_written_before_they_are_read(monkeypatch):
+    """With every new tensor's bytes set to 0xFF (NaN in each type) the results are the same."""
+    from mhc import _lib
+
+    def run():
+        out = []
+        for R, D, dt in ((3, 7, torch.float32), (70, 500, torch.bfloat16), (200, 2050, torch.float16), (600, 96, torch.float32)):
+            x, res, dy = (rand(R, D, seed=i, dtype=dt).requires_grad_() for i in (1, 2, 3))
+            w = rand(D, seed=4).requires_grad_()
+            y, h = branch.rms_norm(x, w, residual=res)
+            out += [y, h, *torch.autograd.grad((y, h), (x, res, w), (dy, dy))]
+            y = branch.dropout(x, 0.4, torch.tensor([1, 2], device=DEV), residual=res)
+            out += [y, *torch.autograd.grad(y, (x, res), dy)]
+            E, N = 5, 40
+            wt, g = rand(E, N, D, seed=5, dtype=dt).requires_grad_(), rand(R, N, seed=6, dtype=dt)
+            off = torch.tensor([R // 3, R // 3, R // 2, R // 2, R - 2], dtype=torch.int32, device=DEV)
+            y = branch.grouped_matmul(x, wt, off)
+            out += [y, *torch.autograd.grad(y, (x, wt), g)]
+        with torch.no_grad():
+            for R, D, E in ((5, 32, 2), (60, 2080, 9), (300, 416, 3)):
+                x, w = rand(R, D, seed=1, dtype=torch.bfloat16), rand(E, 24, D, seed=2, dtype=torch.bfloat16)
+                q, s, h = branch.rms_norm_mx(x, residual=x)
+                wq, ws = branch.quantize_mx(w)
+                off = torch.tensor([R // 3] * (E - 1) + [R - 2], dtype=torch.int32, device=DEV)
+                out += [q, s, h, wq, ws, branch.grouped_matmul_mx(q, s, wq, ws, off)]
+        return [t.detach().contiguous().view(torch.uint8) for t in out]
+
+    class Off:
+        def __getattr__(self, name):
+            return lambda *a: None
+
+    monkeypatch.setattr(_lib, "native", lambda: Off())
+    want = run()
+    for owner, name in ((torch, "empty"), (torch, "empty_like"), (torch.Tensor, "new_empty")):
+        def poisoned(*a, _make=getattr(owner, name), **k):
+            t = _make(*a, **k)
+            if t.is_cuda and t.numel() and t.is_contiguous():
+                t.view(torch.uint8).fill_(0xFF)
+            return t
+        monkeypatch.setattr(owner, name, poisoned)
+    got = run()
+    monkeypatch.undo()
+    same(got, want)
