@@ -628,12 +628,18 @@ extern "C" int mhc_quantize_mx(const void* x, int dtype, void* q, void* scales, 
   hipStream_t st = (hipStream_t)stream;
   return MHC_DISPATCH_DTYPE(dtype, [&] {
     constexpr int W = Vec<T>::N;
-    const int64_t n = (R * ns * (kMxBlock / W) + kThreads - 1) / kThreads;
-    if (n >= ((int64_t)1 << 32) / kThreads) {  // the runtime takes fewer than 2^32 work items
-      set_error("quantize_mx: %lld elements are too many for a call", (long long)(R * D));
+    // the runtime takes fewer than 2^32 work items: whole rows of as many, a launch each
+    const int64_t lanes = ns * (kMxBlock / W), most = (((int64_t)1 << 32) - kThreads) / lanes;
+    if (most < 1) {
+      set_error("quantize_mx: rows of %lld elements are too wide", (long long)D);
       return (int)MHC_ERR_ARG;
     }
-    quantize_mx_kernel<T, W><<<dim3((unsigned)n), kThreads, 0, st>>>((const T*)x, (uint8_t*)q, (uint8_t*)scales, R, D, ns);
-    return hip_status(hipGetLastError(), "quantize_mx launch");
+    for (int64_t r = 0; r < R; r += most) {
+      const int64_t rows = R - r < most ? R - r : most, n = (rows * lanes + kThreads - 1) / kThreads;
+      quantize_mx_kernel<T, W><<<dim3((unsigned)n), kThreads, 0, st>>>(
+          (const T*)x + r * D, (uint8_t*)q + r * D, (uint8_t*)scales + r * ns, rows, D, ns);
+      if (int rc = hip_status(hipGetLastError(), "quantize_mx launch")) return rc;
+    }
+    return (int)MHC_OK;
   });
 }

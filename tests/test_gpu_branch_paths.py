@@ -337,3 +337,20 @@ def test_outputs_and_workspaces_are_written_before_they_are_read(monkeypatch):
     got = run()
     monkeypatch.undo()
     same(got, want)
+
+
+def test_quantize_mx_of_more_elements_than_a_launch_has_work_items():
+    D, R = 8192, (1 << 22) + 5  # eight elements a work item
+    torch.cuda.empty_cache()
+    need = R * D * 3 + R * 256 + (4 << 30)
+    if torch.cuda.mem_get_info()[0] < need:
+        pytest.skip(f"needs {need >> 30} GiB of GPU memory")
+    x = torch.empty(R, D, device=DEV, dtype=torch.bfloat16).fill_(0.5)
+    x[-9:] = rand(9, D, seed=1, dtype=torch.bfloat16)
+    x[:3] = rand(3, D, seed=2, dtype=torch.bfloat16)
+    q, s = (t.view(torch.uint8) for t in branch.quantize_mx(x))
+    for rows in (slice(0, 4), slice(R // 2, R // 2 + 2), slice(R - 9, R)):
+        qa, sa = (t.view(torch.uint8) for t in branch.quantize_mx(x[rows].clone()))
+        assert torch.equal(q[rows], qa) and torch.equal(s[rows], sa)
+    del x, q, s
+    torch.cuda.empty_cache()
