@@ -67,14 +67,31 @@ static int64_t likely_tiles(const GroupedArgs& a) {
   return ((a.R + BM - 1) / BM + (a.E < a.R ? a.E : a.R) / 2) * j;
 }
 
-// Which kernel.  Few rows an expert: at 8 each the kernel that takes weights into registers still wins, past
-// 16 it reads the rows too often (us for 1 / 8 / 16 / 32 rows an expert, registers against tiles: 32 experts of
-// 2048 to 4096 bf16 100 / 111 / 131 / 211 against 133; 8 bits 56 / 64 / 75 / 123 against 74 to 78).  In 8 bits its
-// four waves need four units of four slabs: K = 1024 over 64 experts 38 against 32 us.
+// Which kernel; times in us, a captured launch each.  One rule for all types, made for 16 and 8 bits: where a figure
+// here speaks against it, the rule has not been refined.
+//
+// Few rows an expert: at 8 each the kernel that takes weights into registers still wins, past 16 it reads the rows
+// too often (1 / 8 / 16 / 32 rows an expert, registers against tiles: 32 experts of 2048 to 4096 bf16
+// 100 / 111 / 131 / 211 against 133; 8 bits 56 / 64 / 75 / 123 against 74 to 78).  In 8 bits its four waves need four
+// units of four slabs: K = 1024 over 64 experts 38 against 32 us.  fp32 (1 / 4 / 8 / 16 rows): 173 / 216 / 236 / 305 against
+// 64-tiles' 251 / 288 / 291 / 292 and 32-tiles' 159 / 228 / 227 / 231.  Rows of any alignment, against the general
+// kernel: 1500 to 1001 fp16 18.5 / 21.0 / 23.0 / 27.3 and 21.7 / 22.5 / 22.6 / 23.0, 2047 to 4095 fp32
+// 204 / 273 / 300 / 397 and 266 / 306 / 311 / 320, but bf16 of that odd width 173 / 231 / 268 / 401 and 99 / 113 / 120 / 139.
+//
 // Tiles: the largest of 256, 128, 64 and 32 that gives every CU one, 256 only where experts have as many rows (bf16
 // fwd / dx / dw, 256 against 128: 4096 rows of 4096 to 4096 over 8 experts 118 / 126 / 169 and 154 / 167 / 197 us, 8192 of
 // 1024 to 1024 over 8, half a tile a CU, 29 / 37 / 38 and 25 / 22 / 23, 4096 of 2048 to 1024 over 32 47 / 32 / 50 and
-// 27 / 28 / 45).  The general kernel takes what is not whole aligned 16-byte chunks.
+// 27 / 28 / 45; fp32 dw of 4096 by 1024 over 4, 256 tiles, 452 and 270).
+//   128 against 64, 1024 to 1024 over 8 (fwd / dx), with 352, 264 and 208 likely 128-tiles: bf16 20 / 22 and 28 / 37,
+//   18 / 21 and 20 / 27, 16 / 21 and 18 / 26 (where the rule takes 64); fp32 130 / 130 and 113 / 116, 129 / 129 and
+//   79 / 79, 73 / 74 and 62 / 63.
+//   64 against 32, 1024 to 1024 over 4 with 288 and 160 likely 64-tiles: bf16 10 / 12 and 15 / 20, 8.6 / 10.5 each;
+//   fp32 40 / 40 and 34 / 34, 25 / 25 and 21 / 22.  512 from 2048 with 48: bf16 16.0 and 13.2, fp32 45 and 21.
+//   8 bits, 128 against 64: 288 tiles 22.5 and 32.2, 224 18.3 and 25.4 (where the rule takes 64), 72 10.9 and 7.9.
+//
+// The general kernel takes what is not whole aligned 16-byte chunks, in 128-tiles from two a CU on (against 64, 1001 to
+// 1003 over 4 with 520, 392 and 272 likely 128-tiles: bf16 33 / 39 and 50 / 52, 30 / 37 and 41 / 46,
+// 28 / 36 and 29 / 31; fp32 147 / 155 and 165 / 173, 145 / 153 and 140 / 150, 142 / 152 and 88 / 94).
 template <typename T, typename TO, bool A_KR, bool B_KR, Role ROLE>
 static int launch_grouped(GroupedArgs a, const char* who, hipStream_t st) {
   constexpr bool MX = __is_same(T, Mx);

@@ -363,7 +363,7 @@ __device__ __forceinline__ void store_tile(u32x4* lds, const f32x4 (&acc)[FI][FJ
 // The general kernel: any size and alignment, operands staged through registers (unaligned 16-byte loads,
 // single values at a short row's end).  256 threads, four waves of a quarter of the tile each; the next slab's
 // loads are in flight while one is multiplied, and two slabs of LDS make one barrier a slab enough.  Bound by
-// the slab's loads (any alignment down to the element's): 3069 x 1500 x 1001 fp16 over 9 experts fwd 34, dx 41, dw 38 us,
+// the slab's loads (any alignment down to the element's): 3069 x 1500 x 1001 fp16 over 9 experts fwd 32, dx 40, dw 39-45 us,
 // where 1504 and 1008 take 28, 23 and 22 in the direct kernel.
 template <typename T, bool A_KR, bool B_KR, int BM, int BN, Role ROLE>
 __global__ __launch_bounds__(256) void grouped_kernel(GroupedArgs a) {
@@ -449,7 +449,7 @@ __global__ __launch_bounds__(256) void grouped_kernel(GroupedArgs a) {
 // the slab waited for is complete and the one multiplied before is free.
 //
 // Bound, at 256 x 256, by LDS (256 KB a slab move in the time of its products) and by the clock that the matrix
-// cores leave: 8192^3 bf16 fwd 1382, dx 1328, dw 1125 TFLOP/s, 8 bits 2372.  A k-row operand is read transposed,
+// cores leave: 8192^3 bf16 fwd 1382, dx 1328, dw 1125 TFLOP/s, 8 bits 2372; 4096^3 fp32 144, 142, 141.  A k-row operand is read transposed,
 // with twice the read instructions.
 //
 // Ranges are checked by the buffer: rows past the tile's and, for a k-row operand, k past the group's end

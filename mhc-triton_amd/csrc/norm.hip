@@ -49,7 +49,8 @@ __device__ __forceinline__ double wave_total(double v) {
          both_halves(v, [](uint32_t x) { return __builtin_amdgcn_permlane32_swap(x, x, false, false)[1]; });
 }
 
-// 1 / sqrt(m) to fp64's precision but for a few units: fp32's and a Newton step where fp32 holds m.
+// 1 / sqrt(m) to about 2^-45 of itself: fp32's and one Newton step where fp32 holds m.  What it is for is rounded to
+// fp32.
 __device__ __forceinline__ double rsqrt64(double m) {
   const float f = (float)m;
   if (!(f > 1e-37f && f < 1e37f)) return 1. / sqrt(m);
@@ -182,7 +183,9 @@ struct NormArgs {
 };
 
 // Forward.  Bound by the bus: x and the residual in, y and h out, each once.  16384 x 4096 bf16 with a residual
-// 86.6 us (6.2 TB/s), 8192 x 7168 into 8 bits 72 us (5.7 TB/s), one row of 4096 2.6 us.
+// 86.6 us (6.2 TB/s), the same in fp32 174 (6.2), 8192 x 7168 into 8 bits 72 us (5.7 TB/s), one row of 4096 2.6 us.  Ragged
+// rows of three or four vectors a lane leave one wave a SIMD: 3069 x 1500 fp16 8-9 us, 1504 5.4; beyond a wave bf16
+// 8192 x 4098 with a residual 52 us (5.2 TB/s).
 template <typename T, int W, bool RAG, bool WAVE, int NV, bool RES, bool MX>
 __global__ __launch_bounds__(WAVE ? 256 : 64 * kTeamWaves) void norm_fwd_kernel(NormArgs a) {
   constexpr int ROWS = kTeamRows<WAVE>;
@@ -294,7 +297,10 @@ __device__ __forceinline__ void few_rows_dw(const NormBwdArgs& a) {
 }
 
 // Backward.  Bound by the bus (dy, h and dh in, dx out); the weight gradient stays in registers over all of a team's
-// rows.  16384 x 4096 bf16 with dh 87 us and 4.7 us for the reduction (5.8 TB/s together), 3069 x 1500 fp16 12.5 us.
+// rows.  16384 x 4096 bf16 with dh 87 us and 4.7 us for the reduction (5.8 TB/s together), the same in fp32 177 (6.1);
+// 3069 x 1500 fp16 13 us (one wave a SIMD), 8192 x 4098 bf16 56 (4.8 TB/s).  The launch bound of 16 waves leaves 128
+// registers: some of ragged 16-bit rows beyond a wave and of fp32 rows beyond 8192 are spilled (8 to 66 of them; 4096 x
+// 16384 fp32 228 us, 4.7 TB/s, 16383 370).
 template <typename T, int W, bool RAG, bool WAVE, int NV, bool DH>
 __global__ __launch_bounds__(WAVE ? 256 : 64 * kTeamWaves) void norm_bwd_kernel(NormBwdArgs a) {
   constexpr int ROWS = kTeamRows<WAVE>;
@@ -418,7 +424,8 @@ __global__ __launch_bounds__(kDwCols * kDwGroups) void norm_dw_reduce_kernel(con
   dw[d] = (float)s;
 }
 
-// The quantiser alone: a lane per vector, rows of whole blocks.
+// The quantiser alone: a lane per vector, rows of whole blocks.  Bound by the bus: 8192 x 7168 bf16 35 us (5.1 TB/s),
+// fp32 57 (5.2), experts' weights of 32768 x 7168 bf16 125 us (5.7), 64 x 4096 3.2 us.
 template <typename T, int W>
 __global__ __launch_bounds__(kThreads) void quantize_mx_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
                                                                uint8_t* __restrict__ scales, int64_t R, int64_t D,
@@ -464,8 +471,10 @@ struct Team {
 
 // The team for rows of `nch` vectors of W, fn(Team, threads): a wave up to 256 vectors; beyond, a workgroup
 // of as many waves as two vectors a lane need (four, past 16 waves).  D = 7168 bf16, seven waves of two
-// against four of four: to 8 bits 75.7 -> 72.1 us.  Single elements are rows below one vector, and 16-bit rows
-// end at 16 waves of two.
+// against four of four: to 8 bits 75.7 -> 72.1 us.  A wave against a workgroup of two vectors a lane, 16384 rows of
+// 1024 / 1536 / 2048 bf16 with a residual (us): forward 25 / 37 / 47 and 39 / 47 / 54, backward 29 / 41 / 50 and
+// 57 / 61 / 65; ragged, of 1030 / 2044: backward 35 / 47 and 71 / 67, but forward 60 / 71 and 54 / 59.  Single
+// elements are rows below one vector, and 16-bit rows end at 16 waves of two.
 template <int W, class F>
 static int with_team(int64_t nch, F&& fn) {
   if (W == 1 || nch <= 64) return fn(Team<true, 1>{}, 256);

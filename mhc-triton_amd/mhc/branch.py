@@ -16,8 +16,8 @@ mixture-of-experts feed-forward branch does in between runs on these HIP kernels
 32 of a row (microscaling), which the matrix instructions of gfx950 multiply in.
 
 Tensors are fp32, bf16 or fp16 on a ROCm GPU and are computed in fp32; each op runs on the current stream,
-waits for nothing on the host and may be captured in a HIP graph.  Not part of ``mhc.__all__``, which stays
-the reference's.
+waits for nothing on the host and may be captured in a HIP graph.  Gradients are of the first order in reverse
+mode; second derivatives and, in eager calls, forward mode raise.  Not part of ``mhc.__all__``, which stays the reference's.
 """
 
 from __future__ import annotations
@@ -168,6 +168,9 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor)
     only, so any split, experts without rows among them, serves a captured graph.  Rows past the last offset
     belong to no expert: they give zeros and get zero gradients; offsets out of range count clamped, offsets that
     run backwards as their running maximum.  Differentiable in x and weight.
+
+    Both operands are read as they lie when contiguous; any other view, weights stored (experts, in, out) and passed
+    transposed among them, is copied whole at every call.
     """
     if torch.compiler.is_compiling():
         return _l.grouped_matmul(x, weight, offsets)
