@@ -422,6 +422,86 @@ int mhc_grouped_matmul_mx(const void* x, const void* x_scales, const void* weigh
                           int dtype_y, int64_t R, int64_t K, int64_t N, int64_t E,
                           mhc_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Mixing tokens inside the branch (no reference counterpart): rotary positions,
+ * linear attention with a decay for each head, and the gated product that a
+ * feed-forward begins with.  Row and head strides are in elements, a head's
+ * elements neighbours; outputs are contiguous.
+ * ------------------------------------------------------------------------ */
+
+/* Turns pairs of each head of q [R,q_heads,D] and k [R,k_heads,D]:
+ *   (a, b) -> magnitude (a cos t - b sin t, b cos t + a sin t),  t = position frequency
+ * pair i < pairs is (i, pairs + i), or (2i, 2i + 1) with `interleaved`; elements from
+ * 2 pairs on go through.  `inverse` turns by -t: the backward.  positions i32, or
+ * i64 with `wide`; row r has position r % position_count.  frequencies [pairs] f64,
+ * radians a position; angles are f64.  k may be NULL with k_heads = 0.  D <= 4096. */
+int mhc_rotary(const void* q, int64_t q_row, int64_t q_head, void* q_out, int64_t q_heads,
+               const void* k, int64_t k_row, int64_t k_head, void* k_out, int64_t k_heads,
+               int dtype, const void* positions, int wide, int64_t position_count,
+               const double* frequencies, int64_t pairs, int64_t R, int64_t D,
+               float magnitude, int interleaved, int inverse, mhc_stream_t stream);
+
+/* Linear attention with a decay l = exp(min(log_decay[h], 0)) for each head:
+ *   S_t = l S_{t-1} + k_t^T v_t,   o_t = scale q_t S_t
+ * over N sequences of R / N rows each or, with offsets [N] i32 on the device, packed
+ * ones: sequence n has rows [offsets[n-1], offsets[n]), clamped and as the running
+ * maximum; rows past the last get zeros.  q, k [R,H,Dk], v, o [R,H,Dv] in `dtype`,
+ * Dk, Dv <= 128; first, last [N,H,Dk,Dv] f32, the states before and after (NULL: zeros,
+ * not wanted).  Rows up to 2^22 elements apart. */
+size_t mhc_decay_attention_workspace_bytes(int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv, int packed);
+
+int mhc_decay_attention_forward(const void* q, int64_t q_row, int64_t q_head,
+                                const void* k, int64_t k_row, int64_t k_head,
+                                const void* v, int64_t v_row, int64_t v_head, int dtype,
+                                const float* log_decay, const int32_t* offsets,
+                                const float* first, void* o, float* last, int64_t R,
+                                int64_t N, int64_t H, int64_t Dk, int64_t Dv, float scale,
+                                void* workspace, size_t workspace_bytes, mhc_stream_t stream);
+
+size_t mhc_decay_attention_backward_workspace_bytes(int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv, int packed);
+
+/* dq, dk, dv (as q, k, v, contiguous) and d_first from dout and d_last; any of them,
+ * first and d_last may be NULL.  Rows of no sequence get zeros. */
+int mhc_decay_attention_backward(const void* q, int64_t q_row, int64_t q_head,
+                                 const void* k, int64_t k_row, int64_t k_head,
+                                 const void* v, int64_t v_row, int64_t v_head,
+                                 const void* dout, int64_t do_row, int64_t do_head, int dtype,
+                                 const float* log_decay, const int32_t* offsets,
+                                 const float* first, const float* d_last, void* dq, void* dk,
+                                 void* dv, float* d_first, int64_t R, int64_t N, int64_t H,
+                                 int64_t Dk, int64_t Dv, float scale, void* workspace,
+                                 size_t workspace_bytes, mhc_stream_t stream);
+
+/* One token for each of R rows: state_out[slots[r]] = l state[slots[r]] + k_r^T v_r and
+ * o_r from it.  state, state_out [pool,H,Dk,Dv] f32, the same or apart; slots [R] i32
+ * (NULL: row r has state r).  Rows that share a slot are tokens in their order; a row
+ * whose slot is outside the pool gets zeros and touches no state. */
+int mhc_decay_attention_step(const void* q, int64_t q_row, int64_t q_head,
+                             const void* k, int64_t k_row, int64_t k_head,
+                             const void* v, int64_t v_row, int64_t v_head, int dtype,
+                             const float* log_decay, const int32_t* slots, const float* state,
+                             float* state_out, void* o, int64_t R, int64_t pool, int64_t H,
+                             int64_t Dk, int64_t Dv, float scale, mhc_stream_t stream);
+
+/* Gated product of rows grouped by expert as in mhc_grouped_matmul_forward, or with
+ * offsets NULL (E = 1) all of one weight.  weight [E,2N,K]: N rows that make the gates,
+ * then N that make the values:
+ *   g = x Wg^T,  u = x Wu^T,  y = act(g) * u [R,N]
+ * saved [R,2N] f32 gets g and u for the backward (NULL: none follows). */
+enum { MHC_ACT_SILU = 0, MHC_ACT_GELU = 1, MHC_ACT_GELU_TANH = 2 };
+
+int mhc_gated_matmul_forward(const void* x, const void* weight, int dtype, const int32_t* offsets,
+                             int act, void* y, float* saved, int64_t R, int64_t K, int64_t N,
+                             int64_t E, mhc_stream_t stream);
+
+size_t mhc_gated_matmul_backward_workspace_bytes(int64_t R, int64_t N, int dtype);
+
+/* dx [R,K] and dweight [E,2N,K] (NULL: not wanted) from dy [R,N]. */
+int mhc_gated_matmul_backward(const void* dy, const float* saved, const void* x, const void* weight,
+                              int dtype, const int32_t* offsets, int act, void* dx, void* dweight,
+                              int64_t R, int64_t K, int64_t N, int64_t E, void* workspace,
+                              size_t workspace_bytes, mhc_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -34,6 +34,10 @@ struct GroupedArgs {
   int64_t R, I, J, K;      // rows in all; the product's sizes (kRows: I = R, kWeight: K = R)
   int64_t lda, ldb, ldo, b_expert, o_expert;
   int E, tiles_i, tiles_j, cus;
+  // gated products: `half` rows of a weight make the gates, as many behind them the values
+  float* saved;  // [R, 2 half], or null
+  int64_t half;
+  int act;
 };
 
 // Rows of one expert.  Whatever the offsets hold, they count clamped to [0, R] and as their running maximum, so that
@@ -42,6 +46,11 @@ struct Group {
   int64_t lo, hi;
 };
 
+// Without offsets there is one expert, with all rows.
+__device__ __forceinline__ int end_of(const int32_t* offsets, int e, int64_t R) {
+  return offsets ? min(offsets[e], (int)R) : (int)R;
+}
+
 // Of expert e < E; the whole wave calls.
 __device__ __forceinline__ Group group_of(const int32_t* offsets, int e, int64_t R) {
   int lo = 0;
@@ -49,14 +58,14 @@ __device__ __forceinline__ Group group_of(const int32_t* offsets, int e, int64_t
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) lo = max(lo, __shfl_xor(lo, off, 64));
   lo = min(lo, (int)R);
-  return {lo, max(lo, min(offsets[e], (int)R))};
+  return {lo, max(lo, end_of(offsets, e, R))};
 }
 
 // Of experts base to base + 63, a lane each; expert E has the rows past the last offset.  `end` is the last lane's
 // end, and before the call that of expert base - 1.
 __device__ __forceinline__ Group groups_of(const int32_t* offsets, int base, int E, int64_t R, int* end) {
   const int lane = threadIdx.x & 63, e = base + lane;
-  int hi = max(e < E ? min(offsets[e], (int)R) : (int)R, *end);
+  int hi = max(e < E ? end_of(offsets, e, R) : (int)R, *end);
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
     const int v = __shfl_up(hi, off, 64);
@@ -162,11 +171,18 @@ __device__ __forceinline__ int kr_slot(int r, int c) {
   else return c ^ (2 * ((r >> 3) & 1));  // four do
 }
 
+// Gated products: a tile's BN weight rows make BN / 2 columns, 16 gates and their 16 values in turn, so that a wave's
+// neighbouring fragments hold both of a column and all rows that a wave brings are of one kind.  Tile row r is row
+// gated_row(r) of the gates, or of the values.
+__device__ __forceinline__ int gated_row(int r) { return (r >> 5) * 16 + (r & 15); }
+__device__ __forceinline__ bool gated_value(int r) { return r & 16; }
+
 // Global -> registers -> LDS for one slab of one operand (NTH threads).  16-bit k-rows are loaded in two steps
 // (8000 x 2001 x 3001 bf16: dx 260 -> 200 us, dw 297 -> 204), the others with what is past an end left out: there
 // loads of rows that are none cost more than the branches (the same product's fwd 161 against 183).
-template <typename T, bool KR, int BM, int NTH>
+template <typename T, bool KR, int BM, int NTH, bool GATED = false>
 struct Stage {
+  static_assert(!GATED || !KR, "gates and values are rows");
   static constexpr int CH = BM * 8 / NTH;          // chunks per thread
   static constexpr int PER = BM / kElems<T>;       // KR: chunks per k-row
   static constexpr bool TWO = KR && sizeof(T) == 2;
@@ -174,22 +190,25 @@ struct Stage {
 
   __device__ __forceinline__ static int row(int q) { return (q * NTH + (int)threadIdx.x) / (KR ? PER : 8); }
   __device__ __forceinline__ static int chunk(int q) { return (q * NTH + (int)threadIdx.x) % (KR ? PER : 8); }
+  // Row of the operand: gated_row of a gated product's weight, `second` where it is a value's.
+  __device__ __forceinline__ static int source(int q) { return GATED ? gated_row(row(q)) : row(q); }
+  __device__ __forceinline__ static int64_t second(int q, int64_t half) { return GATED && gated_value(row(q)) ? half : 0; }
   // Values of chunk q that exist.  rows: KC valid rows of the tile; KR valid columns.
   __device__ __forceinline__ static int left(int q, int rows, int k0, int klim) {
     const int c = chunk(q) * kElems<T>;
     if constexpr (KR) return k0 + row(q) < klim ? rows - c : 0;
-    else return row(q) < rows ? klim - k0 - c : 0;
+    else return source(q) < rows ? klim - k0 - c : 0;
   }
 
   // wide: a row in memory has a chunk at least.
-  __device__ __forceinline__ void load(const T* base, int64_t ld, int rows, int k0, int klim, bool wide) {
+  __device__ __forceinline__ void load(const T* base, int64_t ld, int rows, int k0, int klim, bool wide, int64_t half = 0) {
     const bool whole = !KR && k0 + kSlab<T> <= klim;  // no row ends inside the slab
 #pragma unroll
     for (int q = 0; q < CH; ++q) {
       const int c = chunk(q) * kElems<T>, n = left(q, rows, k0, klim);
-      const T* p = base + (KR ? (int64_t)(k0 + row(q)) * ld + c : row(q) * ld + k0 + c);
+      const T* p = base + (KR ? (int64_t)(k0 + row(q)) * ld + c : (source(q) + second(q, half)) * ld + k0 + c);
       if (TWO && wide) r[q] = chunk_load<T>(p, n, base + (int64_t)k0 * ld + min(0, rows - kElems<T>));
-      else if (whole) r[q] = row(q) < rows ? load16_any(p, false) : u32x4{0, 0, 0, 0};
+      else if (whole) r[q] = source(q) < rows ? load16_any(p, false) : u32x4{0, 0, 0, 0};
       else r[q] = load_chunk<T>(p, n, wide);
     }
   }
@@ -360,14 +379,61 @@ __device__ __forceinline__ void store_tile(u32x4* lds, const f32x4 (&acc)[FI][FJ
   }
 }
 
+// act(g), and its derivative.  GELU by erfc, whose small values below zero are exact to a few ulps, and in its tanh form
+// as a logistic function, g / (1 + exp(-2 z)).
+__device__ __forceinline__ float logistic(float x) { return 1.f / (1.f + expf(-x)); }
+__device__ __forceinline__ float gelu_z2(float g) { return 1.5957691216057308f * (g + 0.044715f * g * g * g); }
+__device__ __forceinline__ float activate(int act, float g) {
+  if (act == MHC_ACT_SILU) return g / (1.f + expf(-g));
+  if (act == MHC_ACT_GELU) return 0.5f * g * erfcf(-0.70710678118654752f * g);
+  return g / (1.f + expf(-gelu_z2(g)));
+}
+__device__ __forceinline__ float activate_slope(int act, float g) {
+  if (act == MHC_ACT_SILU) {
+    const float s = logistic(g), rest = logistic(-g);
+    return s * (1.f + (rest == 0.f ? 0.f : g * rest));
+  }
+  if (act == MHC_ACT_GELU) {
+    const float bell = 0.3989422804014327f * expf(-0.5f * g * g);
+    return 0.5f * erfcf(-0.70710678118654752f * g) + (bell == 0.f ? 0.f : g * bell);
+  }
+  const float s = logistic(gelu_z2(g)), bell = s * (1.f - s);
+  return s + (bell == 0.f ? 0.f : g * bell * 1.5957691216057308f * (1.f + 0.134145f * g * g));
+}
+
+// A gated tile's results: act(gate) * value in TO, rounded once, and, wanted for a backward, gate and value in fp32.
+template <typename TO, int BM, int BN, int NTH, int CHUNKS, int FI, int FJ>
+__device__ __forceinline__ void store_gated(const GroupedArgs& a, u32x4* lds, const f32x4 (&acc)[FI][FJ], int wi, int wj,
+                                            int64_t i0, int64_t j0, int rows, int cols) {
+  static_assert(FJ % 2 == 0, "a gate beside each value");
+  f32x4 part[FI][FJ / 2];
+#pragma unroll
+  for (int i = 0; i < FI; ++i)
+#pragma unroll
+    for (int j = 0; j < FJ / 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) part[i][j][r] = activate(a.act, acc[i][2 * j][r]) * acc[i][2 * j + 1][r];
+  store_tile<TO, BM, BN / 2, NTH, CHUNKS>(lds, part, wi, wj / 2, (TO*)a.out + i0 * a.ldo + j0, a.ldo, rows, cols);
+  if (!a.saved) return;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+#pragma unroll
+    for (int i = 0; i < FI; ++i)
+#pragma unroll
+      for (int j = 0; j < FJ / 2; ++j) part[i][j] = acc[i][2 * j + s];
+    store_tile<float, BM, BN / 2, NTH, CHUNKS>(lds, part, wi, wj / 2, a.saved + i0 * 2 * a.half + s * a.half + j0, 2 * a.half,
+                                               rows, cols);
+  }
+}
+
 // The general kernel: any size and alignment, operands staged through registers (unaligned 16-byte loads,
 // single values at a short row's end).  256 threads, four waves of a quarter of the tile each; the next slab's
 // loads are in flight while one is multiplied, and two slabs of LDS make one barrier a slab enough.  Bound by
 // the slab's loads (any alignment down to the element's): 3069 x 1500 x 1001 fp16 over 9 experts fwd 32, dx 40, dw 39-45 us,
 // where 1504 and 1008 take 28, 23 and 22 in the direct kernel.
-template <typename T, bool A_KR, bool B_KR, int BM, int BN, Role ROLE>
+template <typename T, bool A_KR, bool B_KR, int BM, int BN, Role ROLE, bool GATED = false>
 __global__ __launch_bounds__(256) void grouped_kernel(GroupedArgs a) {
-  constexpr int NTH = 256, FI = BM / 32, FJ = BN / 32;
+  constexpr int NTH = 256, FI = BM / 32, FJ = BN / 32, COLS = GATED ? BN / 2 : BN;
   __shared__ u32x4 lds[2 * (BM + BN) * 8];
   const T *A = (const T*)a.A, *B = (const T*)a.B;
   T* out = (T*)a.out;
@@ -400,8 +466,8 @@ __global__ __launch_bounds__(256) void grouped_kernel(GroupedArgs a) {
     A += i0;
     out += (int64_t)e * a.o_expert;
   }
-  j0 = (int64_t)tj * BN;
-  const int cols = (int)(a.J - j0 < BN ? a.J - j0 : BN);
+  j0 = (int64_t)tj * COLS;
+  const int cols = (int)(a.J - j0 < COLS ? a.J - j0 : COLS);
   const bool wa = a.lda >= kElems<T>, wb = a.ldb >= kElems<T>;
   B += B_KR ? j0 : j0 * a.ldb;
   const int wave = threadIdx.x >> 6;
@@ -412,10 +478,10 @@ __global__ __launch_bounds__(256) void grouped_kernel(GroupedArgs a) {
 #pragma unroll
     for (int j = 0; j < FJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   Stage<T, A_KR, BM, NTH> sa;
-  Stage<T, B_KR, BN, NTH> sb;
+  Stage<T, B_KR, BN, NTH, GATED> sb;
   if (k0 < klim) {
     sa.load(A, a.lda, rows, k0, klim, wa);
-    sb.load(B, a.ldb, cols, k0, klim, wb);
+    sb.load(B, a.ldb, cols, k0, klim, wb, a.half);
   }
   for (int s = 0; k0 < klim; k0 += kSlab<T>, s ^= 1) {
     u32x4 *la = lds + s * (BM + BN) * 8, *lb = la + BM * 8;
@@ -424,7 +490,7 @@ __global__ __launch_bounds__(256) void grouped_kernel(GroupedArgs a) {
     __syncthreads();
     if (k0 + kSlab<T> < klim) {
       sa.load(A, a.lda, rows, k0 + kSlab<T>, klim, wa);
-      sb.load(B, a.ldb, cols, k0 + kSlab<T>, klim, wb);
+      sb.load(B, a.ldb, cols, k0 + kSlab<T>, klim, wb, a.half);
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -439,7 +505,8 @@ __global__ __launch_bounds__(256) void grouped_kernel(GroupedArgs a) {
       }
     }
   }
-  store_tile<T, BM, BN, NTH, 2 * (BM + BN) * 8>(lds, acc, wi, wj, out + i0 * a.ldo + j0, a.ldo, rows, cols);
+  if constexpr (GATED) store_gated<T, BM, BN, NTH, 2 * (BM + BN) * 8>(a, lds, acc, wi, wj, i0, j0, rows, cols);
+  else store_tile<T, BM, BN, NTH, 2 * (BM + BN) * 8>(lds, acc, wi, wj, out + i0 * a.ldo + j0, a.ldo, rows, cols);
 }
 
 // ---------------------------------------------------------------------------
@@ -457,8 +524,9 @@ __global__ __launch_bounds__(256) void grouped_kernel(GroupedArgs a) {
 // ---------------------------------------------------------------------------
 constexpr int kNowhere = 0x7ffffff0;
 
-template <typename T, bool KR, int BM, int NTH>
+template <typename T, bool KR, int BM, int NTH, bool GATED = false>
 struct Direct {
+  static_assert(!GATED || (!KR && NTH % 256 == 0), "a wave's rows are all gates' or all values'");
   static constexpr int CH = BM * 8 / NTH;    // loads a lane makes per slab
   static constexpr int PER = BM / kElems<T>; // KR: chunks per k-row
   const char* base;
@@ -467,10 +535,11 @@ struct Direct {
   int col;     // KC: the lane's first value in a slab
   int span;    // KC: the buffer's bytes; KR: bytes of a row that may be read
 
-  // rows: KC rows of the tile, KR columns.
-  __device__ __forceinline__ Direct(const T* p, int64_t ld_, int rows, int klim) {
-    base = reinterpret_cast<const char*>(p);
+  // rows: KC rows of the tile (GATED: of its gates), KR columns.
+  __device__ __forceinline__ Direct(const T* p, int64_t ld_, int rows, int klim, int64_t half = 0) {
     ld = ld_ * (int64_t)sizeof(T);
+    base = reinterpret_cast<const char*>(p);
+    if (GATED && gated_value(__builtin_amdgcn_readfirstlane(threadIdx.x >> 3))) base += half * ld;
 #pragma unroll
     for (int q = 0; q < CH; ++q) {
       const int i = q * NTH + threadIdx.x;
@@ -479,7 +548,7 @@ struct Direct {
         off[q] = c * kElems<T> < rows ? (int)(row * ld) + c * 16 : kNowhere;
       } else {
         const int row = i / 8;
-        off[q] = (int)(row * ld) + (((i % 8) ^ (row & 7)) * 16);
+        off[q] = (int)((GATED ? gated_row(row) : row) * ld) + (((i % 8) ^ (row & 7)) * 16);
       }
     }
     col = (((int)threadIdx.x % 8) ^ (((int)threadIdx.x / 8) & 7)) * kElems<T>;
@@ -560,7 +629,7 @@ template <typename T, int BM, int BN, int NTH>
 constexpr int kSlabChunks = (BM + BN) * 8 + (__is_same(T, Mx) ? NTH / 4 : 0);
 
 #ifdef __HIP_DEVICE_COMPILE__  // the host's compiler drops instantiations with 16-byte loads to LDS
-template <typename T, typename TO, bool A_KR, bool B_KR, int BM, int BN, int WI, int WJ, int ST, Role ROLE>
+template <typename T, typename TO, bool A_KR, bool B_KR, int BM, int BN, int WI, int WJ, int ST, Role ROLE, bool GATED = false>
 __device__ __forceinline__ void direct_tile(const GroupedArgs& a, const Task& task, u32x4* lds) {
   constexpr bool MX = __is_same(T, Mx), AHEAD = sizeof(T) == 2 && BM == 256 && BN == 256;
   constexpr int NTH = 64 * WI * WJ, FI = BM / WI / 16, FJ = BN / WJ / 16;
@@ -582,7 +651,7 @@ __device__ __forceinline__ void direct_tile(const GroupedArgs& a, const Task& ta
     for (int j = 0; j < FJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   const Direct<T, A_KR, BM, NTH> da(A, a.lda, rows, klim);
-  const Direct<T, B_KR, BN, NTH> db(B, a.ldb, cols, klim);
+  const Direct<T, B_KR, BN, NTH, GATED> db(B, a.ldb, cols, klim, a.half);
   constexpr int kLoads = da.CH + db.CH;  // per wave and slab
   ScaleFeed feed{};
   if constexpr (MX) {
@@ -728,7 +797,8 @@ __device__ __forceinline__ void direct_tile(const GroupedArgs& a, const Task& ta
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing lands in LDS after the workgroup's end
   }
-  store_tile<TO, BM, BN, NTH, ST * kSlabChunks>(lds, acc, wi, wj, out + i0 * a.ldo + j0, a.ldo, rows, cols);
+  if constexpr (GATED) store_gated<TO, BM, BN, NTH, ST * kSlabChunks>(a, lds, acc, wi, wj, i0, j0, rows, cols);
+  else store_tile<TO, BM, BN, NTH, ST * kSlabChunks>(lds, acc, wi, wj, out + i0 * a.ldo + j0, a.ldo, rows, cols);
 }
 #endif
 
@@ -747,7 +817,7 @@ __device__ __forceinline__ Task row_task(const GroupedArgs& a, int ti, int tj) {
   return k;
 }
 
-template <typename T, typename TO, bool A_KR, bool B_KR, int BM, int BN, int WI, int WJ, int ST, Role ROLE>
+template <typename T, typename TO, bool A_KR, bool B_KR, int BM, int BN, int WI, int WJ, int ST, Role ROLE, bool GATED = false>
 __global__ __launch_bounds__(64 * WI * WJ, 2) void grouped_direct_kernel(GroupedArgs a) {
 #ifdef __HIP_DEVICE_COMPILE__
   __shared__ u32x4 lds[ST * kSlabChunks<T, BM, BN, 64 * WI * WJ>];
@@ -768,21 +838,22 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void grouped_direct_kernel(Grouped
       t = whole + t / 4;
     }
     band_tile(t, tiles, a.tiles_j, &ti, &tj);
-    k = row_task<BM, BN>(a, ti, tj);
+    k = row_task<BM, GATED ? BN / 2 : BN>(a, ti, tj);
     if (k.e < 0) return;
     if constexpr (QUARTERS) {
       if (part >= 0) {
-        const int di = part / 2 * 128, dj = part % 2 * 128;
+        constexpr int kCols = GATED ? 64 : 128;
+        const int di = part / 2 * 128, dj = part % 2 * kCols;
         if (di >= k.rows || dj >= k.cols) return;
         k.i0 += di;
         k.j0 += dj;
         k.rows = min(k.rows - di, 128);
-        k.cols = min(k.cols - dj, 128);
-        direct_tile<T, TO, A_KR, B_KR, 128, 128, 2, 4, ST, ROLE>(a, k, lds);
+        k.cols = min(k.cols - dj, kCols);
+        direct_tile<T, TO, A_KR, B_KR, 128, 128, 2, 4, ST, ROLE, GATED>(a, k, lds);
         return;
       }
       if (k.rows <= 128) {  // an expert's last rows
-        direct_tile<T, TO, A_KR, B_KR, 128, 256, 2, 4, ST, ROLE>(a, k, lds);
+        direct_tile<T, TO, A_KR, B_KR, 128, 256, 2, 4, ST, ROLE, GATED>(a, k, lds);
         return;
       }
     }
@@ -800,7 +871,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void grouped_direct_kernel(Grouped
     k.k0 = __builtin_amdgcn_readfirstlane((int)g.lo);
     k.klim = __builtin_amdgcn_readfirstlane((int)g.hi);
   }
-  direct_tile<T, TO, A_KR, B_KR, BM, BN, WI, WJ, ST, ROLE>(a, k, lds);
+  direct_tile<T, TO, A_KR, B_KR, BM, BN, WI, WJ, ST, ROLE, GATED>(a, k, lds);
 #endif
 }
 
@@ -813,26 +884,31 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void grouped_direct_kernel(Grouped
 // rows over 30 of 4096 to 4096 in 8 bits 100 us (5.1); with streaming loads, whose lines leave between their
 // halves, 84 and 111.
 // ---------------------------------------------------------------------------
-template <typename T, typename TO, int FI, int NJ, int WAVES, int U, bool CHUNKS>
+template <typename T, typename TO, int FI, int NJ, int WAVES, int U, bool CHUNKS, bool GATED = false>
 __global__ __launch_bounds__(64 * WAVES) void grouped_few_kernel(GroupedArgs a) {
   constexpr bool MX = __is_same(T, Mx);
+  constexpr int COLS = GATED ? 8 * NJ : 16 * NJ;
+  static_assert(!GATED || (NJ == 2 && !MX), "gates, then values");
   __shared__ f32x4 sum[WAVES][FI * NJ][64];
   const int ti = blockIdx.x / a.tiles_j;
-  const int j0 = (int)(blockIdx.x % a.tiles_j) * 16 * NJ;
+  const int j0 = (int)(blockIdx.x % a.tiles_j) * COLS;
   const RowTile t = find_tile<16 * FI>(a.offsets, a.E, a.R, ti);
   if (t.e < 0) return;
   const int e = __builtin_amdgcn_readfirstlane(t.e);
   const int64_t i0 = __builtin_amdgcn_readfirstlane((int)t.lo);
   const int rows = __builtin_amdgcn_readfirstlane((int)(t.hi - t.lo));
   const int klim = e < a.E ? (int)a.K : 0;
-  const int cols = min((int)a.J - j0, 16 * NJ);
+  const int cols = min((int)a.J - j0, COLS);
   const int lane = threadIdx.x & 63, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t wrow = (int64_t)(e < a.E ? e : 0) * a.J + j0;  // the tile's first weight row
+  const int64_t wrow = (int64_t)(e < a.E ? e : 0) * (GATED ? 2 * a.half : a.J) + j0;  // the tile's first weight row
   const int lda = (int)(a.lda * (int64_t)sizeof(T)), ldb = (int)(a.ldb * (int64_t)sizeof(T));
   const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<char*>((const char*)a.A + i0 * lda), 0, (rows - 1) * lda + klim * (int)sizeof(T), kBufRsrcDword3);
   const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<char*>((const char*)a.B + wrow * ldb), 0, (cols - 1) * ldb + klim * (int)sizeof(T), kBufRsrcDword3);
+  const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<char*>((const char*)a.B + (wrow + (GATED ? a.half : 0)) * ldb), 0, (cols - 1) * ldb + klim * (int)sizeof(T),
+      kBufRsrcDword3);
   const int ns = (int)a.ns;
   const __amdgpu_buffer_rsrc_t rsa = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<uint8_t*>(MX ? a.sa + i0 * a.ns : nullptr), 0, MX ? rows * ns : 0, kBufRsrcDword3);
@@ -857,9 +933,9 @@ __global__ __launch_bounds__(64 * WAVES) void grouped_few_kernel(GroupedArgs a) 
       const bool in = c < klim;
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        const int row = 16 * j + (lane & 15);
-        if constexpr (CHUNKS) u.b[j][h] = __builtin_amdgcn_raw_buffer_load_b128(rb, in ? row * ldb + (4 * h + g) * 16 : kNowhere, unit * 128, 0);
-        else u.b[j][h] = load_chunk<T>((const T*)a.B + (wrow + row) * a.ldb + c, row < cols ? klim - c : 0, klim >= kElems<T>);
+        const int row = (GATED ? 0 : 16 * j) + (lane & 15);
+        if constexpr (CHUNKS) u.b[j][h] = __builtin_amdgcn_raw_buffer_load_b128(GATED && j ? rv : rb, in ? row * ldb + (4 * h + g) * 16 : kNowhere, unit * 128, 0);
+        else u.b[j][h] = load_chunk<T>((const T*)a.B + (wrow + (GATED && j ? a.half : 0) + row) * a.ldb + c, row < cols ? klim - c : 0, klim >= kElems<T>);
       }
 #pragma unroll
       for (int i = 0; i < FI; ++i) {
@@ -941,6 +1017,29 @@ __global__ __launch_bounds__(64 * WAVES) void grouped_few_kernel(GroupedArgs a) 
   __syncthreads();
   TO* out = (TO*)a.out;
   const bool vec = a.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(TO) - 1)) == 0;
+  if constexpr (GATED) {
+    for (int f = wave; f < FI; f += WAVES) {
+      f32x4 s[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        s[j] = sum[0][2 * f + j][lane];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) s[j] += sum[w][2 * f + j][lane];
+      }
+      const int r = 16 * f + (lane & 15), c = 4 * g;
+      if (r >= rows) continue;
+      f32x4 y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = activate(a.act, s[0][i]) * s[1][i];
+      store4(out + (i0 + r) * a.ldo + j0 + c, y, cols - c, vec);
+      if (!a.saved) continue;
+      float* to = a.saved + (i0 + r) * 2 * a.half + j0 + c;
+      const bool whole = a.half % 4 == 0 && (reinterpret_cast<uintptr_t>(a.saved) & 15) == 0;
+      store4(to, s[0], cols - c, whole);
+      store4(to + a.half, s[1], cols - c, whole);
+    }
+    return;
+  }
   for (int f = wave; f < FI * NJ; f += WAVES) {
     f32x4 v = sum[0][f][lane];
 #pragma unroll

@@ -15,6 +15,15 @@ mixture-of-experts feed-forward branch does in between runs on these HIP kernels
 ``quantize_mx`` and ``grouped_matmul_mx`` work in 8 bits: e4m3 values with a power-of-two scale for every
 32 of a row (microscaling), which the matrix instructions of gfx950 multiply in.
 
+A branch that mixes tokens, and a feed-forward that begins with a gated product:
+
+    q, k = rotary(q, k, positions, rotary_frequencies(dim))  # (batch, tokens, heads, dim)
+    o, state = decay_attention(q, k, v, log_decay, return_state=True)
+    o = decay_attention_step(q, k, v, log_decay, state)      # the next token of each sequence, (batch, heads, dim)
+    x = gated_matmul(y, w_gate_up, offsets)                  # act(y gate) * (y up), or without offsets of one weight
+
+``examples/decay_layer.py`` is the whole of it, training, prompts and decoding.
+
 Tensors are fp32, bf16 or fp16 on a ROCm GPU and are computed in fp32; each op runs on the current stream,
 waits for nothing on the host and may be captured in a HIP graph.  Gradients are of the first order in reverse
 mode; second derivatives and, in eager calls, forward mode raise.  Not part of ``mhc.__all__``, which stays the reference's.
@@ -22,6 +31,7 @@ mode; second derivatives and, in eager calls, forward mode raise.  Not part of `
 
 from __future__ import annotations
 
+import math
 from typing import Optional, Tuple, Union
 
 import torch
@@ -30,9 +40,12 @@ from torch.autograd.forward_ad import unpack_dual
 from . import _branch as _k
 from . import _branch_library as _l
 from . import _lib
+from . import _mixer as _m
+from . import _mixer_library as _ml
 from ._branch import Rng
 
-__all__ = ["rms_norm", "rms_norm_mx", "quantize_mx", "grouped_matmul", "grouped_matmul_mx", "dropout"]
+__all__ = ["rms_norm", "rms_norm_mx", "quantize_mx", "grouped_matmul", "grouped_matmul_mx", "dropout",
+           "rotary", "rotary_frequencies", "decay_attention", "decay_attention_step", "gated_matmul"]
 
 
 def _first_order(grad: Optional[torch.Tensor], name: str, *differentiable: bool) -> Optional[torch.Tensor]:
@@ -107,6 +120,66 @@ class _GroupedMatmul(torch.autograd.Function):
             dw = _k.grouped_matmul_backward_weight(dy, x, offsets)
             dw = _first_order(dw, "grouped_matmul", dy.requires_grad, x.requires_grad)
         return dx, dw, None
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, frequencies, interleaved: bool, magnitude: float):
+        ctx.save_for_backward(positions, frequencies)
+        ctx.how = interleaved, magnitude
+        ctx.set_materialize_grads(False)
+        a, b = _m.rotary(q, k, positions, frequencies, interleaved, magnitude)
+        return a if k is None else (a, b)
+
+    @staticmethod
+    def backward(ctx, dq, dk=None):
+        grads = [dq if ctx.needs_input_grad[0] else None, dk if ctx.needs_input_grad[1] else None]
+        have = [i for i in (0, 1) if grads[i] is not None]
+        if have:  # both in one launch
+            got = _m.rotary(grads[have[0]], grads[1] if len(have) == 2 else None, *ctx.saved_tensors, *ctx.how, True)
+            for i, g in zip(have, got):
+                grads[i] = _first_order(g, "rotary", grads[i].requires_grad)
+        return (*grads, None, None, None, None)
+
+
+class _DecayAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, offsets, initial_state, scale: float, return_state: bool):
+        ctx.save_for_backward(q, k, v, log_decay, offsets, initial_state)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        o, state = _m.decay_attention_forward(q, k, v, log_decay, offsets, initial_state, scale, return_state)
+        return (o, state) if return_state else o
+
+    @staticmethod
+    def backward(ctx, do, d_state=None):
+        q, k, v, log_decay, offsets, initial = ctx.saved_tensors
+        need = (*ctx.needs_input_grad[:3], ctx.needs_input_grad[5])
+        if do is None and d_state is None:
+            return (None,) * 8
+        if do is None:
+            do = torch.zeros_like(v, memory_format=torch.contiguous_format)
+        got = _m.decay_attention_backward(q, k, v, do, log_decay, offsets, initial, d_state, ctx.scale, need)
+        graph = [t is not None and t.requires_grad for t in (do, d_state, q, k, v, initial)]
+        dq, dk, dv, ds = (_first_order(g, "decay_attention", *graph) for g in got)
+        return dq, dk, dv, None, None, ds, None, None
+
+
+class _GatedMatmul(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, offsets, activation: str):
+        y, saved = _m.gated_matmul_forward(x, weight, offsets, activation, want_saved=any(ctx.needs_input_grad))
+        ctx.save_for_backward(x, weight, offsets, saved)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, weight, offsets, saved = ctx.saved_tensors
+        need = ctx.needs_input_grad[:2]
+        dx, dw = _m.gated_matmul_backward(dy, saved, x, weight, offsets, ctx.activation, *need)
+        graph = (dy.requires_grad, x.requires_grad, weight.requires_grad)
+        return _first_order(dx, "gated_matmul", *graph), _first_order(dw, "gated_matmul", *graph), None, None
 
 
 def _inference_only(name: str, *tensors) -> None:
@@ -211,3 +284,123 @@ def dropout(x: torch.Tensor, p: float, rng: Rng, residual: Optional[torch.Tensor
         if y is not None:
             return y
     return _Dropout.apply(x, residual, float(p), rng)
+
+
+def rotary_frequencies(dim: int, base: float = 10000.0, factor: float = 1.0, original_length: Optional[int] = None,
+                       fast: float = 32.0, slow: float = 1.0, device=None) -> torch.Tensor:
+    """Radians a position for each of the dim / 2 pairs that ``rotary`` turns, in fp64: ``base ** (-2 i / dim)``.
+
+    For contexts ``factor`` times as long as the trained ones every frequency is divided by factor; with
+    ``original_length``, the trained length, only those that turn fewer than ``slow`` times over it are, those that
+    turn more than ``fast`` times stay, and between them the share falls off linearly in the pair's index.  (Such a
+    context usually takes ``magnitude = 0.1 * log(factor) + 1`` in ``rotary``, too.)"""
+    if dim < 0 or dim % 2:
+        raise ValueError(f"dim must be even, got {dim}")
+    if not (base > 0 and factor > 0):
+        raise ValueError(f"base and factor must be positive, got {base} and {factor}")
+    i = torch.arange(dim // 2, dtype=torch.float64)
+    f = base ** (-2.0 * i / max(dim, 1))
+    if original_length is None:
+        f = f / factor
+    elif factor != 1.0:
+        if not (original_length > 0 and fast > slow > 0 and base > 1):
+            raise ValueError(f"original_length, fast > slow and base > 1 must be positive, got {original_length}, {fast}, "
+                             f"{slow}, {base}")
+
+        def pair_of(turns):  # the index, not whole, of the pair that turns so often over the trained length
+            return dim * math.log(original_length / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
+
+        lo, hi = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), max(dim // 2 - 1, 0))
+        stretched = ((i - lo) / max(hi - lo, 1e-3)).clamp(0.0, 1.0)
+        f = f * (1.0 - stretched) + f / factor * stretched
+    return f.to(device) if device is not None else f
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, frequencies: torch.Tensor,
+           interleaved: bool = False, magnitude: float = 1.0) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """Rotary positions of q (..., heads, dim) and k (..., its own number of heads, dim): ``(q, k)``, or with k None q
+    alone.  A pair (a, b) of a head becomes ``magnitude * (a cos t - b sin t, b cos t + a sin t)``,
+    ``t = position * frequency``.
+
+    ``frequencies`` (pairs,) are radians a position, one for each pair of the head's first 2 * pairs elements (at most
+    4096); the others go through.  Pair i is (i, pairs + i), or (2 i, 2 i + 1) when ``interleaved``.  ``positions``
+    (int32 or int64) has q's leading dimensions or the last of them, (tokens,) for (batch, tokens, heads, dim).
+    Angles are taken in fp64: they are exact to 2^-52 of their size however far the position (int64 up to 2^53).
+
+    q and k are read where they lie if a head's elements are neighbours and one stride leads from row to row, parts of
+    a fused projection's output among them; others are copied.  The results are contiguous.  Differentiable in q and k.
+    """
+    _no_gradient("rotary", frequencies=frequencies)
+    if torch.compiler.is_compiling():
+        return _ml.rotary(q, k, positions, frequencies, bool(interleaved), float(magnitude))
+    return _Rotary.apply(q, k, positions, frequencies, bool(interleaved), float(magnitude))
+
+
+def _no_gradient(name: str, **tensors) -> None:
+    """Refuses gradients of arguments that have none."""
+    for what, t in tensors.items():
+        if isinstance(t, torch.Tensor) and t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"mhc: {name} has no gradient of {what}; detach it")
+
+
+def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
+                    initial_state: Optional[torch.Tensor] = None, offsets: Optional[torch.Tensor] = None,
+                    scale: Optional[float] = None, return_state: bool = False):
+    """Linear attention with a decay for each head: ``S_t = exp(log_decay) S_{t-1} + k_t^T v_t``,
+    ``o_t = scale * q_t S_t``; o as v, or ``(o, state)`` with ``return_state``.
+
+    q and k are (batch, tokens, heads, key dim), v (batch, tokens, heads, value dim), dims from 1 to 128.  With
+    ``offsets`` (sequences,) int32 on the GPU (int64 is narrowed) they are packed, (tokens, heads, dim), and sequence n
+    has tokens ``offsets[n-1]`` to ``offsets[n]``; offsets count clamped and as their running maximum, and are read on the
+    GPU only, so a captured graph serves every split.  Tokens past the last offset give zeros and get zero gradients.
+    ``initial_state`` and the state are (sequences, heads, key dim, value dim) fp32; a sequence without tokens hands its own on.
+    ``log_decay`` (heads,) has no gradient; above 0 it counts as 0.  ``scale`` defaults to ``key dim ** -0.5``.
+
+    Differentiable in q, k, v and initial_state.  Inputs are read where they lie as ``rotary`` reads them (rows at most
+    2^22 elements apart), heads that are one expanded among them.  Sums are fp32; products are of bf16 parts whose sum
+    is the operand, exactly for inputs.  A value that is not finite reaches its own and later tokens of its sequence and
+    head, no others; which of them are infinite and which NaN may differ from the recurrence's.
+    """
+    _no_gradient("decay_attention", log_decay=log_decay)
+    scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
+    if torch.compiler.is_compiling():
+        out = _ml.decay_attention(q, k, v, log_decay, offsets, initial_state, scale)
+        return out if return_state else out[0]
+    return _DecayAttention.apply(q, k, v, log_decay, offsets, initial_state, scale, bool(return_state))
+
+
+def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, state: torch.Tensor,
+                         slots: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                         state_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``decay_attention`` of one more token for each row of q, k (rows, heads, key dim) and v (rows, heads, value dim):
+    o as v, and ``state`` (states, heads, key dim, value dim) fp32, contiguous, moved on in place.
+
+    Row r has state ``slots[r]`` (int32 or int64 on the GPU, read there only), or state r without slots.  Rows with the same
+    slot are tokens of one sequence in their order; a row whose slot is outside the pool (negative: padding of a batch)
+    gives zeros and touches no state, and states of no row stay as they are.  With ``state_out`` the rows' new states go
+    there and ``state`` stays: the one before is kept for tokens that may be taken back.  No backward.
+    """
+    _inference_only("decay_attention_step", q, k, v, log_decay, state, state_out)
+    scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
+    if torch.compiler.is_compiling():
+        return _ml.decay_attention_step(q, k, v, log_decay, state, slots, scale, state_out)
+    o = _m.decay_attention_step(q, k, v, log_decay, state, slots, scale, state_out)
+    out = state if state_out is None else state_out
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+    return o
+
+
+def gated_matmul(x: torch.Tensor, weight: torch.Tensor, offsets: Optional[torch.Tensor] = None,
+                 activation: str = "silu") -> torch.Tensor:
+    """``act(x gate^T) * (x up^T)``: the gated product that a feed-forward begins with, (rows, out) in x's dtype.
+
+    ``weight`` is (2 * out, in), the gate's rows and then the up projection's, for all rows of x (rows, in); with
+    ``offsets`` it is (experts, 2 * out, in) and x's rows are sorted by expert, exactly as in ``grouped_matmul``.
+    ``activation`` is "silu", "gelu" (by the error function) or "gelu_tanh".  Both products are summed, activated and
+    multiplied in fp32 and rounded once.  Differentiable in x and weight; for the backward both products are kept
+    in fp32 (8 * rows * out bytes).
+    """
+    if torch.compiler.is_compiling():
+        return _ml.gated_matmul(x, weight, offsets, activation)
+    return _GatedMatmul.apply(x, weight, offsets, activation)
