@@ -448,7 +448,7 @@ int mhc_rotary(const void* q, int64_t q_row, int64_t q_head, void* q_out, int64_
  * maximum; rows past the last get zeros.  q, k [R,H,Dk], v, o [R,H,Dv] in `dtype`,
  * Dk, Dv <= 128; first, last [N,H,Dk,Dv] f32, the states before and after (NULL: zeros,
  * not wanted).  Rows up to 2^22 elements apart. */
-size_t mhc_decay_attention_workspace_bytes(int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv, int packed);
+size_t mhc_decay_attention_workspace_bytes(int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv, int packed, int dtype);
 
 int mhc_decay_attention_forward(const void* q, int64_t q_row, int64_t q_head,
                                 const void* k, int64_t k_row, int64_t k_head,
@@ -458,17 +458,20 @@ int mhc_decay_attention_forward(const void* q, int64_t q_row, int64_t q_head,
                                 int64_t N, int64_t H, int64_t Dk, int64_t Dv, float scale,
                                 void* workspace, size_t workspace_bytes, mhc_stream_t stream);
 
-size_t mhc_decay_attention_backward_workspace_bytes(int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv, int packed);
+size_t mhc_decay_attention_backward_workspace_bytes(int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv, int packed,
+                                                    int dtype);
 
 /* dq, dk, dv (as q, k, v, contiguous) and d_first from dout and d_last; any of them,
- * first and d_last may be NULL.  Rows of no sequence get zeros. */
+ * first and d_last may be NULL.  Rows of no sequence get zeros.  kept: the forward's
+ * workspace as that call (same sizes, operands and first) left it, or NULL: its
+ * segments' states are then computed again. */
 int mhc_decay_attention_backward(const void* q, int64_t q_row, int64_t q_head,
                                  const void* k, int64_t k_row, int64_t k_head,
                                  const void* v, int64_t v_row, int64_t v_head,
                                  const void* dout, int64_t do_row, int64_t do_head, int dtype,
                                  const float* log_decay, const int32_t* offsets,
-                                 const float* first, const float* d_last, void* dq, void* dk,
-                                 void* dv, float* d_first, int64_t R, int64_t N, int64_t H,
+                                 const float* first, const float* kept, const float* d_last,
+                                 void* dq, void* dk, void* dv, float* d_first, int64_t R, int64_t N, int64_t H,
                                  int64_t Dk, int64_t Dv, float scale, void* workspace,
                                  size_t workspace_bytes, mhc_stream_t stream);
 

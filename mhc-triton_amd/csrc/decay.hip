@@ -13,9 +13,12 @@ namespace mhc {
 // kLeast: each costs a state written and read again by those behind it.
 constexpr int64_t kLeast = 512;
 
-static int64_t segment_tokens(int64_t R, int64_t N, int64_t H, int64_t Dv, bool packed) {
+// Columns of the state that a workgroup holds.  fp32 planes of 128 columns do not fit in LDS.
+static int64_t group_cols(int64_t Dv, int dtype) { return Dv <= 64 || dtype == MHC_DTYPE_F32 ? 64 : 128; }
+
+static int64_t segment_tokens(int64_t R, int64_t N, int64_t H, int64_t Dv, bool packed, int dtype) {
   const int64_t longest = packed || N == 0 ? R : R / N;
-  const int64_t heads = H * ((Dv + kStateCols - 1) / kStateCols);
+  const int64_t heads = H * ((Dv + group_cols(Dv, dtype) - 1) / group_cols(Dv, dtype));
   const int64_t sequences = packed ? 1 : N;
   int64_t want = 2 * num_cus() / (heads * sequences > 0 ? heads * sequences : 1);
   if (want < 1) want = 1;
@@ -30,25 +33,32 @@ static int64_t count_tiles(int64_t R, int64_t N, int64_t seg, bool packed) {
   return N * (T > seg ? (T + seg - 1) / seg : 1);
 }
 
-static int64_t parts_bytes(int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv, bool packed) {
-  const int64_t seg = segment_tokens(R, N, H, Dv, packed);
-  if ((packed || N == 0 ? R : R / N) <= seg) return 0;
-  return count_tiles(R, N, seg, packed) * H * Dk * Dv * 4;
+// A scan's segments and what the states that they leave take.
+struct Plan {
+  int64_t seg, tiles, bytes;  // bytes 0: no sequence has a second segment
+};
+static Plan plan_scan(int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv, bool packed, int dtype) {
+  Plan p;
+  p.seg = segment_tokens(R, N, H, Dv, packed, dtype);
+  p.tiles = count_tiles(R, N, p.seg, packed);
+  p.bytes = (packed || N == 0 ? R : R / N) > p.seg ? p.tiles * H * Dk * Dv * 4 : 0;
+  return p;
 }
 
-template <typename T, int DK, bool CHUNKS>
-static int launch_scan(const DecayArgs& a, bool parts, const char* who, hipStream_t st) {
-  const int64_t units = ((int64_t)a.tiles * a.H + 7) / 8 * 8;
-  if (units * a.col_tiles * kThreads >= ((int64_t)1 << 32)) {
-    set_error("%s: %lld workgroups are too many for a call", who, (long long)(units * a.col_tiles));
+template <typename T, int DK, int WAVES, int WEIGHTED, bool CHUNKS>
+static int launch_scan(DecayJobs& jobs, bool states, bool outputs, const char* who, hipStream_t st) {
+  constexpr int NTH = 64 * WAVES;
+  const DecayArgs& a = jobs.job[0];
+  const int col_tiles = (a.Dv + 16 * WAVES - 1) / (16 * WAVES);
+  for (int j = 0; j < jobs.n; ++j) jobs.job[j].col_tiles = col_tiles;
+  const int64_t groups = ((int64_t)a.tiles * a.H + 7) / 8 * 8 * col_tiles * jobs.n;
+  if (groups * NTH >= ((int64_t)1 << 32)) {
+    set_error("%s: %lld workgroups are too many for a call", who, (long long)groups);
     return MHC_ERR_ARG;
   }
-  const dim3 grid((unsigned)(units * a.col_tiles));
-  if (parts) {
-    decay_kernel<T, DK, CHUNKS, true><<<grid, kThreads, 0, st>>>(a);
-    if (int rc = hip_status(hipGetLastError(), who)) return rc;
-  }
-  decay_kernel<T, DK, CHUNKS, false><<<grid, kThreads, 0, st>>>(a);
+  const dim3 grid((unsigned)groups);
+  if (states) decay_kernel<T, DK, WAVES, WEIGHTED, CHUNKS, true><<<grid, NTH, 0, st>>>(jobs);
+  if (outputs) decay_kernel<T, DK, WAVES, WEIGHTED, CHUNKS, false><<<grid, NTH, 0, st>>>(jobs);
   return hip_status(hipGetLastError(), who);
 }
 
@@ -57,25 +67,43 @@ static bool whole_chunks(const void* p, int64_t row, int64_t head, int64_t D) {
   return aligned16(p) && row % kElems<T> == 0 && head % kElems<T> == 0 && D % kElems<T> == 0;
 }
 
+// The segments' states (needed where there are several), or the outputs, of scans alike in their plan and in how many
+// halves of 128 their dims take.  exact: a last state is to come of them.
+enum { kStates = 1, kOutputs = 2 };
 template <typename T>
-static int scan(DecayArgs a, void* workspace, const char* who, hipStream_t st) {
-  const bool packed = a.offsets != nullptr;
-  a.T = a.N ? a.R / a.N : 0;
-  const int64_t seg = segment_tokens(a.R, a.N, a.H, a.Dv, packed);
-  a.seg = (int)seg;
-  const int64_t tiles = count_tiles(a.R, a.N, seg, packed);
-  if (tiles * a.H >= ((int64_t)1 << 31) - 8) {
-    set_error("%s: %lld segments of %d heads are too many for a call", who, (long long)tiles, a.H);
-    return MHC_ERR_ARG;
+static int scan(DecayJobs jobs, const Plan& plan, int what, bool exact, const char* who, hipStream_t st) {
+  bool chunks = true;
+  for (int j = 0; j < jobs.n; ++j) {
+    DecayArgs& a = jobs.job[j];
+    if (plan.tiles * a.H >= ((int64_t)1 << 31) - 8) {
+      set_error("%s: %lld segments of %d heads are too many for a call", who, (long long)plan.tiles, a.H);
+      return MHC_ERR_ARG;
+    }
+    a.T = a.N ? a.R / a.N : 0;
+    a.seg = (int)plan.seg;
+    a.tiles = (int)plan.tiles;
+    chunks = chunks && whole_chunks<T>(a.q, a.q_row, a.q_head, a.Dk) && whole_chunks<T>(a.k, a.k_row, a.k_head, a.Dk) &&
+             whole_chunks<T>(a.v, a.v_row, a.v_head, a.Dv) && aligned16(a.o);
   }
-  a.tiles = (int)tiles;
-  a.col_tiles = (a.Dv + kStateCols - 1) / kStateCols;
-  a.parts = (float*)workspace;
-  const bool parts = parts_bytes(a.R, a.N, a.H, a.Dk, a.Dv, packed) != 0;
-  const bool chunks = whole_chunks<T>(a.q, a.q_row, a.q_head, a.Dk) && whole_chunks<T>(a.k, a.k_row, a.k_head, a.Dk) &&
-                      whole_chunks<T>(a.v, a.v_row, a.v_head, a.Dv);
-  if (chunks) return a.Dk <= 64 ? launch_scan<T, 64, true>(a, parts, who, st) : launch_scan<T, 128, true>(a, parts, who, st);
-  return a.Dk <= 64 ? launch_scan<T, 64, false>(a, parts, who, st) : launch_scan<T, 128, false>(a, parts, who, st);
+  const bool states = what & kStates && plan.bytes, outputs = what & kOutputs;
+  const DecayArgs& a = jobs.job[0];
+  auto launch = [&](auto w, auto parts) {
+    constexpr int WAVES = decltype(w)::value, WEIGHTED = decltype(parts)::value;
+    if (chunks)
+      return a.Dk <= 64 ? launch_scan<T, 64, WAVES, WEIGHTED, true>(jobs, states, outputs, who, st)
+                        : launch_scan<T, 128, WAVES, WEIGHTED, true>(jobs, states, outputs, who, st);
+    return a.Dk <= 64 ? launch_scan<T, 64, WAVES, WEIGHTED, false>(jobs, states, outputs, who, st)
+                      : launch_scan<T, 128, WAVES, WEIGHTED, false>(jobs, states, outputs, who, st);
+  };
+  using std::integral_constant;
+  if constexpr (sizeof(T) == 4) {
+    return launch(integral_constant<int, 4>(), integral_constant<int, 3>());
+  } else {
+    if (exact) return a.Dv > 64 ? launch(integral_constant<int, 8>(), integral_constant<int, 3>())
+                                : launch(integral_constant<int, 4>(), integral_constant<int, 3>());
+    return a.Dv > 64 ? launch(integral_constant<int, 8>(), integral_constant<int, 2>())
+                     : launch(integral_constant<int, 4>(), integral_constant<int, 2>());
+  }
 }
 
 constexpr int64_t kMaxHeadDim = 128;
@@ -124,9 +152,10 @@ static int launch_step(DecayStepArgs a, const char* who, hipStream_t st) {
 
 using namespace mhc;
 
-extern "C" size_t mhc_decay_attention_workspace_bytes(int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv, int packed) {
+extern "C" size_t mhc_decay_attention_workspace_bytes(int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv, int packed,
+                                                      int dtype) {
   if (R <= 0 || N < 0 || H <= 0 || Dk <= 0 || Dv <= 0) return 0;
-  return (size_t)parts_bytes(R, N, H, Dk, Dv, packed);
+  return (size_t)plan_scan(R, N, H, Dk, Dv, packed, dtype).bytes;
 }
 
 extern "C" int mhc_decay_attention_forward(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
@@ -138,72 +167,114 @@ extern "C" int mhc_decay_attention_forward(const void* q, int64_t q_row, int64_t
   if (int rc = check_decay(who, R, N, H, Dk, Dv, offsets != nullptr, {q_row, k_row, v_row})) return rc;
   if (H == 0 || (R == 0 && (N == 0 || !last))) return MHC_OK;
   if (!log_decay || (R && (!q || !k || !v || !o))) return null_in(who);
-  const size_t need = mhc_decay_attention_workspace_bytes(R, N, H, Dk, Dv, offsets != nullptr);
+  const size_t need = mhc_decay_attention_workspace_bytes(R, N, H, Dk, Dv, offsets != nullptr, dtype);
   if (int rc = check_workspace(who, workspace, workspace_bytes, need)) return rc;
-  DecayArgs a{};
+  DecayJobs jobs{};
+  jobs.n = 1;
+  DecayArgs& a = jobs.job[0];
   a.q = q; a.k = k; a.v = v; a.o = o; a.log_decay = log_decay; a.offsets = offsets; a.first = first; a.last = last;
   a.q_row = q_row; a.q_head = q_head; a.k_row = k_row; a.k_head = k_head; a.v_row = v_row; a.v_head = v_head;
-  a.state_row = Dv; a.state_col = 1;
+  a.state_row = (int)Dv; a.state_col = 1;
+  a.parts = (float*)workspace; a.part_row = (int)Dv; a.part_col = 1;
   a.R = R; a.N = (int)N; a.H = (int)H; a.Dk = (int)Dk; a.Dv = (int)Dv;
   a.out_scale = scale; a.in_scale = 1.f; a.lag = 1;
-  return MHC_DISPATCH_DTYPE(dtype, [&] { return scan<T>(a, workspace, who, (hipStream_t)stream); });
+  const Plan plan = plan_scan(R, N, H, Dk, Dv, offsets != nullptr, dtype);
+  return MHC_DISPATCH_DTYPE(dtype, [&] {
+    return scan<T>(jobs, plan, kStates | kOutputs, last != nullptr, who, (hipStream_t)stream);
+  });
 }
 
+// Whether scans over states of Dk x Dv and of Dv x Dk run side by side: the same kernel, segments and column tiles.
+static bool alike(int64_t Dk, int64_t Dv) { return (Dk <= 64) == (Dv <= 64); }
+
+// The states that the segments of the backward scans (dv's and dk's) leave, and those of the forward where the caller
+// did not keep them; scans that are not alike have a plan and states each.
 extern "C" size_t mhc_decay_attention_backward_workspace_bytes(int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv,
-                                                               int packed) {
-  const size_t x = mhc_decay_attention_workspace_bytes(R, N, H, Dk, Dv, packed);
-  const size_t y = mhc_decay_attention_workspace_bytes(R, N, H, Dv, Dk, packed);
-  return x > y ? x : y;
+                                                               int packed, int dtype) {
+  return mhc_decay_attention_workspace_bytes(R, N, H, Dk, Dv, packed, dtype) +
+         mhc_decay_attention_workspace_bytes(R, N, H, Dv, Dk, packed, dtype);
 }
 
 extern "C" int mhc_decay_attention_backward(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
                                             int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const void* dout,
                                             int64_t do_row, int64_t do_head, int dtype, const float* log_decay,
-                                            const int32_t* offsets, const float* first, const float* d_last, void* dq,
-                                            void* dk, void* dv, float* d_first, int64_t R, int64_t N, int64_t H,
-                                            int64_t Dk, int64_t Dv, float scale, void* workspace, size_t workspace_bytes,
-                                            mhc_stream_t stream) {
+                                            const int32_t* offsets, const float* first, const float* kept,
+                                            const float* d_last, void* dq, void* dk, void* dv, float* d_first, int64_t R,
+                                            int64_t N, int64_t H, int64_t Dk, int64_t Dv, float scale, void* workspace,
+                                            size_t workspace_bytes, mhc_stream_t stream) {
   const char* who = "decay_attention_backward";
   if (int rc = check_decay(who, R, N, H, Dk, Dv, offsets != nullptr, {q_row, k_row, v_row, do_row})) return rc;
   if (H == 0 || (R == 0 && (N == 0 || !d_first))) return MHC_OK;
   if (!log_decay || (R && (!q || !k || !v || !dout))) return null_in(who);
-  const size_t need = mhc_decay_attention_backward_workspace_bytes(R, N, H, Dk, Dv, offsets != nullptr);
+  const bool packed = offsets != nullptr, same = alike(Dk, Dv);
+  const size_t need = mhc_decay_attention_backward_workspace_bytes(R, N, H, Dk, Dv, packed, dtype);
   if (int rc = check_workspace(who, workspace, workspace_bytes, need)) return rc;
+  // of states with Dv columns, and of the transposed ones
+  const Plan plan = plan_scan(R, N, H, Dk, Dv, packed, dtype), across = plan_scan(R, N, H, Dv, Dk, packed, dtype);
   DecayArgs base{};
   base.log_decay = log_decay; base.offsets = offsets;
   base.R = R; base.N = (int)N; base.H = (int)H;
+  const int dims[2] = {(int)Dk, (int)Dv};
+
+  // dq: from the first token on, states transposed.  Its segments' states are the forward's.
+  DecayArgs of_q = base;
+  of_q.q = dout; of_q.q_row = do_row; of_q.q_head = do_head;
+  of_q.k = v; of_q.k_row = v_row; of_q.k_head = v_head;
+  of_q.v = k; of_q.v_row = k_row; of_q.v_head = k_head;
+  of_q.o = dq; of_q.first = first; of_q.state_row = 1; of_q.state_col = dims[1];
+  of_q.Dk = dims[1]; of_q.Dv = dims[0];
+  of_q.out_scale = scale; of_q.in_scale = 1.f; of_q.lag = 1;
+  const bool have = same && kept;
+  of_q.parts = have ? const_cast<float*>(kept) : (float*)workspace;
+  of_q.part_row = have ? 1 : dims[0]; of_q.part_col = have ? dims[1] : 1;
+  // dv and dk: from the last token back, with the same states, dk's transposed
+  base.first = d_last;
+  base.out_scale = 1.f; base.in_scale = scale; base.lag = 0; base.reverse = true;
+  base.parts = (float*)((char*)workspace + across.bytes);
+  DecayArgs of_v = base;
+  of_v.q = k; of_v.q_row = k_row; of_v.q_head = k_head;
+  of_v.k = q; of_v.k_row = q_row; of_v.k_head = q_head;
+  of_v.v = dout; of_v.v_row = do_row; of_v.v_head = do_head;
+  of_v.o = dv; of_v.last = d_first; of_v.state_row = dims[1]; of_v.state_col = 1;
+  of_v.part_row = dims[1]; of_v.part_col = 1;
+  of_v.Dk = dims[0]; of_v.Dv = dims[1];
+  DecayArgs of_k = base;
+  of_k.q = v; of_k.q_row = v_row; of_k.q_head = v_head;
+  of_k.k = dout; of_k.k_row = do_row; of_k.k_head = do_head;
+  of_k.v = q; of_k.v_row = q_row; of_k.v_head = q_head;
+  of_k.o = dk; of_k.state_row = 1; of_k.state_col = dims[1];
+  of_k.Dk = dims[1]; of_k.Dv = dims[0];
+
+  const bool want_q = dq && R, want_v = dv || (d_first && !dk), want_k = dk != nullptr, exact = d_first != nullptr;
+  if (want_k && !want_v) of_k.last = d_first;
   return MHC_DISPATCH_DTYPE(dtype, [&]() -> int {
-    if (dq && R) {
-      DecayArgs a = base;
-      a.q = dout; a.q_row = do_row; a.q_head = do_head;
-      a.k = v; a.k_row = v_row; a.k_head = v_head;
-      a.v = k; a.v_row = k_row; a.v_head = k_head;
-      a.o = dq; a.first = first; a.state_row = 1; a.state_col = Dv;
-      a.Dk = (int)Dv; a.Dv = (int)Dk;
-      a.out_scale = scale; a.in_scale = 1.f; a.lag = 1;
-      if (int rc = scan<T>(a, workspace, who, (hipStream_t)stream)) return rc;
+    const hipStream_t st = (hipStream_t)stream;
+    auto one = [&](const DecayArgs& a, const Plan& p, int what, bool fine) {
+      DecayJobs jobs{};
+      jobs.n = 1;
+      jobs.job[0] = a;
+      return scan<T>(jobs, p, what, fine, who, st);
+    };
+    if (!same) {  // each by itself; dk's states take dq's place in the workspace
+      of_k.parts = (float*)workspace; of_k.part_row = dims[0]; of_k.part_col = 1;
+      if (want_q)
+        if (int rc = one(of_q, across, kStates | kOutputs, false)) return rc;
+      if (want_v)
+        if (int rc = one(of_v, plan, kStates | kOutputs, exact)) return rc;
+      if (want_k) return one(of_k, across, kStates | kOutputs, of_k.last != nullptr);
+      return MHC_OK;
     }
-    base.first = d_last;
-    base.out_scale = 1.f; base.in_scale = scale; base.lag = 0; base.reverse = true;
-    if (dv || (d_first && !dk)) {
-      DecayArgs a = base;
-      a.q = k; a.q_row = k_row; a.q_head = k_head;
-      a.k = q; a.k_row = q_row; a.k_head = q_head;
-      a.v = dout; a.v_row = do_row; a.v_head = do_head;
-      a.o = dv; a.last = d_first; a.state_row = Dv; a.state_col = 1;
-      a.Dk = (int)Dk; a.Dv = (int)Dv;
-      if (int rc = scan<T>(a, workspace, who, (hipStream_t)stream)) return rc;
-    }
-    if (dk) {
-      DecayArgs a = base;
-      a.q = v; a.q_row = v_row; a.q_head = v_head;
-      a.k = dout; a.k_row = do_row; a.k_head = do_head;
-      a.v = q; a.v_row = q_row; a.v_head = q_head;
-      a.o = dk; a.last = dv ? nullptr : d_first; a.state_row = 1; a.state_col = Dv;
-      a.Dk = (int)Dv; a.Dv = (int)Dk;
-      if (int rc = scan<T>(a, workspace, who, (hipStream_t)stream)) return rc;
-    }
-    return MHC_OK;
+    // dv's states serve dk, transposed
+    of_k.part_row = want_v ? 1 : dims[0]; of_k.part_col = want_v ? dims[1] : 1;
+    if (want_q && !have)
+      if (int rc = one(of_q, across, kStates, false)) return rc;
+    if (want_v || want_k)
+      if (int rc = one(want_v ? of_v : of_k, want_v ? plan : across, kStates, exact)) return rc;
+    DecayJobs jobs{};
+    if (want_q) jobs.job[jobs.n++] = of_q;
+    if (want_v) jobs.job[jobs.n++] = of_v;
+    if (want_k) jobs.job[jobs.n++] = of_k;
+    return jobs.n ? scan<T>(jobs, plan, kOutputs, exact, who, st) : MHC_OK;
   });
 }
 

@@ -10,15 +10,17 @@
 // a state that the last token has already entered, and the scale is b, because that gradient has none.  A chunk of 64 tokens is matrix products: P = (Q K^T) o (weights, lower triangle),
 // O = P V + weights Q X, X' = l^n X + (K^T) (weighted V).
 //
-// A workgroup takes a segment of a sequence, a head and 64 of the state's columns; each of its four waves holds
+// A workgroup of WAVES waves takes a segment of a sequence, a head and 16 WAVES of the state's columns; each wave holds
 // 16 columns of the state, all rows, in registers from the first chunk to the last, and never passes it on.  Q, K
-// and V of a chunk go through LDS, the next chunk's are in flight.  P is made once for the four waves and passes
-// through LDS.  Segments but the last are first run for their state alone (STATE_ONLY), so that long sequences with
+// and V of a chunk go through LDS; P is made once for all waves and passes through LDS.  Registers are held below 128
+// for bf16, for four waves a SIMD: phases that wait for LDS, for the matrix cores and for the VALU then overlap.
+// Segments but the last are first run for their state alone (STATE_ONLY), so that long sequences with
 // few heads fill the card; each then starts from the sum of the states before it.
 //
 // Precision.  The matrix instructions multiply bf16.  Every operand is a sum of bf16 parts: inputs exactly (bf16 one part,
 // fp16 two, fp32 three), what is computed (P, the state, weighted V) in as many as keep the error far below one rounding to the
-// output's type (two for 16-bit types, three for fp32); the states go out in fp32, so weighted V has three in every type.
+// output's type (two for 16-bit types, three for fp32).  Where the last state is wanted, which is fp32, weighted V has three
+// (WEIGHTED; two in its place are 16 matrix and 40 VALU instructions fewer a wave and chunk).
 // Products of parts whose size is below the last part's are left out.  Sums are fp32.
 #pragma once
 
@@ -26,12 +28,12 @@
 
 namespace mhc {
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
 constexpr int kChunk = 64;     // tokens of a chunk
-constexpr int kStateCols = 64; // columns of the state that a workgroup holds
 
 template <typename T> constexpr int kRaw = sizeof(T) == 4 ? 3 : (__is_same(T, __bf16) ? 1 : 2);  // parts of an input
-template <typename T> constexpr int kMade = sizeof(T) == 4 ? 3 : 2;                             // of P and the state
-constexpr int kWeighted = 3;                                                                     // of weighted V
+template <typename T> constexpr int kMade = sizeof(T) == 4 ? 3 : 2;                              // of P and the state
 
 struct DecayArgs {
   const void *q, *k, *v;
@@ -42,12 +44,21 @@ struct DecayArgs {
   float* last;               // where X goes, or null
   float* parts;              // states that segments leave by themselves, [tile][H][Dk][Dv]
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;  // strides in elements; o is contiguous
-  int64_t state_row, state_col;                         // of first and last: X's rows and columns
+  int state_row, state_col;                             // of first and last: X's rows and columns
+  int part_row, part_col;                               // of parts
   int64_t R, T;
   int H, N, Dk, Dv, seg, tiles, col_tiles;
   float out_scale, in_scale;  // a, b
   int lag;                    // L
   bool reverse;
+};
+
+// Scans that run side by side: the three gradients read the same four tensors, and their workgroups of a segment and
+// head are neighbours, so that the second and the third find them in the caches.
+constexpr int kMaxJobs = 3;
+struct DecayJobs {
+  DecayArgs job[kMaxJobs];
+  int n;
 };
 
 // Segment `s` of sequence e, whose rows are lo to hi; e = N: rows past the last sequence; -1: none.
@@ -133,73 +144,93 @@ __device__ __forceinline__ void split8(float (&f)[8], u32x4 (&out)[P]) {
   for (int p = 0; p < P; ++p) out[p] = u32x4{t[p][0], t[p][1], t[p][2], t[p][3]};
 }
 
-// A plane of 64 rows of bf16, D = 128 or 64 columns, in 16-byte chunks.  Of the rows that half a wave (transposed
-// reads: eight rows of two chunks each) or a quarter (plain reads: 16 rows of one) reads at a time no two meet in a bank.
-template <int D>
-__device__ __forceinline__ int plane_slot(int r, int c) {
-  static_assert(D == 64 || D == 128, "rows of 8 or 16 chunks");
-  const int s = D == 128 ? ((r & 7) << 1 | ((r >> 3) & 1)) : (((r >> 1) & 3) << 1 | ((r >> 3) & 1));
-  return r * (D / 8) + (c ^ s);
-}
-// P: read plainly only; columns in the order in which the lanes' k run (below).
-__device__ __forceinline__ int p_slot(int r, int c) { return r * 8 + (c ^ ((r >> 1) & 7)); }
+// A plane of 64 rows of bf16, D = 128 or 64 columns, as 16-byte chunks, each row followed by an empty one: every lane's
+// accesses lie at constant distances from one address, and of the rows that half a wave (transposed reads: every second
+// of 16 rows, two chunks each) or 16 lanes (plain reads: a chunk of 16 rows) read at a time no two meet in a bank.
+template <int D> constexpr int kPitch = D / 8 + 1;
+template <int D> constexpr int kPlane = kChunk * kPitch<D>;
 
-// Which token (or state row) of 32 the e-th k of lane group g is: two runs of four, because that is what a transposed
-// read or two tiles of a product's result give a lane.
-__device__ __forceinline__ int order(int g, int e) { return 16 * (e >> 2) + 4 * g + (e & 3); }
+// Which of 32 tokens the e-th k of lane group g is, and which of 16 keys row m of a product's tile is, so that a lane's
+// four results are four neighbouring k of P.
+__device__ __forceinline__ int token_of(int g, int e) { return 16 * (e >> 2) + 8 * (g & 1) + 2 * (e & 3) + (g >> 1); }
+__device__ __forceinline__ int key_of(int m) { return 8 * ((m >> 2) & 1) + 2 * (m & 3) + (m >> 3); }
+// Which of 16 rows of X its tile td holds as row 4 g.  Odd tiles swap neighbouring lane groups, so that the two runs of
+// four that a lane reads of a row of Q for two tiles never share a bank with another lane's.
+__device__ __forceinline__ int run_of(int td, int g) { return 4 * (td & 1 ? g ^ 1 : g); }
 
-// Transposed: columns c0 .. c0 + 15 of tokens 32 ks .. 32 ks + 31; lane % 16 gets its column's eight tokens in order().
-template <int D>
+// Transposed: columns c0 .. c0 + 15 of tokens 32 ks .. 32 ks + 31; lane % 16 gets its column's eight, token_of(g, e).
+// SWAP: with neighbouring runs of four columns swapped.
+template <int D, bool SWAP = false>
 __device__ __forceinline__ u32x4 read_columns(const u32x4* plane, int c0, int ks) {
 #ifdef __HIP_DEVICE_COMPILE__
   const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
-  const int r = 32 * ks + 4 * g + (i >> 2), c = (c0 >> 3) + ((i & 3) >> 1);
-  const char* p = reinterpret_cast<const char*>(plane) + (i & 1) * 8;
-  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + plane_slot<D>(r, c) * 16));
-  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + plane_slot<D>(r + 16, c) * 16));
+  const char* p = reinterpret_cast<const char*>(plane) + token_of(g, i >> 2) * kPitch<D> * 16 + ((i & 3) ^ (SWAP ? 1 : 0)) * 8;
+  p += (32 * ks * kPitch<D> + (c0 >> 3)) * 16;
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 16 * kPitch<D> * 16));
   return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 #else
   return u32x4{};
 #endif
 }
-// Row r0 + lane % 16, columns 32 ks .. 32 ks + 31 as they lie, or (ORDERED) in order().
-template <int D, bool ORDERED>
+// Row r0 + lane % 16 (KEYS: r0 + key_of(lane % 16)), columns 32 ks .. 32 ks + 31 as they lie.
+template <int D, bool KEYS = false>
 __device__ __forceinline__ u32x4 read_rows(const u32x4* plane, int r0, int ks) {
-  const int lane = threadIdx.x & 63, g = lane >> 4, r = r0 + (lane & 15);
-  if constexpr (!ORDERED) return plane[plane_slot<D>(r, 4 * ks + g)];
-  const uint64_t* p = reinterpret_cast<const uint64_t*>(plane);
-  const uint64_t lo = p[2 * plane_slot<D>(r, 4 * ks + (g >> 1)) + (g & 1)];
-  const uint64_t hi = p[2 * plane_slot<D>(r, 4 * ks + 2 + (g >> 1)) + (g & 1)];
+  const int lane = threadIdx.x & 63, r = KEYS ? key_of(lane & 15) : lane & 15;
+  return plane[r * kPitch<D> + (lane >> 4) + r0 * kPitch<D> + 4 * ks];
+}
+// The same columns in the order in which two tiles of X hold their rows: run_of(0, g) of the first 16, run_of(1, g) of the
+// second.
+template <int D>
+__device__ __forceinline__ u32x4 read_rows_tiled(const u32x4* plane, int r0, int ks) {
+  const int lane = threadIdx.x & 63, g = lane >> 4;
+  const uint64_t* p = reinterpret_cast<const uint64_t*>(plane) + 2 * (lane & 15) * kPitch<D> + 2 * (r0 * kPitch<D> + 4 * ks);
+  const uint64_t lo = p[g], hi = p[4 + (g ^ 1)];
   return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
 }
 
 // A chunk's rows of one operand: global memory -> registers -> planes of parts.  CHUNKS: whole aligned vectors.
-template <typename T, int D, bool CHUNKS>
+template <typename T, int D, int NTH, bool CHUNKS>
 struct Feed {
-  static constexpr int PER = D / 8, CH = kChunk * PER / kThreads;  // eights of a row; eights of a thread
-  static constexpr int W = sizeof(T) / 2;                          // 16-byte loads of an eight
+  static constexpr int PER = D / 8, CH = kChunk * PER / NTH;  // eights of a row; eights of a thread
+  static constexpr int W = sizeof(T) / 2;                     // 16-byte loads of an eight
+  static constexpr int ROWS = NTH / PER;                      // rows that the workgroup brings at a time
   u32x4 r[CH][W];
+  int first, step;  // CHUNKS: byte offset of the thread's first eight, and from one to the next
 
-  // Token i < n is row i of `base`, or (reverse) row n - 1 - i; rows of `ld` elements, of which `cols` exist.
+  // Rows of `ld` elements, of which `cols` exist.
+  __device__ __forceinline__ Feed(int64_t ld, int cols, bool reverse) {
+    const int i = (int)threadIdx.x / PER, c = (int)threadIdx.x % PER * 8;
+    first = c < cols ? (int)((reverse ? kChunk - 1 - i : i) * ld + c) * (int)sizeof(T) : kNowhere;
+    step = (int)(reverse ? -ROWS * ld : ROWS * ld) * (int)sizeof(T);
+  }
+
+  // The n rows from `base` on become the chunk's last n, in their order or (reverse) the other way round, behind zeros.
+  // Ranges are checked by the buffer, below its start as offsets past its end: a branch around the loads would have the
+  // compiler wait for all of them, and the stores behind them, at once.
   __device__ __forceinline__ void load(const T* base, int64_t ld, int cols, int n, bool reverse) {
-    [[maybe_unused]] const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<T*>(base), 0, (int)(((n - 1) * ld + cols) * (int64_t)sizeof(T)), kBufRsrcDword3);
+    if constexpr (CHUNKS) {
+      const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<T*>(base), 0, n > 0 ? (int)(((n - 1) * ld + cols) * (int64_t)sizeof(T)) : 0, kBufRsrcDword3);
+      const int back = reverse ? 0 : (int)((kChunk - n) * ld) * (int)sizeof(T);
 #pragma unroll
-    for (int q = 0; q < CH; ++q) {
-      const int at = q * kThreads + threadIdx.x, i = at / PER, c = at % PER * 8;
-      const int row = reverse ? n - 1 - i : i;
-      if constexpr (CHUNKS) {
+      for (int q = 0; q < CH; ++q)
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-          const int off = (int)(row * ld + c + 4 * w) * (int)sizeof(T);
-          const bool in = i < n && c + 4 * w < cols;
-          r[q][w] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, in ? off : kNowhere, 0, 0);
+          // an eight of fp32 may end behind its first half
+          const bool in = w == 0 || (int)threadIdx.x % PER * 8 + 4 * w < cols;
+          r[q][w] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, in ? first + q * step - back + 16 * w : kNowhere, 0, 0);
         }
-      } else {
+    } else {
+#pragma unroll
+      for (int q = 0; q < CH; ++q) {
+        const int at = q * NTH + threadIdx.x, i = at / PER, c = at % PER * 8;
+        const int row = reverse ? kChunk - 1 - i : i - (kChunk - n);
+        const bool in = row >= 0 && row < n;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-          const int left = i < n ? cols - c - 4 * w : 0;
-          r[q][w] = load_chunk<T>(base + (i < n ? row * ld + c + 4 * w : 0), left, cols >= kElems<T>);
+          const int left = in ? cols - c - 4 * w : 0;
+          r[q][w] = load_chunk<T>(base + (in ? row * ld + c + 4 * w : 0), left, cols >= kElems<T>);
         }
       }
     }
@@ -209,7 +240,7 @@ struct Feed {
   __device__ __forceinline__ void store(u32x4* planes) const {
 #pragma unroll
     for (int q = 0; q < CH; ++q) {
-      const int at = q * kThreads + threadIdx.x, slot = plane_slot<D>(at / PER, at % PER);
+      const int at = q * NTH + threadIdx.x, slot = at / PER * kPitch<D> + at % PER;
       if constexpr (__is_same(T, __bf16)) {
         planes[slot] = r[q][0];
       } else {
@@ -223,7 +254,7 @@ struct Feed {
         u32x4 p[kRaw<T>];
         split8<kRaw<T>>(f, p);
 #pragma unroll
-        for (int i = 0; i < kRaw<T>; ++i) planes[i * kChunk * PER + slot] = p[i];
+        for (int i = 0; i < kRaw<T>; ++i) planes[i * kPlane<D> + slot] = p[i];
       }
     }
   }
@@ -240,21 +271,32 @@ __device__ __forceinline__ Power power(float log_decay, int64_t n) {
   return {hi, (float)(p - (double)hi)};
 }
 
+// Keeps the compiler from starting the next step's LDS reads here: their registers would cost others' places.
+__device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
+
+// A value that all lanes hold, in a scalar register.
+__device__ __forceinline__ float uniform(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
+
 // LDS in 16-byte chunks: K and V, and for outputs Q and P.
-template <typename T, int DK, bool STATE_ONLY>
-constexpr int kDecayLds = kRaw<T> * kChunk * (DK / 8 * (STATE_ONLY ? 1 : 2) + 8) + (STATE_ONLY ? 0 : kMade<T> * kChunk * 8);
+template <typename T, int DK, int WAVES, bool STATE_ONLY>
+constexpr int kDecayLds = kRaw<T> * (kPlane<DK> * (STATE_ONLY ? 1 : 2) + kPlane<16 * WAVES>) + (STATE_ONLY ? 0 : kMade<T> * kPlane<kChunk>);
+// Waves a SIMD: what two workgroups a CU come to, where their LDS fits.
+template <typename T, int DK, int WAVES, bool STATE_ONLY>
+constexpr int kDecayWaves = WAVES / 4 * (kDecayLds<T, DK, WAVES, STATE_ONLY> * 16 <= 80 * 1024 ? 2 : 1);
 
-template <typename T, int DK, bool CHUNKS, bool STATE_ONLY>
-__global__ __launch_bounds__(kThreads, (kDecayLds<T, DK, STATE_ONLY> * 16 <= 80 * 1024 ? 2 : 1)) void decay_kernel(DecayArgs a) {
+template <typename T, int DK, int WAVES, int WEIGHTED, bool CHUNKS, bool STATE_ONLY>
+__global__ __launch_bounds__(64 * WAVES, (kDecayWaves<T, DK, WAVES, STATE_ONLY>)) void decay_kernel(DecayJobs jobs) {
 #ifdef __HIP_DEVICE_COMPILE__
-  constexpr int RAW = kRaw<T>, MADE = kMade<T>, TD = DK / 16, KS = DK / 32;
-  constexpr int QK = kChunk * DK / 8;  // chunks of a plane of Q or K
-  __shared__ u32x4 lds[kDecayLds<T, DK, STATE_ONLY>];
+  constexpr int RAW = kRaw<T>, MADE = kMade<T>, TD = DK / 16, KS = DK / 32, COLS = 16 * WAVES, NTH = 64 * WAVES;
+  constexpr int QK = kPlane<DK>, VP = kPlane<COLS>;
+  __shared__ u32x4 lds[kDecayLds<T, DK, WAVES, STATE_ONLY>];
   __shared__ float pow_of[kChunk + 1];  // l^0 .. l^64
-  u32x4 *lk = lds, *lv = lk + RAW * QK, *lq = lv + RAW * kChunk * 8, *lp = lq + RAW * QK;
+  u32x4 *lk = lds, *lv = lk + RAW * QK, *lq = lv + RAW * VP, *lp = lq + RAW * QK;
 
-  // column tiles of one (segment, head) side by side on one XCD: they read the same Q and K
-  const int run = blockIdx.x / 8, unit = run / a.col_tiles * 8 + blockIdx.x % 8, col_tile = run % a.col_tiles;
+  // scans and column tiles of one (segment, head) side by side on one XCD
+  const int run = blockIdx.x / 8, part = run / jobs.n;
+  const DecayArgs a = jobs.job[run % jobs.n];
+  const int unit = part / a.col_tiles * 8 + blockIdx.x % 8, col_tile = part % a.col_tiles;
   if (unit >= a.tiles * a.H) return;
   const int tile = unit / a.H, h = unit - tile * a.H;
   const Segment sg = find_segment(a, tile);
@@ -264,205 +306,182 @@ __global__ __launch_bounds__(kThreads, (kDecayLds<T, DK, STATE_ONLY> * 16 <= 80 
   const int len = (int)(hi - lo), begin = seg * a.seg, stop = min(begin + a.seg, len);  // tokens
   const int lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = col_tile * kStateCols + 16 * wave + li;  // of X and V
+  const int col = col_tile * COLS + 16 * wave + li;  // of X and V
   if constexpr (STATE_ONLY) {
     if (e == a.N || stop == len) return;
   } else if (e == a.N) {  // rows of no sequence: zeros
-    const int cols = min(a.Dv - col_tile * kStateCols, kStateCols);
+    const int cols = min(a.Dv - col_tile * COLS, COLS);
     if (!a.o) return;
-    T* o = (T*)a.o + ((lo + begin) * a.H + h) * a.Dv + col_tile * kStateCols;
-    for (int i = threadIdx.x; i < (stop - begin) * cols; i += kThreads) o[(int64_t)(i / cols) * a.H * a.Dv + i % cols] = from_f32<T>(0.f);
+    T* o = (T*)a.o + ((lo + begin) * a.H + h) * a.Dv + col_tile * COLS;
+    for (int i = threadIdx.x; i < (stop - begin) * cols; i += NTH) o[(int64_t)(i / cols) * a.H * a.Dv + i % cols] = from_f32<T>(0.f);
     return;
   }
   const float given = a.log_decay[h], ld = given > 0.f ? 0.f : given;
   if (threadIdx.x <= kChunk) pow_of[threadIdx.x] = power(ld, threadIdx.x).hi;
 
-  // X: rows 16 td + 4 g + r of the wave's columns
+  // X: rows 16 td + run_of(td, g) + r of the wave's columns
   f32x4 x[TD];
 #pragma unroll
   for (int td = 0; td < TD; ++td) x[td] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int64_t size = (int64_t)a.Dk * a.Dv;
+  // where x[td][r] is in a state, for a buffer
+  auto place_of = [&](int td, int r, int row, int column) {
+    const int d = 16 * td + run_of(td, g) + r;
+    return d < a.Dk && col < a.Dv ? (d * row + col * column) * 4 : kNowhere;
+  };
   if constexpr (!STATE_ONLY) {
-    auto add = [&](const float* s, int64_t row, int64_t column, float w) {
+    auto add = [&](const float* s, int row, int column, float w) {
+      const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(s), 0, (int)size * 4, kBufRsrcDword3);
 #pragma unroll
-      for (int td = 0; td < TD; ++td)
+      for (int td = 0; td < TD; ++td) {
+        f32x4 y;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int d = 16 * td + 4 * g + r;
-          if (d < a.Dk && col < a.Dv) x[td][r] += w * s[d * row + col * column];
-        }
+        for (int r = 0; r < 4; ++r)
+          y[r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsrc, place_of(td, r, row, column), 0, 0));
+        x[td] += w * y;
+      }
     };
-    const int64_t size = (int64_t)a.Dk * a.Dv;
     if (a.first) add(a.first + ((int64_t)e * a.H + h) * size, a.state_row, a.state_col, power(ld, begin).hi);
     for (int s = 0; s < seg; ++s)
-      add(a.parts + ((int64_t)(tile - seg + s) * a.H + h) * size, a.Dv, 1, power(ld, (int64_t)(seg - 1 - s) * a.seg).hi);
-    // the halves of P's 32-token rows that lie above the diagonal
-    for (int p = 0; p < MADE; ++p)
-      for (int i = threadIdx.x; i < 32 * 8; i += kThreads) {
-        const int r = i / 8 < 16 ? i / 8 : 16 + i / 8;
-        lp[p * kChunk * 8 + p_slot(r, i % 8)] = u32x4{0, 0, 0, 0};
-      }
+      add(a.parts + ((int64_t)(tile - seg + s) * a.H + h) * size, a.part_row, a.part_col, power(ld, (int64_t)(seg - 1 - s) * a.seg).hi);
+    // P above the diagonal, where a row's 32 tokens reach past it
+    for (int i = threadIdx.x; i < MADE * kPlane<kChunk>; i += NTH) lp[i] = u32x4{0, 0, 0, 0};
   }
   __syncthreads();
 
-  // P's ten tiles in or below the diagonal: wave w makes tiles w, w + 4 and w + 8
-  constexpr int kTiles = 3;
+  // P's ten tiles in or below the diagonal: wave w makes tiles w, w + WAVES, ...
+  constexpr int kTiles = (10 + WAVES - 1) / WAVES;
   int ti[kTiles], tj[kTiles];
-  float pw[kTiles][4], qw[4], vw[2][8];
 #pragma unroll
   for (int n = 0; n < kTiles; ++n) {
-    const int t = wave + 4 * n;
+    const int t = min(wave + WAVES * n, 9);
     ti[n] = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3;
     tj[n] = t - ti[n] * (ti[n] + 1) / 2;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int far = 16 * (ti[n] - tj[n]) + li - 4 * g - r;
-      pw[n][r] = far >= 0 && t < 10 ? a.out_scale * a.in_scale * pow_of[far] : 0.f;
-    }
   }
+  const int key = li - key_of(4 * g);  // query - key of a tile on the diagonal, at r = 0
+  float pw[kTiles][4];
 #pragma unroll
-  for (int it = 0; it < 4; ++it) qw[it] = a.out_scale * pow_of[16 * it + li + a.lag];
-  auto weigh_v = [&](int n) {
+  for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
+    for (int r = 0; r < 4; ++r) pw[n][r] = a.out_scale * a.in_scale * pow_of[max(16 * (ti[n] - tj[n]) + key - 2 * r, 0)];
+  // A chunk's tokens are its last n.  A result's state weight is l^(li + L) times the tile's; a token's weight on the chunk's end one of its lane group's
+  // times one of its place in it, which all lanes share.
+  const float out_w = a.out_scale * pow_of[li + a.lag];
+  float in_w = a.in_scale * pow_of[10 - a.lag - token_of(g, 0)];
+  float place[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) vw[ks][i] = a.in_scale * pow_of[max(n - a.lag - 32 * ks - order(g, i), 0)];
-  };
-  weigh_v(kChunk);
-  Power whole = power(ld, kChunk);
+  for (int i = 0; i < 8; ++i) place[i] = uniform(pow_of[22 - token_of(0, i)]);
+  const float l16 = uniform(pow_of[16]), l32 = uniform(pow_of[32]);
+  // l^64 in fp32 is off by up to 2^-25 of itself, always the same way.  Every 16th chunk puts that right: chunks in
+  // between are off by 2^-21 at most where l^64 is so close to 1 that it matters.
+  constexpr int kMend = 16;
+  const Power p64 = power(ld, kChunk);
+  const float whole = uniform(p64.hi), mend = uniform(p64.hi > 0.f ? 1.f + kMend * (p64.lo / p64.hi) : 1.f);
+  int since = 0;
 
   const T* q = (const T*)a.q + h * a.q_head;
   const T* k = (const T*)a.k + h * a.k_head;
-  const T* v = (const T*)a.v + h * a.v_head + col_tile * kStateCols;
-  Feed<T, DK, CHUNKS> fq, fk;
-  Feed<T, kStateCols, CHUNKS> fv;
+  const T* v = (const T*)a.v + h * a.v_head + col_tile * COLS;
+  Feed<T, DK, NTH, CHUNKS> fq(a.q_row, a.Dk, a.reverse), fk(a.k_row, a.Dk, a.reverse);
+  Feed<T, COLS, NTH, CHUNKS> fv(a.v_row, a.Dv - col_tile * COLS, a.reverse);
+  // where the lane's results go: row li of a tile of 16 in a whole chunk, four columns
+  const int o_col = col_tile * COLS + 16 * wave + 4 * g, o_row = a.H * a.Dv * (int)sizeof(T);
+  const int o_first = o_col < a.Dv ? (a.reverse ? kChunk - 1 - li : li) * o_row + o_col * (int)sizeof(T) : kNowhere;
+  const int o_step = a.reverse ? -16 * o_row : 16 * o_row;
   auto first_row = [&](int t, int n) { return a.reverse ? hi - t - n : lo + t; };
   auto load = [&](int t) {
-    const int n = min(kChunk, stop - t);
-    const int64_t row = first_row(t, n);
+    const int n = max(min(kChunk, stop - t), 0);
+    const int64_t row = n ? first_row(t, n) : lo;
     fk.load(k + row * a.k_row, a.k_row, a.Dk, n, a.reverse);
-    fv.load(v + row * a.v_row, a.v_row, a.Dv - col_tile * kStateCols, n, a.reverse);
+    fv.load(v + row * a.v_row, a.v_row, a.Dv - col_tile * COLS, n, a.reverse);
     if constexpr (!STATE_ONLY) fq.load(q + row * a.q_row, a.q_row, a.Dk, n, a.reverse);
   };
-  if (begin < stop) load(begin);
+  load(begin);
   for (int t = begin; t < stop; t += kChunk) {
     const int n = min(kChunk, stop - t);
+    asm volatile("" : "+v"(in_w));  // its products with `place` are made anew: kept, they would be spilled
     fk.store(lk);
     fv.store(lv);
     if constexpr (!STATE_ONLY) fq.store(lq);
     __syncthreads();
-    if (t + kChunk < stop) load(t + kChunk);
+    if constexpr (STATE_ONLY) load(t + kChunk);
 
-    u32x4 vr[2][RAW];  // the wave's columns of V
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-      for (int p = 0; p < RAW; ++p) vr[ks][p] = read_columns<kStateCols>(lv + p * kChunk * 8, 16 * wave, ks);
-
+    [[maybe_unused]] f32x4 o[4];
     if constexpr (!STATE_ONLY) {
-      // P: keys are the product's rows, so that a lane gets four neighbouring keys of one query
+      // P: keys are the product's rows, so that a lane gets four neighbouring k of one query
 #pragma unroll
       for (int m = 0; m < kTiles; ++m) {
-        if (m == 2 && wave > 1) break;
+        if ((m + 1) * WAVES > 10 && wave + m * WAVES >= 10) break;
         f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           u32x4 kf[RAW], qf[RAW];
 #pragma unroll
           for (int p = 0; p < RAW; ++p) {
-            kf[p] = read_rows<DK, false>(lk + p * QK, 16 * tj[m], ks);
-            qf[p] = read_rows<DK, false>(lq + p * QK, 16 * ti[m], ks);
+            kf[p] = read_rows<DK, true>(lk + p * QK, 16 * tj[m], ks);
+            qf[p] = read_rows<DK>(lq + p * QK, 16 * ti[m], ks);
           }
           s = mm_parts<RAW, RAW, RAW - 1>(kf, qf, s);
         }
         float f[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) f[r] = pw[m][r] != 0.f ? s[r] * pw[m][r] : 0.f;  // a masked NaN goes, too
+        for (int r = 0; r < 4; ++r) {
+          const int far = 16 * (ti[m] - tj[m]) + key - 2 * r;
+          const float w = pw[m][r] * s[r];
+          f[r] = far >= 0 ? w : 0.f;
+        }
         uint32_t parts[MADE][2];
         split<MADE, 2>(f, parts);
-        const int slot = p_slot(16 * ti[m] + li, 4 * (tj[m] >> 1) + g);
+        uint64_t* to = reinterpret_cast<uint64_t*>(lp) + 2 * ((16 * ti[m] + li) * kPitch<kChunk> + 4 * (tj[m] >> 1) + g) + (tj[m] & 1);
 #pragma unroll
-        for (int p = 0; p < MADE; ++p)
-          reinterpret_cast<uint64_t*>(lp + p * kChunk * 8 + slot)[tj[m] & 1] = (uint64_t)parts[p][1] << 32 | parts[p][0];
+        for (int p = 0; p < MADE; ++p) to[2 * p * kPlane<kChunk>] = (uint64_t)parts[p][1] << 32 | parts[p][0];
       }
       // Q X: results are (column, query), a lane's query is li of each tile
-      f32x4 o[4];
 #pragma unroll
       for (int it = 0; it < 4; ++it) o[it] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
+        u32x4 qf[4][RAW], xs[MADE];
+#pragma unroll
+        for (int it = 0; it < 4; ++it)
+#pragma unroll
+          for (int p = 0; p < RAW; ++p) qf[it][p] = read_rows_tiled<DK>(lq + p * QK, 16 * it, ks);
         float f[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] = x[2 * ks + i / 4][i % 4];
-        u32x4 xs[MADE];
         split8<MADE>(f, xs);
 #pragma unroll
-        for (int it = 0; it < 4; ++it) {
-          u32x4 qf[RAW];
+        for (int i = MADE - 1; i >= 0; --i)
 #pragma unroll
-          for (int p = 0; p < RAW; ++p) qf[p] = read_rows<DK, true>(lq + p * QK, 16 * it, ks);
-          o[it] = mm_parts<MADE, RAW, MADE - 1>(xs, qf, o[it]);
-        }
+          for (int j = RAW - 1; j >= 0; --j)
+#pragma unroll
+            for (int it = 0; it < 4; ++it)
+              if (i + j < MADE) o[it] = mm(xs[i], qf[it][j], o[it]);
+        fence();
       }
-      __syncthreads();
-      // P V
-      f32x4 pv[4];
-      float finite = 0.f;
+      float w = out_w;
 #pragma unroll
       for (int it = 0; it < 4; ++it) {
-        pv[it] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int ks = 0; ks <= it / 2; ++ks) {
-          u32x4 pf[MADE];
-#pragma unroll
-          for (int p = 0; p < MADE; ++p) pf[p] = lp[p * kChunk * 8 + p_slot(16 * it + li, 4 * ks + g)];
-          pv[it] = mm_parts<RAW, MADE, MADE - 1>(vr[ks], pf, pv[it]);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) finite = __builtin_fmaf(pv[it][r], 0.f, finite);
-      }
-      if (__any(finite != 0.f)) {
-        // An infinity or a NaN among V: zeros above the diagonal have spread it to earlier tokens.  One by one.
-        for (int it = 0; it < 4; ++it) {
-          pv[it] = f32x4{0.f, 0.f, 0.f, 0.f};
-          const int i = 16 * it + li;
-          for (int j = 0; j <= 16 * it + 15; ++j) {
-            const int at = j & 31, gj = (at >> 2) & 3, ej = (at >> 4) * 4 + (at & 3);  // order(gj, ej) = at
-            float pij = 0.f;
-            for (int p = 0; p < MADE; ++p)
-              pij += to_f32(reinterpret_cast<const __bf16*>(lp + p * kChunk * 8 + p_slot(i, 4 * (j >> 5) + gj))[ej]);
-            for (int r = 0; r < 4; ++r) {
-              const int c = 16 * wave + 4 * g + r;
-              float vj = 0.f;
-              for (int p = 0; p < RAW; ++p)
-                vj += to_f32(reinterpret_cast<const __bf16*>(lv + p * kChunk * 8 + plane_slot<kStateCols>(j, c >> 3))[c & 7]);
-              if (j <= i) pv[it][r] += pij * vj;
-            }
-          }
-        }
-      }
-      T* out = (T*)a.o;
-      const int64_t row = first_row(t, n);
-      const int c = col_tile * kStateCols + 16 * wave + 4 * g;
-      const bool vec = a.Dv % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-#pragma unroll
-      for (int it = 0; it < 4; ++it) {
-        const int i = 16 * it + li;
-        f32x4 y;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) y[r] = pv[it][r] + o[it][r] * qw[it];
-        if (i < n && out) store4(out + ((row + (a.reverse ? n - 1 - i : i)) * a.H + h) * a.Dv + c, y, a.Dv - c, vec);
+        if (__builtin_expect(n < kChunk, false)) w = a.out_scale * pow_of[max(16 * it + li + a.lag - (kChunk - n), 0)];
+        o[it] *= w;
+        w *= l16;
       }
     }
 
     // X' = l^n X + K^T (weighted V)
-    if (n < kChunk) {
-      weigh_v(n);
-      whole = power(ld, n);
+    u32x4 vr[2][RAW];  // the wave's columns of V
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int p = 0; p < RAW; ++p) vr[ks][p] = read_columns<COLS>(lv + p * VP, 16 * wave, ks);
+    float by = whole;
+    if (__builtin_expect(n < kChunk, false)) by = power(ld, n).hi;
+    if (++since == kMend) {  // what rounding l^64 has cost since the last time
+      since = 0;
+      by *= mend;
     }
 #pragma unroll
-    for (int td = 0; td < TD; ++td)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) x[td][r] = __builtin_fmaf(x[td][r], whole.hi, x[td][r] * whole.lo);
+    for (int td = 0; td < TD; ++td) x[td] *= by;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       float f[8];
@@ -471,39 +490,127 @@ __global__ __launch_bounds__(kThreads, (kDecayLds<T, DK, STATE_ONLY> * 16 <= 80 
         f[i] = 0.f;
 #pragma unroll
         for (int p = RAW - 1; p >= 0; --p) f[i] += i % 2 ? high2(vr[ks][p][i / 2]) : low2(vr[ks][p][i / 2]);
-        f[i] *= vw[ks][i];
       }
-      u32x4 vs[kWeighted];
-      split8<kWeighted>(f, vs);
+      const float w = ks ? in_w : in_w * l32;
 #pragma unroll
-      for (int td = 0; td < TD; ++td) {
-        u32x4 kf[RAW];
+      for (int i = 0; i < 8; ++i) f[i] *= w * place[i];
+      u32x4 vs[WEIGHTED];
+      split8<WEIGHTED>(f, vs);
 #pragma unroll
-        for (int p = 0; p < RAW; ++p) kf[p] = read_columns<DK>(lk + p * QK, 16 * td, ks);
-        x[td] = mm_parts<RAW, kWeighted, 2>(kf, vs, x[td]);
+      for (int t4 = 0; t4 < TD; t4 += 4) {
+        u32x4 kf[4][RAW];
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+          for (int p = 0; p < RAW; ++p)
+            kf[m][p] = m & 1 ? read_columns<DK, true>(lk + p * QK, 16 * (t4 + m), ks) : read_columns<DK>(lk + p * QK, 16 * (t4 + m), ks);
+#pragma unroll
+        for (int i = RAW - 1; i >= 0; --i)
+#pragma unroll
+          for (int j = WEIGHTED - 1; j >= 0; --j)
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+              if (i + j < WEIGHTED) x[t4 + m] = mm(kf[m][i], vs[j], x[t4 + m]);
+        fence();
       }
     }
+    if constexpr (!STATE_ONLY) {
+      fence();  // the next chunk's registers are not there before
+      load(t + kChunk);
+    }
     __syncthreads();
+
+    if constexpr (!STATE_ONLY) {
+      // P V.  An infinity or a NaN among V has reached every row of its column of X (then and ever after), and would
+      // through the zeros above the diagonal reach earlier tokens: such a wave takes its tokens one by one.
+      if (__builtin_expect(!__any(x[0][0] * 0.f != 0.f), true)) {
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          u32x4 pf[4][MADE];
+#pragma unroll
+          for (int it = 2 * ks; it < 4; ++it)
+#pragma unroll
+            for (int p = 0; p < MADE; ++p) pf[it][p] = read_rows<kChunk>(lp + p * kPlane<kChunk>, 16 * it, ks);
+#pragma unroll
+          for (int i = RAW - 1; i >= 0; --i)
+#pragma unroll
+            for (int j = MADE - 1; j >= 0; --j)
+#pragma unroll
+              for (int it = 2 * ks; it < 4; ++it)
+                if (i + j < MADE) o[it] = mm(vr[ks][i], pf[it][j], o[it]);
+        }
+      } else {
+#pragma unroll 1
+        for (int j = 0; j < kChunk; ++j) {
+          // token_of(gj, ej) = j & 31
+          const int gj = ((j >> 3) & 1) | (j & 1) << 1, ej = ((j >> 4) & 1) * 4 + ((j >> 1) & 3);
+          float pj[4], vj[4];
+#pragma unroll
+          for (int it = 0; it < 4; ++it) {
+            pj[it] = 0.f;
+            for (int p = 0; p < MADE; ++p)
+              pj[it] += to_f32(reinterpret_cast<const __bf16*>(lp + p * kPlane<kChunk> + (16 * it + li) * kPitch<kChunk> + 4 * (j >> 5) + gj)[ej]);
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {  // column 4 g + r is lane 16 gj + 4 g + r's
+            vj[r] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+              for (int p = 0; p < RAW; ++p)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const uint32_t w = __shfl(vr[ks][p][i], 16 * gj + 4 * g + r, 64);
+                  if (ks == j >> 5 && i == ej >> 1) vj[r] += ej & 1 ? high2(w) : low2(w);
+                }
+          }
+#pragma unroll
+          for (int it = 0; it < 4; ++it)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (j <= 16 * it + li) o[it][r] += pj[it] * vj[r];
+        }
+      }
+      T* out = (T*)a.o + (first_row(t, n) * a.H + h) * a.Dv;
+      [[maybe_unused]] const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+          out, 0, a.o ? (n - 1) * o_row + a.Dv * (int)sizeof(T) : 0, kBufRsrcDword3);
+      const int back = a.reverse ? 0 : (kChunk - n) * o_row;
+#pragma unroll
+      for (int it = 0; it < 4; ++it) {
+        const f32x4 y = o[it];
+        if constexpr (CHUNKS) {
+          const int off = o_first + it * o_step - back;
+          if constexpr (sizeof(T) == 4) {
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), rsrc, off, 0, 0);
+          } else {
+            const T h4[4] = {from_f32<T>(y[0]), from_f32<T>(y[1]), from_f32<T>(y[2]), from_f32<T>(y[3])};
+            uint32_t w[2];
+            __builtin_memcpy(w, h4, 8);
+            __builtin_amdgcn_raw_buffer_store_b64(u32x2{w[0], w[1]}, rsrc, off, 0, 0);
+          }
+        } else {
+          const int at = a.reverse ? kChunk - 1 - 16 * it - li : 16 * it + li - (kChunk - n);
+          if (at >= 0 && at < n && a.o) store4(out + (int64_t)at * a.H * a.Dv + o_col, y, a.Dv - o_col, false);
+        }
+      }
+    }
   }
 
   float* to = nullptr;
-  int64_t row = a.Dv, column = 1;
+  int row = a.Dv, column = 1;
   if constexpr (STATE_ONLY) {
-    to = a.parts + ((int64_t)tile * a.H + h) * a.Dk * a.Dv;
+    to = a.parts + ((int64_t)tile * a.H + h) * size;
   } else if (a.last && stop == len) {
-    to = a.last + ((int64_t)e * a.H + h) * a.Dk * a.Dv;
+    to = a.last + ((int64_t)e * a.H + h) * size;
     row = a.state_row;
     column = a.state_col;
   }
-  if (to) {
+  const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(to, 0, to ? (int)size * 4 : 0, kBufRsrcDword3);
 #pragma unroll
-    for (int td = 0; td < TD; ++td)
+  for (int td = 0; td < TD; ++td)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int d = 16 * td + 4 * g + r;
-        if (d < a.Dk && col < a.Dv) to[d * row + col * column] = x[td][r];
-      }
-  }
+    for (int r = 0; r < 4; ++r)
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[td][r]), rsrc, place_of(td, r, row, column), 0, 0);
 #endif
 }
 

@@ -80,12 +80,12 @@ _SIGNATURES = {
     "mhc_grouped_matmul_backward_weight": (_I, [_P, _P, _I, _P, _P, _I64, _I64, _I64, _I64, _P]),
     "mhc_grouped_matmul_mx": (_I, [_P, _P, _P, _P, _P, _P, _I, _I64, _I64, _I64, _I64, _P]),
     "mhc_rotary": (_I, [*_STRIDED, _P, _I64, *_STRIDED, _P, _I64, _I, _P, _I, _I64, _P, _I64, _I64, _I64, _F, _I, _I, _P]),
-    "mhc_decay_attention_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64, _I]),
+    "mhc_decay_attention_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64, _I, _I]),
     "mhc_decay_attention_forward": (
         _I, [*_STRIDED * 3, _I, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _F, _P, _SZ, _P]),
-    "mhc_decay_attention_backward_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64, _I]),
+    "mhc_decay_attention_backward_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64, _I, _I]),
     "mhc_decay_attention_backward": (
-        _I, [*_STRIDED * 4, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _F, _P, _SZ, _P]),
+        _I, [*_STRIDED * 4, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _F, _P, _SZ, _P]),
     "mhc_decay_attention_step": (
         _I, [*_STRIDED * 3, _I, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _F, _P]),
     "mhc_gated_matmul_forward": (_I, [_P, _P, _I, _P, _I, _P, _P, _I64, _I64, _I64, _I64, _P]),

@@ -151,7 +151,8 @@ def _decay_args(q, k, v, log_decay, offsets, *states):
 
 
 def decay_attention_forward(q, k, v, log_decay, offsets, initial_state, scale: float, want_state: bool):
-    """(o, state): o as v; state (N, H, Dk, Dv) fp32 after each sequence, None unless wanted."""
+    """(o, state, kept): o as v; state (N, H, Dk, Dv) fp32 after each sequence, None unless wanted; kept, or None, spares
+    the backward a pass over k and v."""
     dev, N, H, Dk, Dv, offsets = _decay_args(q, k, v, log_decay, offsets, ("initial_state", initial_state))
     code, log_decay = _lib.dtype_code(q), _f32(log_decay)
     first = None if initial_state is None else initial_state.contiguous()
@@ -159,24 +160,24 @@ def decay_attention_forward(q, k, v, log_decay, offsets, initial_state, scale: f
     o = torch.empty(v.shape, device=dev, dtype=v.dtype)
     last = torch.empty((N, H, Dk, Dv), device=dev, dtype=torch.float32) if want_state else None
     lib = _lib.load()
-    ws = _lib.workspace(lib.mhc_decay_attention_workspace_bytes(a.R, N, H, Dk, Dv, int(offsets is not None)), dev)
+    ws = _lib.workspace(lib.mhc_decay_attention_workspace_bytes(a.R, N, H, Dk, Dv, int(offsets is not None), code), dev)
     with _lib.on_device(dev):
         _lib.check(lib.mhc_decay_attention_forward(*a.args(), *b.args(), *c.args(), code, log_decay.data_ptr(),
                                                    _lib.ptr(offsets), _lib.ptr(first), o.data_ptr(), _lib.ptr(last), a.R, N,
                                                    H, Dk, Dv, float(scale), _lib.ptr(ws), 0 if ws is None else ws.numel(),
                                                    _lib.stream(dev)), "decay_attention_forward")
-    return o, last
+    return o, last, ws
 
 
-def decay_attention_backward(q, k, v, do, log_decay, offsets, initial_state, d_state, scale: float,
+def decay_attention_backward(q, k, v, do, log_decay, offsets, initial_state, kept, d_state, scale: float,
                              need: Tuple[bool, bool, bool, bool]):
-    """(dq, dk, dv, d_initial): None for what is not needed."""
+    """(dq, dk, dv, d_initial): None for what is not needed.  kept: the forward's third result, or None."""
     dev, N, H, Dk, Dv, offsets = _decay_args(q, k, v, log_decay, offsets, ("initial_state", initial_state),
                                              ("the state's gradient", d_state))
     if do.shape != v.shape:
         raise ShapeError(f"the output's gradient must be {tuple(v.shape)}, got {tuple(do.shape)}")
     _same_dtype("the output's gradient", do, q)
-    _lib.require_gpu(q, do)
+    _lib.require_gpu(q, do, kept)
     code, log_decay = _lib.dtype_code(q), _f32(log_decay)
     first = None if initial_state is None else initial_state.contiguous()
     d_last = None if d_state is None else d_state.contiguous()
@@ -184,10 +185,15 @@ def decay_attention_backward(q, k, v, do, log_decay, offsets, initial_state, d_s
     out = [torch.empty(t.shape, device=dev, dtype=t.dtype) if n else None for t, n in zip((q, k, v), need)]
     d_first = torch.empty((N, H, Dk, Dv), device=dev, dtype=torch.float32) if need[3] else None
     lib = _lib.load()
-    ws = _lib.workspace(lib.mhc_decay_attention_backward_workspace_bytes(a.R, N, H, Dk, Dv, int(offsets is not None)), dev)
+    packed = int(offsets is not None)
+    if kept is not None:  # a saved-tensor hook may have changed it
+        if kept.dtype != torch.uint8 or kept.numel() != lib.mhc_decay_attention_workspace_bytes(a.R, N, H, Dk, Dv, packed, code):
+            raise ShapeError(f"kept must be the forward's, got {tuple(kept.shape)} {kept.dtype}")
+        kept = kept.contiguous()
+    ws = _lib.workspace(lib.mhc_decay_attention_backward_workspace_bytes(a.R, N, H, Dk, Dv, packed, code), dev)
     with _lib.on_device(dev):
         _lib.check(lib.mhc_decay_attention_backward(*a.args(), *b.args(), *c.args(), *d.args(), code, log_decay.data_ptr(),
-                                                    _lib.ptr(offsets), _lib.ptr(first), _lib.ptr(d_last),
+                                                    _lib.ptr(offsets), _lib.ptr(first), _lib.ptr(kept), _lib.ptr(d_last),
                                                     *(_lib.ptr(t) for t in out), _lib.ptr(d_first), a.R, N, H, Dk, Dv,
                                                     float(scale), _lib.ptr(ws), 0 if ws is None else ws.numel(),
                                                     _lib.stream(dev)), "decay_attention_backward")

@@ -72,7 +72,7 @@ def _state_shape(q, v, offsets):
 @_op("decay_attention")
 def _decay_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, offsets: Optional[Tensor],
                      initial_state: Optional[Tensor], scale: float) -> Tuple[Tensor, Tensor]:
-    return _k.decay_attention_forward(q, k, v, log_decay, offsets, initial_state, scale, True)
+    return _k.decay_attention_forward(q, k, v, log_decay, offsets, initial_state, scale, True)[:2]
 
 
 @_decay_attention.register_fake
@@ -84,7 +84,7 @@ def _(q, k, v, log_decay, offsets, initial_state, scale):
 def _decay_attention_backward(q: Tensor, k: Tensor, v: Tensor, do: Tensor, log_decay: Tensor, offsets: Optional[Tensor],
                               initial_state: Optional[Tensor], d_state: Optional[Tensor], scale: float,
                               need: List[bool]) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
-    got = _k.decay_attention_backward(q, k, v, do, log_decay, offsets, initial_state, d_state, scale, tuple(need))
+    got = _k.decay_attention_backward(q, k, v, do, log_decay, offsets, initial_state, None, d_state, scale, tuple(need))
     return tuple(_or_empty(g, t) for g, t in zip(got, (q, k, v, log_decay)))
 
 

@@ -145,21 +145,21 @@ class _Rotary(torch.autograd.Function):
 class _DecayAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, offsets, initial_state, scale: float, return_state: bool):
-        ctx.save_for_backward(q, k, v, log_decay, offsets, initial_state)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
-        o, state = _m.decay_attention_forward(q, k, v, log_decay, offsets, initial_state, scale, return_state)
+        o, state, kept = _m.decay_attention_forward(q, k, v, log_decay, offsets, initial_state, scale, return_state)
+        ctx.save_for_backward(q, k, v, log_decay, offsets, initial_state, kept if ctx.needs_input_grad[0] else None)
         return (o, state) if return_state else o
 
     @staticmethod
     def backward(ctx, do, d_state=None):
-        q, k, v, log_decay, offsets, initial = ctx.saved_tensors
+        q, k, v, log_decay, offsets, initial, kept = ctx.saved_tensors
         need = (*ctx.needs_input_grad[:3], ctx.needs_input_grad[5])
         if do is None and d_state is None:
             return (None,) * 8
         if do is None:
             do = torch.zeros_like(v, memory_format=torch.contiguous_format)
-        got = _m.decay_attention_backward(q, k, v, do, log_decay, offsets, initial, d_state, ctx.scale, need)
+        got = _m.decay_attention_backward(q, k, v, do, log_decay, offsets, initial, kept, d_state, ctx.scale, need)
         graph = [t is not None and t.requires_grad for t in (do, d_state, q, k, v, initial)]
         dq, dk, dv, ds = (_first_order(g, "decay_attention", *graph) for g in got)
         return dq, dk, dv, None, None, ds, None, None

@@ -208,12 +208,12 @@ def test_abi_refusals_before_any_device_work():
     assert fwd(q=None) == fwd(o=None) == fwd(ld=None) == fwd(R=7) == fwd(Dk=129) == fwd(Dv=0) == fwd(R=-8) == 1
     assert fwd(row=(1 << 22) + 1) == fwd(row=-1) == fwd(R=1 << 31, N=1) == fwd(N=0) == 1
     assert fwd(R=0, q=None, o=None) == fwd(H=0, q=None) == fwd(R=0, N=0) == 0 and fwd(code=3) == 2
-    need = lib.mhc_decay_attention_workspace_bytes(8192, 1, 2, 64, 64, 0)
-    assert need > 0 and need % (2 * 64 * 64 * 4) == 0 and lib.mhc_decay_attention_workspace_bytes(64, 1, 2, 64, 64, 0) == 0
+    need = lib.mhc_decay_attention_workspace_bytes(8192, 1, 2, 64, 64, 0, 1)
+    assert need > 0 and need % (2 * 64 * 64 * 4) == 0 and lib.mhc_decay_attention_workspace_bytes(64, 1, 2, 64, 64, 0, 1) == 0
     assert fwd(R=8192, N=1, Dk=64, Dv=64) == fwd(R=8192, N=1, Dk=64, Dv=64, ws=16, nb=need - 1) == 3
 
     def bwd(do=16, R=8, N=2, Dk=16, Dv=16, code=1, row=32):
-        return lib.mhc_decay_attention_backward(16, row, 16, 16, row, 16, 16, row, 16, do, row, 16, code, 16, None, None, None, 16,
+        return lib.mhc_decay_attention_backward(16, row, 16, 16, row, 16, 16, row, 16, do, row, 16, code, 16, None, None, None, None, 16,
                                                 16, 16, None, R, N, 2, Dk, Dv, 1.0, None, 0, None)
 
     assert bwd(do=None) == bwd(R=7) == bwd(Dk=200) == bwd(row=(1 << 22) + 1) == 1
