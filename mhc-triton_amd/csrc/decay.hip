@@ -112,7 +112,7 @@ constexpr int64_t kMaxRowStride = (int64_t)1 << 22;  // byte offsets inside a ch
 static int check_decay(const char* who, int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv, bool packed,
                        std::initializer_list<int64_t> row_strides) {
   if (R < 0 || N < 0 || H < 0 || Dk < 1 || Dv < 1 || Dk > kMaxHeadDim || Dv > kMaxHeadDim || R > kMaxRows ||
-      N > ((int64_t)1 << 24) || H * (Dk > Dv ? Dk : Dv) > kMaxRowStride || (!packed && (N ? R % N : R))) {
+      N > ((int64_t)1 << 24) || H * (Dk > Dv ? Dk : Dv) > kMaxRowStride || (!packed && R % N)) {
     set_error("%s: R=%lld N=%lld H=%lld Dk=%lld Dv=%lld (heads of 1 to %lld; sequences of R / N rows)", who, (long long)R,
               (long long)N, (long long)H, (long long)Dk, (long long)Dv, (long long)kMaxHeadDim);
     return MHC_ERR_ARG;
@@ -164,10 +164,11 @@ extern "C" int mhc_decay_attention_forward(const void* q, int64_t q_row, int64_t
                                            float* last, int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv,
                                            float scale, void* workspace, size_t workspace_bytes, mhc_stream_t stream) {
   const char* who = "decay_attention_forward";
-  if (int rc = check_decay(who, R, N, H, Dk, Dv, offsets != nullptr, {q_row, k_row, v_row})) return rc;
+  const bool packed = offsets || N == 0;
+  if (int rc = check_decay(who, R, N, H, Dk, Dv, packed, {q_row, k_row, v_row})) return rc;
   if (H == 0 || (R == 0 && (N == 0 || !last))) return MHC_OK;
   if (!log_decay || (R && (!q || !k || !v || !o))) return null_in(who);
-  const size_t need = mhc_decay_attention_workspace_bytes(R, N, H, Dk, Dv, offsets != nullptr, dtype);
+  const size_t need = mhc_decay_attention_workspace_bytes(R, N, H, Dk, Dv, packed, dtype);
   if (int rc = check_workspace(who, workspace, workspace_bytes, need)) return rc;
   DecayJobs jobs{};
   jobs.n = 1;
@@ -178,7 +179,7 @@ extern "C" int mhc_decay_attention_forward(const void* q, int64_t q_row, int64_t
   a.parts = (float*)workspace; a.part_row = (int)Dv; a.part_col = 1;
   a.R = R; a.N = (int)N; a.H = (int)H; a.Dk = (int)Dk; a.Dv = (int)Dv;
   a.out_scale = scale; a.in_scale = 1.f; a.lag = 1;
-  const Plan plan = plan_scan(R, N, H, Dk, Dv, offsets != nullptr, dtype);
+  const Plan plan = plan_scan(R, N, H, Dk, Dv, packed, dtype);
   return MHC_DISPATCH_DTYPE(dtype, [&] {
     return scan<T>(jobs, plan, kStates | kOutputs, last != nullptr, who, (hipStream_t)stream);
   });
@@ -203,10 +204,11 @@ extern "C" int mhc_decay_attention_backward(const void* q, int64_t q_row, int64_
                                             int64_t N, int64_t H, int64_t Dk, int64_t Dv, float scale, void* workspace,
                                             size_t workspace_bytes, mhc_stream_t stream) {
   const char* who = "decay_attention_backward";
-  if (int rc = check_decay(who, R, N, H, Dk, Dv, offsets != nullptr, {q_row, k_row, v_row, do_row})) return rc;
+  const bool packed = offsets || N == 0;
+  if (int rc = check_decay(who, R, N, H, Dk, Dv, packed, {q_row, k_row, v_row, do_row})) return rc;
   if (H == 0 || (R == 0 && (N == 0 || !d_first))) return MHC_OK;
   if (!log_decay || (R && (!q || !k || !v || !dout))) return null_in(who);
-  const bool packed = offsets != nullptr, same = alike(Dk, Dv);
+  const bool same = alike(Dk, Dv);
   const size_t need = mhc_decay_attention_backward_workspace_bytes(R, N, H, Dk, Dv, packed, dtype);
   if (int rc = check_workspace(who, workspace, workspace_bytes, need)) return rc;
   // of states with Dv columns, and of the transposed ones

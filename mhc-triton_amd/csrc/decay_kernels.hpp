@@ -39,7 +39,7 @@ struct DecayArgs {
   const void *q, *k, *v;
   void* o;
   const float* log_decay;    // [H]
-  const int32_t* offsets;    // ends of the packed sequences; null: N sequences of T rows each
+  const int32_t* offsets;    // ends of the packed sequences; null: N sequences of T rows each, or with N = 0 none
   const float* first;        // X_0 of each sequence, or null
   float* last;               // where X goes, or null
   float* parts;              // states that segments leave by themselves, [tile][H][Dk][Dv]
@@ -69,7 +69,7 @@ struct Segment {
 
 // Tile t: every sequence has a segment at least, so that one without tokens hands its state on.
 __device__ __forceinline__ Segment find_segment(const DecayArgs& a, int t) {
-  if (!a.offsets) {
+  if (!a.offsets && a.N) {
     const int per = (int)max((int64_t)1, (a.T + a.seg - 1) / a.seg);
     const int e = t / per;
     return {e < a.N ? e : -1, t - e * per, e * a.T, (e + 1) * a.T};

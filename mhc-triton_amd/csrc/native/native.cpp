@@ -1020,6 +1020,328 @@ PyObject* py_grouped_matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------------------
+// mhc.branch: rotary, decay_attention, decay_attention_step, gated_matmul
+// ---------------------------------------------------------------------------
+
+bool flag(PyObject* o, bool* v) {
+  *v = o == Py_True;
+  return o == Py_True || o == Py_False;
+}
+
+constexpr int64_t kMaxRowStride = (int64_t)1 << 22;
+
+// Rows (..., heads, dim) as the kernels read them: a head's elements neighbours, rows and heads anywhere.  What no one row
+// stride describes is copied.
+struct Heads {
+  Tensor t;
+  int64_t R, H, D, row, head;
+  explicit Heads(const Tensor& x) {
+    t = x.dim() == 2 ? x.unsqueeze(0) : x.dim() > 3 ? x.flatten(0, -3) : x;
+    R = t.size(0), H = t.size(1), D = t.size(2);
+    if ((D > 1 && t.stride(2) != 1) || (R > 1 && t.stride(0) > kMaxRowStride)) t = t.contiguous();
+    row = R > 1 ? t.stride(0) : H * D;
+    head = H > 1 ? t.stride(1) : D;
+  }
+  void* p() const { return t.data_ptr(); }
+};
+
+Tensor plain_empty(at::IntArrayRef sizes, const Tensor& like) { return at::empty(sizes, like.options().requires_grad(false)); }
+
+struct Pair { Tensor q, k; };
+
+Pair rotary_launch(const Tensor& q, const Tensor& k, const Tensor& pos, const Tensor& freq, bool inter, double mag, bool inverse) {
+  const c10::DeviceGuard guard(q.device());
+  const Tensor p = pos.contiguous(), f = (freq.scalar_type() == at::kDouble ? freq : freq.to(at::kDouble)).contiguous();
+  Pair out{plain_empty(q.sizes(), q), k.defined() ? plain_empty(k.sizes(), k) : Tensor()};
+  if (out.q.numel() == 0 && (!k.defined() || out.k.numel() == 0)) return out;
+  const Heads a(q), b(k.defined() ? k : q);
+  check(mhc_rotary(a.p(), a.row, a.head, ptr(out.q), a.H, k.defined() ? b.p() : nullptr, b.row, b.head, ptr(out.k),
+                   k.defined() ? b.H : 0, code(q), ptr(p), p.scalar_type() == at::kLong, p.numel(),
+                   static_cast<const double*>(ptr(f)), f.size(0), a.R, a.D, (float)mag, inter, inverse, stream(q)),
+        "rotary");
+  return out;
+}
+
+struct Rotary : Function<Rotary> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const std::optional<Tensor>& k, const Tensor& pos,
+                               const Tensor& freq, bool inter, double mag) {
+    ctx->save_for_backward({pos, freq});
+    ctx->saved_data["inter"] = inter;
+    ctx->saved_data["mag"] = mag;
+    ctx->saved_data["k"] = k.has_value();
+    ctx->set_materialize_grads(false);
+    const Pair o = rotary_launch(q, k.value_or(Tensor()), pos, freq, inter, mag, false);
+    if (k) return {o.q, o.k};
+    return {o.q};
+  }
+
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    const variable_list s = saved(ctx);
+    const bool has_k = ctx->saved_data["k"].toBool();
+    const Tensor dq = ctx->needs_input_grad(0) ? g[0] : Tensor(), dk = has_k && ctx->needs_input_grad(1) ? g[1] : Tensor();
+    Tensor gq, gk;
+    if (dq.defined() || dk.defined()) {  // both in one launch
+      const bool both = dq.defined() && dk.defined();
+      const Pair o = rotary_launch(dq.defined() ? dq : dk, both ? dk : Tensor(), s[0], s[1], ctx->saved_data["inter"].toBool(),
+                                   ctx->saved_data["mag"].toDouble(), true);
+      if (dq.defined()) gq = first_order(o.q, "rotary", dq.requires_grad());
+      if (dk.defined()) gk = first_order(both ? o.k : o.q, "rotary", dk.requires_grad());
+    }
+    return {gq, gk, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor q, k, pos, freq;
+  bool inter;
+  double mag;
+  if (n != 6 || !tensors(a, 1, &q) || !optional_tensor(a[1], q, &k) || !optional_tensor(a[2], q, &pos) || !pos.defined() ||
+      !optional_tensor(a[3], q, &freq) || !freq.defined() || !flag(a[4], &inter) || !number(a[5], &mag))
+    return none();
+  if (code(q) < 0 || q.dim() < 2 || q.size(-1) > 4096 || freq.dim() != 1 || 2 * freq.size(0) > q.size(-1) ||
+      !freq.is_floating_point() || (pos.scalar_type() != at::kInt && pos.scalar_type() != at::kLong))
+    return none();
+  const at::IntArrayRef lead = q.sizes().slice(0, q.dim() - 2);
+  if (pos.dim() > (int64_t)lead.size() || pos.sizes() != lead.slice(lead.size() - pos.dim())) return none();
+  if (k.defined() && (k.scalar_type() != q.scalar_type() || k.dim() != q.dim() || k.size(-1) != q.size(-1) ||
+                      k.sizes().slice(0, k.dim() - 2) != lead))
+    return none();
+  variable_list out;
+  {
+    ReleaseGil gil;
+    if (wants_grad({q, k})) {
+      out = Rotary::apply(q, given(k), pos, freq, inter, mag);
+    } else {
+      const Pair o = rotary_launch(q, k, pos, freq, inter, mag, false);
+      out = {o.q};
+      if (k.defined()) out.push_back(o.k);
+    }
+  }
+  return out.size() == 1 ? THPVariable_Wrap(out[0]) : tuple_of(out);
+  END_HANDLE_TH_ERRORS
+}
+
+struct DecayOut { Tensor o, state, kept; };
+
+DecayOut decay_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& decay, const Tensor& offsets,
+                       const Tensor& initial, double scale, bool want_state) {
+  const c10::DeviceGuard guard(q.device());
+  const Heads a(q), b(k), c(v);
+  const Tensor off = offsets.defined() ? int_offsets(offsets) : offsets, ld = f32(decay), first = whole(initial);
+  const int64_t N = off.defined() ? off.size(0) : q.size(0);
+  DecayOut o;
+  o.o = plain_empty(v.sizes(), v);
+  if (want_state) o.state = empty_f32({N, a.H, a.D, c.D}, q);
+  const Workspace ws(mhc_decay_attention_workspace_bytes(a.R, N, a.H, a.D, c.D, off.defined(), code(q)), q);
+  check(mhc_decay_attention_forward(a.p(), a.row, a.head, b.p(), b.row, b.head, c.p(), c.row, c.head, code(q), fptr(ld),
+                                    static_cast<const int32_t*>(ptr(off)), fptr(first), ptr(o.o), wptr(o.state), a.R, N, a.H,
+                                    a.D, c.D, (float)scale, ws.p(), ws.bytes, stream(q)),
+        "decay_attention_forward");
+  o.kept = ws.t;
+  return o;
+}
+
+struct DecayAttention : Function<DecayAttention> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& decay,
+                               const std::optional<Tensor>& offsets, const std::optional<Tensor>& initial, double scale,
+                               bool want_state) {
+    const Tensor off = offsets.value_or(Tensor()), first = initial.value_or(Tensor());
+    const DecayOut o = decay_forward(q, k, v, decay, off, first, scale, want_state);
+    ctx->save_for_backward({q, k, v, decay, off, first, q.requires_grad() ? o.kept : Tensor()});
+    ctx->saved_data["scale"] = scale;
+    ctx->set_materialize_grads(false);
+    if (want_state) return {o.o, o.state};
+    return {o.o};
+  }
+
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    const variable_list s = saved(ctx);
+    const Tensor d_state = g.size() > 1 ? g[1] : Tensor();
+    variable_list out(8);
+    if (!g[0].defined() && !d_state.defined()) return out;
+    const c10::DeviceGuard guard(s[0].device());
+    const at::ScalarType dt = s[0].scalar_type();
+    const Tensor q = s[0], k = s[1].to(dt), v = s[2].to(dt), ld = f32(s[3]);
+    const Tensor off = s[4].defined() ? int_offsets(s[4]) : s[4], first = f32(s[5]), last = f32(d_state);
+    const Tensor dout = g[0].defined() ? g[0].to(dt) : at::zeros(v.sizes(), v.options().requires_grad(false));
+    // inputs that were None do not count
+    const bool need[4] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2),
+                          first.defined() && ctx->needs_input_grad(4 + off.defined())};
+    const Heads a(q), b(k), c(v), d(dout);
+    const int64_t N = off.defined() ? off.size(0) : q.size(0);
+    Tensor kept = whole(s[6]);
+    if (kept.defined() &&
+        (kept.scalar_type() != at::kByte ||
+         kept.numel() != (int64_t)mhc_decay_attention_workspace_bytes(a.R, N, a.H, a.D, c.D, off.defined(), code(q))))
+      kept = Tensor();  // a saved-tensor hook has changed it: computed again
+    Tensor dq, dk, dv, ds;
+    if (need[0]) dq = plain_empty(q.sizes(), q);
+    if (need[1]) dk = plain_empty(k.sizes(), k);
+    if (need[2]) dv = plain_empty(v.sizes(), v);
+    if (need[3]) ds = empty_f32({N, a.H, a.D, c.D}, q);
+    const Workspace ws(mhc_decay_attention_backward_workspace_bytes(a.R, N, a.H, a.D, c.D, off.defined(), code(q)), q);
+    check(mhc_decay_attention_backward(a.p(), a.row, a.head, b.p(), b.row, b.head, c.p(), c.row, c.head, d.p(), d.row, d.head,
+                                       code(q), fptr(ld), static_cast<const int32_t*>(ptr(off)), fptr(first), fptr(kept),
+                                       fptr(last), ptr(dq), ptr(dk), ptr(dv), wptr(ds), a.R, N, a.H, a.D, c.D,
+                                       (float)ctx->saved_data["scale"].toDouble(), ws.p(), ws.bytes, stream(q)),
+          "decay_attention_backward");
+    bool graph = g[0].defined() && g[0].requires_grad();
+    for (const Tensor* t : {&d_state, &s[0], &s[1], &s[2], &s[5]}) graph = graph || (t->defined() && t->requires_grad());
+    out[0] = first_order(dq, "decay_attention", graph);
+    out[1] = first_order(dk, "decay_attention", graph);
+    out[2] = first_order(dv, "decay_attention", graph);
+    out[5] = first_order(ds, "decay_attention", graph);
+    return out;
+  }
+};
+
+// q, k, v (..., heads, dim) and their decays
+bool decay_operands(const Tensor* t) {
+  const Tensor &q = t[0], &k = t[1], &v = t[2];
+  return code(q) >= 0 && k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type() && q.dim() >= 3 &&
+         k.sizes() == q.sizes() && v.dim() == q.dim() && v.sizes().slice(0, v.dim() - 1) == q.sizes().slice(0, q.dim() - 1) &&
+         q.size(-1) >= 1 && q.size(-1) <= 128 && v.size(-1) >= 1 && v.size(-1) <= 128 && t[3].is_floating_point() &&
+         t[3].sizes() == at::IntArrayRef({q.size(-2)});
+}
+
+PyObject* py_decay_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor t[4], initial, off;
+  double scale;
+  bool want_state;
+  if (n != 8 || !tensors(a, 4, t) || !optional_tensor(a[4], t[0], &initial) || !optional_tensor(a[5], t[0], &off) ||
+      !number(a[6], &scale) || !flag(a[7], &want_state) || !decay_operands(t))
+    return none();
+  const Tensor& q = t[0];
+  if (q.dim() != (off.defined() ? 3 : 4) ||
+      (off.defined() && (off.dim() != 1 || (off.scalar_type() != at::kInt && off.scalar_type() != at::kLong))))
+    return none();
+  if (initial.defined() &&
+      (initial.scalar_type() != at::kFloat ||
+       initial.sizes() != at::IntArrayRef({off.defined() ? off.size(0) : q.size(0), q.size(-2), q.size(-1), t[2].size(-1)})))
+    return none();
+  variable_list out;
+  {
+    ReleaseGil gil;
+    if (wants_grad({t[0], t[1], t[2], initial})) {
+      out = DecayAttention::apply(t[0], t[1], t[2], t[3], given(off), given(initial), scale, want_state);
+    } else {
+      const DecayOut o = decay_forward(t[0], t[1], t[2], t[3], off, initial, scale, want_state);
+      out = {o.o};
+      if (want_state) out.push_back(o.state);
+    }
+  }
+  return out.size() == 1 ? THPVariable_Wrap(out[0]) : tuple_of(out);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_decay_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor t[5], slots, state_out;
+  double scale;
+  if (n != 8 || !tensors(a, 5, t) || !optional_tensor(a[5], t[0], &slots) || !number(a[6], &scale) ||
+      !optional_tensor(a[7], t[0], &state_out) || !decay_operands(t) || t[0].dim() != 3)
+    return none();
+  const Tensor &q = t[0], &v = t[2], &state = t[4];
+  const int64_t R = q.size(0), H = q.size(1), Dk = q.size(2), Dv = v.size(2);
+  if (state.dim() != 4 || state.sizes() != at::IntArrayRef({state.size(0), H, Dk, Dv}) || state.scalar_type() != at::kFloat ||
+      !state.is_contiguous() || wants_grad({t[0], t[1], t[2], t[3], t[4], state_out}))
+    return none();
+  if (state_out.defined()) {
+    if (state_out.sizes() != state.sizes() || state_out.scalar_type() != at::kFloat || !state_out.is_contiguous()) return none();
+    const char *x = static_cast<const char*>(ptr(state)), *y = static_cast<const char*>(ptr(state_out));
+    if (x != y && x < y + state.nbytes() && y < x + state.nbytes()) return none();
+  }
+  if (slots.defined() ? slots.sizes() != at::IntArrayRef({R}) || (slots.scalar_type() != at::kInt && slots.scalar_type() != at::kLong)
+                      : R > state.size(0))
+    return none();
+  Tensor o;
+  {
+    ReleaseGil gil;
+    const c10::DeviceGuard guard(q.device());
+    const Tensor to = state_out.defined() ? state_out : state, ld = f32(t[3]);
+    Tensor s = slots;
+    if (s.defined()) s = (s.scalar_type() == at::kInt ? s : at::clamp(s, -1, INT32_MAX).to(at::kInt)).contiguous();
+    const Heads x(q), y(t[1]), z(v);
+    o = plain_empty(v.sizes(), v);
+    check(mhc_decay_attention_step(x.p(), x.row, x.head, y.p(), y.row, y.head, z.p(), z.row, z.head, code(q), fptr(ld),
+                                   static_cast<const int32_t*>(ptr(s)), fptr(state), wptr(to), ptr(o), R, state.size(0), H, Dk,
+                                   Dv, (float)scale, stream(q)),
+          "decay_attention_step");
+    if (!to.is_inference()) to.unsafeGetTensorImpl()->bump_version();
+  }
+  return THPVariable_Wrap(o);
+  END_HANDLE_TH_ERRORS
+}
+
+struct GatedOut { Tensor y, saved; };
+
+GatedOut gated_forward(const Tensor& x_in, const Tensor& w_in, const Tensor& offsets, int64_t act, bool keep) {
+  const c10::DeviceGuard guard(x_in.device());
+  const Tensor x = x_in.contiguous(), w = w_in.contiguous(), off = offsets.defined() ? int_offsets(offsets) : offsets;
+  const int64_t R = x.size(0), K = x.size(1), N = w.size(-2) / 2;
+  GatedOut o{plain_empty({R, N}, x), keep ? empty_f32({R, 2 * N}, x) : Tensor()};
+  check(mhc_gated_matmul_forward(ptr(x), ptr(w), code(x), static_cast<const int32_t*>(ptr(off)), (int)act, ptr(o.y),
+                                 wptr(o.saved), R, K, N, off.defined() ? w.size(0) : 1, stream(x)),
+        "gated_matmul_forward");
+  return o;
+}
+
+struct GatedMatmul : Function<GatedMatmul> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const std::optional<Tensor>& offsets, int64_t act) {
+    const Tensor off = offsets.value_or(Tensor());
+    const GatedOut o = gated_forward(x, w, off, act, true);
+    ctx->save_for_backward({x, w, off, o.saved});
+    ctx->saved_data["act"] = act;
+    return o.y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    const variable_list s = saved(ctx);
+    const c10::DeviceGuard guard(s[0].device());
+    const at::ScalarType dt = s[0].scalar_type();
+    const Tensor x = s[0].contiguous(), w = in_dtype(s[1], dt), off = s[2].defined() ? int_offsets(s[2]) : s[2], kept = f32(s[3]);
+    const Tensor dy = in_dtype(g[0], dt);
+    const int64_t R = x.size(0), K = x.size(1), N = w.size(-2) / 2;
+    Tensor dx, dw;
+    if (ctx->needs_input_grad(0)) dx = plain_empty(x.sizes(), x);
+    if (ctx->needs_input_grad(1)) dw = plain_empty(w.sizes(), w);
+    const Workspace ws(mhc_gated_matmul_backward_workspace_bytes(R, N, code(x)), x);
+    check(mhc_gated_matmul_backward(ptr(dy), fptr(kept), ptr(x), ptr(w), code(x), static_cast<const int32_t*>(ptr(off)),
+                                    (int)ctx->saved_data["act"].toInt(), ptr(dx), ptr(dw), R, K, N, off.defined() ? w.size(0) : 1,
+                                    ws.p(), ws.bytes, stream(x)),
+          "gated_matmul_backward");
+    const bool graph = g[0].requires_grad() || s[0].requires_grad() || s[1].requires_grad();
+    return {first_order(dx, "gated_matmul", graph), first_order(dw, "gated_matmul", graph), Tensor(), Tensor()};
+  }
+};
+
+PyObject* py_gated_matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor t[2], off;
+  if (n != 4 || !tensors(a, 2, t) || !optional_tensor(a[2], t[0], &off) || !PyUnicode_CheckExact(a[3])) return none();
+  const Tensor &x = t[0], &w = t[1];
+  const int64_t act = PyUnicode_CompareWithASCIIString(a[3], "silu") == 0        ? MHC_ACT_SILU
+                      : PyUnicode_CompareWithASCIIString(a[3], "gelu") == 0      ? MHC_ACT_GELU
+                      : PyUnicode_CompareWithASCIIString(a[3], "gelu_tanh") == 0 ? MHC_ACT_GELU_TANH
+                                                                                 : -1;
+  if (act < 0 || code(x) < 0 || w.scalar_type() != x.scalar_type() || x.dim() != 2 || w.dim() != (off.defined() ? 3 : 2) ||
+      w.size(-2) % 2 || x.size(1) != w.size(-1))
+    return none();
+  if (off.defined() && (off.sizes() != w.sizes().slice(0, 1) || (off.scalar_type() != at::kInt && off.scalar_type() != at::kLong)))
+    return none();
+  Tensor y;
+  {
+    ReleaseGil gil;
+    if (wants_grad({x, w})) y = GatedMatmul::apply(x, w, given(off), act);
+    else y = gated_forward(x, w, off, act, false).y;
+  }
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* py_set_error(PyObject*, PyObject* cls) {
   Py_INCREF(cls);
   Py_XDECREF(g_error);
@@ -1036,6 +1358,8 @@ PyMethodDef methods[] = {
     {"dynamic_weights", FAST(py_dynamic_weights)}, {"expand", FAST(py_ends<true>)},
     {"collapse", FAST(py_ends<false>)},          {"rms_norm", FAST(py_rms_norm)},
     {"dropout", FAST(py_dropout)},               {"grouped_matmul", FAST(py_grouped_matmul)},
+    {"rotary", FAST(py_rotary)},                 {"decay_attention", FAST(py_decay_attention)},
+    {"decay_attention_step", FAST(py_decay_step)}, {"gated_matmul", FAST(py_gated_matmul)},
     {"set_error", py_set_error, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

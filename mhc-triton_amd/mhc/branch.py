@@ -330,17 +330,19 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     q and k are read where they lie if a head's elements are neighbours and one stride leads from row to row, parts of
     a fused projection's output among them; others are copied.  The results are contiguous.  Differentiable in q and k.
     """
-    _no_gradient("rotary", frequencies=frequencies)
+    _no_gradient("rotary", "frequencies", frequencies)
     if torch.compiler.is_compiling():
         return _ml.rotary(q, k, positions, frequencies, bool(interleaved), float(magnitude))
+    if q.is_cuda:
+        out = _lib.native().rotary(q, k, positions, frequencies, bool(interleaved), float(magnitude))
+        if out is not None:
+            return out
     return _Rotary.apply(q, k, positions, frequencies, bool(interleaved), float(magnitude))
 
 
-def _no_gradient(name: str, **tensors) -> None:
-    """Refuses gradients of arguments that have none."""
-    for what, t in tensors.items():
-        if isinstance(t, torch.Tensor) and t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError(f"mhc: {name} has no gradient of {what}; detach it")
+def _no_gradient(name: str, what: str, t: torch.Tensor) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"mhc: {name} has no gradient of {what}; detach it")
 
 
 def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
@@ -361,11 +363,15 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     is the operand, exactly for inputs.  A value that is not finite reaches its own and later tokens of its sequence and
     head, no others; which of them are infinite and which NaN may differ from the recurrence's.
     """
-    _no_gradient("decay_attention", log_decay=log_decay)
+    _no_gradient("decay_attention", "log_decay", log_decay)
     scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
     if torch.compiler.is_compiling():
         out = _ml.decay_attention(q, k, v, log_decay, offsets, initial_state, scale)
         return out if return_state else out[0]
+    if q.is_cuda:
+        out = _lib.native().decay_attention(q, k, v, log_decay, initial_state, offsets, scale, bool(return_state))
+        if out is not None:
+            return out
     return _DecayAttention.apply(q, k, v, log_decay, offsets, initial_state, scale, bool(return_state))
 
 
@@ -380,9 +386,14 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
     gives zeros and touches no state, and states of no row stay as they are.  With ``state_out`` the rows' new states go
     there and ``state`` stays: the one before is kept for tokens that may be taken back.  No backward.
     """
-    _inference_only("decay_attention_step", q, k, v, log_decay, state, state_out)
     scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
-    if torch.compiler.is_compiling():
+    compiling = torch.compiler.is_compiling()
+    if q.is_cuda and not compiling:
+        o = _lib.native().decay_attention_step(q, k, v, log_decay, state, slots, scale, state_out)
+        if o is not None:
+            return o
+    _inference_only("decay_attention_step", q, k, v, log_decay, state, state_out)
+    if compiling:
         return _ml.decay_attention_step(q, k, v, log_decay, state, slots, scale, state_out)
     o = _m.decay_attention_step(q, k, v, log_decay, state, slots, scale, state_out)
     out = state if state_out is None else state_out
@@ -403,4 +414,8 @@ def gated_matmul(x: torch.Tensor, weight: torch.Tensor, offsets: Optional[torch.
     """
     if torch.compiler.is_compiling():
         return _ml.gated_matmul(x, weight, offsets, activation)
+    if x.is_cuda:
+        y = _lib.native().gated_matmul(x, weight, offsets, activation)
+        if y is not None:
+            return y
     return _GatedMatmul.apply(x, weight, offsets, activation)

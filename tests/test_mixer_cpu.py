@@ -206,7 +206,7 @@ def test_abi_refusals_before_any_device_work():
                                                1.0, ws, nb, None)
 
     assert fwd(q=None) == fwd(o=None) == fwd(ld=None) == fwd(R=7) == fwd(Dk=129) == fwd(Dv=0) == fwd(R=-8) == 1
-    assert fwd(row=(1 << 22) + 1) == fwd(row=-1) == fwd(R=1 << 31, N=1) == fwd(N=0) == 1
+    assert fwd(row=(1 << 22) + 1) == fwd(row=-1) == fwd(R=1 << 31, N=1) == 1
     assert fwd(R=0, q=None, o=None) == fwd(H=0, q=None) == fwd(R=0, N=0) == 0 and fwd(code=3) == 2
     need = lib.mhc_decay_attention_workspace_bytes(8192, 1, 2, 64, 64, 0, 1)
     assert need > 0 and need % (2 * 64 * 64 * 4) == 0 and lib.mhc_decay_attention_workspace_bytes(64, 1, 2, 64, 64, 0, 1) == 0
