@@ -80,22 +80,34 @@ static int launch_gate_backward(GateArgs a, const char* who, hipStream_t st) {
   return MHC_OK;
 }
 
-// As launch_grouped chooses, a column counting for its gate and its value.
+// As launch_grouped chooses, a column counting for its gate and its value, with limits of its own for fp32, whose loop is
+// bound by the matrix cores at any tile (times in us, cold weights where they matter):
+//   few rows an expert: 4096 to 8192, one expert, 1 / 8 / 16 / 32 / 64 rows: weights into registers 30.0 / 30.3 / 31.7 / 53.4 / 97.6,
+//   64-tiles 30.8 / 31.8 / 31.1 / 31.5 / 32.4 (4.3 TB/s: the weights alone, from memory).
+//   256 against 128 with 288, 320, 512 and 576 likely 256-tiles: bf16 53 / 58, 101 / 112, 229 / 269 and 158 / 181; with 144,
+//   80 and 48 39 / 37, 30 / 21 and 16.5 / 18.5.  fp32, 256 against 64, with 288, 320, 512 and 576: 322 / 324, 626 / 608, 1916 / 2184 and 1114 / 1173.
+//   128 against 64 with 544, 288, 160 and 96 likely 128-tiles: bf16 37 / 46, 21 / 28, 18.5 / 18.7 and 18.0 / 11.5; fp32 200 / 173,
+//   130 / 99, 74 / 63 and 73 / 40.
+//   any alignment, 128 against 64 with 544, 416, 288, 224 and 160 likely 128-tiles: bf16 57 / 51, 32 / 45, 32 / 40, 30 / 29 and 29 / 22; fp32
+//   229 / 164, 145 / 143, 143 / 109, 89 / 87 and 88 / 67.
 template <typename T>
 static int launch_gated(GroupedArgs a, const char* who, hipStream_t st) {
+  constexpr bool F32 = sizeof(T) == 4;
   const bool chunks = a.lda % kElems<T> == 0 && a.ldb % kElems<T> == 0 && aligned16(a.A) && aligned16(a.B);
   const int cus = num_cus();
   const bool few = a.R <= 8 * (int64_t)a.E;
   if (chunks) {
     if (few) return launch_few<T, T, 1, 2, 4, 2, true, true>(a, who, st);
-    if (likely_tiles<Role::kRows, 256, 128>(a) >= cus && a.R >= 256 * (int64_t)a.E)
+    if (likely_tiles<Role::kRows, 256, 128>(a) >= (F32 ? 2 : 1) * cus && a.R >= 256 * (int64_t)a.E)
       return launch_direct<T, T, false, false, 256, 256, 2, 4, 2, Role::kRows, true>(a, who, st);
-    if (likely_tiles<Role::kRows, 128, 64>(a) >= cus)
-      return launch_direct<T, T, false, false, 128, 128, 2, 2, 2, Role::kRows, true>(a, who, st);
+    if constexpr (!F32)
+      if (likely_tiles<Role::kRows, 128, 64>(a) >= cus)
+        return launch_direct<T, T, false, false, 128, 128, 2, 2, 2, Role::kRows, true>(a, who, st);
     return launch_direct<T, T, false, false, 64, 64, 2, 2, 4, Role::kRows, true>(a, who, st);
   }
   if (few) return launch_few<T, T, 1, 2, 4, 2, false, true>(a, who, st);
-  if (likely_tiles<Role::kRows, 128, 64>(a) >= 2 * cus) return launch_general<T, false, false, 128, 128, Role::kRows, true>(a, who, st);
+  if constexpr (!F32)
+    if (likely_tiles<Role::kRows, 128, 64>(a) >= cus) return launch_general<T, false, false, 128, 128, Role::kRows, true>(a, who, st);
   return launch_general<T, false, false, 64, 64, Role::kRows, true>(a, who, st);
 }
 
