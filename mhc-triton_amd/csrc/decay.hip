@@ -12,6 +12,10 @@ namespace mhc {
 // Tokens of a segment.  Enough segments for two workgroups a CU (the kernel's occupancy), but none shorter than
 // kLeast: each costs a state written and read again by those behind it.
 constexpr int64_t kLeast = 512;
+// A segment adds up the states before it, up to this many segments; beyond, decay_join_kernel does it once for all of them.
+// bf16 heads of 128, forward, summed / joined: 32 heads of 8192 tokens (16 segments) 130 / 131 us, 16 of 16384 (32) 150 /
+// 130, 8 of 32768 (64) 192 / 139, one of 65536 (128) 164 / 98.
+constexpr int64_t kSummed = 16;
 
 // Columns of the state that a workgroup holds.  fp32 planes of 128 columns do not fit in LDS.
 static int64_t group_cols(int64_t Dv, int dtype) { return Dv <= 64 || dtype == MHC_DTYPE_F32 ? 64 : 128; }
@@ -36,12 +40,15 @@ static int64_t count_tiles(int64_t R, int64_t N, int64_t seg, bool packed) {
 // A scan's segments and what the states that they leave take.
 struct Plan {
   int64_t seg, tiles, bytes;  // bytes 0: no sequence has a second segment
+  bool joined;
 };
 static Plan plan_scan(int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv, bool packed, int dtype) {
   Plan p;
   p.seg = segment_tokens(R, N, H, Dv, packed, dtype);
   p.tiles = count_tiles(R, N, p.seg, packed);
-  p.bytes = (packed || N == 0 ? R : R / N) > p.seg ? p.tiles * H * Dk * Dv * 4 : 0;
+  const int64_t longest = packed || N == 0 ? R : R / N;
+  p.bytes = longest > p.seg ? p.tiles * H * Dk * Dv * 4 : 0;
+  p.joined = longest > kSummed * p.seg;
   return p;
 }
 
@@ -58,6 +65,11 @@ static int launch_scan(DecayJobs& jobs, bool states, bool outputs, const char* w
   }
   const dim3 grid((unsigned)groups);
   if (states) decay_kernel<T, DK, WAVES, WEIGHTED, CHUNKS, true><<<grid, NTH, 0, st>>>(jobs);
+  if (states && a.joined) {
+    const int64_t most = (((int64_t)1 << 32) / kThreads - 1) / ((int64_t)a.tiles * a.H), want = (a.Dk * a.Dv + kJoin - 1) / kJoin;
+    const int blocks = (int)(want < most ? want : most);
+    decay_join_kernel<<<dim3((unsigned)(a.tiles * a.H * blocks)), kThreads, 0, st>>>(a, blocks);
+  }
   if (outputs) decay_kernel<T, DK, WAVES, WEIGHTED, CHUNKS, false><<<grid, NTH, 0, st>>>(jobs);
   return hip_status(hipGetLastError(), who);
 }
@@ -82,6 +94,7 @@ static int scan(DecayJobs jobs, const Plan& plan, int what, bool exact, const ch
     a.T = a.N ? a.R / a.N : 0;
     a.seg = (int)plan.seg;
     a.tiles = (int)plan.tiles;
+    a.joined = plan.joined;
     chunks = chunks && whole_chunks<T>(a.q, a.q_row, a.q_head, a.Dk) && whole_chunks<T>(a.k, a.k_row, a.k_head, a.Dk) &&
              whole_chunks<T>(a.v, a.v_row, a.v_head, a.Dv) && aligned16(a.o);
   }

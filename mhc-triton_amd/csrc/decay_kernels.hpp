@@ -15,7 +15,8 @@
 // and V of a chunk go through LDS; P is made once for all waves and passes through LDS.  Registers are held below 128
 // for bf16, for four waves a SIMD: phases that wait for LDS, for the matrix cores and for the VALU then overlap.
 // Segments but the last are first run for their state alone (STATE_ONLY), so that long sequences with
-// few heads fill the card; each then starts from the sum of the states before it.
+// few heads fill the card; each then starts from the sum of the states before it, which decay_join_kernel has made where
+// there are many.
 //
 // Precision.  The matrix instructions multiply bf16.  Every operand is a sum of bf16 parts: inputs exactly (bf16 one part,
 // fp16 two, fp32 three), what is computed (P, the state, weighted V) in as many as keep the error far below one rounding to the
@@ -42,10 +43,11 @@ struct DecayArgs {
   const int32_t* offsets;    // ends of the packed sequences; null: N sequences of T rows each, or with N = 0 none
   const float* first;        // X_0 of each sequence, or null
   float* last;               // where X goes, or null
-  float* parts;              // states that segments leave by themselves, [tile][H][Dk][Dv]
+  float* parts;              // [tile][H][Dk][Dv]: states that segments leave by themselves; joined: that the next start from
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;  // strides in elements; o is contiguous
   int state_row, state_col;                             // of first and last: X's rows and columns
   int part_row, part_col;                               // of parts
+  bool joined;
   int64_t R, T;
   int H, N, Dk, Dv, seg, tiles, col_tiles;
   float out_scale, in_scale;  // a, b
@@ -341,8 +343,9 @@ __global__ __launch_bounds__(64 * WAVES, (kDecayWaves<T, DK, WAVES, STATE_ONLY>)
         x[td] += w * y;
       }
     };
-    if (a.first) add(a.first + ((int64_t)e * a.H + h) * size, a.state_row, a.state_col, power(ld, begin).hi);
-    for (int s = 0; s < seg; ++s)
+    const bool joined = a.joined && seg;
+    if (a.first && !joined) add(a.first + ((int64_t)e * a.H + h) * size, a.state_row, a.state_col, power(ld, begin).hi);
+    for (int s = joined ? seg - 1 : 0; s < seg; ++s)
       add(a.parts + ((int64_t)(tile - seg + s) * a.H + h) * size, a.part_row, a.part_col, power(ld, (int64_t)(seg - 1 - s) * a.seg).hi);
     // P above the diagonal, where a row's 32 tokens reach past it
     for (int i = threadIdx.x; i < MADE * kPlane<kChunk>; i += NTH) lp[i] = u32x4{0, 0, 0, 0};
@@ -612,6 +615,53 @@ __global__ __launch_bounds__(64 * WAVES, (kDecayWaves<T, DK, WAVES, STATE_ONLY>)
     for (int r = 0; r < 4; ++r)
       __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[td][r]), rsrc, place_of(td, r, row, column), 0, 0);
 #endif
+}
+
+// From the states that a sequence's segments leave by themselves to those that the next ones start from, in place:
+//   X_0 = first,  X_(s+1) = l^seg X_s + part_s
+// A workgroup has a sequence's first tile, a head and every `blocks`-th kJoin values of the state; the next segments' loads
+// are in flight.
+constexpr int kJoin = 4 * kThreads;
+
+__global__ __launch_bounds__(kThreads) void decay_join_kernel(DecayArgs a, int blocks) {
+  const int unit = blockIdx.x / blocks, tile = unit / a.H, h = unit - tile * a.H;
+  const Segment sg = find_segment(a, tile);
+  if (sg.e < 0 || sg.e == a.N || sg.s) return;
+  const int segments = (int)((sg.hi - sg.lo + a.seg - 1) / a.seg), size = a.Dk * a.Dv;
+  if (segments < 2) return;
+  const float given = a.log_decay[h];
+  const Power l = power(given > 0.f ? 0.f : given, a.seg);
+  const int64_t step = (int64_t)a.H * size;  // from a segment's state to the next one's
+  float* part = a.parts + ((int64_t)tile * a.H + h) * size;
+  const float* first = a.first ? a.first + ((int64_t)sg.e * a.H + h) * size : nullptr;
+  constexpr int V = kJoin / kThreads, AHEAD = 4;
+  for (int block = blockIdx.x % blocks; block * kJoin < size; block += blocks) {
+    int at[V];
+    float x[V], p[AHEAD][V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      at[i] = block * kJoin + i * kThreads + (int)threadIdx.x;
+      // parts are [Dk][Dv]; first has strides
+      x[i] = first && at[i] < size ? first[at[i] / a.Dv * a.state_row + at[i] % a.Dv * a.state_col] : 0.f;
+    }
+    auto load = [&](int s, float (&to)[V]) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) to[i] = s + 1 < segments && at[i] < size ? part[s * step + at[i]] : 0.f;
+    };
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n) load(n, p[n]);
+    for (int s = 0; s + 1 < segments; s += AHEAD) {
+#pragma unroll
+      for (int n = 0; n < AHEAD; ++n) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          x[i] = __builtin_fmaf(x[i], l.hi, __builtin_fmaf(x[i], l.lo, p[n][i]));
+          if (s + n + 1 < segments && at[i] < size) part[(s + n) * step + at[i]] = x[i];
+        }
+        load(s + n + AHEAD, p[n]);
+      }
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------

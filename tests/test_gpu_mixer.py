@@ -145,6 +145,24 @@ def test_decay_attention_in_segments(Dk, Dv, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("Dk,Dv,ends", [(128, 128, None), (64, 40, [8800, 8800, 9290]), (40, 100, [9301]), (100, 70, [30, 9000])])
+def test_decay_attention_in_many_segments(Dk, Dv, ends, dtype):
+    """More segments than each adds up for itself."""
+    dt, H, T = DT[dtype], 1, 9301
+    q, k = (rand(T, H, Dk, seed=i, dtype=dt).requires_grad_() for i in (1, 2))
+    v, do = rand(T, H, Dv, seed=3, dtype=dt).requires_grad_(), rand(T, H, Dv, seed=4, dtype=dt)
+    spans = [(0, T)] if ends is None else M.spans_of(ends, T)
+    N, off = len(spans), None if ends is None else torch.tensor(ends, device=DEV)
+    first, d_last = rand(N, H, Dk, Dv, seed=5).requires_grad_(), rand(N, H, Dk, Dv, seed=6)
+    ld = torch.tensor([-0.0005], device=DEV)
+    if ends is None:
+        q, k, v = (t.detach()[None].requires_grad_() for t in (q, k, v))
+        do = do[None]
+    check_decay(q, k, v, ld, off, first, do, d_last, Dk ** -0.5, spans)
+    check_decay(q, k, v, ld, off, None, do, None, Dk ** -0.5, spans)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("R,pool,H,Dk,Dv", [(1, 1, 1, 1, 1), (3, 5, 2, 128, 128), (4, 4, 3, 64, 72), (5, 9, 2, 33, 95), (300, 310, 1, 16, 8)])
 def test_decay_attention_step(R, pool, H, Dk, Dv, dtype):
     dt = DT[dtype]
