@@ -9,22 +9,24 @@
 
 namespace mhc {
 
-// Tokens of a segment.  Enough segments for two workgroups a CU (the kernel's occupancy), but none shorter than
-// kLeast: each costs a state written and read again by those behind it.
-constexpr int64_t kLeast = 512;
+// Tokens of a segment.  Enough segments for a workgroup a CU, but none shorter than kLeast: each costs a state written and
+// read again.  Forward / backward of bf16 heads of 128: 32 heads of 8192 tokens 112 / 235 us, with two workgroups a CU 118 /
+// 250; 8 heads of 2048 43 / 50 us, with kLeast = 512 53 / 59; the other way round from 256 segments of one head on (65536
+// tokens 109 / 140, with 512 91 / 116).
+constexpr int64_t kLeast = 256;
 // A segment adds up the states before it, up to this many segments; beyond, decay_join_kernel does it once for all of them.
-// bf16 heads of 128, forward, summed / joined: 32 heads of 8192 tokens (16 segments) 130 / 131 us, 16 of 16384 (32) 150 /
-// 130, 8 of 32768 (64) 192 / 139, one of 65536 (128) 164 / 98.
-constexpr int64_t kSummed = 16;
+// Summed / joined, us: backward of 32 heads of 8192 tokens as 16 segments 301 / 246, forward of 8 heads of 32768 as 64
+// 192 / 139; forward of 32 heads of 2048 as 8 47 / 51.
+constexpr int64_t kSummed = 8;
 
-// Columns of the state that a workgroup holds.  fp32 planes of 128 columns do not fit in LDS.
-static int64_t group_cols(int64_t Dv, int dtype) { return Dv <= 64 || dtype == MHC_DTYPE_F32 ? 64 : 128; }
+// Columns of the state that a workgroup holds.
+static int64_t group_cols(int64_t Dv) { return Dv <= 64 ? 64 : 128; }
 
-static int64_t segment_tokens(int64_t R, int64_t N, int64_t H, int64_t Dv, bool packed, int dtype) {
+static int64_t segment_tokens(int64_t R, int64_t N, int64_t H, int64_t Dv, bool packed) {
   const int64_t longest = packed || N == 0 ? R : R / N;
-  const int64_t heads = H * ((Dv + group_cols(Dv, dtype) - 1) / group_cols(Dv, dtype));
+  const int64_t heads = H * ((Dv + group_cols(Dv) - 1) / group_cols(Dv));
   const int64_t sequences = packed ? 1 : N;
-  int64_t want = 2 * num_cus() / (heads * sequences > 0 ? heads * sequences : 1);
+  int64_t want = num_cus() / (heads * sequences > 0 ? heads * sequences : 1);
   if (want < 1) want = 1;
   int64_t seg = (longest + want - 1) / want;
   if (seg < kLeast) seg = kLeast;
@@ -42,9 +44,9 @@ struct Plan {
   int64_t seg, tiles, bytes;  // bytes 0: no sequence has a second segment
   bool joined;
 };
-static Plan plan_scan(int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv, bool packed, int dtype) {
+static Plan plan_scan(int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv, bool packed) {
   Plan p;
-  p.seg = segment_tokens(R, N, H, Dv, packed, dtype);
+  p.seg = segment_tokens(R, N, H, Dv, packed);
   p.tiles = count_tiles(R, N, p.seg, packed);
   const int64_t longest = packed || N == 0 ? R : R / N;
   p.bytes = longest > p.seg ? p.tiles * H * Dk * Dv * 4 : 0;
@@ -110,7 +112,8 @@ static int scan(DecayJobs jobs, const Plan& plan, int what, bool exact, const ch
   };
   using std::integral_constant;
   if constexpr (sizeof(T) == 4) {
-    return launch(integral_constant<int, 4>(), integral_constant<int, 3>());
+    return a.Dv > 64 ? launch(integral_constant<int, 8>(), integral_constant<int, 3>())
+                     : launch(integral_constant<int, 4>(), integral_constant<int, 3>());
   } else {
     if (exact) return a.Dv > 64 ? launch(integral_constant<int, 8>(), integral_constant<int, 3>())
                                 : launch(integral_constant<int, 4>(), integral_constant<int, 3>());
@@ -166,9 +169,9 @@ static int launch_step(DecayStepArgs a, const char* who, hipStream_t st) {
 using namespace mhc;
 
 extern "C" size_t mhc_decay_attention_workspace_bytes(int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv, int packed,
-                                                      int dtype) {
+                                                      int /*dtype*/) {
   if (R <= 0 || N < 0 || H <= 0 || Dk <= 0 || Dv <= 0) return 0;
-  return (size_t)plan_scan(R, N, H, Dk, Dv, packed, dtype).bytes;
+  return (size_t)plan_scan(R, N, H, Dk, Dv, packed).bytes;
 }
 
 extern "C" int mhc_decay_attention_forward(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
@@ -192,7 +195,7 @@ extern "C" int mhc_decay_attention_forward(const void* q, int64_t q_row, int64_t
   a.parts = (float*)workspace; a.part_row = (int)Dv; a.part_col = 1;
   a.R = R; a.N = (int)N; a.H = (int)H; a.Dk = (int)Dk; a.Dv = (int)Dv;
   a.out_scale = scale; a.in_scale = 1.f; a.lag = 1;
-  const Plan plan = plan_scan(R, N, H, Dk, Dv, packed, dtype);
+  const Plan plan = plan_scan(R, N, H, Dk, Dv, packed);
   return MHC_DISPATCH_DTYPE(dtype, [&] {
     return scan<T>(jobs, plan, kStates | kOutputs, last != nullptr, who, (hipStream_t)stream);
   });
@@ -225,7 +228,7 @@ extern "C" int mhc_decay_attention_backward(const void* q, int64_t q_row, int64_
   const size_t need = mhc_decay_attention_backward_workspace_bytes(R, N, H, Dk, Dv, packed, dtype);
   if (int rc = check_workspace(who, workspace, workspace_bytes, need)) return rc;
   // of states with Dv columns, and of the transposed ones
-  const Plan plan = plan_scan(R, N, H, Dk, Dv, packed, dtype), across = plan_scan(R, N, H, Dv, Dk, packed, dtype);
+  const Plan plan = plan_scan(R, N, H, Dk, Dv, packed), across = plan_scan(R, N, H, Dv, Dk, packed);
   DecayArgs base{};
   base.log_decay = log_decay; base.offsets = offsets;
   base.R = R; base.N = (int)N; base.H = (int)H;

@@ -279,9 +279,13 @@ __device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
 // A value that all lanes hold, in a scalar register.
 __device__ __forceinline__ float uniform(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
 
-// LDS in 16-byte chunks: K and V, and for outputs Q and P.
+// LDS in 16-byte chunks: K and V, and for outputs Q and P.  P takes V's place (two barriers more a chunk) where they do not
+// fit side by side: fp32, 128 columns and keys.
+template <typename T, int DK, int WAVES>
+constexpr bool kInPlace = (kRaw<T> * (2 * kPlane<DK> + kPlane<16 * WAVES>) + kMade<T> * kPlane<kChunk>) * 16 > 160 * 1024;
 template <typename T, int DK, int WAVES, bool STATE_ONLY>
-constexpr int kDecayLds = kRaw<T> * (kPlane<DK> * (STATE_ONLY ? 1 : 2) + kPlane<16 * WAVES>) + (STATE_ONLY ? 0 : kMade<T> * kPlane<kChunk>);
+constexpr int kDecayLds = kRaw<T> * (kPlane<DK> * (STATE_ONLY ? 1 : 2) + kPlane<16 * WAVES>) +
+                          (STATE_ONLY || kInPlace<T, DK, WAVES> ? 0 : kMade<T> * kPlane<kChunk>);
 // Waves a SIMD: what two workgroups a CU come to, where their LDS fits.
 template <typename T, int DK, int WAVES, bool STATE_ONLY>
 constexpr int kDecayWaves = WAVES / 4 * (kDecayLds<T, DK, WAVES, STATE_ONLY> * 16 <= 80 * 1024 ? 2 : 1);
@@ -293,7 +297,8 @@ __global__ __launch_bounds__(64 * WAVES, (kDecayWaves<T, DK, WAVES, STATE_ONLY>)
   constexpr int QK = kPlane<DK>, VP = kPlane<COLS>;
   __shared__ u32x4 lds[kDecayLds<T, DK, WAVES, STATE_ONLY>];
   __shared__ float pow_of[kChunk + 1];  // l^0 .. l^64
-  u32x4 *lk = lds, *lv = lk + RAW * QK, *lq = lv + RAW * VP, *lp = lq + RAW * QK;
+  constexpr bool IN_PLACE = !STATE_ONLY && kInPlace<T, DK, WAVES>;
+  u32x4 *lk = lds, *lv = lk + RAW * QK, *lq = lv + RAW * VP, *lp = IN_PLACE ? lv : lq + RAW * QK;
 
   // scans and column tiles of one (segment, head) side by side on one XCD
   const int run = blockIdx.x / 8, part = run / jobs.n;
@@ -334,6 +339,13 @@ __global__ __launch_bounds__(64 * WAVES, (kDecayWaves<T, DK, WAVES, STATE_ONLY>)
   if constexpr (!STATE_ONLY) {
     auto add = [&](const float* s, int row, int column, float w) {
       const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(s), 0, (int)size * 4, kBufRsrcDword3);
+      // transposed: a lane's four rows are neighbours, and its columns lines apart from the other lanes'
+      if (row == 1 && ((column | a.Dk) & 3) == 0 && ((uintptr_t)s & 15) == 0) {
+#pragma unroll
+        for (int td = 0; td < TD; ++td)
+          x[td] += w * __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, place_of(td, 0, 1, column), 0, 0));
+        return;
+      }
 #pragma unroll
       for (int td = 0; td < TD; ++td) {
         f32x4 y;
@@ -348,7 +360,7 @@ __global__ __launch_bounds__(64 * WAVES, (kDecayWaves<T, DK, WAVES, STATE_ONLY>)
     for (int s = joined ? seg - 1 : 0; s < seg; ++s)
       add(a.parts + ((int64_t)(tile - seg + s) * a.H + h) * size, a.part_row, a.part_col, power(ld, (int64_t)(seg - 1 - s) * a.seg).hi);
     // P above the diagonal, where a row's 32 tokens reach past it
-    for (int i = threadIdx.x; i < MADE * kPlane<kChunk>; i += NTH) lp[i] = u32x4{0, 0, 0, 0};
+    for (int i = threadIdx.x; i < MADE * kPlane<kChunk> && !IN_PLACE; i += NTH) lp[i] = u32x4{0, 0, 0, 0};
   }
   __syncthreads();
 
@@ -404,13 +416,31 @@ __global__ __launch_bounds__(64 * WAVES, (kDecayWaves<T, DK, WAVES, STATE_ONLY>)
     const int n = min(kChunk, stop - t);
     asm volatile("" : "+v"(in_w));  // its products with `place` are made anew: kept, they would be spilled
     fk.store(lk);
-    fv.store(lv);
+    if constexpr (!IN_PLACE) fv.store(lv);
     if constexpr (!STATE_ONLY) fq.store(lq);
+    if constexpr (IN_PLACE) {
+      __syncthreads();  // the last chunk's P has been read
+      fv.store(lv);
+    }
     __syncthreads();
     if constexpr (STATE_ONLY) load(t + kChunk);
 
+    u32x4 vr[2][RAW];  // the wave's columns of V
+    auto read_v = [&] {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int p = 0; p < RAW; ++p) vr[ks][p] = read_columns<COLS>(lv + p * VP, 16 * wave, ks);
+    };
     [[maybe_unused]] f32x4 o[4];
     if constexpr (!STATE_ONLY) {
+      if constexpr (IN_PLACE) read_v();
+      auto put = [&](int i, int j, const uint32_t (&parts)[MADE][2]) {
+        uint64_t* to = reinterpret_cast<uint64_t*>(lp) + 2 * ((16 * i + li) * kPitch<kChunk> + 4 * (j >> 1) + g) + (j & 1);
+#pragma unroll
+        for (int p = 0; p < MADE; ++p) to[2 * p * kPlane<kChunk>] = (uint64_t)parts[p][1] << 32 | parts[p][0];
+      };
+      uint32_t made[kTiles][MADE][2];
       // P: keys are the product's rows, so that a lane gets four neighbouring k of one query
 #pragma unroll
       for (int m = 0; m < kTiles; ++m) {
@@ -433,11 +463,16 @@ __global__ __launch_bounds__(64 * WAVES, (kDecayWaves<T, DK, WAVES, STATE_ONLY>)
           const float w = pw[m][r] * s[r];
           f[r] = far >= 0 ? w : 0.f;
         }
-        uint32_t parts[MADE][2];
-        split<MADE, 2>(f, parts);
-        uint64_t* to = reinterpret_cast<uint64_t*>(lp) + 2 * ((16 * ti[m] + li) * kPitch<kChunk> + 4 * (tj[m] >> 1) + g) + (tj[m] & 1);
+        split<MADE, 2>(f, made[m]);
+        if constexpr (!IN_PLACE) put(ti[m], tj[m], made[m]);
+      }
+      if constexpr (IN_PLACE) {
+        __syncthreads();  // V has been read
 #pragma unroll
-        for (int p = 0; p < MADE; ++p) to[2 * p * kPlane<kChunk>] = (uint64_t)parts[p][1] << 32 | parts[p][0];
+        for (int m = 0; m < kTiles; ++m)
+          if ((m + 1) * WAVES <= 10 || wave + m * WAVES < 10) put(ti[m], tj[m], made[m]);
+        // above the diagonal, where a row's 32 tokens reach past it
+        if (wave >= WAVES - 2) put(wave == WAVES - 1 ? 0 : 2, wave == WAVES - 1 ? 1 : 3, {});
       }
       // Q X: results are (column, query), a lane's query is li of each tile
 #pragma unroll
@@ -472,11 +507,7 @@ __global__ __launch_bounds__(64 * WAVES, (kDecayWaves<T, DK, WAVES, STATE_ONLY>)
     }
 
     // X' = l^n X + K^T (weighted V)
-    u32x4 vr[2][RAW];  // the wave's columns of V
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-      for (int p = 0; p < RAW; ++p) vr[ks][p] = read_columns<COLS>(lv + p * VP, 16 * wave, ks);
+    if constexpr (!IN_PLACE) read_v();
     float by = whole;
     if (__builtin_expect(n < kChunk, false)) by = power(ld, n).hi;
     if (++since == kMend) {  // what rounding l^64 has cost since the last time
