@@ -5,8 +5,9 @@
 //
 // Forward the tiles of grouped_kernels.hpp with gates and values side by side: both products, the activation and their
 // product in one launch, x read once.  For a backward it leaves g and u in fp32: rounded to 16 bits they would put
-// two more roundings into every gradient (1.7 times the error that one rounding of [dg du] and one of the result give),
-// and 32 bits cost 4% of a training step at 16384 rows of 4096 to 8192.
+// two more roundings into every gradient (1.7 times the error that one rounding of [dg du] and one of the result give).
+// At 16384 rows of 4096 to 8192 in bf16 writing them is 190 of the forward's 1950 us, and [dg du] from them 340 us of the
+// backward's 4340.
 //
 // Bound by the matrix products, for few rows by reading the weight.
 #include "grouped_launch.hpp"

@@ -361,7 +361,8 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     Differentiable in q, k, v and initial_state.  Inputs are read where they lie as ``rotary`` reads them (rows at most
     2^22 elements apart), heads that are one expanded among them.  Sums are fp32; products are of bf16 parts whose sum
     is the operand, exactly for inputs.  A value that is not finite reaches its own and later tokens of its sequence and
-    head, no others; which of them are infinite and which NaN may differ from the recurrence's.
+    head, no others; which of them are infinite and which NaN may differ from the recurrence's (fp32 magnitudes that round
+    to no bf16, from 3.39e38 on, count as not finite).
     """
     _no_gradient("decay_attention", "log_decay", log_decay)
     scale = float(q.shape[-1] ** -0.5 if scale is None else scale)

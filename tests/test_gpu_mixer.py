@@ -13,13 +13,15 @@ slopes of the activations, below 1.2; expf and erfcf are within 2^-21 of their v
 its products.
 """
 
+import itertools
+
 import numpy as np
 import pytest
 import torch
 
 from helpers import to_np
 from test_gpu_branch import DT, HALF_ULP, close, rand
-from mhc import branch
+from mhc import _mixer, branch
 from oracle import mixer_oracle as M
 
 pytestmark = pytest.mark.gpu
@@ -160,6 +162,28 @@ def test_decay_attention_in_many_segments(Dk, Dv, ends, dtype):
         do = do[None]
     check_decay(q, k, v, ld, off, first, do, d_last, Dk ** -0.5, spans)
     check_decay(q, k, v, ld, off, None, do, None, Dk ** -0.5, spans)
+
+
+@pytest.mark.parametrize("Dk,Dv", [(128, 96), (40, 64), (100, 30)])
+def test_decay_attention_some_gradients_of_many_segments(Dk, Dv):
+    """Each gradient alone and with others, with the forward's states kept and not."""
+    H, T = 1, 2700
+    q, k, v, do = (rand(1, T, H, d, seed=i, dtype=torch.bfloat16) for i, d in enumerate((Dk, Dk, Dv, Dv)))
+    first, d_last = rand(1, H, Dk, Dv, seed=5), rand(1, H, Dk, Dv, seed=6)
+    ld = torch.tensor([-0.002], device=DEV)
+    args = [to_np(t)[0] for t in (q, k, v, do)]
+    states = to_np(first), to_np(d_last)
+    ref = M.decay_attention_backward(*args, to_np(ld), [(0, T)], *states, 0.1)
+    size = M.decay_attention_backward(*map(np.abs, args), to_np(ld), [(0, T)], *map(np.abs, states), 0.1)
+    kept = _mixer.decay_attention_forward(q, k, v, ld, None, first, 0.1, True)[2]
+    assert kept is not None
+    for need in itertools.product((False, True), repeat=4):
+        for states in (kept, None):
+            got = _mixer.decay_attention_backward(q, k, v, do, ld, None, first, states, d_last, 0.1, need)
+            for g, r, z, n in zip(got, ref, size, need):
+                assert (g is not None) == n
+                if n:
+                    close(g if g.dim() == 4 and g.dtype == torch.float32 else g[0], r, z, decay_tol(g.dtype, T), str(need))
 
 
 @pytest.mark.parametrize("dtype", list(DT))
