@@ -7,21 +7,28 @@
 //   X_n = l^n X_0 + b sum_{j < n} l^(n-L-j) k_j^T v_j
 //
 // X is the state that n tokens leave.  Forward L = 1, and the scale is a; backwards L = 0, because X_0 is the gradient of
-// a state that the last token has already entered, and the scale is b, because that gradient has none.  A chunk of 64 tokens is matrix products: P = (Q K^T) o (weights, lower triangle),
-// O = P V + weights Q X, X' = l^n X + (K^T) (weighted V).
+// a state that the last token has already entered, and the scale is b, because that gradient has none.  A chunk of 64
+// tokens is matrix products: P = (Q K^T) o (weights, lower triangle), O = P V + weights Q X, X' = l^n X + (K^T) (weighted V).
 //
 // A workgroup of WAVES waves takes a segment of a sequence, a head and 16 WAVES of the state's columns; each wave holds
 // 16 columns of the state, all rows, in registers from the first chunk to the last, and never passes it on.  Q, K
 // and V of a chunk go through LDS; P is made once for all waves and passes through LDS.  Registers are held below 128
-// for bf16, for four waves a SIMD: phases that wait for LDS, for the matrix cores and for the VALU then overlap.
+// for bf16, for four waves a SIMD: phases that wait for LDS, for the matrix cores and for the VALU then overlap (four
+// waves of 64 columns each and two a SIMD: 198 us where this takes 139; 32 columns a wave: spills, 399 where 16 take 158).
 // Segments but the last are first run for their state alone (STATE_ONLY), so that long sequences with
 // few heads fill the card; each then starts from the sum of the states before it, which decay_join_kernel has made where
 // there are many.
 //
+// Bound by the phases of a chunk, which hardly overlap inside a workgroup (LDS, VALU and matrix cores 2 us each of 8), and
+// not far behind by memory.  bf16, 4 x 4096 tokens of 32 heads of 128: forward 139 us (3.9 TB/s) and 57 for the segments'
+// states, the gradients' scans together 430 us (2.2 TB/s) and 63; left out for a trial no single part gave more than 7%
+// (loads 4, P 3, Q X 7, P V 3), loads and stores together 28%.  fp32, which has six products for one, 3069 packed tokens
+// of 12 heads: forward 44 us, gradients 101, states 20 each.
+//
 // Precision.  The matrix instructions multiply bf16.  Every operand is a sum of bf16 parts: inputs exactly (bf16 one part,
-// fp16 two, fp32 three), what is computed (P, the state, weighted V) in as many as keep the error far below one rounding to the
-// output's type (two for 16-bit types, three for fp32).  Where the last state is wanted, which is fp32, weighted V has three
-// (WEIGHTED; two in its place are 16 matrix and 40 VALU instructions fewer a wave and chunk).
+// fp16 two, fp32 three), what is computed (P, the state, weighted V) in as many as keep the error far below one rounding to
+// the output's type (two for 16-bit types, three for fp32).  Where the last state is wanted, which is fp32, weighted V has
+// three (WEIGHTED; two in its place are 16 matrix and 40 VALU instructions fewer a wave and chunk).
 // Products of parts whose size is below the last part's are left out.  Sums are fp32.
 #pragma once
 
@@ -379,8 +386,8 @@ __global__ __launch_bounds__(64 * WAVES, (kDecayWaves<T, DK, WAVES, STATE_ONLY>)
   for (int n = 0; n < kTiles; ++n)
 #pragma unroll
     for (int r = 0; r < 4; ++r) pw[n][r] = a.out_scale * a.in_scale * pow_of[max(16 * (ti[n] - tj[n]) + key - 2 * r, 0)];
-  // A chunk's tokens are its last n.  A result's state weight is l^(li + L) times the tile's; a token's weight on the chunk's end one of its lane group's
-  // times one of its place in it, which all lanes share.
+  // A chunk's tokens are its last n.  A result's state weight is l^(li + L) times the tile's; a token's weight on the
+  // chunk's end one of its lane group's times one of its place in it, which all lanes share.
   const float out_w = a.out_scale * pow_of[li + a.lag];
   float in_w = a.in_scale * pow_of[10 - a.lag - token_of(g, 0)];
   float place[8];

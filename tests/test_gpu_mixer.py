@@ -147,7 +147,8 @@ def test_decay_attention_in_segments(Dk, Dv, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(DT))
-@pytest.mark.parametrize("Dk,Dv,ends", [(128, 128, None), (64, 40, [8800, 8800, 9290]), (40, 100, [9301]), (100, 70, [30, 9000])])
+@pytest.mark.parametrize("Dk,Dv,ends", [(128, 128, None), (64, 40, [8800, 8800, 9290]), (40, 100, [9301]), (100, 70, [30, 9000]),
+                                        (72, 72, [7000] + list(range(7001, 7040, 3)))])
 def test_decay_attention_in_many_segments(Dk, Dv, ends, dtype):
     """More segments than each adds up for itself."""
     dt, H, T = DT[dtype], 1, 9301
