@@ -77,9 +77,11 @@ static int launch_scan(DecayJobs& jobs, bool states, bool outputs, const char* w
   return hip_status(hipGetLastError(), who);
 }
 
+// Rows that overlap (one row expanded to all tokens among them) are not: what a buffer over the n rows of a short chunk
+// leaves out then lies inside them.
 template <typename T>
 static bool whole_chunks(const void* p, int64_t row, int64_t head, int64_t D) {
-  return aligned16(p) && row % kElems<T> == 0 && head % kElems<T> == 0 && D % kElems<T> == 0;
+  return aligned16(p) && row >= D && row % kElems<T> == 0 && head % kElems<T> == 0 && D % kElems<T> == 0;
 }
 
 // The segments' states (needed where there are several), or the outputs, of scans alike in their plan and in how many
