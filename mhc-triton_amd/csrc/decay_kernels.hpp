@@ -317,7 +317,8 @@ __global__ __launch_bounds__(64 * WAVES, (kDecayWaves<T, DK, WAVES, STATE_ONLY>)
   const int e = __builtin_amdgcn_readfirstlane(sg.e), seg = __builtin_amdgcn_readfirstlane(sg.s);
   if (e < 0) return;
   const int64_t lo = __builtin_amdgcn_readfirstlane((int)sg.lo), hi = __builtin_amdgcn_readfirstlane((int)sg.hi);
-  const int len = (int)(hi - lo), begin = seg * a.seg, stop = min(begin + a.seg, len);  // tokens
+  const int len = (int)(hi - lo), begin = seg * a.seg;
+  const int stop = begin + min(a.seg, len - begin);  // tokens; begin + a.seg may lie past 2^31
   const int lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = col_tile * COLS + 16 * wave + li;  // of X and V

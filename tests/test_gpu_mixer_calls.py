@@ -6,6 +6,7 @@ import torch
 
 from test_gpu_branch import DT, rand
 from test_gpu_mixer import check_decay, decays
+from mhc import branch
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +38,27 @@ def test_tokens_that_are_windows_of_one_row(dtype):
     off = torch.tensor([30, 85], device=DEV)
     first, d_last = rand(2, H, D, D, seed=5).requires_grad_(), rand(2, H, D, D, seed=6)
     check_decay(*(t.detach().requires_grad_() for t in (q, k, v)), decays(H), off, first, do, d_last, 0.1, [(0, 30), (30, 85)])
+
+
+# --------------------------------------------------------------------------
+# The most tokens
+# --------------------------------------------------------------------------
+
+def test_as_many_tokens_as_a_call_takes():
+    """2^31 - 4096 tokens of one head, whose last segment ends within a segment of 2^31.  With nothing kept from token to
+    token the output is v, and so is v's gradient where it is the output's."""
+    R = (1 << 31) - 4096
+    torch.cuda.empty_cache()
+    need = R * 2 * 6 + (4 << 30)
+    if torch.cuda.mem_get_info()[0] < need:
+        pytest.skip(f"needs {need >> 30} GiB of GPU memory")
+    v = torch.empty(1, R, 1, 1, device=DEV, dtype=torch.bfloat16).random_(1, 128, generator=torch.Generator(DEV).manual_seed(1))
+    one = torch.ones((), device=DEV, dtype=v.dtype).expand(1, R, 1, 1)
+    v.requires_grad_()
+    o, state = branch.decay_attention(one, one, v, torch.tensor([-float("inf")], device=DEV), scale=1.0, return_state=True)
+    assert torch.equal(o, v) and float(state) == float(v[0, -1])
+    del state
+    g, = torch.autograd.grad(o, v, v.detach())
+    assert torch.equal(g, v)
+    del o, g, v
+    torch.cuda.empty_cache()
