@@ -49,7 +49,7 @@ static Plan plan_scan(int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv, b
   p.seg = segment_tokens(R, N, H, Dv, packed);
   p.tiles = count_tiles(R, N, p.seg, packed);
   const int64_t longest = packed || N == 0 ? R : R / N;
-  p.bytes = longest > p.seg ? p.tiles * H * Dk * Dv * 4 : 0;
+  p.bytes = longest > p.seg ? (R - 1) / p.seg * H * Dk * Dv * 4 : 0;  // places of part_place
   // packed sequences' lengths are not known here: those up to twice the mean
   p.joined = (packed && N > 1 ? 2 * (R / N) : longest) > kSummed * p.seg;
   return p;

@@ -50,7 +50,7 @@ struct DecayArgs {
   const int32_t* offsets;    // ends of the packed sequences; null: N sequences of T rows each, or with N = 0 none
   const float* first;        // X_0 of each sequence, or null
   float* last;               // where X goes, or null
-  float* parts;              // [tile][H][Dk][Dv]: states that segments leave by themselves; joined: that the next start from
+  float* parts;              // [place][H][Dk][Dv]: states that segments leave by themselves; joined: that the next start from
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;  // strides in elements; o is contiguous
   int state_row, state_col;                             // of first and last: X's rows and columns
   int part_row, part_col;                               // of parts
@@ -69,6 +69,10 @@ struct DecayJobs {
   DecayArgs job[kMaxJobs];
   int n;
 };
+
+// Place among the parts of segment s of a sequence from row lo on.  Only segments with a successor have one; each is `seg` rows,
+// so that places differ and stay below (R - 1) / seg, however the rows are split into sequences.
+__device__ __forceinline__ int64_t part_place(const DecayArgs& a, int64_t lo, int s) { return (int)lo / a.seg + s; }
 
 // Segment `s` of sequence e, whose rows are lo to hi; e = N: rows past the last sequence; -1: none.
 struct Segment {
@@ -366,7 +370,7 @@ __global__ __launch_bounds__(64 * WAVES, (kDecayWaves<T, DK, WAVES, STATE_ONLY>)
     const bool joined = a.joined && seg;
     if (a.first && !joined) add(a.first + ((int64_t)e * a.H + h) * size, a.state_row, a.state_col, power(ld, begin).hi);
     for (int s = joined ? seg - 1 : 0; s < seg; ++s)
-      add(a.parts + ((int64_t)(tile - seg + s) * a.H + h) * size, a.part_row, a.part_col, power(ld, (int64_t)(seg - 1 - s) * a.seg).hi);
+      add(a.parts + (part_place(a, lo, s) * a.H + h) * size, a.part_row, a.part_col, power(ld, (int64_t)(seg - 1 - s) * a.seg).hi);
     // P above the diagonal, where a row's 32 tokens reach past it
     for (int i = threadIdx.x; i < MADE * kPlane<kChunk> && !IN_PLACE; i += NTH) lp[i] = u32x4{0, 0, 0, 0};
   }
@@ -641,7 +645,7 @@ __global__ __launch_bounds__(64 * WAVES, (kDecayWaves<T, DK, WAVES, STATE_ONLY>)
   float* to = nullptr;
   int row = a.Dv, column = 1;
   if constexpr (STATE_ONLY) {
-    to = a.parts + ((int64_t)tile * a.H + h) * size;
+    to = a.parts + (part_place(a, lo, seg) * a.H + h) * size;
   } else if (a.last && stop == len) {
     to = a.last + ((int64_t)e * a.H + h) * size;
     row = a.state_row;
@@ -671,7 +675,7 @@ __global__ __launch_bounds__(kThreads) void decay_join_kernel(DecayArgs a, int b
   const float given = a.log_decay[h];
   const Power l = power(given > 0.f ? 0.f : given, a.seg);
   const int64_t step = (int64_t)a.H * size;  // from a segment's state to the next one's
-  float* part = a.parts + ((int64_t)tile * a.H + h) * size;
+  float* part = a.parts + (part_place(a, sg.lo, 0) * a.H + h) * size;
   const float* first = a.first ? a.first + ((int64_t)sg.e * a.H + h) * size : nullptr;
   constexpr int V = kJoin / kThreads, AHEAD = 4;
   for (int block = blockIdx.x % blocks; block * kJoin < size; block += blocks) {

@@ -41,6 +41,27 @@ def test_tokens_that_are_windows_of_one_row(dtype):
 
 
 # --------------------------------------------------------------------------
+# Segments of many sequences
+# --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("Dk,Dv", [(64, 64), (40, 100)])
+@pytest.mark.parametrize("lens", [None, [257, 256, 512, 513, 1, 0, 769, 255, 300, 300], [2500, 1, 1, 2500]])
+def test_segments_of_many_sequences(lens, Dk, Dv, dtype):
+    """Sequences a token shorter and longer than segments, whose states lie close together; several that are joined."""
+    dt, H = DT[dtype], 1
+    lead = (sum(lens),) if lens else (5, 600)
+    spans = [(n * 600, (n + 1) * 600) for n in range(5)] if lens is None else [(sum(lens[:n]), sum(lens[:n + 1])) for n in range(len(lens))]
+    off = None if lens is None else torch.tensor(lens, device=DEV).cumsum(0)
+    q, k = (rand(*lead, H, Dk, seed=i, dtype=dt).requires_grad_() for i in (1, 2))
+    v, do = rand(*lead, H, Dv, seed=3, dtype=dt).requires_grad_(), rand(*lead, H, Dv, seed=4, dtype=dt)
+    first, d_last = rand(len(spans), H, Dk, Dv, seed=5).requires_grad_(), rand(len(spans), H, Dk, Dv, seed=6)
+    ld = torch.tensor([-0.002], device=DEV)
+    check_decay(q, k, v, ld, off, first, do, d_last, Dk ** -0.5, spans)
+    check_decay(q, k, v, ld, off, None, do, None, Dk ** -0.5, spans)
+
+
+# --------------------------------------------------------------------------
 # The most tokens
 # --------------------------------------------------------------------------
 
