@@ -19,14 +19,10 @@ constexpr int64_t kLeast = 256;
 // 192 / 139; forward of 32 heads of 2048 as 8 47 / 51.
 constexpr int64_t kSummed = 8;
 
-// Columns of the state that a workgroup holds.
-static int64_t group_cols(int64_t Dv) { return Dv <= 64 ? 64 : 128; }
-
-static int64_t segment_tokens(int64_t R, int64_t N, int64_t H, int64_t Dv, bool packed) {
+static int64_t segment_tokens(int64_t R, int64_t N, int64_t H, bool packed) {
   const int64_t longest = packed || N == 0 ? R : R / N;
-  const int64_t heads = H * ((Dv + group_cols(Dv) - 1) / group_cols(Dv));
   const int64_t sequences = packed ? 1 : N;
-  int64_t want = num_cus() / (heads * sequences > 0 ? heads * sequences : 1);
+  int64_t want = num_cus() / (H * sequences > 0 ? H * sequences : 1);
   if (want < 1) want = 1;
   int64_t seg = (longest + want - 1) / want;
   if (seg < kLeast) seg = kLeast;
@@ -46,7 +42,7 @@ struct Plan {
 };
 static Plan plan_scan(int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv, bool packed) {
   Plan p;
-  p.seg = segment_tokens(R, N, H, Dv, packed);
+  p.seg = segment_tokens(R, N, H, packed);
   p.tiles = count_tiles(R, N, p.seg, packed);
   const int64_t longest = packed || N == 0 ? R : R / N;
   p.bytes = longest > p.seg ? (R - 1) / p.seg * H * Dk * Dv * 4 : 0;  // places of part_place
@@ -59,9 +55,7 @@ template <typename T, int DK, int WAVES, int WEIGHTED, bool CHUNKS>
 static int launch_scan(DecayJobs& jobs, bool states, bool outputs, const char* who, hipStream_t st) {
   constexpr int NTH = 64 * WAVES;
   const DecayArgs& a = jobs.job[0];
-  const int col_tiles = (a.Dv + 16 * WAVES - 1) / (16 * WAVES);
-  for (int j = 0; j < jobs.n; ++j) jobs.job[j].col_tiles = col_tiles;
-  const int64_t groups = ((int64_t)a.tiles * a.H + 7) / 8 * 8 * col_tiles * jobs.n;
+  const int64_t groups = ((int64_t)a.tiles * a.H + 7) / 8 * 8 * jobs.n;
   if (groups * NTH >= ((int64_t)1 << 32)) {
     set_error("%s: %lld workgroups are too many for a call", who, (long long)groups);
     return MHC_ERR_ARG;

@@ -10,7 +10,7 @@
 // a state that the last token has already entered, and the scale is b, because that gradient has none.  A chunk of 64
 // tokens is matrix products: P = (Q K^T) o (weights, lower triangle), O = P V + weights Q X, X' = l^n X + (K^T) (weighted V).
 //
-// A workgroup of WAVES waves takes a segment of a sequence, a head and 16 WAVES of the state's columns; each wave holds
+// A workgroup of WAVES waves takes a segment of a sequence and a head, whose state has at most 16 WAVES columns; each wave holds
 // 16 columns of the state, all rows, in registers from the first chunk to the last, and never passes it on.  Q, K
 // and V of a chunk go through LDS; P is made once for all waves and passes through LDS.  Registers are held below 128
 // for bf16, for four waves a SIMD: phases that wait for LDS, for the matrix cores and for the VALU then overlap (four
@@ -56,7 +56,7 @@ struct DecayArgs {
   int part_row, part_col;                               // of parts
   bool joined;
   int64_t R, T;
-  int H, N, Dk, Dv, seg, tiles, col_tiles;
+  int H, N, Dk, Dv, seg, tiles;
   float out_scale, in_scale;  // a, b
   int lag;                    // L
   bool reverse;
@@ -311,10 +311,9 @@ __global__ __launch_bounds__(64 * WAVES, (kDecayWaves<T, DK, WAVES, STATE_ONLY>)
   constexpr bool IN_PLACE = !STATE_ONLY && kInPlace<T, DK, WAVES>;
   u32x4 *lk = lds, *lv = lk + RAW * QK, *lq = lv + RAW * VP, *lp = IN_PLACE ? lv : lq + RAW * QK;
 
-  // scans and column tiles of one (segment, head) side by side on one XCD
-  const int run = blockIdx.x / 8, part = run / jobs.n;
+  // scans of one (segment, head) side by side on one XCD
+  const int run = blockIdx.x / 8, unit = run / jobs.n * 8 + blockIdx.x % 8;
   const DecayArgs a = jobs.job[run % jobs.n];
-  const int unit = part / a.col_tiles * 8 + blockIdx.x % 8, col_tile = part % a.col_tiles;
   if (unit >= a.tiles * a.H) return;
   const int tile = unit / a.H, h = unit - tile * a.H;
   const Segment sg = find_segment(a, tile);
@@ -325,14 +324,13 @@ __global__ __launch_bounds__(64 * WAVES, (kDecayWaves<T, DK, WAVES, STATE_ONLY>)
   const int stop = begin + min(a.seg, len - begin);  // tokens; begin + a.seg may lie past 2^31
   const int lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = col_tile * COLS + 16 * wave + li;  // of X and V
+  const int col = 16 * wave + li;  // of X and V
   if constexpr (STATE_ONLY) {
     if (e == a.N || stop == len) return;
   } else if (e == a.N) {  // rows of no sequence: zeros
-    const int cols = min(a.Dv - col_tile * COLS, COLS);
     if (!a.o) return;
-    T* o = (T*)a.o + ((lo + begin) * a.H + h) * a.Dv + col_tile * COLS;
-    for (int i = threadIdx.x; i < (stop - begin) * cols; i += NTH) o[(int64_t)(i / cols) * a.H * a.Dv + i % cols] = from_f32<T>(0.f);
+    T* o = (T*)a.o + ((lo + begin) * a.H + h) * a.Dv;
+    for (int i = threadIdx.x; i < (stop - begin) * a.Dv; i += NTH) o[(int64_t)(i / a.Dv) * a.H * a.Dv + i % a.Dv] = from_f32<T>(0.f);
     return;
   }
   const float given = a.log_decay[h], ld = given > 0.f ? 0.f : given;
@@ -408,11 +406,11 @@ __global__ __launch_bounds__(64 * WAVES, (kDecayWaves<T, DK, WAVES, STATE_ONLY>)
 
   const T* q = (const T*)a.q + h * a.q_head;
   const T* k = (const T*)a.k + h * a.k_head;
-  const T* v = (const T*)a.v + h * a.v_head + col_tile * COLS;
+  const T* v = (const T*)a.v + h * a.v_head;
   Feed<T, DK, NTH, CHUNKS> fq(a.q_row, a.Dk, a.reverse), fk(a.k_row, a.Dk, a.reverse);
-  Feed<T, COLS, NTH, CHUNKS> fv(a.v_row, a.Dv - col_tile * COLS, a.reverse);
+  Feed<T, COLS, NTH, CHUNKS> fv(a.v_row, a.Dv, a.reverse);
   // where the lane's results go: row li of a tile of 16 in a whole chunk, four columns
-  const int o_col = col_tile * COLS + 16 * wave + 4 * g, o_row = a.H * a.Dv * (int)sizeof(T);
+  const int o_col = 16 * wave + 4 * g, o_row = a.H * a.Dv * (int)sizeof(T);
   const int o_first = o_col < a.Dv ? (a.reverse ? kChunk - 1 - li : li) * o_row + o_col * (int)sizeof(T) : kNowhere;
   const int o_step = a.reverse ? -16 * o_row : 16 * o_row;
   auto first_row = [&](int t, int n) { return a.reverse ? hi - t - n : lo + t; };
@@ -420,7 +418,7 @@ __global__ __launch_bounds__(64 * WAVES, (kDecayWaves<T, DK, WAVES, STATE_ONLY>)
     const int n = max(min(kChunk, stop - t), 0);
     const int64_t row = n ? first_row(t, n) : lo;
     fk.load(k + row * a.k_row, a.k_row, a.Dk, n, a.reverse);
-    fv.load(v + row * a.v_row, a.v_row, a.Dv - col_tile * COLS, n, a.reverse);
+    fv.load(v + row * a.v_row, a.v_row, a.Dv, n, a.reverse);
     if constexpr (!STATE_ONLY) fq.load(q + row * a.q_row, a.q_row, a.Dk, n, a.reverse);
   };
   load(begin);
