@@ -198,15 +198,14 @@ extern "C" int mhc_decay_attention_forward(const void* q, int64_t q_row, int64_t
   });
 }
 
-// Whether scans over states of Dk x Dv and of Dv x Dk run side by side: the same kernel, segments and column tiles.
+// Whether scans over states of Dk x Dv and of Dv x Dk run side by side: the same kernel.
 static bool alike(int64_t Dk, int64_t Dv) { return (Dk <= 64) == (Dv <= 64); }
 
 // The states that the segments of the backward scans (dv's and dk's) leave, and those of the forward where the caller
-// did not keep them; scans that are not alike have a plan and states each.
+// did not keep them.
 extern "C" size_t mhc_decay_attention_backward_workspace_bytes(int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv,
                                                                int packed, int dtype) {
-  return mhc_decay_attention_workspace_bytes(R, N, H, Dk, Dv, packed, dtype) +
-         mhc_decay_attention_workspace_bytes(R, N, H, Dv, Dk, packed, dtype);
+  return 2 * mhc_decay_attention_workspace_bytes(R, N, H, Dk, Dv, packed, dtype);
 }
 
 extern "C" int mhc_decay_attention_backward(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
@@ -224,8 +223,7 @@ extern "C" int mhc_decay_attention_backward(const void* q, int64_t q_row, int64_
   const bool same = alike(Dk, Dv);
   const size_t need = mhc_decay_attention_backward_workspace_bytes(R, N, H, Dk, Dv, packed, dtype);
   if (int rc = check_workspace(who, workspace, workspace_bytes, need)) return rc;
-  // of states with Dv columns, and of the transposed ones
-  const Plan plan = plan_scan(R, N, H, Dk, Dv, packed), across = plan_scan(R, N, H, Dv, Dk, packed);
+  const Plan plan = plan_scan(R, N, H, Dk, Dv, packed);
   DecayArgs base{};
   base.log_decay = log_decay; base.offsets = offsets;
   base.R = R; base.N = (int)N; base.H = (int)H;
@@ -239,13 +237,12 @@ extern "C" int mhc_decay_attention_backward(const void* q, int64_t q_row, int64_
   of_q.o = dq; of_q.first = first; of_q.state_row = 1; of_q.state_col = dims[1];
   of_q.Dk = dims[1]; of_q.Dv = dims[0];
   of_q.out_scale = scale; of_q.in_scale = 1.f; of_q.lag = 1;
-  const bool have = same && kept;
-  of_q.parts = have ? const_cast<float*>(kept) : (float*)workspace;
-  of_q.part_row = have ? 1 : dims[0]; of_q.part_col = have ? dims[1] : 1;
+  of_q.parts = kept ? const_cast<float*>(kept) : (float*)workspace;
+  of_q.part_row = kept ? 1 : dims[0]; of_q.part_col = kept ? dims[1] : 1;
   // dv and dk: from the last token back, with the same states, dk's transposed
   base.first = d_last;
   base.out_scale = 1.f; base.in_scale = scale; base.lag = 0; base.reverse = true;
-  base.parts = (float*)((char*)workspace + across.bytes);
+  base.parts = (float*)((char*)workspace + plan.bytes);
   DecayArgs of_v = base;
   of_v.q = k; of_v.q_row = k_row; of_v.q_head = k_head;
   of_v.k = q; of_v.k_row = q_row; of_v.k_head = q_head;
@@ -264,27 +261,27 @@ extern "C" int mhc_decay_attention_backward(const void* q, int64_t q_row, int64_
   if (want_k && !want_v) of_k.last = d_first;
   return MHC_DISPATCH_DTYPE(dtype, [&]() -> int {
     const hipStream_t st = (hipStream_t)stream;
-    auto one = [&](const DecayArgs& a, const Plan& p, int what, bool fine) {
+    auto one = [&](const DecayArgs& a, int what, bool fine) {
       DecayJobs jobs{};
       jobs.n = 1;
       jobs.job[0] = a;
-      return scan<T>(jobs, p, what, fine, who, st);
+      return scan<T>(jobs, plan, what, fine, who, st);
     };
     if (!same) {  // each by itself; dk's states take dq's place in the workspace
       of_k.parts = (float*)workspace; of_k.part_row = dims[0]; of_k.part_col = 1;
       if (want_q)
-        if (int rc = one(of_q, across, kStates | kOutputs, false)) return rc;
+        if (int rc = one(of_q, kept ? kOutputs : kStates | kOutputs, false)) return rc;
       if (want_v)
-        if (int rc = one(of_v, plan, kStates | kOutputs, exact)) return rc;
-      if (want_k) return one(of_k, across, kStates | kOutputs, of_k.last != nullptr);
+        if (int rc = one(of_v, kStates | kOutputs, exact)) return rc;
+      if (want_k) return one(of_k, kStates | kOutputs, of_k.last != nullptr);
       return MHC_OK;
     }
     // dv's states serve dk, transposed
     of_k.part_row = want_v ? 1 : dims[0]; of_k.part_col = want_v ? dims[1] : 1;
-    if (want_q && !have)
-      if (int rc = one(of_q, across, kStates, false)) return rc;
+    if (want_q && !kept)
+      if (int rc = one(of_q, kStates, false)) return rc;
     if (want_v || want_k)
-      if (int rc = one(want_v ? of_v : of_k, want_v ? plan : across, kStates, exact)) return rc;
+      if (int rc = one(want_v ? of_v : of_k, kStates, exact)) return rc;
     DecayJobs jobs{};
     if (want_q) jobs.job[jobs.n++] = of_q;
     if (want_v) jobs.job[jobs.n++] = of_v;

@@ -6,7 +6,7 @@ import torch
 
 from test_gpu_branch import DT, rand
 from test_gpu_mixer import check_decay, decays
-from mhc import branch
+from mhc import _mixer, branch
 
 pytestmark = pytest.mark.gpu
 
@@ -59,6 +59,20 @@ def test_segments_of_many_sequences(lens, Dk, Dv, dtype):
     ld = torch.tensor([-0.002], device=DEV)
     check_decay(q, k, v, ld, off, first, do, d_last, Dk ** -0.5, spans)
     check_decay(q, k, v, ld, off, None, do, None, Dk ** -0.5, spans)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("Dk,Dv", [(64, 64), (100, 30), (30, 100)])
+def test_the_forwards_states_serve_the_backward(Dk, Dv, dtype):
+    """What the forward keeps is what q's gradient starts from in every segment but the first, and nothing else."""
+    dt, H, T = DT[dtype], 1, 700  # segments of 256
+    q, k, v, do = (rand(1, T, H, d, seed=i, dtype=dt) for i, d in enumerate((Dk, Dk, Dv, Dv)))
+    ld = torch.tensor([-0.002], device=DEV)
+    kept = _mixer.decay_attention_forward(q, k, v, ld, None, None, 0.1, False)[2]
+    want = _mixer.decay_attention_backward(q, k, v, do, ld, None, None, kept, None, 0.1, (True,) * 4)
+    got = _mixer.decay_attention_backward(q, k, v, do, ld, None, None, torch.full_like(kept, 255), None, 0.1, (True,) * 4)
+    assert torch.equal(got[0][:, :256], want[0][:, :256]) and torch.isnan(got[0][:, 256:]).all()
+    assert torch.isfinite(want[0]).all() and all(torch.equal(a, b) for a, b in zip(got[1:], want[1:]))
 
 
 # --------------------------------------------------------------------------
