@@ -464,7 +464,8 @@ size_t mhc_decay_attention_backward_workspace_bytes(int64_t R, int64_t N, int64_
 /* dq, dk, dv (as q, k, v, contiguous) and d_first from dout and d_last; any of them,
  * first and d_last may be NULL.  Rows of no sequence get zeros.  kept: the forward's
  * workspace as that call (same sizes, operands and first) left it, or NULL: its
- * segments' states are then computed again. */
+ * segments' states are then computed again.  With kept the workspace need only be as
+ * large as the forward's. */
 int mhc_decay_attention_backward(const void* q, int64_t q_row, int64_t q_head,
                                  const void* k, int64_t k_row, int64_t k_head,
                                  const void* v, int64_t v_row, int64_t v_head,

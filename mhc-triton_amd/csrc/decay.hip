@@ -221,9 +221,8 @@ extern "C" int mhc_decay_attention_backward(const void* q, int64_t q_row, int64_
   if (H == 0 || (R == 0 && (N == 0 || !d_first))) return MHC_OK;
   if (!log_decay || (R && (!q || !k || !v || !dout))) return null_in(who);
   const bool same = alike(Dk, Dv);
-  const size_t need = mhc_decay_attention_backward_workspace_bytes(R, N, H, Dk, Dv, packed, dtype);
-  if (int rc = check_workspace(who, workspace, workspace_bytes, need)) return rc;
   const Plan plan = plan_scan(R, N, H, Dk, Dv, packed);
+  if (int rc = check_workspace(who, workspace, workspace_bytes, (size_t)plan.bytes * (kept ? 1 : 2))) return rc;
   DecayArgs base{};
   base.log_decay = log_decay; base.offsets = offsets;
   base.R = R; base.N = (int)N; base.H = (int)H;
@@ -242,7 +241,7 @@ extern "C" int mhc_decay_attention_backward(const void* q, int64_t q_row, int64_
   // dv and dk: from the last token back, with the same states, dk's transposed
   base.first = d_last;
   base.out_scale = 1.f; base.in_scale = scale; base.lag = 0; base.reverse = true;
-  base.parts = (float*)((char*)workspace + plan.bytes);
+  base.parts = (float*)((char*)workspace + (kept ? 0 : plan.bytes));
   DecayArgs of_v = base;
   of_v.q = k; of_v.q_row = k_row; of_v.q_head = k_head;
   of_v.k = q; of_v.k_row = q_row; of_v.k_head = q_head;
@@ -267,8 +266,8 @@ extern "C" int mhc_decay_attention_backward(const void* q, int64_t q_row, int64_
       jobs.job[0] = a;
       return scan<T>(jobs, plan, what, fine, who, st);
     };
-    if (!same) {  // each by itself; dk's states take dq's place in the workspace
-      of_k.parts = (float*)workspace; of_k.part_row = dims[0]; of_k.part_col = 1;
+    if (!same) {  // each by itself; dk's states take dv's place in the workspace
+      of_k.part_row = dims[0]; of_k.part_col = 1;
       if (want_q)
         if (int rc = one(of_q, kept ? kOutputs : kStates | kOutputs, false)) return rc;
       if (want_v)

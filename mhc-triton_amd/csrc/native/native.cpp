@@ -1172,16 +1172,16 @@ struct DecayAttention : Function<DecayAttention> {
     const Heads a(q), b(k), c(v), d(dout);
     const int64_t N = off.defined() ? off.size(0) : q.size(0);
     Tensor kept = whole(s[6]);
-    if (kept.defined() &&
-        (kept.scalar_type() != at::kByte ||
-         kept.numel() != (int64_t)mhc_decay_attention_workspace_bytes(a.R, N, a.H, a.D, c.D, off.defined(), code(q))))
+    const size_t states = mhc_decay_attention_workspace_bytes(a.R, N, a.H, a.D, c.D, off.defined(), code(q));
+    if (kept.defined() && (kept.scalar_type() != at::kByte || kept.numel() != (int64_t)states))
       kept = Tensor();  // a saved-tensor hook has changed it: computed again
     Tensor dq, dk, dv, ds;
     if (need[0]) dq = plain_empty(q.sizes(), q);
     if (need[1]) dk = plain_empty(k.sizes(), k);
     if (need[2]) dv = plain_empty(v.sizes(), v);
     if (need[3]) ds = empty_f32({N, a.H, a.D, c.D}, q);
-    const Workspace ws(mhc_decay_attention_backward_workspace_bytes(a.R, N, a.H, a.D, c.D, off.defined(), code(q)), q);
+    const Workspace ws(kept.defined() ? states
+                                      : mhc_decay_attention_backward_workspace_bytes(a.R, N, a.H, a.D, c.D, off.defined(), code(q)), q);
     check(mhc_decay_attention_backward(a.p(), a.row, a.head, b.p(), b.row, b.head, c.p(), c.row, c.head, d.p(), d.row, d.head,
                                        code(q), fptr(ld), static_cast<const int32_t*>(ptr(off)), fptr(first), fptr(kept),
                                        fptr(last), ptr(dq), ptr(dk), ptr(dv), wptr(ds), a.R, N, a.H, a.D, c.D,

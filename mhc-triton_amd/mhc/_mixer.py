@@ -186,11 +186,13 @@ def decay_attention_backward(q, k, v, do, log_decay, offsets, initial_state, kep
     d_first = torch.empty((N, H, Dk, Dv), device=dev, dtype=torch.float32) if need[3] else None
     lib = _lib.load()
     packed = int(offsets is not None)
+    states = lib.mhc_decay_attention_workspace_bytes(a.R, N, H, Dk, Dv, packed, code)
     if kept is not None:  # a saved-tensor hook may have changed it
-        if kept.dtype != torch.uint8 or kept.numel() != lib.mhc_decay_attention_workspace_bytes(a.R, N, H, Dk, Dv, packed, code):
+        if kept.dtype != torch.uint8 or kept.numel() != states:
             raise ShapeError(f"kept must be the forward's, got {tuple(kept.shape)} {kept.dtype}")
         kept = kept.contiguous()
-    ws = _lib.workspace(lib.mhc_decay_attention_backward_workspace_bytes(a.R, N, H, Dk, Dv, packed, code), dev)
+    ws = _lib.workspace(states if kept is not None else
+                        lib.mhc_decay_attention_backward_workspace_bytes(a.R, N, H, Dk, Dv, packed, code), dev)
     with _lib.on_device(dev):
         _lib.check(lib.mhc_decay_attention_backward(*a.args(), *b.args(), *c.args(), *d.args(), code, log_decay.data_ptr(),
                                                     _lib.ptr(offsets), _lib.ptr(first), _lib.ptr(kept), _lib.ptr(d_last),

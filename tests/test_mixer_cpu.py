@@ -290,3 +290,20 @@ def test_decay_workspace_holds_the_states_of_segments_alone():
         for of, times in ((lib.mhc_decay_attention_workspace_bytes, 1), (lib.mhc_decay_attention_backward_workspace_bytes, 2)):
             sizes = {of(R, N, H, Dk, Dv, 1, 1) for N in (1, 64, 512, 2048)}
             assert len(sizes) == 1 and 0 < sizes.pop() <= times * (R - 1) // 256 * H * Dk * Dv * 4
+
+
+def test_decay_backward_workspace_with_the_forwards_states_kept():
+    """Half the workspace of a backward that makes them again; it is checked before the dtype, and both before the device."""
+    from mhc import _lib
+
+    lib = _lib.load()
+
+    def bwd(kept, ws, nb, Dk=64, Dv=64):
+        return lib.mhc_decay_attention_backward(16, 128, 64, 16, 128, 64, 16, 128, 64, 16, 128, 64, 9, 16, None, None, kept, None, 16,
+                                                16, 16, None, 8192, 1, 2, Dk, Dv, 1.0, ws, nb, None)
+
+    for Dk, Dv in ((64, 64), (40, 100)):
+        states = lib.mhc_decay_attention_workspace_bytes(8192, 1, 2, Dk, Dv, 0, 1)
+        assert lib.mhc_decay_attention_backward_workspace_bytes(8192, 1, 2, Dk, Dv, 0, 1) == 2 * states > 0
+        assert bwd(None, 16, 2 * states, Dk, Dv) == 2 and bwd(None, 16, 2 * states - 1, Dk, Dv) == 3
+        assert bwd(16, 16, states, Dk, Dv) == 2 and bwd(16, 16, states - 1, Dk, Dv) == bwd(16, None, 0, Dk, Dv) == 3
