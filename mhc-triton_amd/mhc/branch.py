@@ -292,7 +292,8 @@ def rotary_frequencies(dim: int, base: float = 10000.0, factor: float = 1.0, ori
 
     For contexts ``factor`` times as long as the trained ones every frequency is divided by factor; with
     ``original_length``, the trained length, only those that turn fewer than ``slow`` times over it are, those that
-    turn more than ``fast`` times stay, and between them the share falls off linearly in the pair's index.  (Such a
+    turn more than ``fast`` times stay, and between them the share that stays falls off linearly in the pair's index (between
+    the whole numbers around the two ends, which may lie before the first pair and behind the last).  (Such a
     context usually takes ``magnitude = 0.1 * log(factor) + 1`` in ``rotary``, too.)"""
     if dim < 0 or dim % 2:
         raise ValueError(f"dim must be even, got {dim}")
@@ -310,7 +311,7 @@ def rotary_frequencies(dim: int, base: float = 10000.0, factor: float = 1.0, ori
         def pair_of(turns):  # the index, not whole, of the pair that turns so often over the trained length
             return dim * math.log(original_length / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
 
-        lo, hi = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), max(dim // 2 - 1, 0))
+        lo, hi = math.floor(pair_of(fast)), math.ceil(pair_of(slow))  # the ramp's ends, whether or not there are such pairs
         stretched = ((i - lo) / max(hi - lo, 1e-3)).clamp(0.0, 1.0)
         f = f * (1.0 - stretched) + f / factor * stretched
     return f.to(device) if device is not None else f

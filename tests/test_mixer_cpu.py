@@ -307,3 +307,19 @@ def test_decay_backward_workspace_with_the_forwards_states_kept():
         assert lib.mhc_decay_attention_backward_workspace_bytes(8192, 1, 2, Dk, Dv, 0, 1) == 2 * states > 0
         assert bwd(None, 16, 2 * states, Dk, Dv) == 2 and bwd(None, 16, 2 * states - 1, Dk, Dv) == 3
         assert bwd(16, 16, states, Dk, Dv) == 2 and bwd(16, 16, states - 1, Dk, Dv) == bwd(16, None, 0, Dk, Dv) == 3
+
+
+@pytest.mark.parametrize("dim,length", [(64, 4096), (64, 65536), (128, 131072), (32, 131072), (16, 10 ** 6), (8, 10 ** 9),
+                                        (64, 128), (64, 20), (64, 4), (2, 30)])
+@pytest.mark.parametrize("fast,slow", [(32.0, 1.0), (9.0, 2.5)])
+def test_rotary_frequencies_between_fast_and_slow(dim, length, fast, slow):
+    """The share of a pair that turns between slow and fast times over the trained length is between none and all and linear in
+    its index, whether or not there are pairs at the ramp's ends; beyond them frequencies are divided, or stay."""
+    f = branch.rotary_frequencies(dim)
+    share = (1 - branch.rotary_frequencies(dim, factor=8.0, original_length=length, fast=fast, slow=slow) / f) / (1 - 1 / 8)
+    turns = length * f / (2 * math.pi)
+    # a share is a quotient of fp64 roundings: 1 - 1/8 .. 1 of 2^-53 each
+    assert bool((share[turns >= fast].abs() < 1e-14).all()) and bool(((share[turns <= slow] - 1).abs() < 1e-14).all())
+    ramp = share[(turns > slow) & (turns < fast)]
+    assert bool((ramp > 1e-6).all()) and bool((ramp < 1 - 1e-6).all())
+    assert ramp.numel() < 3 or bool(((ramp.diff().diff()).abs() < 1e-14).all())
