@@ -488,8 +488,8 @@ int mhc_decay_attention_step(const void* q, int64_t q_row, int64_t q_head,
                              int64_t Dk, int64_t Dv, float scale, mhc_stream_t stream);
 
 /* Gated product of rows grouped by expert as in mhc_grouped_matmul_forward, or with
- * offsets NULL (E = 1) all of one weight.  weight [E,2N,K]: N rows that make the gates,
- * then N that make the values:
+ * offsets NULL (E = 1) all of one weight; without experts (E = 0) there are no offsets
+ * to read.  weight [E,2N,K]: N rows that make the gates, then N that make the values:
  *   g = x Wg^T,  u = x Wu^T,  y = act(g) * u [R,N]
  * saved [R,2N] f32 gets g and u for the backward (NULL: none follows). */
 enum { MHC_ACT_SILU = 0, MHC_ACT_GELU = 1, MHC_ACT_GELU_TANH = 2 };

@@ -6,6 +6,7 @@ import torch
 
 from test_gpu_branch import DT, rand
 from test_gpu_mixer import check_decay, decays
+from test_gpu_native_nodes import both
 from mhc import _mixer, branch
 
 pytestmark = pytest.mark.gpu
@@ -97,3 +98,23 @@ def test_as_many_tokens_as_a_call_takes():
     assert torch.equal(g, v)
     del o, g, v
     torch.cuda.empty_cache()
+
+
+# --------------------------------------------------------------------------
+# No experts
+# --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("K", [64, 65])
+def test_gated_matmul_of_no_experts(monkeypatch, K, dtype):
+    """As grouped_matmul: all rows are of no expert."""
+    x, w = rand(70, K, seed=1, dtype=DT[dtype]).requires_grad_(), torch.empty(0, 24, K, dtype=DT[dtype], device=DEV).requires_grad_()
+    off = torch.empty(0, dtype=torch.int32, device=DEV)
+
+    def step():
+        y = branch.gated_matmul(x, w, off)
+        dx, dw = torch.autograd.grad(y, (x, w), rand(70, 12, seed=2, dtype=x.dtype))
+        assert y.shape == (70, 12) and not y.any() and dx.shape == x.shape and not dx.any() and dw.shape == w.shape
+        return [y.detach(), dx, dw]
+
+    both(monkeypatch, step)
