@@ -14,11 +14,6 @@ namespace mhc {
 // 250; 8 heads of 2048 43 / 50 us, with kLeast = 512 53 / 59; the other way round from 256 segments of one head on (65536
 // tokens 109 / 140, with 512 91 / 116).
 constexpr int64_t kLeast = 256;
-// A segment adds up the states before it, up to this many segments; beyond, decay_join_kernel does it once for all of them.
-// Summed / joined, us: backward of 32 heads of 8192 tokens as 16 segments 301 / 246, forward of 8 heads of 32768 as 64
-// 192 / 139; forward of 32 heads of 2048 as 8 47 / 51.
-constexpr int64_t kSummed = 8;
-
 static int64_t segment_tokens(int64_t R, int64_t N, int64_t H, bool packed) {
   const int64_t longest = packed || N == 0 ? R : R / N;
   const int64_t sequences = packed ? 1 : N;
@@ -38,7 +33,7 @@ static int64_t count_tiles(int64_t R, int64_t N, int64_t seg, bool packed) {
 // A scan's segments and what the states that they leave take.
 struct Plan {
   int64_t seg, tiles, bytes;  // bytes 0: no sequence has a second segment
-  bool joined;
+  int64_t joins;              // sequences of more than kSummed segments, at most; 0: decay_join_kernel does not run
 };
 static Plan plan_scan(int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv, bool packed) {
   Plan p;
@@ -46,13 +41,15 @@ static Plan plan_scan(int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv, b
   p.tiles = count_tiles(R, N, p.seg, packed);
   const int64_t longest = packed || N == 0 ? R : R / N;
   p.bytes = longest > p.seg ? (R - 1) / p.seg * H * Dk * Dv * 4 : 0;  // places of part_place
-  // packed sequences' lengths are not known here: those up to twice the mean
-  p.joined = (packed && N > 1 ? 2 * (R / N) : longest) > kSummed * p.seg;
+  // Packed sequences' lengths are not known here, and that one is so long is not likely: from twice as many rows on.  One head of
+  // 65536 tokens in 64 sequences, forward / backward in us without and with the launch: split evenly 44 / 81 and 47 / 83, all but 63 in
+  // the first 281 / 994 and 111 / 145; 12 heads of 16384 in 256 sequences 110 / 300 and 115 / 304, 169 / 437 and 176 / 417.
+  p.joins = longest <= kSummed * p.seg * (packed && N > 1 ? 2 : 1) ? 0 : packed ? (R - 1) / (kSummed * p.seg) : N;
   return p;
 }
 
 template <typename T, int DK, int WAVES, int WEIGHTED, bool CHUNKS>
-static int launch_scan(DecayJobs& jobs, bool states, bool outputs, const char* who, hipStream_t st) {
+static int launch_scan(const DecayJobs& jobs, int64_t joins, bool states, bool outputs, const char* who, hipStream_t st) {
   constexpr int NTH = 64 * WAVES;
   const DecayArgs& a = jobs.job[0];
   const int64_t groups = ((int64_t)a.tiles * a.H + 7) / 8 * 8 * jobs.n;
@@ -62,10 +59,10 @@ static int launch_scan(DecayJobs& jobs, bool states, bool outputs, const char* w
   }
   const dim3 grid((unsigned)groups);
   if (states) decay_kernel<T, DK, WAVES, WEIGHTED, CHUNKS, true><<<grid, NTH, 0, st>>>(jobs);
-  if (states && a.joined) {
-    const int64_t most = (((int64_t)1 << 32) / kThreads - 1) / ((int64_t)a.tiles * a.H), want = (a.Dk * a.Dv + kJoin - 1) / kJoin;
+  if (states && joins) {
+    const int64_t units = joins * a.H, most = (((int64_t)1 << 32) / kThreads - 1) / units, want = (a.Dk * a.Dv + kJoin - 1) / kJoin;
     const int blocks = (int)(want < most ? want : most);
-    decay_join_kernel<<<dim3((unsigned)(a.tiles * a.H * blocks)), kThreads, 0, st>>>(a, blocks);
+    decay_join_kernel<<<dim3((unsigned)(units * blocks)), kThreads, 0, st>>>(a, blocks);
   }
   if (outputs) decay_kernel<T, DK, WAVES, WEIGHTED, CHUNKS, false><<<grid, NTH, 0, st>>>(jobs);
   return hip_status(hipGetLastError(), who);
@@ -93,7 +90,7 @@ static int scan(DecayJobs jobs, const Plan& plan, int what, bool exact, const ch
     a.T = a.N ? a.R / a.N : 0;
     a.seg = (int)plan.seg;
     a.tiles = (int)plan.tiles;
-    a.joined = plan.joined;
+    a.joined = plan.joins > 0;
     chunks = chunks && whole_chunks<T>(a.q, a.q_row, a.q_head, a.Dk) && whole_chunks<T>(a.k, a.k_row, a.k_head, a.Dk) &&
              whole_chunks<T>(a.v, a.v_row, a.v_head, a.Dv) && aligned16(a.o);
   }
@@ -102,10 +99,10 @@ static int scan(DecayJobs jobs, const Plan& plan, int what, bool exact, const ch
   auto launch = [&](auto w, auto parts) {
     constexpr int WAVES = decltype(w)::value, WEIGHTED = decltype(parts)::value;
     if (chunks)
-      return a.Dk <= 64 ? launch_scan<T, 64, WAVES, WEIGHTED, true>(jobs, states, outputs, who, st)
-                        : launch_scan<T, 128, WAVES, WEIGHTED, true>(jobs, states, outputs, who, st);
-    return a.Dk <= 64 ? launch_scan<T, 64, WAVES, WEIGHTED, false>(jobs, states, outputs, who, st)
-                      : launch_scan<T, 128, WAVES, WEIGHTED, false>(jobs, states, outputs, who, st);
+      return a.Dk <= 64 ? launch_scan<T, 64, WAVES, WEIGHTED, true>(jobs, plan.joins, states, outputs, who, st)
+                        : launch_scan<T, 128, WAVES, WEIGHTED, true>(jobs, plan.joins, states, outputs, who, st);
+    return a.Dk <= 64 ? launch_scan<T, 64, WAVES, WEIGHTED, false>(jobs, plan.joins, states, outputs, who, st)
+                      : launch_scan<T, 128, WAVES, WEIGHTED, false>(jobs, plan.joins, states, outputs, who, st);
   };
   using std::integral_constant;
   if constexpr (sizeof(T) == 4) {

@@ -16,8 +16,8 @@
 // for bf16, for four waves a SIMD: phases that wait for LDS, for the matrix cores and for the VALU then overlap (four
 // waves of 64 columns each and two a SIMD: 198 us where this takes 139; 32 columns a wave: spills, 399 where 16 take 158).
 // Segments but the last are first run for their state alone (STATE_ONLY), so that long sequences with
-// few heads fill the card; each then starts from the sum of the states before it, which decay_join_kernel has made where
-// there are many.
+// few heads fill the card; each then starts from the sum of the states before it, which decay_join_kernel has made in
+// sequences of more than kSummed.
 //
 // Bound by the phases of a chunk, which hardly overlap inside a workgroup (LDS, VALU and matrix cores 2 us each of 8), and
 // not far behind by memory.  bf16, 4 x 4096 tokens of 32 heads of 128: forward 139 us (3.9 TB/s) and 57 for the segments'
@@ -54,7 +54,7 @@ struct DecayArgs {
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;  // strides in elements; o is contiguous
   int state_row, state_col;                             // of first and last: X's rows and columns
   int part_row, part_col;                               // of parts
-  bool joined;
+  bool joined;  // decay_join_kernel runs
   int64_t R, T;
   int H, N, Dk, Dv, seg, tiles;
   float out_scale, in_scale;  // a, b
@@ -65,6 +65,11 @@ struct DecayArgs {
 // Scans that run side by side: the three gradients read the same four tensors, and their workgroups of a segment and
 // head are neighbours, so that the second and the third find them in the caches.
 constexpr int kMaxJobs = 3;
+
+// A segment adds up the states before it, in sequences of up to this many segments; in others decay_join_kernel does it once
+// for all of them.  Summed / joined, us: backward of 32 heads of 8192 tokens as 16 segments 301 / 246, forward of 8 heads of
+// 32768 as 64 192 / 139; forward of 32 heads of 2048 as 8 47 / 51.
+constexpr int kSummed = 8;
 struct DecayJobs {
   DecayArgs job[kMaxJobs];
   int n;
@@ -80,10 +85,16 @@ struct Segment {
   int64_t lo, hi;
 };
 
-// Tile t: every sequence has a segment at least, so that one without tokens hands its state on.
+__device__ __forceinline__ int segments_of(const DecayArgs& a, int64_t lo, int64_t hi) {
+  return (int)(((uint32_t)(hi - lo) + (uint32_t)a.seg - 1) / (uint32_t)a.seg);
+}
+
+// Tile t: every sequence has a segment at least, so that one without tokens hands its state on.  JOINED: the first segment
+// of the t-th sequence of more than kSummed.
+template <bool JOINED = false>
 __device__ __forceinline__ Segment find_segment(const DecayArgs& a, int t) {
   if (!a.offsets && a.N) {
-    const int per = (int)max((int64_t)1, (a.T + a.seg - 1) / a.seg);
+    const int per = JOINED ? 1 : max(1, segments_of(a, 0, a.T));
     const int e = t / per;
     return {e < a.N ? e : -1, t - e * per, e * a.T, (e + 1) * a.T};
   }
@@ -91,8 +102,9 @@ __device__ __forceinline__ Segment find_segment(const DecayArgs& a, int t) {
   int before = 0, end = 0;
   for (int base = 0; base <= a.N; base += 64) {
     const Group g = groups_of(a.offsets, base, a.N, a.R, &end);
-    int n = (int)((g.hi - g.lo + a.seg - 1) / a.seg);
-    if (base + lane < a.N) n = max(n, 1);
+    int n = segments_of(a, g.lo, g.hi);
+    if (JOINED) n = base + lane < a.N && n > kSummed;
+    else if (base + lane < a.N) n = max(n, 1);
     int upto = n;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
@@ -365,7 +377,7 @@ __global__ __launch_bounds__(64 * WAVES, (kDecayWaves<T, DK, WAVES, STATE_ONLY>)
         x[td] += w * y;
       }
     };
-    const bool joined = a.joined && seg;
+    const bool joined = a.joined && seg && segments_of(a, lo, hi) > kSummed;
     if (a.first && !joined) add(a.first + ((int64_t)e * a.H + h) * size, a.state_row, a.state_col, power(ld, begin).hi);
     for (int s = joined ? seg - 1 : 0; s < seg; ++s)
       add(a.parts + (part_place(a, lo, s) * a.H + h) * size, a.part_row, a.part_col, power(ld, (int64_t)(seg - 1 - s) * a.seg).hi);
@@ -660,16 +672,15 @@ __global__ __launch_bounds__(64 * WAVES, (kDecayWaves<T, DK, WAVES, STATE_ONLY>)
 
 // From the states that a sequence's segments leave by themselves to those that the next ones start from, in place:
 //   X_0 = first,  X_(s+1) = l^seg X_s + part_s
-// A workgroup has a sequence's first tile, a head and every `blocks`-th kJoin values of the state; the next segments' loads
-// are in flight.
+// A workgroup has a sequence of more than kSummed segments, a head and every `blocks`-th kJoin values of the state; the next
+// segments' loads are in flight.
 constexpr int kJoin = 4 * kThreads;
 
 __global__ __launch_bounds__(kThreads) void decay_join_kernel(DecayArgs a, int blocks) {
-  const int unit = blockIdx.x / blocks, tile = unit / a.H, h = unit - tile * a.H;
-  const Segment sg = find_segment(a, tile);
-  if (sg.e < 0 || sg.e == a.N || sg.s) return;
-  const int segments = (int)((sg.hi - sg.lo + a.seg - 1) / a.seg), size = a.Dk * a.Dv;
-  if (segments < 2) return;
+  const int unit = blockIdx.x / blocks, nth = unit / a.H, h = unit - nth * a.H;
+  const Segment sg = find_segment<true>(a, nth);
+  if (sg.e < 0) return;
+  const int segments = segments_of(a, sg.lo, sg.hi), size = a.Dk * a.Dv;
   const float given = a.log_decay[h];
   const Power l = power(given > 0.f ? 0.f : given, a.seg);
   const int64_t step = (int64_t)a.H * size;  // from a segment's state to the next one's

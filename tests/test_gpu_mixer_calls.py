@@ -62,6 +62,31 @@ def test_segments_of_many_sequences(lens, Dk, Dv, dtype):
     check_decay(q, k, v, ld, off, None, do, None, Dk ** -0.5, spans)
 
 
+def test_a_long_sequence_among_many_short_ones():
+    """Its many segments' states are joined whatever it is packed with: the bits are those of the sequence alone.  Packed with
+    another one, sequences of a few segments are summed beside it as among themselves."""
+    H, D, T = 1, 64, 7000  # segments of 256
+    ld = torch.tensor([-0.0005], device=DEV)
+
+    def run(ends, R):
+        q, k, v = (rand(9400, H, D, seed=i)[:R].contiguous().requires_grad_() for i in (1, 2, 3))
+        off = torch.tensor(ends, dtype=torch.int32, device=DEV)
+        o, state = branch.decay_attention(q, k, v, ld, offsets=off, return_state=True)
+        do, d_state = rand(9400, H, D, seed=4)[:R], rand(200, H, D, D, seed=5)[:len(ends)]
+        return [o, state, *torch.autograd.grad((o, state), (q, k, v), (do, d_state))]
+
+    alone = run([T], T)
+    for i, ends in enumerate(([T, T + 1500, T + 2000], [T, *range(T + 1, T + 200)])):
+        got = run(ends, 9400)
+        for a, b in zip(got, alone):
+            assert torch.equal(a[:len(b)], b)
+        if i == 0:  # two of 1500 and 500 tokens
+            rows = slice(T, T + 2000)
+            q, k, v = (rand(9400, H, D, seed=s)[rows] for s in (1, 2, 3))
+            o = branch.decay_attention(q, k, v, ld, offsets=torch.tensor([1500, 2000], device=DEV))
+            assert torch.equal(got[0][rows], o)
+
+
 @pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("Dk,Dv", [(64, 64), (100, 30), (30, 100)])
 def test_the_forwards_states_serve_the_backward(Dk, Dv, dtype):
