@@ -4,10 +4,12 @@ test_gpu_mixer_paths.py do not make."""
 import pytest
 import torch
 
-from test_gpu_branch import DT, rand
-from test_gpu_mixer import check_decay, decays
+from helpers import to_np
+from test_gpu_branch import DT, close, rand
+from test_gpu_mixer import check_decay, check_gated, decays
 from test_gpu_native_nodes import both
 from mhc import _mixer, branch
+from oracle import mixer_oracle as M
 
 pytestmark = pytest.mark.gpu
 
@@ -123,6 +125,34 @@ def test_as_many_tokens_as_a_call_takes():
     assert torch.equal(g, v)
     del o, g, v
     torch.cuda.empty_cache()
+
+
+def test_rotary_of_more_row_tiles_than_a_launch_has_workgroups():
+    """2^24 - 1 workgroups of four rows: those of the first rows take the last ones, too."""
+    R, f = 4 * ((1 << 24) - 1 + 1000) + 3, torch.tensor([0.37], dtype=torch.float64, device=DEV)
+    q = torch.empty(R, 1, 2, device=DEV, dtype=torch.bfloat16).normal_(generator=torch.Generator(DEV).manual_seed(1))
+    pos = torch.arange(R, device=DEV, dtype=torch.int32) % 100003
+    y = branch.rotary(q, None, pos, f)
+    second = 4 * ((1 << 24) - 1)
+    for lo, hi in ((0, 4096), (second - 100, second + 4003)):
+        ref, size = M.rotary(to_np(q[lo:hi]), to_np(pos[lo:hi]), to_np(f))
+        # an angle is off by its fp64 rounding, 2^-53 of up to 2^16 radians
+        close(y[lo:hi], ref, size, 2.0 ** -21, "rows")
+    # every row: turning keeps a pair's length, to the rounding of its two bf16 elements
+    a, b = (t.float().square().sum((1, 2)).sqrt() for t in (q, y))
+    assert bool(((a - b).abs() <= 2.0 ** -8 * a * 1.01 + 1e-30).all())
+
+
+# --------------------------------------------------------------------------
+# Gated products: fp32 in the largest tiles
+# --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("R,K,N,off", [(6000, 64, 2864, None), (6000, 72, 2800, [2900, 2900, 5950])])
+def test_gated_matmul_in_256_tiles_of_fp32(R, K, N, off):
+    """Two likely tiles a CU and more: the last round in quarters, experts' last rows in half tiles, rows of no expert."""
+    x = rand(R, K, seed=1).requires_grad_()
+    w = rand(*(() if off is None else (len(off),)), 2 * N, K, seed=2, scale=K ** -0.5).requires_grad_()
+    check_gated(x, w, off, "gelu", rand(R, N, seed=3))
 
 
 # --------------------------------------------------------------------------
