@@ -19,11 +19,12 @@
 // few heads fill the card; each then starts from the sum of the states before it, which decay_join_kernel has made in
 // sequences of more than kSummed.
 //
-// Bound by the phases of a chunk, which hardly overlap inside a workgroup (LDS, VALU and matrix cores 2 us each of 8), and
-// not far behind by memory.  bf16, 4 x 4096 tokens of 32 heads of 128: forward 139 us (3.9 TB/s) and 57 for the segments'
-// states, the gradients' scans together 430 us (2.2 TB/s) and 63; left out for a trial no single part gave more than 7%
-// (loads 4, P 3, Q X 7, P V 3), loads and stores together 28%.  fp32, which has six products for one, 3069 packed tokens
-// of 12 heads: forward 44 us, gradients 101, states 20 each.
+// Bound by the phases of a chunk, which follow one another, and not far behind by memory.  bf16, 4 x 4096 tokens of 32 heads
+// of 128: forward 142 us (3.8 TB/s) and 46 for the segments' states, the gradients' three scans together 375 us (2.5 TB/s) and
+// 45.  That is 4.4 us a chunk with one workgroup a CU; a second one gains 14% (the scans of k and v side by side 247 us, one
+// alone 143).  Left out for a trial (of 195 us, then): stores 18%, Q X 7, loads 4, P 3, P V 3, loads and stores together
+// 28%.  fp32, which has six products for one, 3069 packed tokens of 12 heads of 100 and 72: forward 44 us, gradients 102, states 20
+// each; waves whose columns lie past Dv, and zeros past Dk, cost as much as others.
 //
 // Precision.  The matrix instructions multiply bf16.  Every operand is a sum of bf16 parts: inputs exactly (bf16 one part,
 // fp16 two, fp32 three), what is computed (P, the state, weighted V) in as many as keep the error far below one rounding to

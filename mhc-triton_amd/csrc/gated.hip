@@ -9,7 +9,8 @@
 // At 16384 rows of 4096 to 8192 in bf16 writing them is 190 of the forward's 1950 us, and [dg du] from them 340 us of the
 // backward's 4340.
 //
-// Bound by the matrix products, for few rows by reading the weight.
+// Bound by the matrix products, for few rows by reading the weight.  fp32, 8192 rows of 2048 to 4096: forward 1950 us
+// (141 TFLOP/s, the library's plain product 148), backward 4000 (137).
 #include "grouped_launch.hpp"
 
 namespace mhc {
@@ -85,12 +86,15 @@ static int launch_gate_backward(GateArgs a, const char* who, hipStream_t st) {
 // bound by the matrix cores at any tile (times in us, cold weights where they matter):
 //   few rows an expert: 4096 to 8192, one expert, 1 / 8 / 16 / 32 / 64 rows: weights into registers 30.0 / 30.3 / 31.7 / 53.4 / 97.6,
 //   64-tiles 30.8 / 31.8 / 31.1 / 31.5 / 32.4 (4.3 TB/s: the weights alone, from memory).
-//   256 against 128 with 288, 320, 512 and 576 likely 256-tiles: bf16 53 / 58, 101 / 112, 229 / 269 and 158 / 181; with 144,
-//   80 and 48 39 / 37, 30 / 21 and 16.5 / 18.5.  fp32, 256 against 64, with 288, 320, 512 and 576: 322 / 324, 626 / 608, 1916 / 2184 and 1114 / 1173.
-//   128 against 64 with 544, 288, 160 and 96 likely 128-tiles: bf16 37 / 46, 21 / 28, 18.5 / 18.7 and 18.0 / 11.5; fp32 200 / 173,
-//   130 / 99, 74 / 63 and 73 / 40.
-//   any alignment, 128 against 64 with 544, 416, 288, 224 and 160 likely 128-tiles: bf16 57 / 51, 32 / 45, 32 / 40, 30 / 29 and 29 / 22; fp32
-//   229 / 164, 145 / 143, 143 / 109, 89 / 87 and 88 / 67.
+//   256 against 128, 2048 to 4096, 2304 / 2560 / 4096 / 4608 rows (288 to 576 likely 256-tiles): bf16 85 / 91 / 126 / 152 and
+//   92 / 93 / 143 / 163; 2048 to 2048, 1280 / 2304 rows (80 and 144) 50 / 54 and 34 / 58 (the rule takes 128 for both).
+//   fp32, 256 against 64, the same: 620 / 628 / 981 / 1113 and 641 / 711 / 1133 / 1274 (the rule takes 64 for the first two);
+//   264 / 488 and 186 / 324.
+//   128 against 64, 2048 to 2048, 384 / 640 / 896 / 1152 / 1664 / 2176 rows (96 to 544 likely 128-tiles): bf16
+//   26.8 / 27.5 / 27.9 / 31.6 / 34.8 / 58.4 and 16.4 / 26.7 / 31.8 / 41.4 / 55.7 / 70.3; fp32 137 / 139 / 139 / 253 / 257 / 385 and
+//   76 / 115 / 144 / 185 / 254 / 325.
+//   any alignment, 2047 to 2048, the same rows: bf16 44 / 46 / 46 / 51 / 52 / 94 and 29 / 37 / 49 / 66 / 77 / 106; fp32
+//   165 / 166 / 166 / 276 / 278 / 439 and 90 / 126 / 162 / 207 / 275 / 357.
 template <typename T>
 static int launch_gated(GroupedArgs a, const char* who, hipStream_t st) {
   constexpr bool F32 = sizeof(T) == 4;

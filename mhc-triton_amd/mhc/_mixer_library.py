@@ -115,6 +115,7 @@ torch.library.register_autograd("mhc_mixer::decay_attention", _decay_bwd, setup_
 
 
 def decay_attention(q, k, v, log_decay, offsets, initial_state, scale):
+    """(o, state).  The state is always made and the segments' states are not kept for the backward, which makes them again."""
     return torch.ops.mhc_mixer.decay_attention(q, k, v, log_decay, offsets, initial_state, scale)
 
 

@@ -363,7 +363,9 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     2^22 elements apart), heads that are one expanded among them.  Sums are fp32; products are of bf16 parts whose sum
     is the operand, exactly for inputs.  A value that is not finite reaches its own and later tokens of its sequence and
     head, no others; which of them are infinite and which NaN may differ from the recurrence's (fp32 magnitudes that round
-    to no bf16, from 3.39e38 on, count as not finite).
+    to no bf16, from 3.39e38 on, count as not finite).  What is computed (weights, states) enters the products as two bf16
+    parts for 16-bit types, 2^-16 of itself or better, three for fp32.  With ``return_state``, and in traced calls, weighted values have a
+    part more than without, so that the last bits of o may differ.
     """
     _no_gradient("decay_attention", "log_decay", log_decay)
     scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
@@ -412,7 +414,8 @@ def gated_matmul(x: torch.Tensor, weight: torch.Tensor, offsets: Optional[torch.
     ``offsets`` it is (experts, 2 * out, in) and x's rows are sorted by expert, exactly as in ``grouped_matmul``.
     ``activation`` is "silu", "gelu" (by the error function) or "gelu_tanh".  Both products are summed, activated and
     multiplied in fp32 and rounded once.  Differentiable in x and weight; for the backward both products are kept
-    in fp32 (8 * rows * out bytes).
+    in fp32 (8 * rows * out bytes).  Gradients are rounded twice: the gradients of the two products, computed in fp32, to x's
+    dtype before their own products, and the results.
     """
     if torch.compiler.is_compiling():
         return _ml.gated_matmul(x, weight, offsets, activation)
