@@ -447,7 +447,7 @@ int mhc_rotary(const void* q, int64_t q_row, int64_t q_head, void* q_out, int64_
  * ones: sequence n has rows [offsets[n-1], offsets[n]), clamped and as the running
  * maximum; rows past the last, all of them where N = 0, get zeros.  q, k [R,H,Dk], v, o [R,H,Dv] in `dtype`,
  * Dk, Dv <= 128; first, last [N,H,Dk,Dv] f32, the states before and after (NULL: zeros,
- * not wanted).  Rows up to 2^22 elements apart. */
+ * not wanted).  Rows up to 2^22 elements apart, at most 2^24 sequences. */
 size_t mhc_decay_attention_workspace_bytes(int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv, int packed, int dtype);
 
 int mhc_decay_attention_forward(const void* q, int64_t q_row, int64_t q_head,

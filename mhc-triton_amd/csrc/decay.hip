@@ -30,21 +30,30 @@ static int64_t count_tiles(int64_t R, int64_t N, int64_t seg, bool packed) {
   return N * (T > seg ? (T + seg - 1) / seg : 1);
 }
 
-// A scan's segments and what the states that they leave take.
+// From so many packed sequences on a table says which segment a tile has; the tiles' own searches grow with the square of their
+// number.  Heads of 128, sequences of 64 tokens, forward without / with in us: 4 heads, 32 / 64 / 128 / 256 / 1024 sequences
+// 15 / 16 / 28 / 53 / 254 and 17 / 18 / 26 / 41 / 141; 32 heads, 32 / 64 / 128 / 256 / 1024 39 / 69 / 150 / 307 / 1694 and
+// 39 / 66 / 137 / 264 / 1004.
+constexpr int64_t kTableSequences = 128;
+
+// A scan's segments and what they take of the workspace: the states that they leave, then the table.
 struct Plan {
-  int64_t seg, tiles, bytes;  // bytes 0: no sequence has a second segment
-  int64_t joins;              // sequences of more than kSummed segments, at most; 0: decay_join_kernel does not run
+  int64_t seg, tiles;
+  int64_t parts;  // bytes; 0: no sequence has a second segment
+  int64_t joins;  // sequences of more than kSummed segments, at most; 0: decay_join_kernel does not run
+  int64_t table;  // bytes; 0: without
 };
 static Plan plan_scan(int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv, bool packed) {
   Plan p;
   p.seg = segment_tokens(R, N, H, packed);
   p.tiles = count_tiles(R, N, p.seg, packed);
   const int64_t longest = packed || N == 0 ? R : R / N;
-  p.bytes = longest > p.seg ? (R - 1) / p.seg * H * Dk * Dv * 4 : 0;  // places of part_place
+  p.parts = longest > p.seg ? (R - 1) / p.seg * H * Dk * Dv * 4 : 0;  // places of part_place
   // Packed sequences' lengths are not known here, and that one is so long is not likely: from twice as many rows on.  One head of
   // 65536 tokens in 64 sequences, forward / backward in us without and with the launch: split evenly 44 / 81 and 47 / 83, all but 63 in
   // the first 281 / 994 and 111 / 145; 12 heads of 16384 in 256 sequences 110 / 300 and 115 / 304, 169 / 437 and 176 / 417.
   p.joins = longest <= kSummed * p.seg * (packed && N > 1 ? 2 : 1) ? 0 : packed ? (R - 1) / (kSummed * p.seg) : N;
+  p.table = packed && N >= kTableSequences ? (p.tiles + p.joins) * 16 : 0;
   return p;
 }
 
@@ -75,6 +84,22 @@ static bool whole_chunks(const void* p, int64_t row, int64_t head, int64_t D) {
   return aligned16(p) && row >= D && row % kElems<T> == 0 && head % kElems<T> == 0 && D % kElems<T> == 0;
 }
 
+// What the scans of a call share, and its table made at `table` where it is null and there is to be one.
+static int set_plan(DecayArgs& a, const Plan& plan, void* table, const char* who, hipStream_t st) {
+  if (plan.tiles * a.H >= ((int64_t)1 << 31) - 8) {
+    set_error("%s: %lld segments of %d heads are too many for a call", who, (long long)plan.tiles, a.H);
+    return MHC_ERR_ARG;
+  }
+  a.T = a.N ? a.R / a.N : 0;
+  a.seg = (int)plan.seg;
+  a.tiles = (int)plan.tiles;
+  a.joined = plan.joins > 0;
+  if (!plan.table || a.table) return MHC_OK;
+  a.table = (const int32_t*)table;
+  decay_table_kernel<<<dim3(1), kTableThreads, 0, st>>>(a, (int32_t*)table, (int)plan.joins);
+  return hip_status(hipGetLastError(), who);
+}
+
 // The segments' states (needed where there are several), or the outputs, of scans alike in their plan and in how many
 // halves of 128 their dims take.  exact: a last state is to come of them.
 enum { kStates = 1, kOutputs = 2 };
@@ -83,18 +108,10 @@ static int scan(DecayJobs jobs, const Plan& plan, int what, bool exact, const ch
   bool chunks = true;
   for (int j = 0; j < jobs.n; ++j) {
     DecayArgs& a = jobs.job[j];
-    if (plan.tiles * a.H >= ((int64_t)1 << 31) - 8) {
-      set_error("%s: %lld segments of %d heads are too many for a call", who, (long long)plan.tiles, a.H);
-      return MHC_ERR_ARG;
-    }
-    a.T = a.N ? a.R / a.N : 0;
-    a.seg = (int)plan.seg;
-    a.tiles = (int)plan.tiles;
-    a.joined = plan.joins > 0;
     chunks = chunks && whole_chunks<T>(a.q, a.q_row, a.q_head, a.Dk) && whole_chunks<T>(a.k, a.k_row, a.k_head, a.Dk) &&
              whole_chunks<T>(a.v, a.v_row, a.v_head, a.Dv) && aligned16(a.o);
   }
-  const bool states = what & kStates && plan.bytes, outputs = what & kOutputs;
+  const bool states = what & kStates && plan.parts, outputs = what & kOutputs;
   const DecayArgs& a = jobs.job[0];
   auto launch = [&](auto w, auto parts) {
     constexpr int WAVES = decltype(w)::value, WEIGHTED = decltype(parts)::value;
@@ -164,8 +181,9 @@ using namespace mhc;
 
 extern "C" size_t mhc_decay_attention_workspace_bytes(int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv, int packed,
                                                       int /*dtype*/) {
-  if (R <= 0 || N < 0 || H <= 0 || Dk <= 0 || Dv <= 0) return 0;
-  return (size_t)plan_scan(R, N, H, Dk, Dv, packed).bytes;
+  if (R < 0 || N < 0 || H <= 0 || Dk <= 0 || Dv <= 0) return 0;
+  const Plan p = plan_scan(R, N, H, Dk, Dv, packed);
+  return (size_t)(p.parts + p.table);
 }
 
 extern "C" int mhc_decay_attention_forward(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
@@ -178,8 +196,8 @@ extern "C" int mhc_decay_attention_forward(const void* q, int64_t q_row, int64_t
   if (int rc = check_decay(who, R, N, H, Dk, Dv, packed, {q_row, k_row, v_row})) return rc;
   if (H == 0 || (R == 0 && (N == 0 || !last))) return MHC_OK;
   if (!log_decay || (R && (!q || !k || !v || !o))) return null_in(who);
-  const size_t need = mhc_decay_attention_workspace_bytes(R, N, H, Dk, Dv, packed, dtype);
-  if (int rc = check_workspace(who, workspace, workspace_bytes, need)) return rc;
+  const Plan plan = plan_scan(R, N, H, Dk, Dv, packed);
+  if (int rc = check_workspace(who, workspace, workspace_bytes, (size_t)(plan.parts + plan.table))) return rc;
   DecayJobs jobs{};
   jobs.n = 1;
   DecayArgs& a = jobs.job[0];
@@ -189,20 +207,23 @@ extern "C" int mhc_decay_attention_forward(const void* q, int64_t q_row, int64_t
   a.parts = (float*)workspace; a.part_row = (int)Dv; a.part_col = 1;
   a.R = R; a.N = (int)N; a.H = (int)H; a.Dk = (int)Dk; a.Dv = (int)Dv;
   a.out_scale = scale; a.in_scale = 1.f; a.lag = 1;
-  const Plan plan = plan_scan(R, N, H, Dk, Dv, packed);
-  return MHC_DISPATCH_DTYPE(dtype, [&] {
-    return scan<T>(jobs, plan, kStates | kOutputs, last != nullptr, who, (hipStream_t)stream);
+  return MHC_DISPATCH_DTYPE(dtype, [&]() -> int {
+    const hipStream_t st = (hipStream_t)stream;
+    if (int rc = set_plan(a, plan, (char*)workspace + plan.parts, who, st)) return rc;
+    return scan<T>(jobs, plan, kStates | kOutputs, last != nullptr, who, st);
   });
 }
 
 // Whether scans over states of Dk x Dv and of Dv x Dk run side by side: the same kernel.
 static bool alike(int64_t Dk, int64_t Dv) { return (Dk <= 64) == (Dv <= 64); }
 
-// The states that the segments of the backward scans (dv's and dk's) leave, and those of the forward where the caller
-// did not keep them.
+// The states that the segments of the backward scans (dv's and dk's) leave, and those of the forward, and the table, where the
+// caller did not keep them.
 extern "C" size_t mhc_decay_attention_backward_workspace_bytes(int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv,
                                                                int packed, int dtype) {
-  return 2 * mhc_decay_attention_workspace_bytes(R, N, H, Dk, Dv, packed, dtype);
+  if (R < 0 || N < 0 || H <= 0 || Dk <= 0 || Dv <= 0) return 0;
+  const Plan p = plan_scan(R, N, H, Dk, Dv, packed);
+  return (size_t)(2 * p.parts + p.table);
 }
 
 extern "C" int mhc_decay_attention_backward(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
@@ -219,10 +240,11 @@ extern "C" int mhc_decay_attention_backward(const void* q, int64_t q_row, int64_
   if (!log_decay || (R && (!q || !k || !v || !dout))) return null_in(who);
   const bool same = alike(Dk, Dv);
   const Plan plan = plan_scan(R, N, H, Dk, Dv, packed);
-  if (int rc = check_workspace(who, workspace, workspace_bytes, (size_t)plan.bytes * (kept ? 1 : 2))) return rc;
+  if (int rc = check_workspace(who, workspace, workspace_bytes, (size_t)(kept ? plan.parts : 2 * plan.parts + plan.table))) return rc;
   DecayArgs base{};
   base.log_decay = log_decay; base.offsets = offsets;
   base.R = R; base.N = (int)N; base.H = (int)H;
+  if (kept && plan.table) base.table = (const int32_t*)((const char*)kept + plan.parts);
   const int dims[2] = {(int)Dk, (int)Dv};
 
   // dq: from the first token on, states transposed.  Its segments' states are the forward's.
@@ -238,7 +260,7 @@ extern "C" int mhc_decay_attention_backward(const void* q, int64_t q_row, int64_
   // dv and dk: from the last token back, with the same states, dk's transposed
   base.first = d_last;
   base.out_scale = 1.f; base.in_scale = scale; base.lag = 0; base.reverse = true;
-  base.parts = (float*)((char*)workspace + (kept ? 0 : plan.bytes));
+  base.parts = (float*)((char*)workspace + (kept ? 0 : plan.parts));
   DecayArgs of_v = base;
   of_v.q = k; of_v.q_row = k_row; of_v.q_head = k_head;
   of_v.k = q; of_v.k_row = q_row; of_v.k_head = q_head;
@@ -257,6 +279,11 @@ extern "C" int mhc_decay_attention_backward(const void* q, int64_t q_row, int64_
   if (want_k && !want_v) of_k.last = d_first;
   return MHC_DISPATCH_DTYPE(dtype, [&]() -> int {
     const hipStream_t st = (hipStream_t)stream;
+    if (int rc = set_plan(of_q, plan, (char*)workspace + 2 * plan.parts, who, st)) return rc;
+    for (DecayArgs* a : {&of_v, &of_k}) {
+      a->table = of_q.table;
+      if (int rc = set_plan(*a, plan, nullptr, who, st)) return rc;
+    }
     auto one = [&](const DecayArgs& a, int what, bool fine) {
       DecayJobs jobs{};
       jobs.n = 1;

@@ -51,6 +51,7 @@ struct DecayArgs {
   const int32_t* offsets;    // ends of the packed sequences; null: N sequences of T rows each, or with N = 0 none
   const float* first;        // X_0 of each sequence, or null
   float* last;               // where X goes, or null
+  const int32_t* table;      // [tiles + joins][4]: what find_segment finds, or null
   float* parts;              // [place][H][Dk][Dv]: states that segments leave by themselves; joined: that the next start from
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;  // strides in elements; o is contiguous
   int state_row, state_col;                             // of first and last: X's rows and columns
@@ -94,6 +95,10 @@ __device__ __forceinline__ int segments_of(const DecayArgs& a, int64_t lo, int64
 // of the t-th sequence of more than kSummed.
 template <bool JOINED = false>
 __device__ __forceinline__ Segment find_segment(const DecayArgs& a, int t) {
+  if (a.table) {
+    const int32_t* p = a.table + 4 * ((int64_t)t + (JOINED ? a.tiles : 0));
+    return {p[0], p[1], p[2], p[3]};
+  }
   if (!a.offsets && a.N) {
     const int per = JOINED ? 1 : max(1, segments_of(a, 0, a.T));
     const int e = t / per;
@@ -121,6 +126,64 @@ __device__ __forceinline__ Segment find_segment(const DecayArgs& a, int t) {
     before = __shfl(upto, 63, 64);
   }
   return {-1, 0, 0, 0};
+}
+
+// The table: every tile's Segment, then the first segments of the sequences of more than kSummed; entries without one have
+// e = -1.  One workgroup, a thread a sequence.  For many packed sequences: a tile's own search reads the offsets of all before
+// it.
+constexpr int kTableThreads = 1024;
+
+__global__ __launch_bounds__(kTableThreads) void decay_table_kernel(DecayArgs a, int32_t* table, int joins) {
+  constexpr int W = kTableThreads / 64;
+  __shared__ int most[W];
+  __shared__ uint64_t sums[W];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int end = 0;        // of the sequences so far
+  uint64_t done = 0;  // their segments; above 2^32 those of more than kSummed
+  auto put = [&](int64_t at, int e, int s, int lo, int hi) {
+    int32_t* p = table + 4 * at;
+    p[0] = e, p[1] = s, p[2] = lo, p[3] = hi;
+  };
+  for (int64_t base = 0; base <= a.N; base += kTableThreads) {
+    const int64_t e = base + threadIdx.x;
+    int hi = e < a.N ? end_of(a.offsets, (int)e, a.R) : (int)a.R;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int v = __shfl_up(hi, off, 64);
+      if (lane >= off) hi = max(hi, v);
+    }
+    if (lane == 63) most[wave] = hi;
+    __syncthreads();
+    int before = end;
+    for (int w = 0; w < W; ++w) {
+      if (w < wave) before = max(before, most[w]);
+      end = max(end, most[w]);
+    }
+    hi = max(hi, before);
+    const int up = __shfl_up(hi, 1, 64), lo = lane ? up : before;
+    int n = segments_of(a, lo, hi);
+    const bool joined = e < a.N && n > kSummed;
+    n = e < a.N ? max(n, 1) : e == a.N ? n : 0;
+    const uint64_t mine = (uint64_t)joined << 32 | (uint32_t)n;
+    uint64_t upto = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const uint64_t v = __shfl_up(upto, off, 64);
+      if (lane >= off) upto += v;
+    }
+    if (lane == 63) sums[wave] = upto;
+    __syncthreads();
+    uint64_t at = done + upto - mine;
+    for (int w = 0; w < W; ++w) {
+      if (w < wave) at += sums[w];
+      done += sums[w];
+    }
+    for (int s = 0; s < n; ++s) put((int64_t)(uint32_t)at + s, (int)e, s, lo, hi);
+    if (joined && (int)(at >> 32) < joins) put(a.tiles + (int64_t)(at >> 32), (int)e, 0, lo, hi);
+    __syncthreads();  // sums and most have been read
+  }
+  for (int64_t t = (uint32_t)done + threadIdx.x; t < a.tiles; t += kTableThreads) put(t, -1, 0, 0, 0);
+  for (int64_t t = (done >> 32) + threadIdx.x; t < joins; t += kTableThreads) put(a.tiles + t, -1, 0, 0, 0);
 }
 
 // D[m][n] += sum_k A[m][k] B[n][k] of 16 x 16 x 32: a lane gives row (column) lane % 16 and the eight k of its group

@@ -1,6 +1,7 @@
 """The operators that mix tokens on the GPU: calls that their documentation allows and that test_gpu_mixer.py and
 test_gpu_mixer_paths.py do not make."""
 
+import numpy as np
 import pytest
 import torch
 
@@ -87,6 +88,100 @@ def test_a_long_sequence_among_many_short_ones():
             q, k, v = (rand(9400, H, D, seed=s)[rows] for s in (1, 2, 3))
             o = branch.decay_attention(q, k, v, ld, offsets=torch.tensor([1500, 2000], device=DEV))
             assert torch.equal(got[0][rows], o)
+
+
+def _lengths(N, seed):
+    """Mostly a few tokens or none, now and then some hundreds."""
+    r = np.random.default_rng(seed)
+    return np.where(r.random(N) < 0.005, r.integers(200, 700, N), r.integers(0, 4, N))
+
+
+@pytest.mark.parametrize("N,long,extra", [(127, 0, 3), (128, 0, 0), (1023, 300, 5), (1024, 0, 300), (1025, 5000, 0), (2500, 4000, 700)])
+def test_many_sequences(N, long, extra):
+    """Around the sizes at which a table says where tiles begin and at which it takes another round; long sequences, whose
+    segments are joined, among the first and the last; rows behind the last."""
+    H, Dk, Dv = 1, 24, 40
+    lens = _lengths(N, N)
+    lens[3], lens[N - 2] = long or lens[3], long // 2 or lens[N - 2]
+    ends = np.cumsum(lens)
+    R = int(ends[-1]) + extra
+    q, k = (rand(R, H, Dk, seed=i, dtype=torch.bfloat16).requires_grad_() for i in (1, 2))
+    v, do = rand(R, H, Dv, seed=3, dtype=q.dtype).requires_grad_(), rand(R, H, Dv, seed=4, dtype=q.dtype)
+    first, d_last = rand(N, H, Dk, Dv, seed=5).requires_grad_(), rand(N, H, Dk, Dv, seed=6)
+    off, ld = torch.tensor(ends, device=DEV), torch.tensor([-0.002], device=DEV)
+    check_decay(q, k, v, ld, off, first, do, d_last, Dk ** -0.5, M.spans_of(ends.tolist(), R))
+    # each gradient by itself, which makes the table again
+    o, state = branch.decay_attention(q, k, v, ld, initial_state=first, offsets=off, return_state=True)
+    for a, b in zip((k, v, first), torch.autograd.grad((o, state), (k, v, first), (do, d_last), retain_graph=True)):
+        got = _mixer.decay_attention_backward(q, k, v, do, ld, off, first, None, d_last, Dk ** -0.5,
+                                              (False, a is k, a is v, a is first))
+        close(next(g for g in got if g is not None), to_np(b), np.abs(to_np(b)).max(), 2.0 ** -7)
+
+
+def test_many_sequences_of_any_offsets():
+    """Offsets that fall, lie below 0 and past the rows; sequences without any token at all."""
+    H, D, R, N = 2, 16, 500, 1500
+    r = np.random.default_rng(1)
+    ends = np.sort(r.integers(-50, R + 50, N)) + r.integers(-20, 20, N)
+    q, k, v = (rand(R, H, D, seed=i).requires_grad_() for i in (1, 2, 3))
+    first, d_last, do = rand(N, H, D, D, seed=5).requires_grad_(), rand(N, H, D, D, seed=6), rand(R, H, D, seed=4)
+    check_decay(q, k, v, decays(H), torch.tensor(ends, device=DEV), first, do, d_last, 0.2, M.spans_of(ends.tolist(), R))
+    e = torch.empty(0, H, D, device=DEV).requires_grad_()
+    o, state = branch.decay_attention(e, e, e, decays(H), initial_state=first, offsets=torch.tensor(ends, device=DEV), return_state=True)
+    g, = torch.autograd.grad(state, first, d_last)
+    assert o.shape == e.shape and torch.equal(state, first) and torch.equal(g, d_last)
+
+
+def test_many_sequences_in_a_graph():
+    """A captured training step whose sequences change between replays."""
+    H, D, R, N = 1, 32, 3500, 200
+    q, k, v = (rand(R, H, D, seed=i, dtype=torch.bfloat16).requires_grad_() for i in (1, 2, 3))
+    do, ld, off = rand(R, H, D, seed=4, dtype=q.dtype), decays(H), torch.zeros(N, dtype=torch.int32, device=DEV)
+    splits = [np.cumsum(_lengths(N, s)) for s in range(3)] + [np.arange(N) // 150 * 3000 + 5]
+
+    def step():
+        o = branch.decay_attention(q, k, v, ld, offsets=off)
+        return [o.detach(), *torch.autograd.grad(o, (q, k, v), do)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for ends in splits:
+        off.copy_(torch.tensor(ends))
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [t.clone() for t in got]
+        for a, b in zip(kept, step()):
+            assert torch.equal(a, b)
+
+
+def test_many_sequences_take_no_longer_than_their_tokens():
+    """32768 packed sequences of 4 tokens against the same in a batch.  A search of the offsets by every workgroup took 50 times as
+    long, a table 1.1 times."""
+    N, T, H, D = 32768, 4, 8, 64
+    q, k, v = (rand(N, T, H, D, seed=i, dtype=torch.bfloat16) for i in (1, 2, 3))
+    ld, off = decays(H), torch.arange(T, N * T + 1, T, device=DEV, dtype=torch.int32)
+
+    def time(f):
+        out, best = f(), float("inf")
+        for _ in range(3):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            f()
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return out, best
+
+    want, dense = time(lambda: branch.decay_attention(q, k, v, ld))
+    got, packed = time(lambda: branch.decay_attention(q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1), ld, offsets=off))
+    print(f"packed {packed:.2f} ms, dense {dense:.2f} ms", flush=True)
+    assert torch.equal(got.view_as(want), want) and packed < 8 * dense
 
 
 @pytest.mark.parametrize("dtype", list(DT))
