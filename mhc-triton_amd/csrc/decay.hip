@@ -217,8 +217,8 @@ extern "C" int mhc_decay_attention_forward(const void* q, int64_t q_row, int64_t
 // Whether scans over states of Dk x Dv and of Dv x Dk run side by side: the same kernel.
 static bool alike(int64_t Dk, int64_t Dv) { return (Dk <= 64) == (Dv <= 64); }
 
-// The states that the segments of the backward scans (dv's and dk's) leave, and those of the forward, and the table, where the
-// caller did not keep them.
+// The states that the segments of the backward scans (dv's and dk's) leave, those of the forward where the caller did not keep
+// them, and the table: it is made again, because it says where to write, and what was kept may have been changed since.
 extern "C" size_t mhc_decay_attention_backward_workspace_bytes(int64_t R, int64_t N, int64_t H, int64_t Dk, int64_t Dv,
                                                                int packed, int dtype) {
   if (R < 0 || N < 0 || H <= 0 || Dk <= 0 || Dv <= 0) return 0;
@@ -240,11 +240,11 @@ extern "C" int mhc_decay_attention_backward(const void* q, int64_t q_row, int64_
   if (!log_decay || (R && (!q || !k || !v || !dout))) return null_in(who);
   const bool same = alike(Dk, Dv);
   const Plan plan = plan_scan(R, N, H, Dk, Dv, packed);
-  if (int rc = check_workspace(who, workspace, workspace_bytes, (size_t)(kept ? plan.parts : 2 * plan.parts + plan.table))) return rc;
+  const int64_t states = (kept ? 1 : 2) * plan.parts;
+  if (int rc = check_workspace(who, workspace, workspace_bytes, (size_t)(states + plan.table))) return rc;
   DecayArgs base{};
   base.log_decay = log_decay; base.offsets = offsets;
   base.R = R; base.N = (int)N; base.H = (int)H;
-  if (kept && plan.table) base.table = (const int32_t*)((const char*)kept + plan.parts);
   const int dims[2] = {(int)Dk, (int)Dv};
 
   // dq: from the first token on, states transposed.  Its segments' states are the forward's.
@@ -279,7 +279,7 @@ extern "C" int mhc_decay_attention_backward(const void* q, int64_t q_row, int64_
   if (want_k && !want_v) of_k.last = d_first;
   return MHC_DISPATCH_DTYPE(dtype, [&]() -> int {
     const hipStream_t st = (hipStream_t)stream;
-    if (int rc = set_plan(of_q, plan, (char*)workspace + 2 * plan.parts, who, st)) return rc;
+    if (int rc = set_plan(of_q, plan, (char*)workspace + states, who, st)) return rc;
     for (DecayArgs* a : {&of_v, &of_k}) {
       a->table = of_q.table;
       if (int rc = set_plan(*a, plan, nullptr, who, st)) return rc;

@@ -132,6 +132,26 @@ def test_many_sequences_of_any_offsets():
     assert o.shape == e.shape and torch.equal(state, first) and torch.equal(g, d_last)
 
 
+def test_many_sequences_whose_forward_left_nothing():
+    """Without tokens and with no state wanted the forward does nothing; the gradient of the first states is there all the same.
+    Whatever becomes of the states that a forward kept, gradients stay in their places."""
+    H, D, N = 2, 16, 300
+    off, ld = torch.zeros(N, dtype=torch.int32, device=DEV), decays(H)
+    e, first = torch.empty(0, H, D, device=DEV).requires_grad_(), rand(N, H, D, D, seed=1).requires_grad_()
+    o = branch.decay_attention(e, e, e, ld, initial_state=first, offsets=off)
+    g, dq = torch.autograd.grad(o, (first, e), torch.empty_like(o))
+    assert not g.any() and dq.shape == e.shape
+    ends = torch.tensor(np.cumsum(_lengths(N, 7)) + 900, device=DEV)
+    R = int(ends[-1]) + 9
+    q, k, v, do = (rand(R, H, D, seed=i) for i in range(4))
+    kept = _mixer.decay_attention_forward(q, k, v, ld, ends, None, 0.1, False)[2]
+    want = _mixer.decay_attention_backward(q, k, v, do, ld, ends, None, kept, None, 0.1, (True,) * 4)
+    got = _mixer.decay_attention_backward(q, k, v, do, ld, ends, None, torch.full_like(kept, 255), None, 0.1, (True,) * 4)
+    for a, b in zip(got[1:], want[1:]):
+        assert torch.equal(a, b)
+    assert torch.equal(got[0][:256], want[0][:256]) and torch.isnan(got[0][256:900]).all()
+
+
 def test_many_sequences_in_a_graph():
     """A captured training step whose sequences change between replays."""
     H, D, R, N = 1, 32, 3500, 200
